@@ -1,0 +1,414 @@
+"""Operators of a key/value cache kept in pages, for serving.
+
+The cache of one layer is two tensors of pages ``k_pages`` and ``v_pages``,
+each ``(n_pages, Hkv, page_size, d)`` with a contiguous last axis (any other
+strides: pass a ``(n_pages, page_size, Hkv, d)`` storage transposed).  Key
+``j`` of sequence ``b`` lies in slot ``j % page_size`` of page
+``block_table[b, j // page_size]``; one table serves every layer.  Lengths,
+tables, positions and slots are device tensors that no call reads back, so a
+step recorded into a hipGraph replays with new ones.
+
+A layer's step over new tokens:
+
+* :func:`qk_norm_rope_append` norms and rotates their queries and keys and
+  writes keys and values into the cache (:func:`qk_norm_rope` returns them
+  instead);
+* :func:`paged_attention` attends from each sequence's new tokens to its
+  cached keys, a prompt, a chunk of one or a single token alike, and can add
+  up every key's attention weight;
+* :func:`paged_evict` moves each head's most attended and most recent keys
+  into a smaller cache.
+
+As in :mod:`catopt_amd.kernels`, operands are device tensors checked on the
+host before any launch, outputs and workspace come from torch's caching
+allocator, and work is enqueued on torch's current stream of the operands'
+device.  What only the device knows (a length past the table, a page index
+outside the pages) never leads out of bounds: lengths are cut to the table's
+reach, keys of an invalid page count as masked, and a write to one is dropped.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib as L
+from .kernels import _DT, _need_device, _ptr, _stream, _workspace
+
+__all__ = ["qk_norm_rope", "qk_norm_rope_append", "paged_attention", "paged_evict", "PAGED_ATTENTION_MAX_HEAD_DIM",
+           "QK_NORM_ROPE_MAX_HEAD_DIM"]
+
+PAGED_ATTENTION_MAX_HEAD_DIM = 128
+QK_NORM_ROPE_MAX_HEAD_DIM = 256
+
+_I12, _I14, _I16 = C.c_int64 * 12, C.c_int64 * 14, C.c_int64 * 16
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The byte range that a tensor's elements lie in."""
+    p = t.data_ptr()
+    if t.numel() == 0:
+        return p, p
+    return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _apart(name: str, out: torch.Tensor, *ins: torch.Tensor | None) -> None:
+    lo, hi = _span(out)
+    for t in ins:
+        if t is not None:
+            a, b = _span(t)
+            if a < hi and lo < b:
+                raise ValueError(f"{name} overlaps one of the call's other operands")
+
+
+def _no_overlap_within(name: str, t: torch.Tensor) -> None:
+    """An output whose elements share memory (an expanded tensor) is refused."""
+    need = 1
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s < need:
+            raise ValueError(f"{name} has elements that share memory (strides {t.stride()})")
+        need = s * n
+
+
+class _on:
+    """The operands' device as the current one for a call's launches."""
+
+    __slots__ = ("dev", "old")
+
+    def __init__(self, dev: int) -> None:
+        self.dev = dev
+
+    def __enter__(self) -> None:
+        self.old = torch.cuda.current_device()
+        if self.old != self.dev:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc) -> None:
+        if self.old != self.dev:
+            torch.cuda.set_device(self.old)
+
+
+def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
+    """``(N, H, d)`` with a contiguous last axis, rows readable in 16-byte pieces."""
+    if t.dim() != 3:
+        raise ValueError(f"{name} is (tokens, heads, head dim), got {tuple(t.shape)}")
+    step = 16 // t.element_size()
+    s = t.stride()
+    if s[2] != 1 or s[0] % step or s[1] % step or t.data_ptr() % 16:
+        t = t.contiguous()
+    return t
+
+
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, what: str = "") -> tuple[int, int, int, int]:
+    """The shape of a cache's two page tensors, checked: they are used in place, so nothing is copied to fit."""
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        raise ValueError(f"the {what}pages are two tensors (n_pages, heads, page size, head dim) of one type, got "
+                         f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
+    step = 16 // k_pages.element_size()
+    for t in (k_pages, v_pages):
+        s = t.stride()
+        if s[3] != 1 or s[0] % step or s[1] % step or s[2] % step or t.data_ptr() % 16:
+            raise ValueError(f"{what}pages need a contiguous head dim and 16-byte aligned rows, got strides {s}")
+    return tuple(k_pages.shape)
+
+
+def _two_tensors(a: torch.Tensor, b: torch.Tensor) -> None:
+    """Keys and values are not one tensor (they may be two parts of one, so their ranges may interleave)."""
+    if a.data_ptr() == b.data_ptr() and a.numel():
+        raise ValueError("keys and values need pages of their own")
+
+
+def _ints(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
+    if t.dtype != dtype or t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
+        want = tuple("any" if w is None else w for w in shape)
+        raise ValueError(f"{name} is an {dtype} tensor of shape {want}, got {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _table(name: str, t: torch.Tensor, B: int) -> torch.Tensor:
+    _ints(name, t, torch.int32, (B, None))
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleaved, k_pages, v_pages, slots):
+    append = slots is not None
+    dev = _need_device(q, k, v, cos, sin, positions, q_weight, k_weight, k_pages, v_pages, slots)
+    lib = L.load()
+    dt = _DT.get(q.dtype)
+    if dt is None:
+        raise NotImplementedError(f"qk_norm_rope runs on fp32 and bf16 operands, got {q.dtype}")
+    q, k = _heads("q", q), _heads("k", k)
+    N, Hq, d = q.shape
+    Hkv = k.shape[1]
+    if k.dtype != q.dtype or k.shape[0] != N or k.shape[2] != d:
+        raise ValueError(f"q and k share tokens, head dim and type: {tuple(q.shape)} {q.dtype}, "
+                         f"{tuple(k.shape)} {k.dtype}")
+    if not 1 <= d <= QK_NORM_ROPE_MAX_HEAD_DIM:
+        raise NotImplementedError(f"qk_norm_rope takes head dims up to {QK_NORM_ROPE_MAX_HEAD_DIM}, got {d}")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError("cos and sin are fp32 tables (positions, rotated dims / 2) of one shape")
+    rot = 2 * cos.shape[1]
+    if rot > d:
+        raise ValueError(f"the tables rotate {rot} dims of a head of {d}")
+    if rot and (cos.stride(1) != 1 or sin.stride() != cos.stride()):
+        cos, sin = cos.contiguous(), sin.contiguous()
+    for w in (q_weight, k_weight):
+        if w is not None and (w.dtype != q.dtype or w.numel() != d):
+            raise ValueError("a norm weight holds one value of q's type for each head dim")
+    q_weight = None if q_weight is None else q_weight.contiguous()
+    k_weight = None if k_weight is None else k_weight.contiguous()
+    _ints("positions", positions, torch.int64, (N,))
+    positions = positions.contiguous()
+    q_out = torch.empty((N, Hq, d), dtype=q.dtype, device=q.device)
+    n_pages = page = 0
+    if append:
+        v = _heads("v", v)
+        if v.shape != k.shape or v.dtype != q.dtype:
+            raise ValueError(f"v has k's shape and type: {tuple(v.shape)} {v.dtype}, {tuple(k.shape)} {k.dtype}")
+        n_pages, ph, page, pd = _pages(k_pages, v_pages)
+        if (ph, pd) != (Hkv, d) or k_pages.dtype != q.dtype:
+            raise ValueError(f"the pages hold {ph} heads of {pd} {k_pages.dtype}, k has {Hkv} of {d} {q.dtype}")
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            _no_overlap_within(name, t)
+            _apart(name, t, q, k, v, cos, sin, positions, slots)
+        _two_tensors(k_pages, v_pages)
+        _ints("slots", slots, torch.int64, (N,))
+        slots = slots.contiguous()
+        k_out, v_out = k_pages, v_pages
+        ks, vs = k_pages.stride(), v_pages.stride()
+        strides = _I12(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *ks[:3], *vs[:3])
+    else:
+        k_out = torch.empty((N, Hkv, d), dtype=q.dtype, device=q.device)
+        v_out = None
+        strides = _I12(*q.stride()[:2], *k.stride()[:2])
+    with _on(dev):
+        st = lib.catopt_hip_qk_norm_rope(dt, N, Hq, Hkv, d, rot, int(bool(interleaved)), _ptr(q), _ptr(k), _ptr(v),
+                                         _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
+                                         cos.shape[0], cos.stride(0) if rot else 0, _ptr(positions), _ptr(q_out),
+                                         _ptr(k_out), _ptr(v_out), strides, _ptr(slots), n_pages, page, _stream(q))
+    L.check("catopt_hip_qk_norm_rope", st)
+    return q_out, k_out
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6, *,
+                 interleaved: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """The RMS norm of every head of ``q (N, Hq, d)`` and ``k (N, Hkv, d)``
+    and their position rotation, in one pass (fp32 or bf16; computed in fp32,
+    rounded once).
+
+    ``x * rsqrt(mean(x²) + eps) * weight`` over the head dim (a weight of
+    ``None``: no norm), then each pair ``(a, b)`` of the first ``rot`` dims
+    becomes ``(a c - b s, b c + a s)``: pairs ``(i, i + rot/2)``, or ``(2i,
+    2i+1)`` when ``interleaved``, with ``c, s`` of row ``positions[n]`` of the
+    fp32 tables ``cos, sin (positions, rot/2)``.  ``q`` and ``k`` may be views
+    of one projection's rows.  ``positions`` is int64; one outside the tables
+    gives NaN in the rotated dims.  Returns new ``(q, k)``."""
+    return _norm_rope(q, k, None, cos, sin, positions, q_weight, k_weight, eps, interleaved, None, None, None)
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                        positions: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor,
+                        q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                        *, interleaved: bool = False) -> torch.Tensor:
+    """:func:`qk_norm_rope` whose keys go into the cache, with ``v (N, Hkv,
+    d)`` as it is: token ``n`` to slot ``slots[n] % page_size`` of page
+    ``slots[n] // page_size`` of ``k_pages`` and ``v_pages``.  ``slots`` is
+    int64 and names no slot twice; a token whose slot lies outside the pages
+    (-1 for padding) is not written.  Returns the new ``q``."""
+    if slots is None or k_pages is None or v_pages is None or v is None:
+        raise TypeError("qk_norm_rope_append needs v, k_pages, v_pages and slots")
+    return _norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleaved, k_pages, v_pages, slots)[0]
+
+
+def _weight_rows(name: str, w: torch.Tensor, B: int, H: int, width: int) -> tuple[int, int]:
+    if w.dtype != torch.float32 or w.dim() != 3 or w.shape[0] != B or w.shape[1] != H or w.shape[2] < width:
+        raise ValueError(f"{name} is an fp32 ({B}, {H}, at least {width}) tensor, got {w.dtype} {tuple(w.shape)}")
+    if w.shape[2] > 1 and w.stride(2) != 1:
+        raise ValueError(f"{name} needs a contiguous last axis, got strides {w.stride()}")
+    return w.stride(0), w.stride(1)
+
+
+def _in_place_or_apart(name: str, out: torch.Tensor, src: torch.Tensor | None) -> None:
+    """``out`` is ``src`` itself, element for element, or shares no memory with it."""
+    if src is not None and (out.data_ptr() != src.data_ptr() or out.stride() != src.stride()):
+        _apart(name, out, src)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    kv_lens: torch.Tensor, q_starts: torch.Tensor, scale: float, *, causal: bool = True,
+                    weights: torch.Tensor | None = None, weights_out: torch.Tensor | None = None,
+                    return_ml: bool = False, empty_rows: str = "nan", out: torch.Tensor | None = None):
+    """Attention of each sequence's new tokens over its cached keys (bf16).
+
+    ``q (N, Hq, d)`` holds the tokens of all sequences, sequence ``b``'s in
+    rows ``q_starts[b]`` to ``q_starts[b + 1]`` (int32, ``B + 1`` ascending
+    values); ``kv_lens (B,)`` int32 counts its cached keys, the new tokens'
+    own the last of them (write them first, :func:`qk_norm_rope_append`).
+    ``block_table (B, n)`` is int32.  With ``causal`` token ``i`` of ``n``
+    sees keys ``j <= kv_len - n + i``, else every key.  Query head ``h`` reads
+    key head ``h // (Hq // Hkv)``.  ``d`` is a multiple of 8 up to 128, the
+    page size a multiple of 8.
+
+    Returns ``o (N, Hq, d)``, written to ``out`` when given; rows behind the
+    last sequence are neither read nor written.  ``return_ml`` adds the fp32
+    ``(m, l)`` om carriers of the rows, ``(N, Hq)``, so that a part of the
+    keys kept elsewhere can be combined.  A row that sees no key is NaN
+    (``empty_rows="nan"``) or 0 (``"zero"``), as in
+    :func:`catopt_amd.kernels.attention`.
+
+    ``weights_out (B, Hkv, L)`` fp32, ``L`` at least the table's reach,
+    receives the sum over the new tokens and the key head's query heads of
+    each key's softmax weight, on top of ``weights`` (the sums so far; none:
+    zeros), which is not read for the new tokens' own keys.  Entries from
+    ``kv_lens[b]`` on are left as they were.  ``weights_out`` may be
+    ``weights``."""
+    if empty_rows not in ("nan", "zero"):
+        raise ValueError(f"empty_rows is 'nan' or 'zero', got {empty_rows!r}")
+    dev = _need_device(q, k_pages, v_pages, block_table, kv_lens, q_starts, weights, weights_out, out)
+    lib = L.load()
+    if q.dtype != torch.bfloat16 or k_pages.dtype != q.dtype:
+        raise NotImplementedError(f"paged attention runs on bf16 operands, got {q.dtype} and {k_pages.dtype} pages")
+    q = _heads("q", q)
+    N, Hq, d = q.shape
+    n_pages, Hkv, page, pd = _pages(k_pages, v_pages)
+    if pd != d or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"q has {Hq} heads of {d}, the pages {Hkv} heads of {pd}: the head dims agree and the query "
+                         "heads are a multiple of the key heads")
+    if d % 8 or not 8 <= d <= PAGED_ATTENTION_MAX_HEAD_DIM:
+        raise NotImplementedError(f"paged attention takes head dims that are multiples of 8 up to "
+                                  f"{PAGED_ATTENTION_MAX_HEAD_DIM}, got {d}")
+    if page < 1 or page % 8:
+        raise NotImplementedError(f"paged attention takes page sizes that are multiples of 8, got {page}")
+    scale = float(scale)
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"the scale is a positive number, got {scale}")
+    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+    _ints("kv_lens", kv_lens, torch.int32, (None,))
+    _ints("q_starts", q_starts, torch.int32, (B + 1,))
+    table = _table("block_table", block_table, B)
+    n_table = table.shape[1]
+    kv_lens, q_starts = kv_lens.contiguous(), q_starts.contiguous()
+    if out is None:
+        o = torch.empty((N, Hq, d), dtype=q.dtype, device=q.device)
+    else:
+        o = out
+        if o.shape != q.shape or o.dtype != q.dtype:
+            raise ValueError(f"out has q's shape and type, got {tuple(o.shape)} {o.dtype}")
+        so = o.stride()
+        if so[2] != 1 or so[0] % 8 or so[1] % 8 or o.data_ptr() % 16:
+            raise ValueError(f"out needs a contiguous head dim and 16-byte aligned rows, got strides {so}")
+        _no_overlap_within("out", o)
+        _apart("out", o, q, k_pages, v_pages, weights, weights_out)
+    w_in, w_out = (0, 0), (0, 0)
+    if weights_out is not None:
+        w_out = _weight_rows("weights_out", weights_out, B, Hkv, n_table * page)
+        _no_overlap_within("weights_out", weights_out)
+        if weights is not None:
+            w_in = _weight_rows("weights", weights, B, Hkv, n_table * page)
+        _in_place_or_apart("weights_out", weights_out, weights)
+        _apart("weights_out", weights_out, q, k_pages, v_pages)
+    elif weights is not None:
+        raise ValueError("weights need a weights_out to go to")
+    m = l = None
+    if return_ml:
+        m = torch.empty((N, Hq), dtype=torch.float32, device=q.device)
+        l = torch.empty((N, Hq), dtype=torch.float32, device=q.device)
+    if N and B:
+        ks, vs, qs, so = k_pages.stride(), v_pages.stride(), q.stride(), o.stride()
+        strides = _I14(qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], so[0], so[1], *w_in, *w_out)
+        with _on(dev):
+            wsb = lib.catopt_hip_paged_attn_workspace_bytes(B, N, Hq, Hkv, d, n_table, page,
+                                                            int(weights_out is not None))
+            if wsb < 0:
+                raise NotImplementedError("paged attention: the call is beyond what one launch takes")
+            ws = _workspace(wsb, q.device)
+            st = lib.catopt_hip_paged_attn_fwd(L.BF16, B, N, Hq, Hkv, d, q.data_ptr(), k_pages.data_ptr(),
+                                               v_pages.data_ptr(), n_pages, page, table.data_ptr(), table.stride(0),
+                                               n_table, kv_lens.data_ptr(), q_starts.data_ptr(), scale,
+                                               int(bool(causal)), 2 if empty_rows == "zero" else 1, o.data_ptr(),
+                                               _ptr(m), _ptr(l), _ptr(weights), _ptr(weights_out), strides, _ptr(ws),
+                                               wsb, _stream(q))
+        L.check("catopt_hip_paged_attn_fwd", st)
+    return (o, m, l) if return_ml else o
+
+
+def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                weights: torch.Tensor, out_table: torch.Tensor, budget: int, recent: int = 0, *,
+                k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None,
+                weights_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cut each sequence's cache to ``budget`` keys a head, by accumulated
+    attention weight (fp32 or bf16 pages).
+
+    Of the ``n = kv_lens[b]`` keys of head ``h``, ``min(n, budget)`` stay: the
+    last ``recent`` ones and, of the others, those of the largest ``weights[b,
+    h, :]`` (:func:`paged_attention`'s sums; the lowest index first among
+    equals, a NaN above every number).  Each head keeps its own, in their
+    order: they move to slots 0, 1, … of the pages ``out_table (B, n')`` names
+    in ``k_out, v_out (n_out_pages, Hkv, out_page_size, d)``, a cache of its
+    own (say of a fixed size for generation) or, by default, ``k_pages,
+    v_pages``.  In that case the pages of ``out_table`` are free ones: none
+    may be in ``block_table``, whose pages can be given back afterwards.
+    Rows behind the last kept key are left as they were.
+
+    Returns ``kept (B, Hkv, budget)`` int32 (the keys' indices, -1 behind the
+    last), ``new_lens (B,)`` int32 and their weights, in ``weights_out (B,
+    Hkv, at least budget)`` when given (it may be ``weights``), else in a new
+    tensor whose entries behind the last kept key are 0."""
+    if (k_out is None) != (v_out is None):
+        raise ValueError("give both k_out and v_out, or neither")
+    dev = _need_device(k_pages, v_pages, block_table, kv_lens, weights, out_table, k_out, v_out, weights_out)
+    lib = L.load()
+    dt = _DT.get(k_pages.dtype)
+    if dt is None:
+        raise NotImplementedError(f"eviction runs on fp32 and bf16 pages, got {k_pages.dtype}")
+    n_pages, Hkv, page, d = _pages(k_pages, v_pages)
+    own = k_out is None
+    k_to, v_to = (k_pages, v_pages) if own else (k_out, v_out)
+    n_out, ho, page_out, do = _pages(k_to, v_to, "output ")
+    if (ho, do) != (Hkv, d) or k_to.dtype != k_pages.dtype:
+        raise ValueError(f"the output pages hold {ho} heads of {do} {k_to.dtype}, the cache {Hkv} of {d} {k_pages.dtype}")
+    if d < 1 or Hkv < 1 or page < 1 or page_out < 1 or d * k_pages.element_size() % 16:
+        raise NotImplementedError(f"eviction takes rows of a multiple of 16 bytes, got {d} of {k_pages.dtype}")
+    budget, recent = int(budget), int(recent)
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"a budget of at least 1 with 0 <= recent <= budget, got {budget} and {recent}")
+    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+    _ints("kv_lens", kv_lens, torch.int32, (None,))
+    table, to = _table("block_table", block_table, B), _table("out_table", out_table, B)
+    n_table, n_to = table.shape[1], to.shape[1]
+    if n_to * page_out < budget:
+        raise ValueError(f"out_table reaches {n_to * page_out} keys, the budget is {budget}")
+    _two_tensors(k_to, v_to)
+    for name, t, src in (("k_out", k_to, k_pages), ("v_out", v_to, v_pages)):
+        _no_overlap_within(name, t)
+        _apart(name, t, weights, table, to, kv_lens)
+        _in_place_or_apart(name, t, src)
+    if not own:
+        _two_tensors(k_to, v_pages)
+        _two_tensors(v_to, k_pages)
+    if B > 0 and n_table and to.data_ptr() == table.data_ptr() and k_to.data_ptr() == k_pages.data_ptr():
+        raise ValueError("out_table names pages of its own, not those of block_table")
+    kv_lens = kv_lens.contiguous()
+    w_in = _weight_rows("weights", weights, B, Hkv, n_table * page)
+    if weights_out is None:
+        weights_out = torch.zeros((B, Hkv, budget), dtype=torch.float32, device=weights.device)
+    w_out = _weight_rows("weights_out", weights_out, B, Hkv, budget)
+    _no_overlap_within("weights_out", weights_out)
+    _in_place_or_apart("weights_out", weights_out, weights)
+    _apart("weights_out", weights_out, k_pages, v_pages, k_to, v_to)
+    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=k_pages.device)
+    new_lens = torch.empty((B,), dtype=torch.int32, device=k_pages.device)
+    if B:
+        strides = _I16(*k_pages.stride()[:3], *v_pages.stride()[:3], *k_to.stride()[:3], *v_to.stride()[:3],
+                       *w_in, *w_out)
+        with _on(dev):
+            st = lib.catopt_hip_paged_evict(dt, B, Hkv, d, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page,
+                                            _ptr(table), table.stride(0), n_table, kv_lens.data_ptr(),
+                                            weights.data_ptr(), budget, recent, k_to.data_ptr(), v_to.data_ptr(),
+                                            n_out, page_out, to.data_ptr(), to.stride(0), n_to, kept.data_ptr(),
+                                            new_lens.data_ptr(), weights_out.data_ptr(), strides, _stream(k_pages))
+        L.check("catopt_hip_paged_evict", st)
+    return kept, new_lens, weights_out

@@ -557,6 +557,116 @@ int32_t catopt_hip_silu(int32_t dtype, int64_t n, const void* x, void* y,
 int32_t catopt_hip_silu_mul(int32_t dtype, int64_t n, const void* g,
                             const void* u, void* y, void* stream);
 
+/*
+ * ---- A key/value cache in pages
+ *
+ * The cache of one layer is two tensors of pages, k_pages and v_pages, each
+ * [n_pages, Hkv, page_size, d] with a contiguous last axis and explicit
+ * strides (element counts, order page, head, slot; multiples of 16 bytes, so
+ * that a (n_pages, page_size, Hkv, d) storage is the same call).  Key j of
+ * sequence b lies in slot j % page_size of page block_table[b, j / page_size]
+ * (int32, rows table_ld apart, n_table entries each); entries behind a
+ * sequence's last page are never read.  A page index outside [0, n_pages) is
+ * never followed: its keys count as masked, and nothing is written there.
+ * Lengths, tables and positions are device memory, so a captured graph
+ * replays with new ones.  These entries have no counterpart in the reference,
+ * whose decode loop keeps an om carrier and no cache (om_lower.py:871-1040).
+ */
+
+/*
+ * RMS norm of each head of q and k and their position rotation, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * w          (w NULL: y = x)
+ *   (y[i], y[p]) = (y[i] c - y[p] s, y[p] c + y[i] s),  i < rot / 2
+ * with p = i + rot / 2, or the pairs (2i, 2i + 1) when interleaved; c, s the
+ * i-th entries of row positions[n] of the fp32 tables cos, sin [n_pos, rot /
+ * 2] (rows ld_table apart).  Columns past rot are normed only.  fp32
+ * arithmetic, one rounding.  q: [N, Hq, d], k: [N, Hkv, d], contiguous last
+ * axis; the weights are [d] of `dtype` (F32 or BF16).
+ * d <= 256, rot even and at most d.
+ * slots == NULL: q_out and k_out are [N, H, d], contiguous (v, v_out unused).
+ * slots != NULL: q_out as before; token n's key, and its row of v [N, Hkv,
+ * d], go to slot slots[n] % page_size of page slots[n] / page_size of k_out
+ * and v_out (pages as above); a slot outside the pages (-1 for a padded
+ * token) writes nothing.  The slots of one call are distinct.  A position
+ * outside the tables gives NaN in the rotated columns.  No output may overlap
+ * an input.
+ * strides (host, 12 values): q and k and v (token, head); pages k_out and
+ * v_out (page, head, slot; not read without slots).
+ */
+int32_t catopt_hip_qk_norm_rope(
+    int32_t dtype, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t rot,
+    int32_t interleaved, const void* q, const void* k, const void* v,
+    const void* q_weight, const void* k_weight, float eps, const float* cos,
+    const float* sin, int64_t n_pos, int64_t ld_table,
+    const int64_t* positions, void* q_out, void* k_out, void* v_out,
+    const int64_t* strides, const int64_t* slots, int64_t n_pages,
+    int64_t page_size, void* stream);
+
+/*
+ * Attention of each sequence's new tokens over its cached keys.  q: [N, Hq,
+ * d], sequence b's tokens in rows q_starts[b] ..
+ * q_starts[b + 1] (int32 [B + 1], ascending; rows outside are neither read
+ * nor written); kv_lens[b] (int32) keys are cached, the new tokens' own among
+ * them as the last ones.  Query head h reads key head h / (Hq / Hkv).
+ *   s = scale q k^T;  causal: token i of n sees keys j <= kv_len - n + i
+ *   o = softmax(s) v                    (o: [N, Hq, d])
+ * A row that sees no key is NaN (normalize 1) or 0 (normalize 2).  m_out,
+ * l_out (fp32 [N, Hq], optional): the row's om carrier, max s and sum of
+ * exp(s - m); (-inf, 0) for an empty row.
+ * weights_out (fp32 [B, Hkv, >= n_table * page_size], optional) receives each key's attention weight summed over the tokens and
+ * the query heads of its group, on top of weights_in (the same layout; NULL:
+ * zeros), which is not read for the new tokens' own keys:
+ *   weights_out[b, h, j] = (j < kv_len - n ? weights_in[b, h, j] : 0)
+ *                          + sum_rows exp(s - m) / l,      j < kv_len
+ * Entries from kv_len on are left as they were.  weights_out may be
+ * weights_in.  bf16; d a multiple of 8 up to 128; page_size a multiple of 8;
+ * q, pages and o 16-byte aligned.
+ * strides (host, 14 values): q (token, head); k_pages, v_pages (page, head,
+ * slot); o (token, head); weights_in, weights_out (sequence, head).
+ * Workspace: catopt_hip_paged_attn_workspace_bytes(...) bytes, 16-byte
+ * aligned, any contents (-1: invalid arguments).
+ */
+int64_t catopt_hip_paged_attn_workspace_bytes(int64_t B, int64_t N, int64_t Hq,
+                                              int64_t Hkv, int64_t d,
+                                              int64_t n_table,
+                                              int64_t page_size,
+                                              int32_t weights);
+int32_t catopt_hip_paged_attn_fwd(
+    int32_t dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d,
+    const void* q, const void* k_pages, const void* v_pages, int64_t n_pages,
+    int64_t page_size, const int32_t* block_table, int64_t table_ld,
+    int64_t n_table, const int32_t* kv_lens, const int32_t* q_starts,
+    float scale, int32_t causal, int32_t normalize, void* o, float* m_out,
+    float* l_out, const float* weights_in, float* weights_out,
+    const int64_t* strides, void* workspace, int64_t workspace_bytes,
+    void* stream);
+
+/*
+ * Eviction by accumulated attention weight.  For each sequence b and key head
+ * h, of its n = kv_lens[b] keys min(n, budget) stay: the last `recent` ones
+ * (recent <= budget) and, of the others, those of the largest weights[b, h,
+ * :] (fp32 [B, Hkv, >= n_table * page_size]; the lowest index first among
+ * equals; a NaN ranks above every number).  They keep their order and move to
+ * slots 0, 1, ... of the pages out_table[b, :] of k_out and v_out, whose page
+ * count and size are their own (n_out_table * out_page_size >= budget).
+ * kept (int32 [B, Hkv, budget]) holds their indices, then -1; new_lens
+ * (int32 [B]) the counts; weights_out (fp32 [B, Hkv, >= budget], optional)
+ * their weights.  The row of a key whose page index is invalid moves as zeros.  k_out / v_out may be k_pages / v_pages where no
+ * page of out_table is one of block_table's; weights_out may be weights.
+ * F32 or BF16 rows of a multiple of 16 bytes; 1 <= budget.
+ * strides (host, 16 values): k_pages, v_pages, k_out, v_out (page, head,
+ * slot); weights, weights_out (sequence, head).
+ */
+int32_t catopt_hip_paged_evict(
+    int32_t dtype, int64_t B, int64_t Hkv, int64_t d, const void* k_pages,
+    const void* v_pages, int64_t n_pages, int64_t page_size,
+    const int32_t* block_table, int64_t table_ld, int64_t n_table,
+    const int32_t* kv_lens, const float* weights, int64_t budget,
+    int64_t recent, void* k_out, void* v_out, int64_t n_out_pages,
+    int64_t out_page_size, const int32_t* out_table, int64_t out_table_ld,
+    int64_t n_out_table, int32_t* kept, int32_t* new_lens, float* weights_out,
+    const int64_t* strides, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

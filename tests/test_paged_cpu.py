@@ -1,0 +1,138 @@
+"""The paged cache's operators on the host: what the C ABI refuses before any launch (the operand addresses are never
+read) and the checks of layouts and overlaps that the Python entry points make."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+from catopt_amd import _lib as L
+from catopt_amd import paged as P
+
+FAKE = 4096
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not L.LIB_PATH.exists():
+        from catopt_amd import build
+
+        build.build()
+    return L.load()
+
+
+def _attn(lib, dtype=L.BF16, B=1, N=4, Hq=4, Hkv=2, d=64, q=FAKE, k=FAKE, v=FAKE, n_pages=8, page=16, table=FAKE, ld=4,
+          n_table=4, lens=FAKE, starts=FAKE, scale=1.0, causal=1, norm=1, o=FAKE, w_in=None, w_out=None, strides=None,
+          ws=FAKE, wsb=1 << 40):
+    st = (C.c_int64 * 14)(*(strides or [256, 64, 2048, 1024, 64, 2048, 1024, 64, 256, 64, 128, 64, 128, 64]))
+    return lib.catopt_hip_paged_attn_fwd(dtype, B, N, Hq, Hkv, d, q, k, v, n_pages, page, table, ld, n_table, lens,
+                                         starts, scale, causal, norm, o, None, None, w_in, w_out, st, ws, wsb, None)
+
+
+def test_attention_refuses(lib):
+    # nothing to do is no error, and touches nothing
+    assert _attn(lib, B=0) == L.OK and _attn(lib, N=0) == L.OK
+    for kw in ({"B": -1}, {"N": -1}, {"Hq": 3}, {"Hkv": 0}, {"n_pages": -1}, {"n_table": -1}, {"ld": -1}, {"norm": 0},
+               {"norm": 3}, {"q": None}, {"o": None}, {"k": None}, {"v": None}, {"table": None}, {"lens": None},
+               {"starts": None}, {"q": FAKE + 8}, {"o": FAKE + 2}, {"k": FAKE + 4}, {"v": FAKE + 4}, {"w_in": FAKE},
+               {"strides": [-256] + [64] * 13}, {"strides": [4] + [64] * 13}, {"strides": [64] * 10 + [-1] * 4}):
+        assert _attn(lib, **kw) == L.E_INVAL, kw
+    for kw in ({"dtype": L.F32}, {"d": 60}, {"d": 136}, {"d": 0}, {"page": 12}, {"scale": 0.0}, {"scale": float("inf")},
+               {"scale": float("nan")}, {"N": 1 << 40}, {"B": 1 << 40}, {"n_table": 1 << 30}, {"page": 1 << 40}):
+        assert _attn(lib, **kw) == L.E_UNSUPPORTED, kw
+    need = lib.catopt_hip_paged_attn_workspace_bytes(1, 4, 4, 2, 64, 4, 16, 1)
+    assert need > 0
+    assert _attn(lib, w_out=FAKE, ws=None) == L.E_WORKSPACE
+    assert _attn(lib, w_out=FAKE, wsb=need - 1) == L.E_WORKSPACE
+    assert _attn(lib, w_out=FAKE, ws=FAKE + 8, wsb=need) == L.E_WORKSPACE
+
+
+def test_workspace_query(lib):
+    f = lib.catopt_hip_paged_attn_workspace_bytes
+    ok = [1, 4, 4, 2, 64, 4, 16, 0]
+    assert f(*ok) >= 0 and f(*ok[:-1], 1) > 0
+    for i, x in ((0, -1), (1, -1), (2, 3), (3, 0), (4, 0), (4, 132), (4, 60), (5, -1), (6, 0), (6, 12), (1, 1 << 31),
+                 (2, 1 << 20), (5, 1 << 31), (6, 1 << 31)):
+        bad = list(ok)
+        bad[i] = x
+        assert f(*bad) == -1, bad
+
+
+def _rope(lib, dtype=L.BF16, N=4, Hq=4, Hkv=2, d=64, rot=64, q=FAKE, k=FAKE, v=FAKE, cos=FAKE, sin=FAKE, n_pos=8, ld=32,
+          pos=FAKE, qo=FAKE, ko=FAKE, vo=FAKE, strides=None, slots=None, n_pages=4, page=16):
+    st = (C.c_int64 * 12)(*(strides or [256, 64, 128, 64, 128, 64, 2048, 1024, 64, 2048, 1024, 64]))
+    return lib.catopt_hip_qk_norm_rope(dtype, N, Hq, Hkv, d, rot, 0, q, k, v, None, None, 1e-6, cos, sin, n_pos, ld, pos,
+                                       qo, ko, vo, st, slots, n_pages, page, None)
+
+
+def test_norm_rope_refuses(lib):
+    assert _rope(lib, N=0) == L.OK and _rope(lib, Hq=0, Hkv=0) == L.OK
+    for kw in ({"N": -1}, {"Hq": -1}, {"d": 0}, {"rot": 66}, {"rot": 3}, {"rot": -2}, {"n_pos": -1}, {"pos": None},
+               {"q": None}, {"qo": None}, {"k": None}, {"ko": None}, {"cos": None}, {"sin": None}, {"ld": 31},
+               {"strides": [-1] * 12}, {"slots": FAKE, "v": None}, {"slots": FAKE, "vo": None},
+               {"slots": FAKE, "page": 0}, {"slots": FAKE, "n_pages": -1}):
+        assert _rope(lib, **kw) == L.E_INVAL, kw
+    for kw in ({"dtype": 2}, {"d": 257}, {"N": 1 << 41}, {"N": 1 << 36}, {"Hq": 1 << 21}):
+        assert _rope(lib, **kw) == L.E_UNSUPPORTED, kw
+
+
+def _evict(lib, dtype=L.BF16, B=1, H=2, d=64, k=FAKE, v=FAKE, n_pages=8, page=16, table=FAKE, ld=4, n_table=4, lens=FAKE,
+           w=FAKE, budget=8, recent=2, ko=FAKE, vo=FAKE, n_out=8, page_out=16, to=FAKE, to_ld=4, n_to=4, kept=FAKE,
+           new=FAKE, wo=None, strides=None):
+    st = (C.c_int64 * 16)(*(strides or [2048, 1024, 64] * 4 + [128, 64] * 2))
+    return lib.catopt_hip_paged_evict(dtype, B, H, d, k, v, n_pages, page, table, ld, n_table, lens, w, budget, recent,
+                                      ko, vo, n_out, page_out, to, to_ld, n_to, kept, new, wo, st, None)
+
+
+def test_evict_refuses(lib):
+    assert _evict(lib, B=0) == L.OK
+    for kw in ({"B": -1}, {"H": 0}, {"d": 0}, {"n_pages": -1}, {"page": 0}, {"n_table": -1}, {"ld": -1}, {"n_out": -1},
+               {"page_out": 0}, {"n_to": -1}, {"to_ld": -1}, {"budget": 0}, {"recent": -1}, {"recent": 9},
+               {"budget": 65}, {"lens": None}, {"kept": None}, {"new": None}, {"to": None}, {"table": None}, {"w": None},
+               {"k": None}, {"v": None}, {"ko": None}, {"vo": None}, {"k": FAKE + 8}, {"vo": FAKE + 8},
+               {"strides": [4] * 16}, {"strides": [64] * 12 + [-1] * 4}):
+        assert _evict(lib, **kw) == L.E_INVAL, kw
+    for kw in ({"dtype": 2}, {"d": 4}, {"d": 1 << 14}, {"B": 1 << 21}, {"H": 1 << 21}, {"B": 1 << 11, "H": 1 << 11},
+               {"n_table": 1 << 27}, {"budget": 1 << 31, "n_to": 1 << 28}):
+        assert _evict(lib, **kw) == L.E_UNSUPPORTED, kw
+
+
+def test_host_tensors_are_refused():
+    q = torch.zeros((2, 4, 64), dtype=torch.bfloat16)
+    p = torch.zeros((2, 4, 16, 64), dtype=torch.bfloat16)
+    i = torch.zeros((1,), dtype=torch.int32)
+    with pytest.raises(ValueError, match="ROCm device"):
+        P.paged_attention(q, p, p.clone(), i[None], i, torch.zeros((2,), dtype=torch.int32), 1.0)
+    with pytest.raises(ValueError, match="ROCm device"):
+        P.qk_norm_rope(q, q, torch.ones((4, 32)), torch.ones((4, 32)), torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="ROCm device"):
+        P.paged_evict(p, p.clone(), i[None], i, torch.zeros((1, 4, 16)), i[None], 1)
+    with pytest.raises(TypeError):
+        P.qk_norm_rope_append(q, q, q, None, None, None, p, p, None)
+
+
+def test_layout_checks():
+    t = torch.zeros((4, 6, 8))
+    P._no_overlap_within("t", t)
+    P._no_overlap_within("t", t.transpose(0, 2))
+    P._no_overlap_within("t", t[::2, :, 1:3])
+    P._no_overlap_within("t", t[:1].expand(1, 6, 8))
+    for bad in (t[:1].expand(4, 6, 8), t.as_strided((4, 4), (2, 1)), t[0, 0, :1].expand(3)):
+        with pytest.raises(ValueError):
+            P._no_overlap_within("t", bad)
+    P._apart("t", t[:2], t[2:], None)
+    P._apart("t", t[:0], t)
+    for a, b in ((t, t), (t[:3], t[2:]), (t[0], t[:, 0])):
+        with pytest.raises(ValueError):
+            P._apart("t", a, b)
+    P._in_place_or_apart("t", t, t.view(4, 6, 8))
+    P._in_place_or_apart("t", t[:2], t[2:])
+    with pytest.raises(ValueError):
+        P._in_place_or_apart("t", t[:3], t[1:])
+    u = torch.zeros((3, 4, 12))
+    assert P._heads("t", u[..., :7]).data_ptr() == u.data_ptr()  # rows of 48 bytes: read in place
+    assert P._heads("t", u[..., 1:8]).is_contiguous()  # misaligned: copied
+    with pytest.raises(ValueError):
+        P._pages(t, t)
