@@ -1,120 +1,128 @@
-// Attention of each sequence's new tokens over its paged cache, and the sum of
-// every key's attention weight.
-//
-// One workgroup per (token, query head): its lanes take one key each, the row's
-// softmax statistics meet in LDS, and each thread then adds one column of the
-// values.  The weights follow in a second launch, one thread per key.
-#include "paged.hpp"
+// Paged attention: the choice of kernel, its workspace, and the combination of
+// split keys.
+#include "paged_attn.hpp"
 
 namespace catopt {
 namespace {
 
-struct PagedArgs {
-  const uint16_t *q, *k, *v;
-  uint16_t* o;
-  int64_t q_t, q_h, k_p, k_h, k_s, v_p, v_h, v_s, o_t, o_h, wi_b, wi_h, wo_b, wo_h;
-  const int32_t *table, *lens, *starts;
-  int64_t table_ld, n_pages, N;
-  float *m_out, *l_out, *w_out, *stats;
-  const float* w_in;
-  FastDiv page;
-  int B, Hq, Hkv, G, d, cap, normalize, causal;
-  float scale;
+// One wave per row (token, query head): the carriers of its key ranges, in
+// their order.  R: the rows of the tiles they were made with.
+template <int D, int R>
+__global__ __launch_bounds__(256) void paged_combine(PagedArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.N * a.Hq) return;
+  const int n = (int)(row / a.Hq), hq = (int)(row - (int64_t)n * a.Hq);
+  int b = -1;
+  for (int c0 = 0; c0 < a.B; c0 += 64) {  // the last sequence that starts at or before the token
+    const int i = c0 + lane;
+    const int k = __popcll(__ballot(i < a.B && min(max(a.starts[i < a.B ? i : 0], 0), (int)a.N) <= n));
+    b += k;
+    if (k < 64) break;
+  }
+  if (b < 0) return;
+  PagedTile x{};
+  x.b = b;
+  seq_rows(a.starts, b, a.N, x.row0, x.nq);
+  if (n < x.row0 || n >= x.row0 + x.nq) return;
+  x.len = min(max(a.lens[b], 0), a.cap);
+  x.r0 = ((n - x.row0) * a.G + hq % a.G) / R * R;
+  x.rows = min(R, x.nq * a.G - x.r0);
+  paged_ranges(a, x);
+  if (x.splits == 1) return;  // written by the tile
+  constexpr int V = D / 64;   // numerators per lane
+  const float c = a.scale * kLog2e;
+  const float* ml = a.part + 2 * row * a.splits;
+  const float* num = a.part + ((2 * a.N * a.Hq * a.splits + 3) & ~(int64_t)3) + row * a.splits * D + V * lane;
+  float mx = kNegInf;
+  for (int s = lane; s < x.splits; s += 64) mx = fmaxf(mx, ml[2 * s]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  float lt = 0.f, y[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) y[e] = 0.f;
+  constexpr int U = 8;  // loads ahead of their additions
+  for (int s0 = 0; s0 < x.splits; s0 += U) {
+    float f[U], ls[U], ys[U][V];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int s = min(s0 + i, x.splits - 1);
+      f[i] = s0 + i < x.splits ? move_factor(ml[2 * s], mx, c) : 0.f;
+      ls[i] = s0 + i < x.splits ? ml[2 * s + 1] : 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) ys[i][e] = s0 + i < x.splits ? num[(int64_t)s * D + e] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      lt += ls[i] * f[i];
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] += ys[i][e] * f[i];
+    }
+  }
+  uint16_t* orow = a.o + (int64_t)n * a.o_t + (int64_t)hq * a.o_h;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (V * lane + e < a.d) orow[V * lane + e] = f32_to_bf16(finish(y[e], lt, a.normalize));
+  if (lane == 0) {
+    if (a.m_out) a.m_out[row] = mx * a.scale;
+    if (a.l_out) a.l_out[row] = lt;
+  }
+}
+
+struct Plan {
+  bool few;
+  int splits, min_keys, parts;
+  int64_t tiles, part_floats, stat_floats, score_floats, weight_floats;
+  int64_t bytes() const { return 4 * (part_floats + stat_floats + score_floats + weight_floats); }
 };
 
-constexpr int NT = 256;
-constexpr float kNegInf = -__builtin_inff();
-
-// The sequence of row n, its rows and its keys; -1 behind the last sequence.
-__device__ __forceinline__ int seq_of(const PagedArgs& a, int64_t n, int& row0, int& nq, int& len) {
-  for (int b = 0; b < a.B; ++b) {
-    seq_rows(a.starts, b, a.N, row0, nq);
-    if (row0 <= n && n < row0 + nq) {
-      len = min(max(a.lens[b], 0), a.cap);
-      return b;
+// The kernel and the key ranges by sizes that the host knows.
+//
+// Few rows: 32-row tiles whenever the sequences have 32 rows per key head or
+// fewer on average.
+//
+// Ranges: few-row calls read K and V at the rate of HBM, so their ranges only
+// have to fill the CUs and even out the sequences: at most 64 to a tile and
+// 16384 workgroups in all (those behind a sequence's keys end at once), each
+// of 256 keys at least, or of 128 where the table's reach gives fewer than 512
+// such ranges.  Tiles of 128 rows are split only where they are fewer than the
+// 512 workgroups that the CUs hold, into ranges of 256 keys at least.
+Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t cap, bool weights) {
+  Plan p{};
+  const int64_t G = Hq / Hkv, D = d <= 64 ? 64 : 128;
+  p.few = N * G <= kFewRows * B;
+  p.tiles = paged_tiles(N, G, B, p.few ? kFewRows : kTileRows);
+  const int64_t groups = p.tiles * Hkv;
+  int64_t s = p.few ? 16384 / groups : 512 / groups;
+  p.min_keys = p.few && groups * cap < 512 * 256 ? 128 : 256;
+  const int64_t most = (cap + p.min_keys - 1) / p.min_keys;
+  if (s > 64) s = 64;
+  if (s > most) s = most;
+  p.splits = s < 1 ? 1 : (int)s;
+  const int64_t rows = N * Hq;
+  p.part_floats = p.splits > 1 ? ((2 * rows * p.splits + 3) & ~(int64_t)3) + rows * p.splits * D : 0;
+  if (weights) {
+    p.stat_floats = (2 * rows + 3) & ~(int64_t)3;
+    if (p.few && rows * cap <= (1LL << 28)) {
+      p.score_floats = rows * cap;
+    } else {
+      p.parts = paged_weight_parts(B, Hkv, cap, N, G);
+      p.weight_floats = p.parts > 1 ? p.parts * B * Hkv * cap : 0;
     }
   }
-  return -1;
+  return p;
 }
 
-// q . k of one key, -inf where its page is invalid
-__device__ __forceinline__ float score(const PagedArgs& a, const uint16_t* q, int b, int h, int j) {
-  const uint32_t tp = a.page.div(j);
-  const int64_t page = a.table[b * a.table_ld + tp];
-  if (page < 0 || page >= a.n_pages) return kNegInf;
-  const uint16_t* k = a.k + page * a.k_p + h * a.k_h + (int64_t)(j - tp * a.page.d) * a.k_s;
-  float s = 0.f;
-  for (int e = 0; e < a.d; ++e) s += bf16_to_f32(q[e]) * bf16_to_f32(k[e]);
-  return s * a.scale;
-}
-
-__global__ __launch_bounds__(NT) void paged_attn_rows(PagedArgs a) {
-  __shared__ float red[NT], p[NT];
-  const int64_t n = blockIdx.x / a.Hq;
-  const int hq = blockIdx.x - (int)(n * a.Hq), h = hq / a.G, tid = threadIdx.x;
-  int row0, nq, len;
-  const int b = seq_of(a, n, row0, nq, len);
-  if (b < 0) return;
-  const int64_t lim = a.causal ? (int64_t)len - nq + (n - row0) : (int64_t)len - 1;  // last key seen
-  const int end = lim < 0 ? 0 : (int)(lim + 1 < len ? lim + 1 : len);
-  const uint16_t* q = a.q + n * a.q_t + hq * a.q_h;
-  float m = kNegInf, l = 0.f, acc = 0.f;
-  for (int j0 = 0; j0 < end; j0 += NT) {
-    const int j = j0 + tid;
-    const float s = j < end ? score(a, q, b, h, j) : kNegInf;
-    red[tid] = s;
-    __syncthreads();
-    float mx = m;
-    for (int i = 0; i < NT; ++i) mx = fmaxf(mx, red[i]);
-    const float old = m == kNegInf ? 0.f : __expf(m - mx);
-    p[tid] = s == kNegInf ? 0.f : __expf(s - mx);
-    __syncthreads();
-    m = mx;
-    l *= old;
-    acc *= old;
-    for (int i = 0; i < NT && j0 + i < end; ++i) {
-      const int64_t page = a.table[b * a.table_ld + a.page.div(j0 + i)];
-      l += p[i];
-      if (tid < a.d && page >= 0 && page < a.n_pages) {
-        const uint32_t slot = (j0 + i) - a.page.div(j0 + i) * a.page.d;
-        acc += p[i] * bf16_to_f32(a.v[page * a.v_p + h * a.v_h + slot * a.v_s + tid]);
-      }
-    }
-    __syncthreads();
-  }
-  if (tid < a.d) {
-    const float x = l == 0.f ? (a.normalize == 2 ? 0.f : __builtin_nanf("")) : acc / l;
-    a.o[n * a.o_t + hq * a.o_h + tid] = f32_to_bf16(x);
-  }
-  if (tid == 0) {
-    if (a.m_out) a.m_out[n * a.Hq + hq] = m;
-    if (a.l_out) a.l_out[n * a.Hq + hq] = l;
-    if (a.stats) {
-      a.stats[2 * (n * a.Hq + hq)] = m;
-      a.stats[2 * (n * a.Hq + hq) + 1] = l;
-    }
-  }
-}
-
-__global__ __launch_bounds__(NT) void paged_attn_weights(PagedArgs a, int blocks) {
-  const int bh = blockIdx.x / blocks, b = bh / a.Hkv, h = bh - b * a.Hkv;
-  const int j = (blockIdx.x - bh * blocks) * NT + threadIdx.x;
-  int row0, nq;
-  seq_rows(a.starts, b, a.N, row0, nq);
-  const int len = min(max(a.lens[b], 0), a.cap);
-  if (j >= len) return;
-  float w = 0.f;
-  for (int i = 0; i < nq; ++i) {
-    if (a.causal && j > len - nq + i) continue;
-    for (int g = 0; g < a.G; ++g) {
-      const int64_t n = row0 + i, hq = h * a.G + g;
-      const float m = a.stats[2 * (n * a.Hq + hq)], l = a.stats[2 * (n * a.Hq + hq) + 1];
-      if (l == 0.f) continue;
-      w += __expf(score(a, a.q + n * a.q_t + hq * a.q_h, b, h, j) - m) / l;
-    }
-  }
-  if (a.w_in && j < len - nq) w += a.w_in[b * a.wi_b + h * a.wi_h + j];
-  a.w_out[b * a.wo_b + h * a.wo_h + j] = w;
+template <int R>
+int32_t combine(const PagedArgs& a, int D, hipStream_t s) {
+  const int64_t blocks = (a.N * a.Hq + 3) / 4;
+  if (!grid_fits(blocks, 256)) return CATOPT_E_UNSUPPORTED;
+  if (D == 128)
+    paged_combine<128, R><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(a);
+  else
+    paged_combine<64, R><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(a);
+  CATOPT_LAUNCH_CHECK();
+  return CATOPT_OK;
 }
 
 }  // namespace
@@ -127,8 +135,10 @@ extern "C" int64_t catopt_hip_paged_attn_workspace_bytes(int64_t B, int64_t N, i
   const int64_t lim = 1LL << 30;
   if (B < 0 || N < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || d < 8 || d > 128 || d % 8) return -1;
   if (n_table < 0 || page_size < 8 || page_size % 8) return -1;
-  if (B > lim || N > lim || Hq > 65535 || n_table > lim || page_size > lim || n_table * page_size > lim) return -1;
-  return weights ? 8 * N * Hq : 0;
+  if (B > (1 << 20) || N >= lim || Hq > 65535 || N * Hq >= lim || B * Hkv >= lim) return -1;
+  if (n_table > lim || page_size > lim || n_table * page_size >= lim) return -1;
+  if (B == 0 || N == 0) return 0;
+  return plan_of(B, N, Hq, Hkv, d, n_table * page_size, weights != 0).bytes();
 }
 
 extern "C" int32_t catopt_hip_paged_attn_fwd(
@@ -150,6 +160,8 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   if (!strides_fit(strides, 10, 8) || !strides_fit(strides + 10, 4, 1)) return CATOPT_E_INVAL;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o)) return CATOPT_E_INVAL;
   if (weights_in && !weights_out) return CATOPT_E_INVAL;
+  // the rows of one load lie within 31 bits of its resource's base
+  if (strides[4] > (1 << 26) || strides[7] > (1 << 26)) return CATOPT_E_UNSUPPORTED;
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return CATOPT_E_WORKSPACE;
   PagedArgs a{};
   const int64_t* s = strides;
@@ -159,19 +171,25 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   a.o_t = s[8], a.o_h = s[9], a.wi_b = s[10], a.wi_h = s[11], a.wo_b = s[12], a.wo_h = s[13];
   a.table = block_table, a.lens = kv_lens, a.starts = q_starts, a.table_ld = table_ld, a.n_pages = n_pages, a.N = N;
   a.m_out = m_out, a.l_out = l_out, a.w_in = weights_in, a.w_out = weights_out;
-  a.stats = weights_out ? static_cast<float*>(workspace) : nullptr;
-  a.page = FastDiv::of(page_size);
+  a.page = FastDiv::of(page_size), a.group = FastDiv::of(Hq / Hkv);
   a.B = (int)B, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.d = (int)d, a.cap = (int)(n_table * page_size);
   a.normalize = normalize, a.causal = causal != 0, a.scale = scale;
-  const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (!grid_fits(N * Hq, NT)) return CATOPT_E_UNSUPPORTED;
-  paged_attn_rows<<<dim3((uint32_t)(N * Hq)), dim3(NT), 0, st>>>(a);
-  CATOPT_LAUNCH_CHECK();
-  if (weights_out && a.cap > 0) {
-    const int64_t blocks = (a.cap + NT - 1) / NT;
-    if (!grid_fits(B * Hkv * blocks, NT)) return CATOPT_E_UNSUPPORTED;
-    paged_attn_weights<<<dim3((uint32_t)(B * Hkv * blocks)), dim3(NT), 0, st>>>(a, (int)blocks);
-    CATOPT_LAUNCH_CHECK();
+  const Plan p = plan_of(B, N, Hq, Hkv, d, a.cap, weights_out != nullptr);
+  float* ws = static_cast<float*>(workspace);
+  a.splits = p.splits, a.min_keys = p.min_keys;
+  a.part = ws;
+  ws += p.part_floats;
+  if (weights_out) {  // the weights need every row's statistics
+    if (!a.m_out) a.m_out = ws;
+    if (!a.l_out) a.l_out = ws + N * Hq;
+    ws += p.stat_floats;
+    a.scores = p.score_floats ? ws : nullptr;
+    ws += p.score_floats;
   }
-  return CATOPT_OK;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int D = d <= 64 ? 64 : 128;
+  int32_t r = p.few ? paged_few_launch(a, D, p.tiles, st) : paged_tile_launch(a, D, p.tiles, st);
+  if (r == CATOPT_OK && p.splits > 1) r = p.few ? combine<kFewRows>(a, D, st) : combine<kTileRows>(a, D, st);
+  if (r == CATOPT_OK && weights_out) r = paged_weights_launch(a, D, p.parts, ws, st);
+  return r;
 }

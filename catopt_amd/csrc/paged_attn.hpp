@@ -1,0 +1,215 @@
+// What the paged attention kernels share: a call's arguments, the tiles of
+// query rows, the page reads, the products and the split keys' bookkeeping.
+#pragma once
+#include "attention.hpp"
+#include "paged.hpp"
+
+namespace catopt {
+
+constexpr float kNegInf = -__builtin_inff();
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct PagedArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t* o;
+  int64_t q_t, q_h, k_p, k_h, k_s, v_p, v_h, v_s, o_t, o_h, wi_b, wi_h, wo_b, wo_h;
+  const int32_t *table, *lens, *starts;
+  int64_t table_ld, n_pages, N;
+  float *m_out, *l_out;  // [N, Hq], optional
+  float* part;           // split keys' carriers: [row][split] (m, l), then [row][split][D]; row = n Hq + hq
+  float* scores;         // [row][cap] q . k of the keys that the row's tile sees, -inf where masked; optional
+  const float* w_in;
+  float* w_out;
+  FastDiv page, group;  // by the page size, by the query heads of a key head
+  int B, Hq, Hkv, G, d, cap, normalize, causal;
+  int splits, min_keys;  // key ranges per tile at most, keys of one at least
+  float scale;
+};
+
+// Query rows of one key head are its G query heads of every token, a token's
+// heads next to each other: row r of a sequence is token r / G, head r % G.
+// A tile is R such rows; the tiles of sequence b begin at tile
+// floor(row0 G / R) + b, which leaves each sequence as many as it needs
+// whatever the lengths are, so the grid depends on N and B alone.
+inline int64_t paged_tiles(int64_t N, int64_t G, int64_t B, int64_t R) { return N * G / R + B; }
+
+struct PagedTile {
+  int b, row0, nq, len, r0, rows;  // sequence, its tokens and keys; the tile's first row and its rows (0: no such tile)
+  int off;                         // token i sees keys <= off + i
+  int kend;                        // keys that some row of the tile sees
+  int splits, keys;                // its key ranges and the keys of each
+};
+
+template <int R>
+__device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, int t) {
+  const int lane = threadIdx.x & 63;
+  int b = -1;
+  for (int c = 0; c < a.B; c += 64) {  // the last sequence whose first tile is not behind t
+    const int i = c + lane;
+    bool le = false;
+    if (i < a.B) {
+      const int64_t s = min(max(a.starts[i], 0), (int)a.N);
+      le = s * a.G / R + i <= t;
+    }
+    const int n = __popcll(__ballot(le));
+    b += n;
+    if (n < 64) break;
+  }
+  PagedTile x{};
+  x.b = __builtin_amdgcn_readfirstlane(b);
+  if (x.b < 0) return x;
+  seq_rows(a.starts, x.b, a.N, x.row0, x.nq);
+  x.len = min(max(a.lens[x.b], 0), a.cap);
+  const int64_t first = (int64_t)x.row0 * a.G / R + x.b, rows = (int64_t)x.nq * a.G, r0 = (t - first) * R;
+  x.r0 = (int)r0;
+  x.rows = r0 >= 0 && r0 < rows ? (int)min((int64_t)R, rows - r0) : 0;  // r0 < 0: starts that do not ascend
+  return x;
+}
+
+// The keys a tile of rows [r0, r0 + rows) sees, and how they are split: in
+// ranges of at least min_keys and a multiple of 128 (whole stages of every
+// kernel).
+__device__ __forceinline__ void paged_ranges(const PagedArgs& a, PagedTile& x) {
+  x.off = a.causal ? x.len - x.nq : 0x3fffffff;
+  const int64_t last = (int64_t)x.off + (x.r0 + x.rows - 1) / a.G;
+  x.kend = last < 0 ? 0 : (int)min((int64_t)x.len, last + 1);
+  int keys = (x.kend + a.splits - 1) / a.splits;
+  keys = (max(keys, a.min_keys) + 127) & ~127;
+  x.keys = keys;
+  x.splits = max((x.kend + keys - 1) / keys, 1);
+}
+
+// exp2((from - to) c), 0 for an empty `from`.
+__device__ __forceinline__ float move_factor(float from, float to, float c) {
+  return from == kNegInf ? 0.f : __builtin_amdgcn_exp2f((from - to) * c);
+}
+
+// A row of the result: numerator piece x of a row with sum l.
+__device__ __forceinline__ float finish(float x, float l, int normalize) {
+  if (l == 0.f) return normalize == 2 ? 0.f : __builtin_nanf("");
+  return x * (1.0f / l);
+}
+
+// Page ids and first slots of the 8-key groups from `key0` on: lane i holds
+// group i (pages hold a multiple of 8 keys, so a group lies in one).  `bad`
+// has a bit for each group of real keys whose page is invalid; groups behind
+// the keys, like invalid ones, hold page -1.
+struct PageIds {
+  int page, slot;
+};
+__device__ __forceinline__ PageIds page_ids(const PagedArgs& a, const int32_t* table, int key0, int len) {
+  const int key = key0 + 8 * (threadIdx.x & 7);
+  PageIds r{-1, 0};
+  if (key < len) {
+    const uint32_t tp = a.page.div(key);
+    r.page = table[tp];
+    r.slot = key - (int)(tp * a.page.d);
+  }
+  return r;
+}
+__device__ __forceinline__ uint32_t bad_groups(const PagedArgs& a, const PageIds& r, int key0, int len) {
+  const bool bad = key0 + 8 * (int)(threadIdx.x & 7) < len && (r.page < 0 || r.page >= a.n_pages);
+  return (uint32_t)__ballot(bad) & 0xffu;
+}
+
+// Resource over the `rows` rows from slot `slot` of page `page` (head offset
+// in `base`): rows past them, and every row of an invalid page, read as zeros.
+__device__ __forceinline__ u32x4 page_rsrc(const uint16_t* base, int page, int slot, int64_t s_page, int64_t s_slot,
+                                           int rows, int d, int64_t n_pages) {
+  const bool ok = rows > 0 && page >= 0 && page < n_pages;
+  const uint16_t* p = ok ? base + page * s_page + slot * s_slot : base;
+  return make_rsrc(p, ok ? (uint32_t)(((rows - 1) * s_slot + d) * 2) : 0u);
+}
+
+// V^T fragments of 32 keys from an LDS tile: vf[2 db + u], keys 16 u + {4 (G /
+// 2) + j / 4, 8 further} and d block 32 db + 16 (G % 2) + 4 (j % 4) for lane
+// group G = lane / 16, j = lane % 16 (the order of the score accumulator).
+template <int D>
+__device__ __forceinline__ void read_v(const char* Vs, int key0, bf16x8* vf) {
+  const int lane = threadIdx.x & 63, G = lane >> 4, jj = lane & 15;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = key0 + 16 * u + 4 * (G >> 1) + (jj >> 2);
+      const int d = 32 * db + 16 * (G & 1) + 4 * (jj & 3);
+      const s16x4 lo = ds_read_tr(Vs, vtile_off<D>(key, d >> 3) + (d & 7) * 2);
+      const s16x4 hi = ds_read_tr(Vs, vtile_off<D>(key + 8, d >> 3) + (d & 7) * 2);
+      const u32x2 lw = __builtin_bit_cast(u32x2, lo), hw = __builtin_bit_cast(u32x2, hi);
+      vf[2 * db + u] = __builtin_bit_cast(bf16x8, u32x4{lw[0], lw[1], hw[0], hw[1]});
+    }
+  }
+}
+
+// Both bf16 values of a word at once, by arithmetic in 16-bit halves whose top
+// bits catch the carry (one comparison per value would cost a lane mask each).
+// 0x8000 in the halves that are not zero / infinite or NaN / NaN:
+__device__ __forceinline__ uint32_t halves_set(uint32_t w) {
+  return (((w & 0x7fff7fffu) + 0x7fff7fffu) | w) & 0x80008000u;
+}
+__device__ __forceinline__ uint32_t halves_odd(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t halves_nan(uint32_t w) { return ((w & 0x7fff7fffu) + 0x007f007fu) & 0x80008000u; }
+
+// Whether some value of the fragments is infinite or NaN (exponent all ones).
+template <int D>
+__device__ __forceinline__ bool odd_values(const bf16x8* vf) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    const u32x4 w = __builtin_bit_cast(u32x4, vf[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) any |= halves_odd(w[e]);
+  }
+  return __ballot(any != 0) != 0;
+}
+
+// For a product O^T += V^T P^T in which a row may not see a key whose value is
+// infinite or NaN: 0 times that value is NaN, so the fragments are left with
+// finite values only, and products of ones count, for each row and column, the
+// seen keys (weight not 0) that hold +inf, -inf or NaN, and add those.
+template <int D>
+__device__ __forceinline__ void take_odd_values(bf16x8* vf, const bf16x8* p, f32x16* acc) {
+#pragma unroll 1
+  for (int kind = 0; kind < 3; ++kind) {
+    const float add = kind == 0 ? __builtin_inff() : kind == 1 ? kNegInf : __builtin_nanf("");
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+      f32x16 cnt;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) cnt[r] = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        u32x4 v = __builtin_bit_cast(u32x4, vf[2 * db + u]), w = __builtin_bit_cast(u32x4, p[u]), x, y;
+        // opaque: nothing of this is worked out for all blocks before the loop,
+        // which would cost the attention loop its registers
+        asm volatile("" : "+v"(v), "+v"(w));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t inf = halves_set(v[e] ^ (kind == 0 ? 0x7f807f80u : 0xff80ff80u)) ^ 0x80008000u;
+          x[e] = ((kind < 2 ? inf : halves_nan(v[e])) >> 15) * 0x3f80u;  // 1.0
+          y[e] = (halves_set(w[e]) >> 15) * 0x3f80u;
+        }
+        cnt = mfma32x32x16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), cnt);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[db][r] += cnt[r] > 0.f ? add : 0.f;
+      __builtin_amdgcn_sched_barrier(0);  // one block's counts at a time: this path must not cost the others registers
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) {
+    u32x4 v = __builtin_bit_cast(u32x4, vf[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] &= ~((halves_odd(v[e]) >> 15) * 0xffffu);
+    vf[i] = __builtin_bit_cast(bf16x8, v);
+  }
+}
+
+// Host side of each kernel.
+constexpr int kFewRows = 32, kTileRows = 128;
+int32_t paged_few_launch(const PagedArgs& a, int D, int64_t tiles, hipStream_t s);    // tiles of kFewRows
+int32_t paged_tile_launch(const PagedArgs& a, int D, int64_t tiles, hipStream_t s);   // tiles of kTileRows
+int paged_weight_parts(int64_t B, int64_t Hkv, int64_t cap, int64_t N, int64_t G);
+int32_t paged_weights_launch(const PagedArgs& a, int D, int parts, float* part, hipStream_t s);
+
+}  // namespace catopt

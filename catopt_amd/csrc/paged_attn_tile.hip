@@ -1,0 +1,308 @@
+// Paged attention with many query rows per key head (prompts and chunks): the
+// tile loop of the contiguous 32-query kernel over cache pages.
+//
+// One workgroup = 4 waves = 128 rows of one key head, 32 per wave, a token's G
+// query heads in neighbouring rows, so that they share every K and V tile.
+// S^T = K Q^T and O^T += V^T P^T on the 32x32x16 MFMA: the accumulator's
+// column is the query row, and the softmax statistics are lane-local.  Tiles
+// of 64 keys are double buffered in LDS; each 1 KB of one comes by a direct
+// global->LDS load whose 4 or 8 rows lie in one page, through a buffer
+// resource of its own that ends behind the last key.
+//
+// A tile runs as two key halves of 32, each its own online-softmax step, so
+// that the exponentials of one half issue between the MFMAs of the other.  The
+// reference max moves only when a half exceeds it by kLazy (log2 units);
+// until then p <= 2^kLazy, exact in range for fp32 and bf16.
+//
+// The grid takes the key heads of a tile next to each other: consecutive
+// workgroups go to the 8 XCDs in turn, so with a multiple of 8 key heads each
+// XCD's L2 serves its own heads.  Tiles go from the last one down, which
+// starts the longest of a causal sequence first.
+#include <type_traits>
+
+#include "paged_attn.hpp"
+
+namespace catopt {
+namespace {
+
+constexpr int NT = 256;  // 4 waves
+constexpr int KVB = 64;  // keys per tile
+constexpr float kLazy = 8.0f;
+
+template <int D>
+struct TileLds {
+  static constexpr int TILE = KVB * AttnRow<D>::BYTES, STAGE = 2 * TILE, BYTES = 2 * STAGE;
+  static constexpr int LOADS = TILE / 4096;  // 1 KB loads of K (and of V) per wave
+  static constexpr int ROWS = 1024 / AttnRow<D>::BYTES;  // rows of one
+};
+
+// An empty asm use: the value is computed before this point.
+__device__ __forceinline__ void pin(const bf16x8& x) { asm volatile("" ::"v"(__builtin_bit_cast(u32x4, x))); }
+__device__ __forceinline__ void pin(float x) { asm volatile("" ::"v"(x)); }
+
+template <int D>
+__global__ __launch_bounds__(NT, 2) void paged_tile_kernel(PagedArgs a, int tiles) {
+  using L = TileLds<D>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = blockIdx.x % a.Hkv, ts = blockIdx.x / a.Hkv, tr = ts / a.splits, split = ts - tr * a.splits;
+  PagedTile x = paged_tile<kTileRows>(a, tiles - 1 - tr);
+  if (x.rows == 0) return;
+  paged_ranges(a, x);
+  if (split >= x.splits) return;
+  const float c = a.scale * kLog2e;
+
+  const int row = x.r0 + 32 * wave + l32, tok = (int)a.group.div(row), hq = h * a.G + row - tok * a.G;
+  const bool live = 32 * wave + l32 < x.rows;
+  const uint16_t* q = a.q + (int64_t)(x.row0 + tok) * a.q_t + (int64_t)hq * a.q_h;
+  bf16x8 qf[D / 16];
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) {
+    u32x4 w = u32x4{0, 0, 0, 0};
+    if (live && 16 * j + 8 * g < a.d) w = *reinterpret_cast<const u32x4*>(q + 16 * j + 8 * g);
+    qf[j] = __builtin_bit_cast(bf16x8, w);
+  }
+  const int lim = x.off + tok;  // last key this row sees
+  // of the wave's rows the first sees the fewest keys, the last the most
+  const int w0 = x.r0 + 32 * wave, w1 = min(w0 + 31, x.r0 + x.rows - 1);
+  const int lim0 = __builtin_amdgcn_readfirstlane(x.off + (int)a.group.div(w0));
+  const int lim1 = __builtin_amdgcn_readfirstlane(x.off + (int)a.group.div(max(w1, 0)));
+  const bool wave_live = 32 * wave < x.rows;
+
+  f32x16 acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+  float m_run = kNegInf, m_true = kNegInf, l_run = 0.f;  // maxima in units of q . k
+
+  const int k_end = min(x.kend, (split + 1) * x.keys);
+  const int t0 = split * x.keys / KVB, t1 = (k_end + KVB - 1) / KVB;
+  const int wave_end = wave_live ? min(k_end, lim1 + 1) : 0;
+  const int32_t* table = a.table + (int64_t)x.b * a.table_ld;
+  const uint16_t *kb = a.k + (int64_t)h * a.k_h, *vb = a.v + (int64_t)h * a.v_h;
+  // a lane's 16 bytes of a load: row `sub` of the wave's rows of it.  Load i
+  // holds tile rows (4 i + wave) ROWS + sub, whose swizzles do not depend on i.
+  const int sub = lane / AttnRow<D>::CH, cp = lane % AttnRow<D>::CH, trow = wave * L::ROWS + sub;
+  const int kc = cp ^ (trow & (AttnRow<D>::CH - 1) & 15), vc = cp ^ vswz<D>(trow);
+  const uint32_t koff = kc * 8 < a.d ? (uint32_t)(sub * (int)a.k_s + kc * 8) * 2u : 0x7ffffff0u;
+  const uint32_t voff = vc * 8 < a.d ? (uint32_t)(sub * (int)a.v_s + vc * 8) * 2u : 0x7ffffff0u;
+  const uint32_t lds0 = lds_u32(lds) + wave * 1024;
+  auto issue = [&](int t, int stage, const PageIds& ids) {
+#pragma unroll
+    for (int i = 0; i < L::LOADS; ++i) {
+      const int r0 = (4 * i + wave) * L::ROWS;  // of the tile
+      const int page = __builtin_amdgcn_readlane(ids.page, r0 >> 3);
+      const int slot = __builtin_amdgcn_readlane(ids.slot, r0 >> 3) + (r0 & 7);
+      const int rows = min(x.len - (t * KVB + r0), L::ROWS);
+      const uint32_t to = lds0 + stage * L::STAGE + i * 4096;
+      dma_buf(page_rsrc(kb, page, slot, a.k_p, a.k_s, rows, a.d, a.n_pages), koff, to);
+      dma_buf(page_rsrc(vb, page, slot, a.v_p, a.v_s, rows, a.d, a.n_pages), voff, to + L::TILE);
+    }
+  };
+
+  PageIds next{-1, 0};  // of the tile after the one in flight
+  uint32_t bad = 0, bad_next = 0;
+  if (t0 < t1) {
+    const PageIds ids = page_ids(a, table, t0 * KVB, x.len);
+    bad = bad_groups(a, ids, t0 * KVB, x.len);
+    issue(t0, 0, ids);
+    next = page_ids(a, table, (t0 + 1) * KVB, x.len);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+
+  auto tile = [&](int t, auto stage_tag) {
+    constexpr int cur = decltype(stage_tag)::value;
+    if (t + 1 < t1) {
+      bad_next = bad_groups(a, next, (t + 1) * KVB, x.len);
+      issue(t + 1, cur ^ 1, next);
+      next = page_ids(a, table, (t + 2) * KVB, x.len);
+    }
+    const char* Ks = lds + cur * L::STAGE;
+    const char* Vs = Ks + L::TILE;
+    const int kv0 = t * KVB;
+    if (kv0 < wave_end) {
+      //   QK(0) | max(0) | QK(1) + exp(0) | max(1) | PV(0) + exp(1) | PV(1)
+      const bool masked = kv0 + KVB > x.len || kv0 + KVB - 1 > lim0 || bad;
+      bf16x8 kf[2][D / 16], vf[2][D / 16];
+      auto read_k = [&](int kb2) {
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+          kf[kb2][j] = *reinterpret_cast<const bf16x8*>(Ks + tile_off<D>(32 * kb2 + l32, 2 * j + g));
+      };
+      auto qk = [&](int kb2, f32x16& s) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) s = mfma32x32x16(kf[kb2][j], qf[j], s);
+      };
+      auto pv = [&](int kb2, const bf16x8* p) {
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) acc[db] = mfma32x32x16(vf[kb2][2 * db + u], p[u], acc[db]);
+      };
+      auto apply_mask = [&](int kb2, f32x16& s) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int in = 32 * kb2 + acc_row(r, g), key = kv0 + in;
+          const bool keep = key < x.len && key <= lim && !((bad >> (in >> 3)) & 1);
+          s[r] = keep ? s[r] : kNegInf;
+        }
+      };
+      // row max of a half over both lane halves, the true max, and the lazy
+      // move of the reference max; returns the factor for O^T (1: no move)
+      auto half_max = [&](const f32x16& s) -> float {
+        float mt = kNegInf;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[r]);
+        {
+          const auto sw = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mt),
+                                                           __builtin_bit_cast(uint32_t, mt), false, false);
+          mt = fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]));
+        }
+        m_true = fmaxf(m_true, mt);
+        float alpha = 1.f;
+        if (__builtin_amdgcn_ballot_w64((mt - m_run) * c > kLazy) != 0) {
+          const float m_new = fmaxf(m_run, mt);
+          alpha = move_factor(m_run, m_new, c);
+          l_run *= alpha;
+          m_run = m_new;
+        }
+        return alpha;
+      };
+      auto rescale = [&](float alpha) {
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
+      };
+      auto half_exp = [&](const f32x16& s, bf16x8* p) {
+        const float mc = (m_run == kNegInf ? 0.f : m_run) * c;
+        float lsum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -mc));
+          lsum += e;
+          p[r >> 3][r & 7] = static_cast<__bf16>(e);
+        }
+        l_run += lsum;
+      };
+
+      f32x16 s0, s1;
+      bf16x8 p0[2], p1[2];
+      read_k(0);
+      read_k(1);
+      qk(0, s0);
+      if (masked) apply_mask(0, s0);
+      const float a0 = half_max(s0);
+      if (__builtin_amdgcn_ballot_w64(a0 != 1.f) != 0) rescale(a0);
+      __builtin_amdgcn_sched_barrier(0);
+      qk(1, s1);
+      half_exp(s0, p0);
+      read_v<D>(Vs, 0, vf[0]);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // VALU
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // DS read
+      }
+      pin(p0[0]);
+      pin(p0[1]);
+      pin(l_run);
+      __builtin_amdgcn_sched_barrier(0);
+      if (masked) apply_mask(1, s1);
+      const float a1 = half_max(s1);
+      if (masked && odd_values<D>(vf[0])) take_odd_values<D>(vf[0], p0, acc);
+      __builtin_amdgcn_sched_barrier(0);
+      pv(0, p0);
+      half_exp(s1, p1);
+      read_v<D>(Vs, 32, vf[1]);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // VALU
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // DS read
+      }
+      pin(p1[0]);
+      pin(p1[1]);
+      pin(l_run);
+      __builtin_amdgcn_sched_barrier(0);
+      if (__builtin_amdgcn_ballot_w64(a1 != 1.f) != 0) rescale(a1);
+      if (masked && odd_values<D>(vf[1])) take_odd_values<D>(vf[1], p1, acc);
+      pv(1, p1);
+    }
+    bad = bad_next;
+    if (t + 1 < t1) {
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    }
+  };
+  for (int t = t0; t < t1; t += 2) {
+    tile(t, std::integral_constant<int, 0>{});
+    if (t + 1 < t1) tile(t + 1, std::integral_constant<int, 1>{});
+  }
+
+  // ---- epilogue: back to the true max, then the row or its range's carrier
+  const float fix = m_true != kNegInf && m_run != kNegInf ? __builtin_amdgcn_exp2f((m_run - m_true) * c) : 1.f;
+  const float l_sum = l_run + __shfl_xor(l_run, 32, 64);
+  if (!live) return;
+  const int64_t i = (int64_t)(x.row0 + tok) * a.Hq + hq;
+  if (x.splits > 1) {
+    const int64_t rows = a.N * a.Hq, at = i * a.splits + split;
+    if (g == 0) {
+      a.part[2 * at] = m_true;
+      a.part[2 * at + 1] = l_sum * fix;
+    }
+    float* num = a.part + ((2 * rows * a.splits + 3) & ~(int64_t)3) + at * D;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg)
+        *reinterpret_cast<f32x4*>(num + 32 * db + 8 * rg + 4 * g) =
+            f32x4{acc[db][4 * rg] * fix, acc[db][4 * rg + 1] * fix, acc[db][4 * rg + 2] * fix, acc[db][4 * rg + 3] * fix};
+    return;
+  }
+  uint16_t* orow = a.o + (int64_t)(x.row0 + tok) * a.o_t + (int64_t)hq * a.o_h;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) {
+#pragma unroll
+    for (int rg = 0; rg < 4; ++rg) {
+      const int d = 32 * db + 8 * rg + 4 * g;
+      if (d < a.d)
+        *reinterpret_cast<u32x2*>(orow + d) =
+            u32x2{pack_bf16x2(finish(acc[db][4 * rg], l_sum, a.normalize), finish(acc[db][4 * rg + 1], l_sum, a.normalize)),
+                  pack_bf16x2(finish(acc[db][4 * rg + 2], l_sum, a.normalize), finish(acc[db][4 * rg + 3], l_sum, a.normalize))};
+    }
+  }
+  if (g == 0) {
+    if (a.m_out) a.m_out[i] = m_true * a.scale;
+    if (a.l_out) a.l_out[i] = l_sum * fix;
+  }
+}
+
+template <int D>
+int32_t launch(const PagedArgs& a, int64_t tiles, hipStream_t s) {
+  static bool attr_done = false;  // idempotent; benign race (same value written)
+  if (!attr_done) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_tile_kernel<D>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<D>::BYTES);
+    if (e != hipSuccess) return set_hip_error(e);
+    attr_done = true;
+  }
+  const int64_t blocks = tiles * a.splits * a.Hkv;
+  if (!grid_fits(blocks, NT)) return CATOPT_E_UNSUPPORTED;
+  paged_tile_kernel<D><<<dim3((uint32_t)blocks), dim3(NT), TileLds<D>::BYTES, s>>>(a, (int)tiles);
+  CATOPT_LAUNCH_CHECK();
+  return CATOPT_OK;
+}
+
+}  // namespace
+
+int32_t paged_tile_launch(const PagedArgs& a, int D, int64_t tiles, hipStream_t s) {
+  return D == 128 ? launch<128>(a, tiles, s) : launch<64>(a, tiles, s);
+}
+
+}  // namespace catopt

@@ -1,0 +1,242 @@
+// Every cached key's attention weight, summed over the new tokens and the
+// query heads of its key head:
+//   w[j] = sum_rows exp(s_rj - m_r) / l_r = sum_rows exp2(q_r . k_j c - o_r),
+//   c = scale log2 e,  o_r = m_r log2 e + log2 l_r  (m, l: the finished rows')
+// on top of the weight so far (nothing for the new tokens' own keys).
+//
+// Few rows: the attention kernel has stored its products (4 bytes a row and
+// key, against 4 d bytes for K and V), and one thread adds four keys' rows.
+// Many rows: the products are formed again, half of the attention's.  A
+// workgroup keeps 128 keys in registers, 32 per wave, and streams the rows by
+// 32 through LDS; the score accumulator's columns are rows, so each lane adds
+// its rows for 16 keys and the lanes meet once at the end.  The exponentials
+// bound it.  Where the keys leave CUs idle the rows are split over workgroups
+// and the parts added in their order by another launch.
+#include "paged_attn.hpp"
+
+namespace catopt {
+namespace {
+
+constexpr int NT = 256;
+
+// o_r of a row, +inf where it sees nothing (its terms are then 0)
+__device__ __forceinline__ float row_offset(const PagedArgs& a, int64_t i) {
+  const float m = a.m_out[i], l = a.l_out[i];
+  return l == 0.f ? __builtin_inff() : m * kLog2e + __builtin_amdgcn_logf(l);
+}
+
+__device__ __forceinline__ void add_weight(const PagedArgs& a, int b, int h, int key, int old, float w) {
+  if (a.w_in && key < old) w += a.w_in[b * a.wi_b + h * a.wi_h + key];
+  a.w_out[b * a.wo_b + h * a.wo_h + key] = w;
+}
+
+__global__ __launch_bounds__(NT) void weights_from_scores(PagedArgs a, int blocks) {
+  const int bh = blockIdx.x / blocks, b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const int key = ((blockIdx.x - bh * blocks) * NT + threadIdx.x) * 4;
+  int row0, nq;
+  seq_rows(a.starts, b, a.N, row0, nq);
+  const int len = min(max(a.lens[b], 0), a.cap);
+  if (key >= len) return;
+  const int old = len - nq;
+  const float c = a.scale * kLog2e;
+  f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int tok = 0; tok < nq; ++tok) {
+    const int seen = a.causal ? old + tok : len;  // last key
+    if (key > seen) continue;
+    for (int g = 0; g < a.G; ++g) {
+      const int64_t i = (int64_t)(row0 + tok) * a.Hq + h * a.G + g;
+      const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + i * a.cap + key);
+      const float o = row_offset(a, i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -o));
+        w[e] += key + e <= seen ? x : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (key + e < len) add_weight(a, b, h, key + e, old, w[e]);
+}
+
+constexpr int kKeys = 128;  // of a workgroup
+
+template <int D>
+__global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks, int parts, float* part) {
+  __shared__ __attribute__((aligned(16))) char lds[2][32 * D * 2];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int u = blockIdx.x;
+  const int h = u % a.Hkv;
+  u /= a.Hkv;
+  const int pt = u % parts;
+  u /= parts;
+  const int blk = u % blocks, b = u / blocks;
+  int row0, nq;
+  seq_rows(a.starts, b, a.N, row0, nq);
+  const int len = min(max(a.lens[b], 0), a.cap);
+  if (blk * kKeys >= len) return;
+  const int old = len - nq, off = a.causal ? old : 0x3fffffff;
+  const int key0 = blk * kKeys + 32 * wave, key = key0 + l32;
+  const float c = a.scale * kLog2e;
+
+  bf16x8 kf[D / 16];
+  bool valid = key < len;
+  {
+    const uint32_t tp = a.page.div(valid ? key : 0);
+    const int64_t page = valid ? a.table[(int64_t)b * a.table_ld + tp] : -1;
+    valid = page >= 0 && page < a.n_pages;
+    const uint16_t* k = a.k + (valid ? page * a.k_p + h * a.k_h + (int64_t)(key - tp * a.page.d) * a.k_s : 0);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      u32x4 w = u32x4{0, 0, 0, 0};
+      if (valid && 16 * j + 8 * g < a.d) w = *reinterpret_cast<const u32x4*>(k + 16 * j + 8 * g);
+      kf[j] = __builtin_bit_cast(bf16x8, w);
+    }
+  }
+
+  // tiles of 32 rows from the first that sees the block's first key; this part's share
+  const int rows = nq * a.G, tok0 = max(blk * kKeys - off, 0);
+  const int ta = (int)min((int64_t)tok0 * a.G, (int64_t)rows) / 32, tb = (rows + 31) / 32;
+  const int t0 = ta + (int)((int64_t)(tb - ta) * pt / parts), t1 = ta + (int)((int64_t)(tb - ta) * (pt + 1) / parts);
+
+  constexpr int CH = AttnRow<D>::CH, LD = 32 * CH / NT;  // 16-byte pieces of a tile per thread
+  static_assert(LD >= 1 && LD <= 2, "a tile is one or two pieces per thread");
+  u32x4 qr[2];
+  float o_next = __builtin_inff();
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const int piece = i * NT + tid, r = 32 * t + piece / CH, ch = piece % CH;
+      qr[i] = u32x4{0, 0, 0, 0};
+      if (r < rows && ch * 8 < a.d) {
+        const int tok = (int)a.group.div(r);
+        qr[i] = *reinterpret_cast<const u32x4*>(a.q + (int64_t)(row0 + tok) * a.q_t +
+                                                (int64_t)(h * a.G + r - tok * a.G) * a.q_h + ch * 8);
+      }
+    }
+    const int r = 32 * t + l32;
+    o_next = __builtin_inff();
+    if (r < rows) {
+      const int tok = (int)a.group.div(r);
+      o_next = row_offset(a, (int64_t)(row0 + tok) * a.Hq + h * a.G + r - tok * a.G);
+    }
+  };
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const int piece = i * NT + tid;
+      *reinterpret_cast<u32x4*>(lds[buf] + tile_off<D>(piece / CH, piece % CH)) = qr[i];
+    }
+  };
+
+  float w[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) w[r] = 0.f;
+  if (t0 < t1) {
+    fetch(t0);
+    stage(0);
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    const float o = o_next;
+    __syncthreads();  // the tile is staged, and the other buffer is free
+    if (t + 1 < t1) fetch(t + 1);
+    const int first = off + (int)a.group.div(32 * t);                          // last key of the tile's first row
+    const int last = off + (int)a.group.div(min(32 * t + 31, rows - 1));       // and of its last row
+    if (key0 <= last && key0 < len) {
+      f32x16 s;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+        s = mfma32x32x16(kf[j], *reinterpret_cast<const bf16x8*>(lds[buf] + tile_off<D>(l32, 2 * j + g)), s);
+      if (key0 + 31 > first) {
+        const int lim = off + (int)a.group.div(32 * t + l32);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -o));
+          w[r] += key0 + acc_row(r, g) <= lim ? x : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -o));
+      }
+    }
+    if (t + 1 < t1) stage(buf ^ 1);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) w[r] += __shfl_xor(w[r], x, 64);
+  }
+  // lane r of each half takes the key of accumulator register r, and whether
+  // that key's page is one
+  const uint64_t ok = __ballot(valid);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    if (l32 == r) {
+      const int in = acc_row(r, g), j = key0 + in;
+      if (j < len) {
+        const float x = (ok >> in) & 1 ? w[r] : 0.f;
+        if (parts > 1)
+          part[((int64_t)(pt * a.B + b) * a.Hkv + h) * a.cap + j] = x;
+        else
+          add_weight(a, b, h, j, old, x);
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(NT) void weights_add_parts(PagedArgs a, int blocks, int parts, const float* part) {
+  const int bh = blockIdx.x / blocks, b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const int key = (blockIdx.x - bh * blocks) * NT + threadIdx.x;
+  int row0, nq;
+  seq_rows(a.starts, b, a.N, row0, nq);
+  const int len = min(max(a.lens[b], 0), a.cap);
+  if (key >= len) return;
+  float w = 0.f;
+  for (int p = 0; p < parts; ++p) w += part[((int64_t)p * a.B * a.Hkv + bh) * a.cap + key];
+  add_weight(a, b, h, key, len - nq, w);
+}
+
+}  // namespace
+
+// Parts of the rows: as many as give four workgroups to a CU, were every
+// sequence as long as its table.
+int paged_weight_parts(int64_t B, int64_t Hkv, int64_t cap, int64_t N, int64_t G) {
+  const int64_t groups = B * Hkv * ((cap + kKeys - 1) / kKeys);
+  int64_t n = groups > 0 ? 1024 / groups : 1;
+  const int64_t tiles = N * G / 32;
+  if (n > tiles / 8) n = tiles / 8;  // of the call: a part has work for a few tiles at least
+  return n < 1 ? 1 : n > 16 ? 16 : (int)n;
+}
+
+int32_t paged_weights_launch(const PagedArgs& a, int D, int parts, float* part, hipStream_t s) {
+  if (a.cap == 0) return CATOPT_OK;
+  const int64_t heads = (int64_t)a.B * a.Hkv;
+  if (a.scores) {
+    const int64_t blocks = (a.cap + 4 * NT - 1) / (4 * NT);
+    if (!grid_fits(heads * blocks, NT)) return CATOPT_E_UNSUPPORTED;
+    weights_from_scores<<<dim3((uint32_t)(heads * blocks)), dim3(NT), 0, s>>>(a, (int)blocks);
+    CATOPT_LAUNCH_CHECK();
+    return CATOPT_OK;
+  }
+  const int64_t blocks = (a.cap + kKeys - 1) / kKeys;
+  if (!grid_fits(heads * blocks * parts, NT)) return CATOPT_E_UNSUPPORTED;
+  const dim3 grid((uint32_t)(heads * blocks * parts));
+  if (D == 128)
+    weights_of_rows<128><<<grid, dim3(NT), 0, s>>>(a, (int)blocks, parts, part);
+  else
+    weights_of_rows<64><<<grid, dim3(NT), 0, s>>>(a, (int)blocks, parts, part);
+  CATOPT_LAUNCH_CHECK();
+  if (parts > 1) {
+    const int64_t n = (a.cap + NT - 1) / NT;
+    if (!grid_fits(heads * n, NT)) return CATOPT_E_UNSUPPORTED;
+    weights_add_parts<<<dim3((uint32_t)(heads * n)), dim3(NT), 0, s>>>(a, (int)n, parts, part);
+    CATOPT_LAUNCH_CHECK();
+  }
+  return CATOPT_OK;
+}
+
+}  // namespace catopt
