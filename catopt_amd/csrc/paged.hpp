@@ -42,4 +42,58 @@ inline bool strides_fit(const int64_t* s, int n, int64_t step) {
   return true;
 }
 
+// A tensor's layout for the checks of what may overlap what: up to four axes,
+// extents and strides in elements, and the size of one.
+struct Layout {
+  const void* p;
+  int n;
+  int64_t extent[4], stride[4], size;
+
+  bool empty() const {
+    for (int i = 0; i < n; ++i)
+      if (extent[i] < 1) return true;
+    return !p;
+  }
+  uintptr_t begin() const { return reinterpret_cast<uintptr_t>(p); }
+  // One byte behind the last element.
+  uintptr_t end() const {
+    int64_t last = 0;
+    for (int i = 0; i < n; ++i) last += (extent[i] - 1) * stride[i];
+    return begin() + (uintptr_t)((last + 1) * size);
+  }
+  // Whether two elements share memory (an expanded tensor).
+  bool folded() const {
+    if (empty()) return false;
+    int64_t s[4], e[4];
+    int m = 0;
+    for (int i = 0; i < n; ++i) {
+      if (extent[i] < 2) continue;
+      int at = m++;
+      for (; at > 0 && s[at - 1] > stride[i]; --at) s[at] = s[at - 1], e[at] = e[at - 1];
+      s[at] = stride[i], e[at] = extent[i];
+    }
+    int64_t need = 1;
+    for (int i = 0; i < m; ++i) {
+      if (s[i] < need) return true;
+      need = s[i] * e[i];
+    }
+    return false;
+  }
+  bool overlaps(const Layout& o) const { return !empty() && !o.empty() && begin() < o.end() && o.begin() < end(); }
+  bool same(const Layout& o) const {
+    if (p != o.p) return false;
+    for (int i = 0; i < n; ++i)
+      if (extent[i] > 1 && stride[i] != o.stride[i]) return false;
+    return true;
+  }
+};
+
+inline Layout layout3(const void* p, int64_t size, int64_t a, int64_t sa, int64_t b, int64_t sb, int64_t c) {
+  return Layout{p, 3, {a, b, c, 1}, {sa, sb, 1, 1}, size};
+}
+inline Layout layout_pages(const void* p, int64_t size, int64_t n_pages, int64_t H, int64_t page, int64_t d,
+                           const int64_t* s) {
+  return Layout{p, 4, {n_pages, H, page, d}, {s[0], s[1], s[2], 1}, size};
+}
+
 }  // namespace catopt

@@ -5,13 +5,15 @@
 namespace catopt {
 namespace {
 
-// One wave per row (token, query head): the carriers of its key ranges, in
-// their order.  R: the rows of the tiles they were made with.
+// One workgroup per row (token, query head): the carriers of its key ranges,
+// D / 4 threads to a range's numerators, so that 8 (D = 64: 16) ranges load at
+// once.  R: the rows of the tiles they were made with.
 template <int D, int R>
 __global__ __launch_bounds__(256) void paged_combine(PagedArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.N * a.Hq) return;
+  constexpr int TPR = D / 4, GROUPS = 256 / TPR;
+  __shared__ f32x4 sums[GROUPS][TPR];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t row = blockIdx.x;
   const int n = (int)(row / a.Hq), hq = (int)(row - (int64_t)n * a.Hq);
   int b = -1;
   for (int c0 = 0; c0 < a.B; c0 += 64) {  // the last sequence that starts at or before the token
@@ -30,40 +32,41 @@ __global__ __launch_bounds__(256) void paged_combine(PagedArgs a) {
   x.rows = min(R, x.nq * a.G - x.r0);
   paged_ranges(a, x);
   if (x.splits == 1) return;  // written by the tile
-  constexpr int V = D / 64;   // numerators per lane
   const float c = a.scale * kLog2e;
   const float* ml = a.part + 2 * row * a.splits;
-  const float* num = a.part + ((2 * a.N * a.Hq * a.splits + 3) & ~(int64_t)3) + row * a.splits * D + V * lane;
-  float mx = kNegInf;
-  for (int s = lane; s < x.splits; s += 64) mx = fmaxf(mx, ml[2 * s]);
+  const float* num = a.part + ((2 * a.N * a.Hq * a.splits + 3) & ~(int64_t)3) + row * a.splits * D + 4 * (tid % TPR);
+  // lane s of every wave: range s (64 at most)
+  const bool mine = lane < x.splits;
+  const float ms = mine ? ml[2 * lane] : kNegInf, ls = mine ? ml[2 * lane + 1] : 0.f;
+  constexpr int STEPS = kMaxSplits / GROUPS;
+  f32x4 ys[STEPS];
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int s = i * GROUPS + tid / TPR;
+    ys[i] = s < x.splits ? *reinterpret_cast<const f32x4*>(num + (int64_t)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  float mx = ms;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-  float lt = 0.f, y[V];
+  const float f = mine ? move_factor(ms, mx, c) : 0.f;
+  float lt = ls * f;
 #pragma unroll
-  for (int e = 0; e < V; ++e) y[e] = 0.f;
-  constexpr int U = 8;  // loads ahead of their additions
-  for (int s0 = 0; s0 < x.splits; s0 += U) {
-    float f[U], ls[U], ys[U][V];
+  for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o, 64);
+  f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int s = min(s0 + i, x.splits - 1);
-      f[i] = s0 + i < x.splits ? move_factor(ml[2 * s], mx, c) : 0.f;
-      ls[i] = s0 + i < x.splits ? ml[2 * s + 1] : 0.f;
+  for (int i = 0; i < STEPS; ++i) y += ys[i] * __shfl(f, i * GROUPS + tid / TPR, 64);
+  sums[tid / TPR][tid % TPR] = y;
+  __syncthreads();
+  if (tid < TPR && 4 * tid < a.d) {
+    y = sums[0][tid];
 #pragma unroll
-      for (int e = 0; e < V; ++e) ys[i][e] = s0 + i < x.splits ? num[(int64_t)s * D + e] : 0.f;
-    }
+    for (int i = 1; i < GROUPS; ++i) y += sums[i][tid];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      lt += ls[i] * f[i];
-#pragma unroll
-      for (int e = 0; e < V; ++e) y[e] += ys[i][e] * f[i];
-    }
+    for (int e = 0; e < 4; ++e) y[e] = finish(y[e], lt, a.normalize);
+    *reinterpret_cast<u32x2*>(a.o + (int64_t)n * a.o_t + (int64_t)hq * a.o_h + 4 * tid) =
+        u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
   }
-  uint16_t* orow = a.o + (int64_t)n * a.o_t + (int64_t)hq * a.o_h;
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    if (V * lane + e < a.d) orow[V * lane + e] = f32_to_bf16(finish(y[e], lt, a.normalize));
-  if (lane == 0) {
+  if (tid == 0) {
     if (a.m_out) a.m_out[row] = mx * a.scale;
     if (a.l_out) a.l_out[row] = lt;
   }
@@ -96,7 +99,7 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t c
   int64_t s = p.few ? 16384 / groups : 512 / groups;
   p.min_keys = p.few && groups * cap < 512 * 256 ? 128 : 256;
   const int64_t most = (cap + p.min_keys - 1) / p.min_keys;
-  if (s > 64) s = 64;
+  if (s > kMaxSplits) s = kMaxSplits;
   if (s > most) s = most;
   p.splits = s < 1 ? 1 : (int)s;
   const int64_t rows = N * Hq;
@@ -115,7 +118,7 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t c
 
 template <int R>
 int32_t combine(const PagedArgs& a, int D, hipStream_t s) {
-  const int64_t blocks = (a.N * a.Hq + 3) / 4;
+  const int64_t blocks = a.N * a.Hq;
   if (!grid_fits(blocks, 256)) return CATOPT_E_UNSUPPORTED;
   if (D == 128)
     paged_combine<128, R><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(a);
@@ -160,6 +163,17 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   if (!strides_fit(strides, 10, 8) || !strides_fit(strides + 10, 4, 1)) return CATOPT_E_INVAL;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o)) return CATOPT_E_INVAL;
   if (weights_in && !weights_out) return CATOPT_E_INVAL;
+  const Layout out = layout3(o, 2, N, strides[8], Hq, strides[9], d), lq = layout3(q, 2, N, strides[0], Hq, strides[1], d);
+  const Layout lk = layout_pages(k_pages, 2, n_pages, Hkv, page_size, d, strides + 2);
+  const Layout lv = layout_pages(v_pages, 2, n_pages, Hkv, page_size, d, strides + 5);
+  if (out.folded() || out.overlaps(lq) || out.overlaps(lk) || out.overlaps(lv)) return CATOPT_E_INVAL;
+  if (weights_out) {
+    const int64_t cap = n_table * page_size;
+    const Layout wo = layout3(weights_out, 4, B, strides[12], Hkv, strides[13], cap);
+    const Layout wi = layout3(weights_in, 4, B, strides[10], Hkv, strides[11], cap);
+    if (wo.folded() || wo.overlaps(lq) || wo.overlaps(lk) || wo.overlaps(lv) || wo.overlaps(out)) return CATOPT_E_INVAL;
+    if (weights_in && ((wo.overlaps(wi) && !wo.same(wi)) || out.overlaps(wi))) return CATOPT_E_INVAL;
+  }
   // the rows of one load lie within 31 bits of its resource's base
   if (strides[4] > (1 << 26) || strides[7] > (1 << 26)) return CATOPT_E_UNSUPPORTED;
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return CATOPT_E_WORKSPACE;

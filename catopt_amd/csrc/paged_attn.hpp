@@ -207,6 +207,7 @@ __device__ __forceinline__ void take_odd_values(bf16x8* vf, const bf16x8* p, f32
 
 // Host side of each kernel.
 constexpr int kFewRows = 32, kTileRows = 128;
+constexpr int kMaxSplits = 64;  // key ranges of a tile: one per lane of the wave that combines them
 int32_t paged_few_launch(const PagedArgs& a, int D, int64_t tiles, hipStream_t s);    // tiles of kFewRows
 int32_t paged_tile_launch(const PagedArgs& a, int D, int64_t tiles, hipStream_t s);   // tiles of kTileRows
 int paged_weight_parts(int64_t B, int64_t Hkv, int64_t cap, int64_t N, int64_t G);

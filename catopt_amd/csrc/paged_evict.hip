@@ -26,83 +26,135 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One workgroup per (sequence, head).  Radix select over 8 bits at a time
-// finds the rank of the last key that stays and how many of its equals do
-// (the first ones); one pass in key order then lists the kept keys.
+constexpr int kWaves = NT / 64, kRegs = 16;  // weights per lane held in registers: NT * kRegs keys
+constexpr int kBins = 2048;
+
+// One workgroup per (sequence, head); wave i takes the i-th of 16 runs of the
+// keys.  A radix select by 11, 11 and 10 bits of the rank finds the rank of the
+// last key that stays and how many of its equals do (the first ones); each wave
+// then counts its keys above and at that rank, one exchange of the counts gives
+// every wave its place, and a second sweep lists the kept keys in order.
+// HELD: a lane's weights stay in registers over the five sweeps (they cover
+// tables of up to 16384 keys); else each sweep reads them again, from L2.
+template <bool HELD>
 __global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {
-  __shared__ uint32_t hist[256], sh_bin, sh_left, wave_sum[2][NT / 64];
-  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ uint32_t hist[kBins], wave_sum[kWaves], sh_bin, sh_left, cnt_above[kWaves], cnt_equal[kWaves];
+  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = min(max(a.lens[b], 0), a.cap), m = min(n, a.budget);
   const int old = n - min(a.recent, m);  // keys from here on stay
   const float* w = a.w + b * a.w_b + h * a.w_h;
-  float* w_out = a.w_out ? a.w_out + b * a.wo_b + h * a.wo_h : nullptr;
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
   if (h == 0 && tid == 0) a.new_lens[b] = m;
-  uint32_t need = (uint32_t)(m - (n - old)), prefix = 0;  // of the first `old` keys, `need` stay
-  if (need > 0 && need < (uint32_t)old) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-      for (int j = tid; j < old; j += NT) {
-        const uint32_t r = rank_of(w[j]);
-        if ((r & mask) == prefix) atomicAdd(&hist[(r >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        uint32_t left = need;
-        int bin = 255;
-        while (bin > 0 && hist[bin] < left) left -= hist[bin--];
-        sh_bin = (uint32_t)bin;
-        sh_left = left;
-      }
-      __syncthreads();
-      prefix |= sh_bin << shift;
-      need = sh_left;
-      __syncthreads();
+  const int steps = (n + NT - 1) / NT, first = wave * steps * 64;  // this wave's keys: `steps` of 64
+
+  uint32_t held[HELD ? kRegs : 1];
+  if (HELD) {
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) {
+      const int j = first + 64 * i + lane;
+      held[i] = i < steps && j < old ? rank_of(w[j]) : 0u;
     }
-  } else if (need > 0) {
-    need = 0, prefix = 0;  // every old key stays: every rank is at least 0
-  } else {
-    prefix = 0xffffffffu;  // none does
   }
-  // keys above the last rank stay, and the first `need` of that rank itself
-  // (all of them where every old key stays)
-  const bool all = m - (n - old) == old, none = m == n - old;
-  uint32_t base = 0, base_eq = 0;
-  for (int j0 = 0; j0 < n; j0 += NT) {
-    const int j = j0 + tid;
-    const float wj = j < n ? w[j] : 0.f;
-    const uint32_t r = rank_of(wj);
+  // f(key, rank, whether the key is one of the old ones)
+  auto sweep = [&](auto f) {
+    if (HELD) {
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i)
+        if (i < steps) f(first + 64 * i + lane, held[i]);
+    } else {
+      constexpr int U = 8;
+      for (int i0 = 0; i0 < steps; i0 += U) {
+        uint32_t r[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int j = first + 64 * (i0 + i) + lane;
+          r[i] = i0 + i < steps && j < old ? rank_of(w[j]) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+          if (i0 + i < steps) f(first + 64 * (i0 + i) + lane, r[i]);
+      }
+    }
+  };
+
+  // of the first `old` keys `need` stay: those above the rank `limit` and the
+  // first `equals` of that rank
+  const uint32_t need = (uint32_t)(m - (n - old));
+  uint32_t limit = 0, equals = need;
+  const bool some = need > 0 && need < (uint32_t)old;
+  if (some) {
+    for (int round = 0; round < 3; ++round) {
+      const int shift = round == 0 ? 21 : round == 1 ? 10 : 0, bits = round == 2 ? 10 : 11;
+      const uint32_t mask = round == 0 ? 0u : round == 1 ? 0xffe00000u : 0xfffffc00u;
+      hist[tid] = 0;
+      hist[tid + NT] = 0;
+      __syncthreads();
+      sweep([&](int j, uint32_t r) {
+        if (j < old && (r & mask) == limit) atomicAdd(&hist[(r >> shift) & ((1u << bits) - 1)], 1u);
+      });
+      __syncthreads();
+      // keys in this thread's two bins and in all bins above them
+      const uint32_t hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
+      uint32_t sum = hi + lo;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += x;
+      }
+      if (lane == 63) wave_sum[wave] = sum;
+      __syncthreads();
+      uint32_t above = sum - hi - lo;
+      for (int i = 0; i < wave; ++i) above += wave_sum[i];
+      if (above < equals && equals <= above + hi + lo) {  // one thread
+        const bool in_hi = equals <= above + hi;
+        sh_bin = kBins - 1 - 2 * tid - (in_hi ? 0 : 1);
+        sh_left = equals - above - (in_hi ? 0u : hi);
+      }
+      __syncthreads();
+      limit |= sh_bin << shift;
+      equals = sh_left;
+    }
+  } else if (need == 0) {
+    limit = 0xffffffffu, equals = 0;  // none of them stays
+  }  // else all do: every rank is at least 0, and all `need` of rank 0 would stay
+
+  uint32_t na = 0, ne = 0;
+  sweep([&](int j, uint32_t r) {
     const bool is_old = j < old;
-    const bool above = j < n && (!is_old || all || (!none && r > prefix));
-    const bool equal = is_old && !all && !none && r == prefix;
-    const uint64_t below = (1ull << lane) - 1, be = __ballot(equal);
-    if (lane == 0) wave_sum[0][wave] = __popcll(be);
-    __syncthreads();
-    uint32_t eq_before = base_eq + __popcll(be & below), eq_total = 0;
-    for (int i = 0; i < NT / 64; ++i) {
-      if (i < wave) eq_before += wave_sum[0][i];
-      eq_total += wave_sum[0][i];
-    }
-    const bool stay = above || (equal && eq_before < need);
-    const uint64_t bs = __ballot(stay);
-    if (lane == 0) wave_sum[1][wave] = __popcll(bs);
-    __syncthreads();
-    uint32_t at = base + __popcll(bs & below), total = 0;
-    for (int i = 0; i < NT / 64; ++i) {
-      if (i < wave) at += wave_sum[1][i];
-      total += wave_sum[1][i];
-    }
-    if (stay && at < (uint32_t)m) {
-      kept[at] = j;
-      if (w_out) w_out[at] = wj;  // at <= j, and every weight up to j0 + NT has been read
-    }
-    base += total;
-    base_eq += eq_total;
-    __syncthreads();
+    na += __popcll(__ballot(j < n && (!is_old || r > limit)));
+    ne += __popcll(__ballot(is_old && r == limit));
+  });
+  if (lane == 0) cnt_above[wave] = na, cnt_equal[wave] = ne;
+  __syncthreads();
+  uint32_t at = 0, eq = 0;  // kept keys, and keys at the limit, before this wave's
+  for (int i = 0; i < wave; ++i) {
+    at += cnt_above[i] + (eq < equals ? min(cnt_equal[i], equals - eq) : 0u);
+    eq += cnt_equal[i];
   }
+  const uint64_t below = (1ull << lane) - 1;
+  sweep([&](int j, uint32_t r) {
+    const bool is_old = j < old;
+    const uint64_t be = __ballot(is_old && r == limit);
+    const bool stay = j < n && (!is_old || r > limit || (r == limit && eq + __popcll(be & below) < equals));
+    const uint64_t bs = __ballot(stay);
+    const uint32_t to = at + __popcll(bs & below);
+    if (stay && to < (uint32_t)m) kept[to] = j;
+    at += __popcll(bs);
+    eq += __popcll(be);
+  });
   for (int j = m + tid; j < a.budget; j += NT) kept[j] = -1;
+  if (!a.w_out) return;
+  // the kept weights, which may go where the weights are: a kept key's place is
+  // never behind it, so a step's writes lie before every later step's reads
+  float* w_out = a.w_out + b * a.wo_b + h * a.wo_h;
+  __syncthreads();
+  for (int i0 = 0; i0 < m; i0 += NT) {
+    const int i = i0 + tid;
+    const float x = i < m ? w[kept[i]] : 0.f;
+    __syncthreads();
+    if (i < m) w_out[i] = x;
+  }
 }
 
 // 16 bytes of one kept row of k and of v per thread.
@@ -150,7 +202,7 @@ extern "C" int32_t catopt_hip_paged_evict(int32_t dtype, int64_t B, int64_t Hkv,
   if (row % 16 || row > (1 << 14)) return CATOPT_E_UNSUPPORTED;
   if (page_size > lim || out_page_size > lim || n_table > lim || n_out_table > lim || budget > lim || B > (1 << 20) || Hkv > (1 << 20))
     return CATOPT_E_UNSUPPORTED;
-  if (n_table * page_size > lim) return CATOPT_E_UNSUPPORTED;
+  if (n_table * page_size > lim || !grid_fits(B * Hkv, NT)) return CATOPT_E_UNSUPPORTED;  // B Hkv < 2^22
   if (n_out_table * out_page_size < budget) return CATOPT_E_INVAL;
   if (B == 0) return CATOPT_OK;
   const int64_t step = 16 / (dtype == CATOPT_BF16 ? 2 : 4);
@@ -158,8 +210,26 @@ extern "C" int32_t catopt_hip_paged_evict(int32_t dtype, int64_t B, int64_t Hkv,
   if (!kv_lens || !kept || !new_lens || !out_table || (n_table > 0 && (!block_table || !weights))) return CATOPT_E_INVAL;
   if ((n_pages > 0 && (!k_pages || !v_pages)) || (n_out_pages > 0 && (!k_out || !v_out))) return CATOPT_E_INVAL;
   if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(k_out) || !aligned16(v_out)) return CATOPT_E_INVAL;
-  EvictArgs a{};
   const int64_t* s = strides;
+  const int64_t size = 16 / step;
+  const Layout lk = layout_pages(k_pages, size, n_pages, Hkv, page_size, d, s);
+  const Layout lv = layout_pages(v_pages, size, n_pages, Hkv, page_size, d, s + 3);
+  const Layout ko = layout_pages(k_out, size, n_out_pages, Hkv, out_page_size, d, s + 6);
+  const Layout vo = layout_pages(v_out, size, n_out_pages, Hkv, out_page_size, d, s + 9);
+  const Layout w = layout3(weights, 4, B, s[12], Hkv, s[13], n_table * page_size);
+  const Layout wo = layout3(weights_out, 4, B, s[14], Hkv, s[15], budget);
+  // the same pool keeps its place in both roles; keys and values may be parts
+  // of one storage, so only their beginnings tell them apart
+  const bool pool = k_out == k_pages;
+  if (ko.folded() || vo.folded() || (!ko.empty() && (k_out == v_out || k_out == v_pages || v_out == k_pages)))
+    return CATOPT_E_INVAL;
+  if (pool ? !ko.same(lk) || !vo.same(lv) || n_out_pages != n_pages || (n_table > 0 && out_table == block_table)
+           : ko.overlaps(lk) || vo.overlaps(lv))
+    return CATOPT_E_INVAL;
+  if (ko.overlaps(w) || vo.overlaps(w) || ko.overlaps(wo) || vo.overlaps(wo) || lk.overlaps(wo) || lv.overlaps(wo))
+    return CATOPT_E_INVAL;
+  if (wo.folded() || (wo.overlaps(w) && !wo.same(w))) return CATOPT_E_INVAL;
+  EvictArgs a{};
   a.k = Pages{k_pages, s[0] / step, s[1] / step, s[2] / step};
   a.v = Pages{v_pages, s[3] / step, s[4] / step, s[5] / step};
   a.ko = Pages{k_out, s[6] / step, s[7] / step, s[8] / step};
@@ -171,11 +241,13 @@ extern "C" int32_t catopt_hip_paged_evict(int32_t dtype, int64_t B, int64_t Hkv,
   a.page = FastDiv::of(page_size), a.out_page = FastDiv::of(out_page_size);
   a.B = (int)B, a.H = (int)Hkv, a.cap = (int)(n_table * page_size), a.budget = (int)budget, a.recent = (int)recent;
   a.row16 = (int)(row / 16);
-  if (!grid_fits(B * Hkv, NT)) return CATOPT_E_UNSUPPORTED;  // so B Hkv < 2^22 and the product below < 2^62
-  const int64_t blocks = (B * Hkv * budget * a.row16 + 255) / 256;
+  const int64_t blocks = (B * Hkv * budget * a.row16 + 255) / 256;  // the product is below 2^62
   if (!grid_fits(blocks, 256)) return CATOPT_E_UNSUPPORTED;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  evict_select<<<dim3((uint32_t)(B * Hkv)), dim3(NT), 0, st>>>(a);
+  if (a.cap <= NT * kRegs)
+    evict_select<true><<<dim3((uint32_t)(B * Hkv)), dim3(NT), 0, st>>>(a);
+  else
+    evict_select<false><<<dim3((uint32_t)(B * Hkv)), dim3(NT), 0, st>>>(a);
   CATOPT_LAUNCH_CHECK();
   evict_move<<<dim3((uint32_t)blocks), dim3(256), 0, st>>>(a);
   CATOPT_LAUNCH_CHECK();

@@ -46,32 +46,6 @@ QK_NORM_ROPE_MAX_HEAD_DIM = 256
 _I12, _I14, _I16 = C.c_int64 * 12, C.c_int64 * 14, C.c_int64 * 16
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """The byte range that a tensor's elements lie in."""
-    p = t.data_ptr()
-    if t.numel() == 0:
-        return p, p
-    return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-
-def _apart(name: str, out: torch.Tensor, *ins: torch.Tensor | None) -> None:
-    lo, hi = _span(out)
-    for t in ins:
-        if t is not None:
-            a, b = _span(t)
-            if a < hi and lo < b:
-                raise ValueError(f"{name} overlaps one of the call's other operands")
-
-
-def _no_overlap_within(name: str, t: torch.Tensor) -> None:
-    """An output whose elements share memory (an expanded tensor) is refused."""
-    need = 1
-    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
-        if s < need:
-            raise ValueError(f"{name} has elements that share memory (strides {t.stride()})")
-        need = s * n
-
-
 class _on:
     """The operands' device as the current one for a call's launches."""
 
@@ -81,7 +55,7 @@ class _on:
         self.dev = dev
 
     def __enter__(self) -> None:
-        self.old = torch.cuda.current_device()
+        self.old = torch._C._cuda_getDevice()
         if self.old != self.dev:
             torch.cuda.set_device(self.dev)
 
@@ -94,42 +68,46 @@ def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
     """``(N, H, d)`` with a contiguous last axis, rows readable in 16-byte pieces."""
     if t.dim() != 3:
         raise ValueError(f"{name} is (tokens, heads, head dim), got {tuple(t.shape)}")
+    a, b, c = t.stride()
     step = 16 // t.element_size()
-    s = t.stride()
-    if s[2] != 1 or s[0] % step or s[1] % step or t.data_ptr() % 16:
+    if c != 1 or a % step or b % step or t.data_ptr() % 16:
         t = t.contiguous()
     return t
 
 
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, what: str = "") -> tuple[int, int, int, int]:
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, what: str = "") -> torch.Size:
     """The shape of a cache's two page tensors, checked: they are used in place, so nothing is copied to fit."""
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype:
         raise ValueError(f"the {what}pages are two tensors (n_pages, heads, page size, head dim) of one type, got "
-                         f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
+                         f"{tuple(shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
     step = 16 // k_pages.element_size()
     for t in (k_pages, v_pages):
-        s = t.stride()
-        if s[3] != 1 or s[0] % step or s[1] % step or s[2] % step or t.data_ptr() % 16:
-            raise ValueError(f"{what}pages need a contiguous head dim and 16-byte aligned rows, got strides {s}")
-    return tuple(k_pages.shape)
+        a, b, c, e = t.stride()
+        if e != 1 or a % step or b % step or c % step or t.data_ptr() % 16:
+            raise ValueError(f"{what}pages need a contiguous head dim and 16-byte aligned rows, got strides {t.stride()}")
+    return shape
 
 
-def _two_tensors(a: torch.Tensor, b: torch.Tensor) -> None:
-    """Keys and values are not one tensor (they may be two parts of one, so their ranges may interleave)."""
-    if a.data_ptr() == b.data_ptr() and a.numel():
-        raise ValueError("keys and values need pages of their own")
-
-
-def _ints(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
-    if t.dtype != dtype or t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
-        want = tuple("any" if w is None else w for w in shape)
-        raise ValueError(f"{name} is an {dtype} tensor of shape {want}, got {t.dtype} {tuple(t.shape)}")
-    return t
+def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, n: int | None = None) -> torch.Tensor:
+    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} is an {dtype} vector{'' if n is None else f' of {n}'}, got {t.dtype} {tuple(t.shape)}")
+    return t.contiguous()
 
 
 def _table(name: str, t: torch.Tensor, B: int) -> torch.Tensor:
-    _ints(name, t, torch.int32, (B, None))
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B:
+        raise ValueError(f"{name} is an int32 ({B}, pages of a sequence) tensor, got {t.dtype} {tuple(t.shape)}")
     return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _check(fn: str, status: int) -> None:
+    """A refusal of the library's own checks (what overlaps what) as the argument error that it is."""
+    if status == L.E_INVAL:
+        raise ValueError(f"{fn}: an output overlaps another operand or itself, or a stride does not fit")
+    if status == L.E_UNSUPPORTED:
+        raise NotImplementedError(f"{fn}: the call is beyond what one launch takes")
+    L.check(fn, status)
 
 
 def _norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleaved, k_pages, v_pages, slots):
@@ -159,36 +137,31 @@ def _norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleave
             raise ValueError("a norm weight holds one value of q's type for each head dim")
     q_weight = None if q_weight is None else q_weight.contiguous()
     k_weight = None if k_weight is None else k_weight.contiguous()
-    _ints("positions", positions, torch.int64, (N,))
-    positions = positions.contiguous()
+    positions = _vector("positions", positions, torch.int64, N)
     q_out = torch.empty((N, Hq, d), dtype=q.dtype, device=q.device)
     n_pages = page = 0
+    qs, ks = q.stride(), k.stride()
     if append:
         v = _heads("v", v)
         if v.shape != k.shape or v.dtype != q.dtype:
             raise ValueError(f"v has k's shape and type: {tuple(v.shape)} {v.dtype}, {tuple(k.shape)} {k.dtype}")
         n_pages, ph, page, pd = _pages(k_pages, v_pages)
-        if (ph, pd) != (Hkv, d) or k_pages.dtype != q.dtype:
+        if ph != Hkv or pd != d or k_pages.dtype != q.dtype:
             raise ValueError(f"the pages hold {ph} heads of {pd} {k_pages.dtype}, k has {Hkv} of {d} {q.dtype}")
-        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-            _no_overlap_within(name, t)
-            _apart(name, t, q, k, v, cos, sin, positions, slots)
-        _two_tensors(k_pages, v_pages)
-        _ints("slots", slots, torch.int64, (N,))
-        slots = slots.contiguous()
+        slots = _vector("slots", slots, torch.int64, N)
         k_out, v_out = k_pages, v_pages
-        ks, vs = k_pages.stride(), v_pages.stride()
-        strides = _I12(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *ks[:3], *vs[:3])
+        vs, ko, vo = v.stride(), k_pages.stride(), v_pages.stride()
+        strides = _I12(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], ko[0], ko[1], ko[2], vo[0], vo[1], vo[2])
     else:
         k_out = torch.empty((N, Hkv, d), dtype=q.dtype, device=q.device)
         v_out = None
-        strides = _I12(*q.stride()[:2], *k.stride()[:2])
+        strides = _I12(qs[0], qs[1], ks[0], ks[1])
     with _on(dev):
         st = lib.catopt_hip_qk_norm_rope(dt, N, Hq, Hkv, d, rot, int(bool(interleaved)), _ptr(q), _ptr(k), _ptr(v),
                                          _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
                                          cos.shape[0], cos.stride(0) if rot else 0, _ptr(positions), _ptr(q_out),
                                          _ptr(k_out), _ptr(v_out), strides, _ptr(slots), n_pages, page, _stream(q))
-    L.check("catopt_hip_qk_norm_rope", st)
+    _check("qk_norm_rope", st)
     return q_out, k_out
 
 
@@ -229,12 +202,6 @@ def _weight_rows(name: str, w: torch.Tensor, B: int, H: int, width: int) -> tupl
     if w.shape[2] > 1 and w.stride(2) != 1:
         raise ValueError(f"{name} needs a contiguous last axis, got strides {w.stride()}")
     return w.stride(0), w.stride(1)
-
-
-def _in_place_or_apart(name: str, out: torch.Tensor, src: torch.Tensor | None) -> None:
-    """``out`` is ``src`` itself, element for element, or shares no memory with it."""
-    if src is not None and (out.data_ptr() != src.data_ptr() or out.stride() != src.stride()):
-        _apart(name, out, src)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -285,31 +252,25 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     scale = float(scale)
     if not (math.isfinite(scale) and scale > 0):
         raise ValueError(f"the scale is a positive number, got {scale}")
-    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    _ints("kv_lens", kv_lens, torch.int32, (None,))
-    _ints("q_starts", q_starts, torch.int32, (B + 1,))
+    kv_lens = _vector("kv_lens", kv_lens, torch.int32)
+    B = kv_lens.shape[0]
+    q_starts = _vector("q_starts", q_starts, torch.int32, B + 1)
     table = _table("block_table", block_table, B)
     n_table = table.shape[1]
-    kv_lens, q_starts = kv_lens.contiguous(), q_starts.contiguous()
     if out is None:
         o = torch.empty((N, Hq, d), dtype=q.dtype, device=q.device)
     else:
         o = out
         if o.shape != q.shape or o.dtype != q.dtype:
             raise ValueError(f"out has q's shape and type, got {tuple(o.shape)} {o.dtype}")
-        so = o.stride()
-        if so[2] != 1 or so[0] % 8 or so[1] % 8 or o.data_ptr() % 16:
-            raise ValueError(f"out needs a contiguous head dim and 16-byte aligned rows, got strides {so}")
-        _no_overlap_within("out", o)
-        _apart("out", o, q, k_pages, v_pages, weights, weights_out)
-    w_in, w_out = (0, 0), (0, 0)
+    so = o.stride()
+    if so[2] != 1 or so[0] % 8 or so[1] % 8 or o.data_ptr() % 16:
+        raise ValueError(f"out needs a contiguous head dim and 16-byte aligned rows, got strides {so}")
+    w_in = w_out = (0, 0)
     if weights_out is not None:
         w_out = _weight_rows("weights_out", weights_out, B, Hkv, n_table * page)
-        _no_overlap_within("weights_out", weights_out)
         if weights is not None:
             w_in = _weight_rows("weights", weights, B, Hkv, n_table * page)
-        _in_place_or_apart("weights_out", weights_out, weights)
-        _apart("weights_out", weights_out, q, k_pages, v_pages)
     elif weights is not None:
         raise ValueError("weights need a weights_out to go to")
     m = l = None
@@ -317,7 +278,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         m = torch.empty((N, Hq), dtype=torch.float32, device=q.device)
         l = torch.empty((N, Hq), dtype=torch.float32, device=q.device)
     if N and B:
-        ks, vs, qs, so = k_pages.stride(), v_pages.stride(), q.stride(), o.stride()
+        ks, vs, qs = k_pages.stride(), v_pages.stride(), q.stride()
         strides = _I14(qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], so[0], so[1], *w_in, *w_out)
         with _on(dev):
             wsb = lib.catopt_hip_paged_attn_workspace_bytes(B, N, Hq, Hkv, d, n_table, page,
@@ -331,7 +292,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                                                int(bool(causal)), 2 if empty_rows == "zero" else 1, o.data_ptr(),
                                                _ptr(m), _ptr(l), _ptr(weights), _ptr(weights_out), strides, _ptr(ws),
                                                wsb, _stream(q))
-        L.check("catopt_hip_paged_attn_fwd", st)
+        _check("paged_attention", st)
     return (o, m, l) if return_ml else o
 
 
@@ -375,40 +336,26 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     budget, recent = int(budget), int(recent)
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"a budget of at least 1 with 0 <= recent <= budget, got {budget} and {recent}")
-    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    _ints("kv_lens", kv_lens, torch.int32, (None,))
+    kv_lens = _vector("kv_lens", kv_lens, torch.int32)
+    B = kv_lens.shape[0]
     table, to = _table("block_table", block_table, B), _table("out_table", out_table, B)
     n_table, n_to = table.shape[1], to.shape[1]
     if n_to * page_out < budget:
         raise ValueError(f"out_table reaches {n_to * page_out} keys, the budget is {budget}")
-    _two_tensors(k_to, v_to)
-    for name, t, src in (("k_out", k_to, k_pages), ("v_out", v_to, v_pages)):
-        _no_overlap_within(name, t)
-        _apart(name, t, weights, table, to, kv_lens)
-        _in_place_or_apart(name, t, src)
-    if not own:
-        _two_tensors(k_to, v_pages)
-        _two_tensors(v_to, k_pages)
-    if B > 0 and n_table and to.data_ptr() == table.data_ptr() and k_to.data_ptr() == k_pages.data_ptr():
-        raise ValueError("out_table names pages of its own, not those of block_table")
-    kv_lens = kv_lens.contiguous()
     w_in = _weight_rows("weights", weights, B, Hkv, n_table * page)
     if weights_out is None:
         weights_out = torch.zeros((B, Hkv, budget), dtype=torch.float32, device=weights.device)
     w_out = _weight_rows("weights_out", weights_out, B, Hkv, budget)
-    _no_overlap_within("weights_out", weights_out)
-    _in_place_or_apart("weights_out", weights_out, weights)
-    _apart("weights_out", weights_out, k_pages, v_pages, k_to, v_to)
     kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=k_pages.device)
     new_lens = torch.empty((B,), dtype=torch.int32, device=k_pages.device)
     if B:
-        strides = _I16(*k_pages.stride()[:3], *v_pages.stride()[:3], *k_to.stride()[:3], *v_to.stride()[:3],
-                       *w_in, *w_out)
+        a, b, c, e = k_pages.stride(), v_pages.stride(), k_to.stride(), v_to.stride()
+        strides = _I16(a[0], a[1], a[2], b[0], b[1], b[2], c[0], c[1], c[2], e[0], e[1], e[2], *w_in, *w_out)
         with _on(dev):
             st = lib.catopt_hip_paged_evict(dt, B, Hkv, d, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page,
                                             _ptr(table), table.stride(0), n_table, kv_lens.data_ptr(),
                                             weights.data_ptr(), budget, recent, k_to.data_ptr(), v_to.data_ptr(),
                                             n_out, page_out, to.data_ptr(), to.stride(0), n_to, kept.data_ptr(),
                                             new_lens.data_ptr(), weights_out.data_ptr(), strides, _stream(k_pages))
-        L.check("catopt_hip_paged_evict", st)
+        _check("paged_evict", st)
     return kept, new_lens, weights_out
