@@ -90,35 +90,50 @@ __device__ __forceinline__ float finish(float x, float l, int normalize) {
   return x * (1.0f / l);
 }
 
-// Page ids and first slots of the 8-key groups from `key0` on: lane i holds
-// group i (pages hold a multiple of 8 keys, so a group lies in one).  `bad`
-// has a bit for each group of real keys whose page is invalid; groups behind
-// the keys, like invalid ones, hold page -1.
-struct PageIds {
-  int page, slot;
+// Where 8 keys (a lane's) lie: pages hold a multiple of 8 keys, so the rows of 8
+// are in one, and one buffer resource over them serves all loads of them.  Its
+// range ends behind the last key; for keys of an invalid page, or behind the
+// last key, it is empty, so that they read as zeros.  The lanes work these out
+// for many groups at once; a load takes its group's from the lane by readlane.
+struct KeyGroup {
+  uint32_t k_lo, k_hi, k_bytes, v_lo, v_hi, v_bytes;
 };
-__device__ __forceinline__ PageIds page_ids(const PagedArgs& a, const int32_t* table, int key0, int len) {
-  const int key = key0 + 8 * (threadIdx.x & 7);
-  PageIds r{-1, 0};
-  if (key < len) {
-    const uint32_t tp = a.page.div(key);
-    r.page = table[tp];
-    r.slot = key - (int)(tp * a.page.d);
-  }
-  return r;
-}
-__device__ __forceinline__ uint32_t bad_groups(const PagedArgs& a, const PageIds& r, int key0, int len) {
-  const bool bad = key0 + 8 * (int)(threadIdx.x & 7) < len && (r.page < 0 || r.page >= a.n_pages);
-  return (uint32_t)__ballot(bad) & 0xffu;
+
+__device__ __forceinline__ int group_page(const PagedArgs& a, const int32_t* table, int key, int len) {
+  return key < len ? table[a.page.div(key)] : -1;
 }
 
-// Resource over the `rows` rows from slot `slot` of page `page` (head offset
-// in `base`): rows past them, and every row of an invalid page, read as zeros.
-__device__ __forceinline__ u32x4 page_rsrc(const uint16_t* base, int page, int slot, int64_t s_page, int64_t s_slot,
-                                           int rows, int d, int64_t n_pages) {
-  const bool ok = rows > 0 && page >= 0 && page < n_pages;
-  const uint16_t* p = ok ? base + page * s_page + slot * s_slot : base;
-  return make_rsrc(p, ok ? (uint32_t)(((rows - 1) * s_slot + d) * 2) : 0u);
+// `bad`: keys before `len` whose page is invalid.
+__device__ __forceinline__ KeyGroup key_group(const PagedArgs& a, const uint16_t* kb, const uint16_t* vb, int page, int key,
+                                              int len, bool& bad) {
+  const bool real = key < len, ok = real && page >= 0 && page < a.n_pages;
+  bad = real && !ok;
+  const int64_t pg = ok ? page : 0, slot = ok ? key - (int)(a.page.div(key) * a.page.d) : 0;
+  const int rows = min(len - key, 8);
+  const uint64_t k = reinterpret_cast<uint64_t>(kb + pg * a.k_p + slot * a.k_s);
+  const uint64_t v = reinterpret_cast<uint64_t>(vb + pg * a.v_p + slot * a.v_s);
+  KeyGroup r;
+  r.k_lo = (uint32_t)k, r.k_hi = (uint32_t)(k >> 32), r.v_lo = (uint32_t)v, r.v_hi = (uint32_t)(v >> 32);
+  r.k_bytes = ok ? ((rows - 1) * (uint32_t)a.k_s + a.d) * 2u : 0u;
+  r.v_bytes = ok ? ((rows - 1) * (uint32_t)a.v_s + a.d) * 2u : 0u;
+  return r;
+}
+
+__device__ __forceinline__ u32x4 lane_rsrc(uint32_t lo, uint32_t hi, uint32_t bytes, int lane) {
+  u32x4 r;
+  r.x = __builtin_amdgcn_readlane(lo, lane);
+  r.y = __builtin_amdgcn_readlane(hi, lane);
+  r.z = __builtin_amdgcn_readlane(bytes, lane);
+  r.w = 0x00020000;
+  return r;
+}
+__device__ __forceinline__ u32x4 k_rsrc(const KeyGroup& x, int lane) { return lane_rsrc(x.k_lo, x.k_hi, x.k_bytes, lane); }
+__device__ __forceinline__ u32x4 v_rsrc(const KeyGroup& x, int lane) { return lane_rsrc(x.v_lo, x.v_hi, x.v_bytes, lane); }
+
+// A lane's byte offset from its group's first row: row `row` of the 8, 16-byte
+// piece `piece` of it; pieces past d lie outside every resource.
+__device__ __forceinline__ uint32_t group_offset(int64_t s_slot, int row, int piece, int d) {
+  return piece * 8 < d ? (uint32_t)(row * (int)s_slot + piece * 8) * 2u : 0x7ffffff0u;
 }
 
 // V^T fragments of 32 keys from an LDS tile: vf[2 db + u], keys 16 u + {4 (G /

@@ -8,10 +8,11 @@
 //
 // Products as in the contiguous kernels: S^T = K Q^T and O^T += V^T P^T on the
 // 32x32x16 MFMA, the accumulator column the query row.  A wave's rows of K and
-// V go global->LDS directly, one stage ahead; a 1 KB load covers 4 or 8 rows,
-// which lie in one page, so each has a buffer resource of its own whose range
-// ends behind the last key.  The page ids of a stage are loaded one stage
-// before its rows.
+// V go global->LDS directly into two stages of its own.  A stage is loaded again
+// as soon as it has been used, and the wait for the other one leaves the new
+// loads in flight: the waves read nothing of each other's, so there is no
+// barrier in the loop.  A lane works out the place of 8 keys, the wave those of
+// 16 stages at once.
 #include "paged_attn.hpp"
 
 namespace catopt {
@@ -20,14 +21,25 @@ namespace {
 template <int D>
 struct Few {
   static constexpr int WAVES = D == 128 ? 2 : 4, NT = 64 * WAVES;
-  static constexpr int KEYS = 32 * WAVES;              // per stage
+  static constexpr int KEYS = 32 * WAVES;              // of a round of stages, 32 per wave
   static constexpr int HALF = 32 * AttnRow<D>::BYTES;  // a wave's K (or V) rows of a stage
-  static constexpr int WAVE_BYTES = 2 * HALF, STAGE = WAVES * WAVE_BYTES, BYTES = 2 * STAGE;
+  static constexpr int STAGE = 2 * HALF, WAVE_BYTES = 2 * STAGE, BYTES = WAVES * WAVE_BYTES;
   static constexpr int LOADS = HALF / 1024;            // 1 KB loads of K (and of V) per stage
   static constexpr int ROWS = 32 / LOADS;              // rows of one
   static constexpr int OLD = D + 4;                    // row of the merge buffer, floats
   static_assert(WAVES * 32 * OLD * 4 + WAVES * 64 * 4 <= BYTES, "the merge reuses the stages");
 };
+
+// Wait for all but the newest LOADS * 2 loads (one stage's), or for all.  The
+// stage waited for is older than those whatever else the compiler has issued in
+// between, and the asm keeps the stage's LDS reads behind it.
+template <int N>
+__device__ __forceinline__ void wait_stage(bool newer) {
+  if (newer)
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  else
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
 
 template <int D>
 __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
@@ -55,34 +67,31 @@ __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
   }
   const int lim = x.off + tok;  // last key this row sees
 
-  const int k_end = min(x.kend, (split + 1) * x.keys);
-  const int t0 = split * x.keys / L::KEYS, t1 = (k_end + L::KEYS - 1) / L::KEYS;
+  // this wave's stages: 32 keys each from key_of(i) on
+  const int k_begin = split * x.keys + 32 * wave, k_end = min(x.kend, (split + 1) * x.keys);
+  const int stages = k_end > k_begin ? (k_end - k_begin + L::KEYS - 1) / L::KEYS : 0;
+  auto key_of = [&](int i) { return k_begin + i * L::KEYS; };
   const int32_t* table = a.table + (int64_t)x.b * a.table_ld;
   const uint16_t *kb = a.k + (int64_t)h * a.k_h, *vb = a.v + (int64_t)h * a.v_h;
-  // a lane's 16 bytes of a load: row lane / CH of it.  The swizzles depend on a
-  // row's place among 16 (K, D = 128: loads i and i + 4 agree), 8 or 4 rows.
-  // Columns past d lie outside every resource.
+  // a lane's 16 bytes of load k: row k ROWS + lane / CH of the stage, row & 7 of
+  // its group; the swizzles depend on a row's place among 16 (K, D = 128: loads
+  // k and k + 4 agree), 8 or 4 rows
   const int sub = lane / AttnRow<D>::CH, cp = lane % AttnRow<D>::CH;
-  uint32_t koff[4];
+  uint32_t koff[4], voff[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int kc = cp ^ ((i * L::ROWS + sub) & (AttnRow<D>::CH - 1) & 15);
-    koff[i] = kc * 8 < a.d ? (uint32_t)(sub * (int)a.k_s + kc * 8) * 2u : 0x7ffffff0u;
+  for (int k = 0; k < 4; ++k) {
+    const int r = k * L::ROWS + sub;
+    koff[k] = group_offset(a.k_s, r & 7, cp ^ (r & (AttnRow<D>::CH - 1) & 15), a.d);
+    if (k < 2) voff[k] = group_offset(a.v_s, r & 7, cp ^ vswz<D>(r), a.d);
   }
-  const int vc = cp ^ vswz<D>(sub);
-  const uint32_t voff = vc * 8 < a.d ? (uint32_t)(sub * (int)a.v_s + vc * 8) * 2u : 0x7ffffff0u;
   const uint32_t lds0 = lds_u32(lds) + wave * L::WAVE_BYTES;
-  auto issue = [&](int st, int stage, const PageIds& ids) {
-    const int key0 = st * L::KEYS + 32 * wave;
+  auto issue = [&](int i, int lane0, const KeyGroup& at) {  // stage i, its groups in lanes lane0 to lane0 + 3
 #pragma unroll
-    for (int i = 0; i < L::LOADS; ++i) {
-      const int grp = i * L::ROWS / 8;
-      const int page = __builtin_amdgcn_readlane(ids.page, grp);
-      const int slot = __builtin_amdgcn_readlane(ids.slot, grp) + i * L::ROWS % 8;
-      const int rows = min(x.len - (key0 + i * L::ROWS), L::ROWS);
-      dma_buf(page_rsrc(kb, page, slot, a.k_p, a.k_s, rows, a.d, a.n_pages), koff[i & 3], lds0 + stage * L::STAGE + i * 1024);
-      dma_buf(page_rsrc(vb, page, slot, a.v_p, a.v_s, rows, a.d, a.n_pages), voff,
-              lds0 + stage * L::STAGE + L::HALF + i * 1024);
+    for (int k = 0; k < L::LOADS; ++k) {
+      const int ln = lane0 + k * L::ROWS / 8;
+      const uint32_t to = lds0 + (i & 1) * L::STAGE + k * 1024;
+      dma_buf(k_rsrc(at, ln), koff[k & 3], to);
+      dma_buf(v_rsrc(at, ln), voff[k & 1], to + L::HALF);
     }
   };
 
@@ -94,30 +103,27 @@ __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
   float m = kNegInf, l = 0.f;
   float* srow = a.scores ? a.scores + ((int64_t)(x.row0 + tok) * a.Hq + hq) * a.cap : nullptr;
 
-  PageIds ids{-1, 0}, next{-1, 0};
-  uint32_t bad = 0, bad_next = 0;
-  if (t0 < t1) {
-    ids = page_ids(a, table, t0 * L::KEYS + 32 * wave, x.len);
-    bad = bad_groups(a, ids, t0 * L::KEYS + 32 * wave, x.len) & 15u;
-    issue(t0, 0, ids);
-    next = page_ids(a, table, (t0 + 1) * L::KEYS + 32 * wave, x.len);
-  }
-  for (int st = t0; st < t1; ++st) {
-    const int stage = (st - t0) & 1;
-    // this stage has landed (for every wave: an LDS-DMA write is read only past
-    // a barrier), and every wave is done with the other half of the ring
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (st + 1 < t1) {
-      bad_next = bad_groups(a, next, (st + 1) * L::KEYS + 32 * wave, x.len) & 15u;
-      issue(st + 1, stage ^ 1, next);
-      next = page_ids(a, table, (st + 2) * L::KEYS + 32 * wave, x.len);
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j)  // the queries have arrived: no wait for them below, which would wait for K and V
+    asm volatile("" ::"v"(__builtin_bit_cast(u32x4, qf[j])));
+
+  KeyGroup at{};
+  uint64_t bad = 0;
+  for (int st = 0; st < stages; ++st) {
+    const int in = st & 15;  // of the 16 stages whose groups the lanes hold
+    if (in == 0) {
+      const int key = key_of(st + (lane >> 2)) + 8 * (lane & 3), end = key < k_end ? x.len : 0;
+      bool odd;
+      at = key_group(a, kb, vb, group_page(a, table, key, end), key, end, odd);
+      bad = __ballot(odd);
+      issue(st, 0, at);
     }
-    const int key0 = st * L::KEYS + 32 * wave;
-    const uint32_t bad_now = bad;
-    bad = bad_next;
-    if (key0 >= k_end) continue;
-    const char* Ks = lds + stage * L::STAGE + wave * L::WAVE_BYTES;
+    const bool newer = in < 15 && st + 1 < stages;
+    if (newer) issue(st + 1, 4 * in + 4, at);
+    wait_stage<2 * L::LOADS>(newer);
+    const int key0 = key_of(st);
+    const uint32_t bad_now = (uint32_t)(bad >> (4 * in)) & 15u;
+    const char* Ks = lds + wave * L::WAVE_BYTES + (st & 1) * L::STAGE;
     const char* Vs = Ks + L::HALF;
 
     f32x16 s;
@@ -174,6 +180,7 @@ __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
       for (int u = 0; u < 2; ++u) acc[db] = mfma32x32x16(vf[2 * db + u], p[u], acc[db]);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage's LDS reads are done: it may be loaded again
   }
 
   // ---- the waves' carriers meet in LDS: [wave][row][d] numerators, then

@@ -82,33 +82,40 @@ __global__ __launch_bounds__(NT, 2) void paged_tile_kernel(PagedArgs a, int tile
   const int wave_end = wave_live ? min(k_end, lim1 + 1) : 0;
   const int32_t* table = a.table + (int64_t)x.b * a.table_ld;
   const uint16_t *kb = a.k + (int64_t)h * a.k_h, *vb = a.v + (int64_t)h * a.v_h;
-  // a lane's 16 bytes of a load: row `sub` of the wave's rows of it.  Load i
-  // holds tile rows (4 i + wave) ROWS + sub, whose swizzles do not depend on i.
+  // a lane's 16 bytes of load i: tile row (4 i + wave) ROWS + sub, whose place
+  // in its 8 keys and whose swizzles do not depend on i
   const int sub = lane / AttnRow<D>::CH, cp = lane % AttnRow<D>::CH, trow = wave * L::ROWS + sub;
-  const int kc = cp ^ (trow & (AttnRow<D>::CH - 1) & 15), vc = cp ^ vswz<D>(trow);
-  const uint32_t koff = kc * 8 < a.d ? (uint32_t)(sub * (int)a.k_s + kc * 8) * 2u : 0x7ffffff0u;
-  const uint32_t voff = vc * 8 < a.d ? (uint32_t)(sub * (int)a.v_s + vc * 8) * 2u : 0x7ffffff0u;
+  const uint32_t koff = group_offset(a.k_s, trow & 7, cp ^ (trow & (AttnRow<D>::CH - 1) & 15), a.d);
+  const uint32_t voff = group_offset(a.v_s, trow & 7, cp ^ vswz<D>(trow), a.d);
   const uint32_t lds0 = lds_u32(lds) + wave * 1024;
-  auto issue = [&](int t, int stage, const PageIds& ids) {
+  // the lanes hold the places of eight tiles, lane 8 i + j keys 8 j on of the
+  // i-th; the page ids of the next eight are loaded one tile before they are used
+  KeyGroup at{};
+  uint64_t bads = 0;
+  int next_page = -1;
+  auto key_of = [&](int t) { return t * KVB + 8 * lane; };  // of the eight tiles from t on
+  auto places = [&](int t) {
+    bool odd;
+    at = key_group(a, kb, vb, next_page, key_of(t), x.len, odd);
+    bads = __ballot(odd);
+  };
+  auto issue = [&](int t, int stage) {
+    const int lane0 = 8 * ((t - t0) & 7);
 #pragma unroll
     for (int i = 0; i < L::LOADS; ++i) {
-      const int r0 = (4 * i + wave) * L::ROWS;  // of the tile
-      const int page = __builtin_amdgcn_readlane(ids.page, r0 >> 3);
-      const int slot = __builtin_amdgcn_readlane(ids.slot, r0 >> 3) + (r0 & 7);
-      const int rows = min(x.len - (t * KVB + r0), L::ROWS);
+      const int ln = lane0 + ((4 * i + wave) * L::ROWS >> 3);
       const uint32_t to = lds0 + stage * L::STAGE + i * 4096;
-      dma_buf(page_rsrc(kb, page, slot, a.k_p, a.k_s, rows, a.d, a.n_pages), koff, to);
-      dma_buf(page_rsrc(vb, page, slot, a.v_p, a.v_s, rows, a.d, a.n_pages), voff, to + L::TILE);
+      dma_buf(k_rsrc(at, ln), koff, to);
+      dma_buf(v_rsrc(at, ln), voff, to + L::TILE);
     }
   };
 
-  PageIds next{-1, 0};  // of the tile after the one in flight
-  uint32_t bad = 0, bad_next = 0;
+  uint32_t bad = 0, bad_next = 0;  // a bit for each 8 keys of the tile whose page is invalid
   if (t0 < t1) {
-    const PageIds ids = page_ids(a, table, t0 * KVB, x.len);
-    bad = bad_groups(a, ids, t0 * KVB, x.len);
-    issue(t0, 0, ids);
-    next = page_ids(a, table, (t0 + 1) * KVB, x.len);
+    next_page = group_page(a, table, key_of(t0), x.len);
+    places(t0);
+    bad = (uint32_t)bads & 0xffu;
+    issue(t0, 0);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   }
@@ -116,9 +123,11 @@ __global__ __launch_bounds__(NT, 2) void paged_tile_kernel(PagedArgs a, int tile
   auto tile = [&](int t, auto stage_tag) {
     constexpr int cur = decltype(stage_tag)::value;
     if (t + 1 < t1) {
-      bad_next = bad_groups(a, next, (t + 1) * KVB, x.len);
-      issue(t + 1, cur ^ 1, next);
-      next = page_ids(a, table, (t + 2) * KVB, x.len);
+      const int in = (t + 1 - t0) & 7;
+      if (in == 0) places(t + 1);
+      bad_next = (uint32_t)(bads >> (8 * in)) & 0xffu;
+      issue(t + 1, cur ^ 1);
+      if (in == 6) next_page = group_page(a, table, key_of(t + 3), x.len);
     }
     const char* Ks = lds + cur * L::STAGE;
     const char* Vs = Ks + L::TILE;
