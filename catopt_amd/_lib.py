@@ -105,19 +105,19 @@ SIGNATURES: dict[str, tuple] = {
     "catopt_hip_silu_mul": (_i32, [_i32, _i64, _p, _p, _p, _p]),
     "catopt_hip_qk_norm_rope": (
         _i32,
-        [_i32, _i64, _i64, _i64, _i64, _i64, _i32, _p, _p, _p, _p, _p, _f32, _p, _p, _i64, _i64, _p, _p, _p, _p, _pi64,
+        [_i32, _i64, _i64, _i64, _i64, _i64, _i32, _p, _p, _p, _p, _p, _f32, _p, _p, _i64, _i64, _p, _p, _p, _p, _p,
          _p, _i64, _i64, _p],
     ),
     "catopt_hip_paged_attn_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "catopt_hip_paged_attn_fwd": (
         _i32,
         [_i32, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _f32, _i32, _i32, _p, _p,
-         _p, _p, _p, _pi64, _p, _i64, _p],
+         _p, _p, _p, _p, _p, _i64, _p],
     ),
     "catopt_hip_paged_evict": (
         _i32,
         [_i32, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64,
-         _i64, _p, _p, _p, _pi64, _p],
+         _i64, _p, _p, _p, _p, _p],
     ),
 }
 

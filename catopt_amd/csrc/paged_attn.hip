@@ -66,10 +66,7 @@ __global__ __launch_bounds__(256) void paged_combine(PagedArgs a) {
     *reinterpret_cast<u32x2*>(a.o + (int64_t)n * a.o_t + (int64_t)hq * a.o_h + 4 * tid) =
         u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
   }
-  if (tid == 0) {
-    if (a.m_out) a.m_out[row] = mx * a.scale;
-    if (a.l_out) a.l_out[row] = lt;
-  }
+  if (tid == 0) row_stats(a, row, mx, lt);
 }
 
 struct Plan {
@@ -86,9 +83,11 @@ struct Plan {
 //
 // Ranges: few-row calls read K and V at the rate of HBM, so their ranges only
 // have to fill the CUs and even out the sequences: at most 64 to a tile and
-// 16384 workgroups in all (those behind a sequence's keys end at once), each
-// of 256 keys at least, or of 128 where the table's reach gives fewer than 512
-// such ranges.  Tiles of 128 rows are split only where they are fewer than the
+// 16384 workgroups in all (those behind a sequence's keys end at once).  A range
+// is 256 keys at least; 128 where the table's reach is less than 256 for each
+// of the 512 workgroups that the CUs hold; 1024 where it is 4096 for each (a
+// step of 32 sequences of 300 to 16000 keys: 115 us, 124 with 256; at eight
+// sequences of 2000 to 12000 they are level).  Tiles of 128 rows are split only where they are fewer than the
 // 512 workgroups that the CUs hold, into ranges of 256 keys at least.
 Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t cap, bool weights) {
   Plan p{};
@@ -97,7 +96,8 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t c
   p.tiles = paged_tiles(N, G, B, p.few ? kFewRows : kTileRows);
   const int64_t groups = p.tiles * Hkv;
   int64_t s = p.few ? 16384 / groups : 512 / groups;
-  p.min_keys = p.few && groups * cap < 512 * 256 ? 128 : 256;
+  const int64_t per_slot = p.few ? groups * cap / 512 : 256;
+  p.min_keys = per_slot >= 4096 ? 1024 : per_slot >= 256 ? 256 : 128;
   const int64_t most = (cap + p.min_keys - 1) / p.min_keys;
   if (s > kMaxSplits) s = kMaxSplits;
   if (s > most) s = most;
@@ -105,7 +105,7 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t c
   const int64_t rows = N * Hq;
   p.part_floats = p.splits > 1 ? ((2 * rows * p.splits + 3) & ~(int64_t)3) + rows * p.splits * D : 0;
   if (weights) {
-    p.stat_floats = (2 * rows + 3) & ~(int64_t)3;
+    p.stat_floats = (rows + 3) & ~(int64_t)3;
     if (p.few && rows * cap <= (1LL << 28)) {
       p.score_floats = rows * cap;
     } else {
@@ -193,9 +193,8 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   a.splits = p.splits, a.min_keys = p.min_keys;
   a.part = ws;
   ws += p.part_floats;
-  if (weights_out) {  // the weights need every row's statistics
-    if (!a.m_out) a.m_out = ws;
-    if (!a.l_out) a.l_out = ws + N * Hq;
+  if (weights_out) {
+    a.row_log = ws;
     ws += p.stat_floats;
     a.scores = p.score_floats ? ws : nullptr;
     ws += p.score_floats;

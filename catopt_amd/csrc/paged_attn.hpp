@@ -16,6 +16,7 @@ struct PagedArgs {
   const int32_t *table, *lens, *starts;
   int64_t table_ld, n_pages, N;
   float *m_out, *l_out;  // [N, Hq], optional
+  float* row_log;        // [N, Hq] m + log l of the row in log2 units, +inf where it sees no key; for the weights
   float* part;           // split keys' carriers: [row][split] (m, l), then [row][split][D]; row = n Hq + hq
   float* scores;         // [row][cap] q . k of the keys that the row's tile sees, -inf where masked; optional
   const float* w_in;
@@ -88,6 +89,13 @@ __device__ __forceinline__ float move_factor(float from, float to, float c) {
 __device__ __forceinline__ float finish(float x, float l, int normalize) {
   if (l == 0.f) return normalize == 2 ? 0.f : __builtin_nanf("");
   return x * (1.0f / l);
+}
+
+// A finished row's statistics: max m (units of q . k) and sum l.
+__device__ __forceinline__ void row_stats(const PagedArgs& a, int64_t i, float m, float l) {
+  if (a.m_out) a.m_out[i] = m * a.scale;
+  if (a.l_out) a.l_out[i] = l;
+  if (a.row_log) a.row_log[i] = l == 0.f ? __builtin_inff() : m * (a.scale * kLog2e) + __builtin_amdgcn_logf(l);
 }
 
 // Where 8 keys (a lane's) lie: pages hold a multiple of 8 keys, so the rows of 8

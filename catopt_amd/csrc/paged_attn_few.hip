@@ -231,10 +231,7 @@ __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = finish(y[e], lt, a.normalize);
       if (d < a.d) *reinterpret_cast<u32x2*>(orow + d) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-      if (d == 0) {
-        if (a.m_out) a.m_out[i] = mx * a.scale;
-        if (a.l_out) a.l_out[i] = lt;
-      }
+      if (d == 0) row_stats(a, i, mx, lt);
     }
   }
 }

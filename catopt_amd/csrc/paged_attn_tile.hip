@@ -286,10 +286,7 @@ __global__ __launch_bounds__(NT, 2) void paged_tile_kernel(PagedArgs a, int tile
                   pack_bf16x2(finish(acc[db][4 * rg + 2], l_sum, a.normalize), finish(acc[db][4 * rg + 3], l_sum, a.normalize))};
     }
   }
-  if (g == 0) {
-    if (a.m_out) a.m_out[i] = m_true * a.scale;
-    if (a.l_out) a.l_out[i] = l_sum * fix;
-  }
+  if (g == 0) row_stats(a, i, m_true, l_sum * fix);
 }
 
 template <int D>

@@ -1,15 +1,16 @@
 // Every cached key's attention weight, summed over the new tokens and the
 // query heads of its key head:
 //   w[j] = sum_rows exp(s_rj - m_r) / l_r = sum_rows exp2(q_r . k_j c - o_r),
-//   c = scale log2 e,  o_r = m_r log2 e + log2 l_r  (m, l: the finished rows')
+//   c = scale log2 e,  o_r = m_r log2 e + log2 l_r  (PagedArgs::row_log)
 // on top of the weight so far (nothing for the new tokens' own keys).
 //
 // Few rows: the attention kernel has stored its products (4 bytes a row and
 // key, against 4 d bytes for K and V), and one thread adds four keys' rows.
 // Many rows: the products are formed again, half of the attention's.  A
-// workgroup keeps 128 keys in registers, 32 per wave, and streams the rows by
-// 32 through LDS; the score accumulator's columns are rows, so each lane adds
-// its rows for 16 keys and the lanes meet once at the end.  The exponentials
+// workgroup keeps 256 keys in registers, 64 per wave, and streams the rows by
+// 32 through LDS, each fragment of them feeding two MFMAs; the score
+// accumulator's columns are rows, so each lane adds its rows for 32 keys and
+// the lanes meet once at the end.  The exponentials
 // bound it.  Where the keys leave CUs idle the rows are split over workgroups
 // and the parts added in their order by another launch.
 #include "paged_attn.hpp"
@@ -18,12 +19,6 @@ namespace catopt {
 namespace {
 
 constexpr int NT = 256;
-
-// o_r of a row, +inf where it sees nothing (its terms are then 0)
-__device__ __forceinline__ float row_offset(const PagedArgs& a, int64_t i) {
-  const float m = a.m_out[i], l = a.l_out[i];
-  return l == 0.f ? __builtin_inff() : m * kLog2e + __builtin_amdgcn_logf(l);
-}
 
 __device__ __forceinline__ void add_weight(const PagedArgs& a, int b, int h, int key, int old, float w) {
   if (a.w_in && key < old) w += a.w_in[b * a.wi_b + h * a.wi_h + key];
@@ -46,7 +41,7 @@ __global__ __launch_bounds__(NT) void weights_from_scores(PagedArgs a, int block
     for (int g = 0; g < a.G; ++g) {
       const int64_t i = (int64_t)(row0 + tok) * a.Hq + h * a.G + g;
       const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + i * a.cap + key);
-      const float o = row_offset(a, i);
+      const float o = a.row_log[i];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -o));
@@ -59,11 +54,13 @@ __global__ __launch_bounds__(NT) void weights_from_scores(PagedArgs a, int block
     if (key + e < len) add_weight(a, b, h, key + e, old, w[e]);
 }
 
-constexpr int kKeys = 128;  // of a workgroup
+constexpr int KB = 2;            // blocks of 32 keys per wave
+constexpr int kKeys = 128 * KB;  // of a workgroup
+constexpr int RT = 1;            // blocks of 32 rows per step
 
 template <int D>
 __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks, int parts, float* part) {
-  __shared__ __attribute__((aligned(16))) char lds[2][32 * D * 2];
+  __shared__ __attribute__((aligned(16))) char lds[2][32 * RT * D * 2];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int u = blockIdx.x;
@@ -77,49 +74,82 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks
   const int len = min(max(a.lens[b], 0), a.cap);
   if (blk * kKeys >= len) return;
   const int old = len - nq, off = a.causal ? old : 0x3fffffff;
-  const int key0 = blk * kKeys + 32 * wave, key = key0 + l32;
+  const int key0 = blk * kKeys + 32 * KB * wave;
   const float c = a.scale * kLog2e;
 
-  bf16x8 kf[D / 16];
-  bool valid = key < len;
-  {
+  bf16x8 kf[KB][D / 16];
+  uint64_t ok[KB];  // keys whose page is one
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    const int key = key0 + 32 * kb + l32;
+    bool valid = key < len;
     const uint32_t tp = a.page.div(valid ? key : 0);
     const int64_t page = valid ? a.table[(int64_t)b * a.table_ld + tp] : -1;
     valid = page >= 0 && page < a.n_pages;
-    const uint16_t* k = a.k + (valid ? page * a.k_p + h * a.k_h + (int64_t)(key - tp * a.page.d) * a.k_s : 0);
+    const uint16_t* k = a.k + (valid ? page * a.k_p + h * a.k_h + (int64_t)(key - (int)(tp * a.page.d)) * a.k_s : 0);
 #pragma unroll
     for (int j = 0; j < D / 16; ++j) {
       u32x4 w = u32x4{0, 0, 0, 0};
       if (valid && 16 * j + 8 * g < a.d) w = *reinterpret_cast<const u32x4*>(k + 16 * j + 8 * g);
-      kf[j] = __builtin_bit_cast(bf16x8, w);
+      kf[kb][j] = __builtin_bit_cast(bf16x8, w);
     }
+    ok[kb] = __ballot(valid);
   }
 
-  // tiles of 32 rows from the first that sees the block's first key; this part's share
+  // steps of 32 RT rows from the first that sees the block's first key; this part's share
   const int rows = nq * a.G, tok0 = max(blk * kKeys - off, 0);
-  const int ta = (int)min((int64_t)tok0 * a.G, (int64_t)rows) / 32, tb = (rows + 31) / 32;
+  const int ta = (int)min((int64_t)tok0 * a.G, (int64_t)rows) / (32 * RT), tb = (rows + 32 * RT - 1) / (32 * RT);
   const int t0 = ta + (int)((int64_t)(tb - ta) * pt / parts), t1 = ta + (int)((int64_t)(tb - ta) * (pt + 1) / parts);
 
-  constexpr int CH = AttnRow<D>::CH, LD = 32 * CH / NT;  // 16-byte pieces of a tile per thread
-  static_assert(LD >= 1 && LD <= 2, "a tile is one or two pieces per thread");
-  u32x4 qr[2];
-  float o_next = __builtin_inff();
-  auto fetch = [&](int t) {
+  constexpr int CH = AttnRow<D>::CH, LD = 32 * RT * CH / NT;  // 16-byte pieces of a step per thread
+  static_assert(LD >= 1 && LD <= 4, "the pieces' registers");
+  u32x4 qr[4];
+  float o_next[RT];
+  // Row r of the sequence is token r / G, head r % G.  The rows that a lane
+  // reads advance by 32 RT a step, so their tokens and heads, and with them the
+  // offsets of their queries and offsets o, advance by constants and a carry.
+  struct Walk {
+    int r, g;
+    int64_t q, o;
+  };
+  const int step_t = 32 * RT / a.G, step_g = 32 * RT - step_t * a.G;
+  const int64_t step_q = step_t * a.q_t + step_g * a.q_h, wrap_q = a.q_t - a.G * a.q_h;
+  const int64_t step_o = (int64_t)step_t * a.Hq + step_g, wrap_o = a.Hq - a.G;
+  auto walk_from = [&](int r) {
+    const int tok = (int)a.group.div(r), gr = r - tok * a.G;
+    return Walk{r, gr, (int64_t)(row0 + tok) * a.q_t + (int64_t)(h * a.G + gr) * a.q_h,
+                (int64_t)(row0 + tok) * a.Hq + h * a.G + gr};
+  };
+  auto advance = [&](Walk& x, bool queries) {
+    x.r += 32 * RT;
+    x.g += step_g;
+    const bool wrap = x.g >= a.G;
+    x.g -= wrap ? a.G : 0;
+    if (queries)
+      x.q += step_q + (wrap ? wrap_q : 0);
+    else
+      x.o += step_o + (wrap ? wrap_o : 0);
+  };
+  Walk wq[4], wo[RT];
+#pragma unroll
+  for (int i = 0; i < LD; ++i) {
+    wq[i] = walk_from(32 * RT * t0 + (i * NT + tid) / CH);
+    wq[i].q += (tid % CH) * 8;
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) wo[rt] = walk_from(32 * (RT * t0 + rt) + l32);
+  const bool column = (tid % CH) * 8 < a.d;
+  auto fetch = [&]() {
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
-      const int piece = i * NT + tid, r = 32 * t + piece / CH, ch = piece % CH;
       qr[i] = u32x4{0, 0, 0, 0};
-      if (r < rows && ch * 8 < a.d) {
-        const int tok = (int)a.group.div(r);
-        qr[i] = *reinterpret_cast<const u32x4*>(a.q + (int64_t)(row0 + tok) * a.q_t +
-                                                (int64_t)(h * a.G + r - tok * a.G) * a.q_h + ch * 8);
-      }
+      if (wq[i].r < rows && column) qr[i] = *reinterpret_cast<const u32x4*>(a.q + wq[i].q);
+      advance(wq[i], true);
     }
-    const int r = 32 * t + l32;
-    o_next = __builtin_inff();
-    if (r < rows) {
-      const int tok = (int)a.group.div(r);
-      o_next = row_offset(a, (int64_t)(row0 + tok) * a.Hq + h * a.G + r - tok * a.G);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      o_next[rt] = wo[rt].r < rows ? a.row_log[wo[rt].o] : __builtin_inff();
+      advance(wo[rt], false);
     }
   };
   auto stage = [&](int buf) {
@@ -130,59 +160,80 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks
     }
   };
 
-  float w[16];
+  float w[KB][16];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) w[r] = 0.f;
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[kb][r] = 0.f;
   if (t0 < t1) {
-    fetch(t0);
+    fetch();
     stage(0);
   }
+  // Sᵀ of the wave's keys and 32 staged rows, and the rows' terms of it
+  auto qk = [&](int buf, int rt, f32x16* s) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      const bf16x8 q = *reinterpret_cast<const bf16x8*>(lds[buf] + tile_off<D>(32 * rt + l32, 2 * j + g));
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) s[kb] = mfma32x32x16(kf[kb][j], q, s[kb]);
+    }
+  };
+  auto mask = [&](int r0, f32x16* s) {
+    const int lim = off + (int)a.group.div(r0 + l32);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = key0 + 32 * kb + acc_row(r, g) <= lim ? s[kb][r] : kNegInf;
+  };
+  auto add = [&](const f32x16* s, float o) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w[kb][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], c, -o));
+  };
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
-    const float o = o_next;
-    __syncthreads();  // the tile is staged, and the other buffer is free
-    if (t + 1 < t1) fetch(t + 1);
-    const int first = off + (int)a.group.div(32 * t);                          // last key of the tile's first row
-    const int last = off + (int)a.group.div(min(32 * t + 31, rows - 1));       // and of its last row
+    float o[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) o[rt] = o_next[rt];
+    __syncthreads();  // the step is staged, and the other buffer is free
+    if (t + 1 < t1) fetch();
+    const int r0 = 32 * RT * t;
+    const int first = off + (int)a.group.div(r0);                          // last key of the step's first row
+    const int last = off + (int)a.group.div(min(r0 + 32 * RT, rows) - 1);  // and of its last row
     if (key0 <= last && key0 < len) {
-      f32x16 s;
+      const bool masked = key0 + 32 * KB - 1 > first;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j)
-        s = mfma32x32x16(kf[j], *reinterpret_cast<const bf16x8*>(lds[buf] + tile_off<D>(l32, 2 * j + g)), s);
-      if (key0 + 31 > first) {
-        const int lim = off + (int)a.group.div(32 * t + l32);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -o));
-          w[r] += key0 + acc_row(r, g) <= lim ? x : 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) w[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -o));
+      for (int rt = 0; rt < RT; ++rt) {
+        f32x16 s[KB];
+        qk(buf, rt, s);
+        if (masked) mask(r0 + 32 * rt, s);
+        add(s, o[rt]);
       }
     }
     if (t + 1 < t1) stage(buf ^ 1);
   }
+  // lane r of each half takes the key of accumulator register r
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
+  for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) w[r] += __shfl_xor(w[r], x, 64);
-  }
-  // lane r of each half takes the key of accumulator register r, and whether
-  // that key's page is one
-  const uint64_t ok = __ballot(valid);
+    for (int r = 0; r < 16; ++r) {
+      float y = w[kb][r];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    if (l32 == r) {
-      const int in = acc_row(r, g), j = key0 + in;
-      if (j < len) {
-        const float x = (ok >> in) & 1 ? w[r] : 0.f;
-        if (parts > 1)
-          part[((int64_t)(pt * a.B + b) * a.Hkv + h) * a.cap + j] = x;
-        else
-          add_weight(a, b, h, j, old, x);
+      for (int x = 16; x > 0; x >>= 1) y += __shfl_xor(y, x, 64);
+      if (l32 == r) {
+        const int in = acc_row(r, g), j = key0 + 32 * kb + in;
+        if (j < len) {
+          const float x = (ok[kb] >> in) & 1 ? y : 0.f;
+          if (parts > 1)
+            part[((int64_t)(pt * a.B + b) * a.Hkv + h) * a.cap + j] = x;
+          else
+            add_weight(a, b, h, j, old, x);
+        }
       }
     }
   }
@@ -202,13 +253,13 @@ __global__ __launch_bounds__(NT) void weights_add_parts(PagedArgs a, int blocks,
 
 }  // namespace
 
-// Parts of the rows: as many as give four workgroups to a CU, were every
+// Parts of the rows: as many as give eight workgroups to a CU, were every
 // sequence as long as its table.
 int paged_weight_parts(int64_t B, int64_t Hkv, int64_t cap, int64_t N, int64_t G) {
   const int64_t groups = B * Hkv * ((cap + kKeys - 1) / kKeys);
-  int64_t n = groups > 0 ? 1024 / groups : 1;
-  const int64_t tiles = N * G / 32;
-  if (n > tiles / 8) n = tiles / 8;  // of the call: a part has work for a few tiles at least
+  int64_t n = groups > 0 ? 2048 / groups : 1;
+  const int64_t steps = N * G / (32 * RT);
+  if (n > steps / 4) n = steps / 4;  // of the call: a part has a few steps at least
   return n < 1 ? 1 : n > 16 ? 16 : (int)n;
 }
 

@@ -29,13 +29,14 @@ reach, keys of an invalid page count as masked, and a write to one is dropped.
 
 from __future__ import annotations
 
-import ctypes as C
+import functools
 import math
+import struct
 
 import torch
 
 from . import _lib as L
-from .kernels import _DT, _need_device, _ptr, _stream, _workspace
+from .kernels import _DT, _need_device, _stream
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_append", "paged_attention", "paged_evict", "PAGED_ATTENTION_MAX_HEAD_DIM",
            "QK_NORM_ROPE_MAX_HEAD_DIM"]
@@ -43,50 +44,54 @@ __all__ = ["qk_norm_rope", "qk_norm_rope_append", "paged_attention", "paged_evic
 PAGED_ATTENTION_MAX_HEAD_DIM = 128
 QK_NORM_ROPE_MAX_HEAD_DIM = 256
 
-_I12, _I14, _I16 = C.c_int64 * 12, C.c_int64 * 14, C.c_int64 * 16
+# host arrays of strides, as the C entries take them
+_S12, _S14, _S16 = (struct.Struct(f"{n}q").pack for n in (12, 14, 16))
 
 
-class _on:
-    """The operands' device as the current one for a call's launches."""
-
-    __slots__ = ("dev", "old")
-
-    def __init__(self, dev: int) -> None:
-        self.dev = dev
-
-    def __enter__(self) -> None:
-        self.old = torch._C._cuda_getDevice()
-        if self.old != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc) -> None:
-        if self.old != self.dev:
-            torch.cuda.set_device(self.old)
+def _device(*ts: torch.Tensor | None) -> int:
+    """The device index that all operands share; raises as ``kernels`` does where they do not."""
+    try:
+        dev = ts[0].get_device()
+        for t in ts:
+            if t is not None and t.get_device() != dev:
+                break
+        else:
+            if dev >= 0:
+                return dev
+    except AttributeError:
+        pass
+    return _need_device(*ts)
 
 
-def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
-    """``(N, H, d)`` with a contiguous last axis, rows readable in 16-byte pieces."""
+def _launch(dev: int, fn, *args) -> int:
+    """``fn(*args)`` with the operands' device as the current one."""
+    if torch._C._cuda_getDevice() == dev:
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
+
+
+def _heads(name: str, t: torch.Tensor) -> tuple[torch.Tensor, torch.Size, tuple]:
+    """``(N, H, d)`` with a contiguous last axis, rows readable in 16-byte pieces; its shape and strides."""
     if t.dim() != 3:
         raise ValueError(f"{name} is (tokens, heads, head dim), got {tuple(t.shape)}")
-    a, b, c = t.stride()
+    s = t.stride()
     step = 16 // t.element_size()
-    if c != 1 or a % step or b % step or t.data_ptr() % 16:
+    if s[2] != 1 or s[0] % step or s[1] % step or t.data_ptr() % 16:
         t = t.contiguous()
-    return t
+        s = t.stride()
+    return t, t.shape, s
 
 
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, what: str = "") -> torch.Size:
-    """The shape of a cache's two page tensors, checked: they are used in place, so nothing is copied to fit."""
-    shape = k_pages.shape
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, what: str = "") -> tuple[torch.Size, tuple, tuple]:
+    """The shape and strides of a cache's two page tensors, which are used in place: nothing is copied to fit."""
+    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
     if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype:
         raise ValueError(f"the {what}pages are two tensors (n_pages, heads, page size, head dim) of one type, got "
                          f"{tuple(shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
-    step = 16 // k_pages.element_size()
-    for t in (k_pages, v_pages):
-        a, b, c, e = t.stride()
-        if e != 1 or a % step or b % step or c % step or t.data_ptr() % 16:
-            raise ValueError(f"{what}pages need a contiguous head dim and 16-byte aligned rows, got strides {t.stride()}")
-    return shape
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError(f"the {what}pages need a contiguous head dim, got strides {ks} and {vs}")
+    return shape, ks, vs
 
 
 def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, n: int | None = None) -> torch.Tensor:
@@ -104,7 +109,7 @@ def _table(name: str, t: torch.Tensor, B: int) -> torch.Tensor:
 def _check(fn: str, status: int) -> None:
     """A refusal of the library's own checks (what overlaps what) as the argument error that it is."""
     if status == L.E_INVAL:
-        raise ValueError(f"{fn}: an output overlaps another operand or itself, or a stride does not fit")
+        raise ValueError(f"{fn}: an output overlaps another operand or itself, or rows are not 16-byte aligned")
     if status == L.E_UNSUPPORTED:
         raise NotImplementedError(f"{fn}: the call is beyond what one launch takes")
     L.check(fn, status)
@@ -112,57 +117,62 @@ def _check(fn: str, status: int) -> None:
 
 def _norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleaved, k_pages, v_pages, slots):
     append = slots is not None
-    dev = _need_device(q, k, v, cos, sin, positions, q_weight, k_weight, k_pages, v_pages, slots)
+    dev = _device(q, k, v, cos, sin, positions, q_weight, k_weight, k_pages, v_pages, slots)
     lib = L.load()
     dt = _DT.get(q.dtype)
     if dt is None:
         raise NotImplementedError(f"qk_norm_rope runs on fp32 and bf16 operands, got {q.dtype}")
-    q, k = _heads("q", q), _heads("k", k)
-    N, Hq, d = q.shape
-    Hkv = k.shape[1]
-    if k.dtype != q.dtype or k.shape[0] != N or k.shape[2] != d:
+    q, (N, Hq, d), qs = _heads("q", q)
+    k, (kn, Hkv, kd), ks = _heads("k", k)
+    if k.dtype != q.dtype or kn != N or kd != d:
         raise ValueError(f"q and k share tokens, head dim and type: {tuple(q.shape)} {q.dtype}, "
                          f"{tuple(k.shape)} {k.dtype}")
     if not 1 <= d <= QK_NORM_ROPE_MAX_HEAD_DIM:
         raise NotImplementedError(f"qk_norm_rope takes head dims up to {QK_NORM_ROPE_MAX_HEAD_DIM}, got {d}")
     if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError("cos and sin are fp32 tables (positions, rotated dims / 2) of one shape")
-    rot = 2 * cos.shape[1]
+    n_pos, half = cos.shape
+    rot = 2 * half
     if rot > d:
         raise ValueError(f"the tables rotate {rot} dims of a head of {d}")
-    if rot and (cos.stride(1) != 1 or sin.stride() != cos.stride()):
+    if rot and (cos.stride() != sin.stride() or cos.stride(1) != 1):
         cos, sin = cos.contiguous(), sin.contiguous()
-    for w in (q_weight, k_weight):
-        if w is not None and (w.dtype != q.dtype or w.numel() != d):
-            raise ValueError("a norm weight holds one value of q's type for each head dim")
-    q_weight = None if q_weight is None else q_weight.contiguous()
-    k_weight = None if k_weight is None else k_weight.contiguous()
+    qw = kw = vp = slots_p = None
+    if q_weight is not None:
+        q_weight = _norm_weight(q_weight, q, d)
+        qw = q_weight.data_ptr()
+    if k_weight is not None:
+        k_weight = _norm_weight(k_weight, q, d)
+        kw = k_weight.data_ptr()
     positions = _vector("positions", positions, torch.int64, N)
-    q_out = torch.empty((N, Hq, d), dtype=q.dtype, device=q.device)
+    q_out = q.new_empty((N, Hq, d))
     n_pages = page = 0
-    qs, ks = q.stride(), k.stride()
     if append:
-        v = _heads("v", v)
-        if v.shape != k.shape or v.dtype != q.dtype:
+        v, vshape, vs = _heads("v", v)
+        if vshape != k.shape or v.dtype != q.dtype:
             raise ValueError(f"v has k's shape and type: {tuple(v.shape)} {v.dtype}, {tuple(k.shape)} {k.dtype}")
-        n_pages, ph, page, pd = _pages(k_pages, v_pages)
+        (n_pages, ph, page, pd), ko, vo = _pages(k_pages, v_pages)
         if ph != Hkv or pd != d or k_pages.dtype != q.dtype:
             raise ValueError(f"the pages hold {ph} heads of {pd} {k_pages.dtype}, k has {Hkv} of {d} {q.dtype}")
         slots = _vector("slots", slots, torch.int64, N)
-        k_out, v_out = k_pages, v_pages
-        vs, ko, vo = v.stride(), k_pages.stride(), v_pages.stride()
-        strides = _I12(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], ko[0], ko[1], ko[2], vo[0], vo[1], vo[2])
+        slots_p, vp = slots.data_ptr(), v.data_ptr()
+        k_out, v_out = k_pages, v_pages.data_ptr()
+        strides = _S12(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], ko[0], ko[1], ko[2], vo[0], vo[1], vo[2])
     else:
-        k_out = torch.empty((N, Hkv, d), dtype=q.dtype, device=q.device)
-        v_out = None
-        strides = _I12(qs[0], qs[1], ks[0], ks[1])
-    with _on(dev):
-        st = lib.catopt_hip_qk_norm_rope(dt, N, Hq, Hkv, d, rot, int(bool(interleaved)), _ptr(q), _ptr(k), _ptr(v),
-                                         _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(cos), _ptr(sin),
-                                         cos.shape[0], cos.stride(0) if rot else 0, _ptr(positions), _ptr(q_out),
-                                         _ptr(k_out), _ptr(v_out), strides, _ptr(slots), n_pages, page, _stream(q))
+        k_out, v_out = q.new_empty((N, Hkv, d)), None
+        strides = _S12(qs[0], qs[1], ks[0], ks[1], 0, 0, 0, 0, 0, 0, 0, 0)
+    st = _launch(dev, lib.catopt_hip_qk_norm_rope, dt, N, Hq, Hkv, d, rot, 1 if interleaved else 0, q.data_ptr(),
+                 k.data_ptr(), vp, qw, kw, eps, cos.data_ptr(), sin.data_ptr(), n_pos, cos.stride(0) if rot else 0,
+                 positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), v_out, strides, slots_p, n_pages, page,
+                 _stream(q))
     _check("qk_norm_rope", st)
     return q_out, k_out
+
+
+def _norm_weight(w: torch.Tensor, x: torch.Tensor, d: int) -> torch.Tensor:
+    if w.dtype != x.dtype or w.numel() != d:
+        raise ValueError(f"a norm weight holds one value of q's type for each head dim, got {tuple(w.shape)} {w.dtype}")
+    return w.contiguous()
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
@@ -194,6 +204,14 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: 
     if slots is None or k_pages is None or v_pages is None or v is None:
         raise TypeError("qk_norm_rope_append needs v, k_pages, v_pages and slots")
     return _norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleaved, k_pages, v_pages, slots)[0]
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_workspace(B: int, N: int, Hq: int, Hkv: int, d: int, n_table: int, page: int, weights: int) -> int:
+    n = L.load().catopt_hip_paged_attn_workspace_bytes(B, N, Hq, Hkv, d, n_table, page, weights)
+    if n < 0:
+        raise NotImplementedError("paged attention: the call is beyond what one launch takes")
+    return n
 
 
 def _weight_rows(name: str, w: torch.Tensor, B: int, H: int, width: int) -> tuple[int, int]:
@@ -234,13 +252,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``weights``."""
     if empty_rows not in ("nan", "zero"):
         raise ValueError(f"empty_rows is 'nan' or 'zero', got {empty_rows!r}")
-    dev = _need_device(q, k_pages, v_pages, block_table, kv_lens, q_starts, weights, weights_out, out)
+    dev = _device(q, k_pages, v_pages, block_table, kv_lens, q_starts, weights, weights_out, out)
     lib = L.load()
     if q.dtype != torch.bfloat16 or k_pages.dtype != q.dtype:
         raise NotImplementedError(f"paged attention runs on bf16 operands, got {q.dtype} and {k_pages.dtype} pages")
-    q = _heads("q", q)
-    N, Hq, d = q.shape
-    n_pages, Hkv, page, pd = _pages(k_pages, v_pages)
+    q, (N, Hq, d), qs = _heads("q", q)
+    (n_pages, Hkv, page, pd), ks, vs = _pages(k_pages, v_pages)
     if pd != d or Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"q has {Hq} heads of {d}, the pages {Hkv} heads of {pd}: the head dims agree and the query "
                          "heads are a multiple of the key heads")
@@ -258,40 +275,36 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     table = _table("block_table", block_table, B)
     n_table = table.shape[1]
     if out is None:
-        o = torch.empty((N, Hq, d), dtype=q.dtype, device=q.device)
+        o = q.new_empty((N, Hq, d))
     else:
         o = out
         if o.shape != q.shape or o.dtype != q.dtype:
             raise ValueError(f"out has q's shape and type, got {tuple(o.shape)} {o.dtype}")
     so = o.stride()
-    if so[2] != 1 or so[0] % 8 or so[1] % 8 or o.data_ptr() % 16:
-        raise ValueError(f"out needs a contiguous head dim and 16-byte aligned rows, got strides {so}")
-    w_in = w_out = (0, 0)
+    if so[2] != 1:
+        raise ValueError(f"out needs a contiguous head dim, got strides {so}")
+    wi0 = wi1 = wo0 = wo1 = 0
+    wi = wo = m = l = mp = lp = ws = None
     if weights_out is not None:
-        w_out = _weight_rows("weights_out", weights_out, B, Hkv, n_table * page)
+        wo0, wo1 = _weight_rows("weights_out", weights_out, B, Hkv, n_table * page)
+        wo = weights_out.data_ptr()
         if weights is not None:
-            w_in = _weight_rows("weights", weights, B, Hkv, n_table * page)
+            wi0, wi1 = _weight_rows("weights", weights, B, Hkv, n_table * page)
+            wi = weights.data_ptr()
     elif weights is not None:
         raise ValueError("weights need a weights_out to go to")
-    m = l = None
     if return_ml:
-        m = torch.empty((N, Hq), dtype=torch.float32, device=q.device)
-        l = torch.empty((N, Hq), dtype=torch.float32, device=q.device)
+        m, l = (q.new_empty((N, Hq), dtype=torch.float32) for _ in range(2))
+        mp, lp = m.data_ptr(), l.data_ptr()
     if N and B:
-        ks, vs, qs = k_pages.stride(), v_pages.stride(), q.stride()
-        strides = _I14(qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], so[0], so[1], *w_in, *w_out)
-        with _on(dev):
-            wsb = lib.catopt_hip_paged_attn_workspace_bytes(B, N, Hq, Hkv, d, n_table, page,
-                                                            int(weights_out is not None))
-            if wsb < 0:
-                raise NotImplementedError("paged attention: the call is beyond what one launch takes")
-            ws = _workspace(wsb, q.device)
-            st = lib.catopt_hip_paged_attn_fwd(L.BF16, B, N, Hq, Hkv, d, q.data_ptr(), k_pages.data_ptr(),
-                                               v_pages.data_ptr(), n_pages, page, table.data_ptr(), table.stride(0),
-                                               n_table, kv_lens.data_ptr(), q_starts.data_ptr(), scale,
-                                               int(bool(causal)), 2 if empty_rows == "zero" else 1, o.data_ptr(),
-                                               _ptr(m), _ptr(l), _ptr(weights), _ptr(weights_out), strides, _ptr(ws),
-                                               wsb, _stream(q))
+        strides = _S14(qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], so[0], so[1], wi0, wi1, wo0, wo1)
+        wsb = _attn_workspace(B, N, Hq, Hkv, d, n_table, page, wo is not None)
+        if wsb:
+            ws = q.new_empty(wsb // 2)
+        st = _launch(dev, lib.catopt_hip_paged_attn_fwd, L.BF16, B, N, Hq, Hkv, d, q.data_ptr(), k_pages.data_ptr(),
+                     v_pages.data_ptr(), n_pages, page, table.data_ptr(), table.stride(0), n_table, kv_lens.data_ptr(),
+                     q_starts.data_ptr(), scale, 1 if causal else 0, 2 if empty_rows == "zero" else 1, o.data_ptr(),
+                     mp, lp, wi, wo, strides, None if ws is None else ws.data_ptr(), wsb, _stream(q))
         _check("paged_attention", st)
     return (o, m, l) if return_ml else o
 
@@ -320,16 +333,15 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     tensor whose entries behind the last kept key are 0."""
     if (k_out is None) != (v_out is None):
         raise ValueError("give both k_out and v_out, or neither")
-    dev = _need_device(k_pages, v_pages, block_table, kv_lens, weights, out_table, k_out, v_out, weights_out)
+    dev = _device(k_pages, v_pages, block_table, kv_lens, weights, out_table, k_out, v_out, weights_out)
     lib = L.load()
     dt = _DT.get(k_pages.dtype)
     if dt is None:
         raise NotImplementedError(f"eviction runs on fp32 and bf16 pages, got {k_pages.dtype}")
-    n_pages, Hkv, page, d = _pages(k_pages, v_pages)
-    own = k_out is None
-    k_to, v_to = (k_pages, v_pages) if own else (k_out, v_out)
-    n_out, ho, page_out, do = _pages(k_to, v_to, "output ")
-    if (ho, do) != (Hkv, d) or k_to.dtype != k_pages.dtype:
+    (n_pages, Hkv, page, d), ks, vs = _pages(k_pages, v_pages)
+    k_to, v_to = (k_pages, v_pages) if k_out is None else (k_out, v_out)
+    (n_out, ho, page_out, do), kt, vt = _pages(k_to, v_to, "output ")
+    if ho != Hkv or do != d or k_to.dtype != k_pages.dtype:
         raise ValueError(f"the output pages hold {ho} heads of {do} {k_to.dtype}, the cache {Hkv} of {d} {k_pages.dtype}")
     if d < 1 or Hkv < 1 or page < 1 or page_out < 1 or d * k_pages.element_size() % 16:
         raise NotImplementedError(f"eviction takes rows of a multiple of 16 bytes, got {d} of {k_pages.dtype}")
@@ -342,20 +354,18 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     n_table, n_to = table.shape[1], to.shape[1]
     if n_to * page_out < budget:
         raise ValueError(f"out_table reaches {n_to * page_out} keys, the budget is {budget}")
-    w_in = _weight_rows("weights", weights, B, Hkv, n_table * page)
+    wi0, wi1 = _weight_rows("weights", weights, B, Hkv, n_table * page)
     if weights_out is None:
         weights_out = torch.zeros((B, Hkv, budget), dtype=torch.float32, device=weights.device)
-    w_out = _weight_rows("weights_out", weights_out, B, Hkv, budget)
-    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=k_pages.device)
-    new_lens = torch.empty((B,), dtype=torch.int32, device=k_pages.device)
+    wo0, wo1 = _weight_rows("weights_out", weights_out, B, Hkv, budget)
+    kept = kv_lens.new_empty((B, Hkv, budget))
+    new_lens = kv_lens.new_empty((B,))
     if B:
-        a, b, c, e = k_pages.stride(), v_pages.stride(), k_to.stride(), v_to.stride()
-        strides = _I16(a[0], a[1], a[2], b[0], b[1], b[2], c[0], c[1], c[2], e[0], e[1], e[2], *w_in, *w_out)
-        with _on(dev):
-            st = lib.catopt_hip_paged_evict(dt, B, Hkv, d, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page,
-                                            _ptr(table), table.stride(0), n_table, kv_lens.data_ptr(),
-                                            weights.data_ptr(), budget, recent, k_to.data_ptr(), v_to.data_ptr(),
-                                            n_out, page_out, to.data_ptr(), to.stride(0), n_to, kept.data_ptr(),
-                                            new_lens.data_ptr(), weights_out.data_ptr(), strides, _stream(k_pages))
+        strides = _S16(ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kt[0], kt[1], kt[2], vt[0], vt[1], vt[2],
+                       wi0, wi1, wo0, wo1)
+        st = _launch(dev, lib.catopt_hip_paged_evict, dt, B, Hkv, d, k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
+                     page, table.data_ptr(), table.stride(0), n_table, kv_lens.data_ptr(), weights.data_ptr(), budget,
+                     recent, k_to.data_ptr(), v_to.data_ptr(), n_out, page_out, to.data_ptr(), to.stride(0), n_to,
+                     kept.data_ptr(), new_lens.data_ptr(), weights_out.data_ptr(), strides, _stream(k_pages))
         _check("paged_evict", st)
     return kept, new_lens, weights_out

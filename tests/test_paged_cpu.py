@@ -146,8 +146,9 @@ def test_host_tensors_are_refused():
 
 def test_layout_checks():
     u = torch.zeros((3, 4, 12))
-    assert P._heads("t", u[..., :7]).data_ptr() == u.data_ptr()  # rows of 48 bytes: read in place
-    assert P._heads("t", u[..., 1:8]).is_contiguous()  # misaligned: copied
+    assert P._heads("t", u[..., :7])[0].data_ptr() == u.data_ptr()  # rows of 48 bytes: read in place
+    t, shape, strides = P._heads("t", u[..., 1:8])
+    assert t.is_contiguous() and shape == (3, 4, 7) and strides == (28, 7, 1)  # misaligned: copied
     with pytest.raises(ValueError):
         P._heads("t", u[0])
     with pytest.raises(ValueError):

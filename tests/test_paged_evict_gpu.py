@@ -164,7 +164,7 @@ def test_refusals():
     bad(ValueError, wo=torch.zeros((1, 2, 31), device=DEV))
     bad(ValueError, wo=w[..., 8:])
     c12 = Cache([64], 2, 12, 16)
-    bad(ValueError, k=c12.k, v=c12.v, ko=c12.k, vo=c12.v)
+    bad(NotImplementedError, k=c12.k, v=c12.v, ko=c12.k, vo=c12.v)
     torch.cuda.synchronize()
 
 
