@@ -5,15 +5,15 @@
 namespace catopt {
 namespace {
 
-// One workgroup per row (token, query head): the carriers of its key ranges,
-// D / 4 threads to a range's numerators, so that 8 (D = 64: 16) ranges load at
-// once.  R: the rows of the tiles they were made with.
-template <int D, int R>
+// WAVES waves per row (token, query head): the carriers of its key ranges, D / 4
+// lanes to a range's numerators, so that 2 WAVES (D = 64: 4 WAVES) ranges load
+// at once.  R: the rows of the tiles they were made with.
+template <int D, int R, int WAVES>
 __global__ __launch_bounds__(256) void paged_combine(PagedArgs a) {
-  constexpr int TPR = D / 4, GROUPS = 256 / TPR;
-  __shared__ f32x4 sums[GROUPS][TPR];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t row = blockIdx.x;
+  constexpr int TPR = D / 4, GROUPS = 64 * WAVES / TPR;
+  const int lane = threadIdx.x & 63, tid = WAVES == 4 ? threadIdx.x : lane;
+  const int64_t row = WAVES == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.N * a.Hq) return;
   const int n = (int)(row / a.Hq), hq = (int)(row - (int64_t)n * a.Hq);
   int b = -1;
   for (int c0 = 0; c0 < a.B; c0 += 64) {  // the last sequence that starts at or before the token
@@ -38,13 +38,6 @@ __global__ __launch_bounds__(256) void paged_combine(PagedArgs a) {
   // lane s of every wave: range s (64 at most)
   const bool mine = lane < x.splits;
   const float ms = mine ? ml[2 * lane] : kNegInf, ls = mine ? ml[2 * lane + 1] : 0.f;
-  constexpr int STEPS = kMaxSplits / GROUPS;
-  f32x4 ys[STEPS];
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int s = i * GROUPS + tid / TPR;
-    ys[i] = s < x.splits ? *reinterpret_cast<const f32x4*>(num + (int64_t)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
-  }
   float mx = ms;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
@@ -53,14 +46,32 @@ __global__ __launch_bounds__(256) void paged_combine(PagedArgs a) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o, 64);
   f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 8;  // loads ahead of their additions
+  for (int s0 = 0; s0 < x.splits; s0 += U * GROUPS) {  // every lane stays: the factors come from lanes
+    f32x4 ys[U];
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) y += ys[i] * __shfl(f, i * GROUPS + tid / TPR, 64);
-  sums[tid / TPR][tid % TPR] = y;
-  __syncthreads();
+    for (int i = 0; i < U; ++i) {
+      const int s = s0 + i * GROUPS + tid / TPR;
+      ys[i] = s < x.splits ? *reinterpret_cast<const f32x4*>(num + (int64_t)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) y += ys[i] * __shfl(f, min(s0 + i * GROUPS + tid / TPR, 63), 64);
+  }
+  if constexpr (WAVES == 4) {
+    __shared__ f32x4 sums[GROUPS][TPR];
+    sums[tid / TPR][tid % TPR] = y;
+    __syncthreads();
+    if (tid < TPR) {
+#pragma unroll
+      for (int i = 1; i < GROUPS; ++i) y += sums[i][tid];
+    }
+  } else {
+#pragma unroll
+    for (int o = TPR; o < 64; o <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], o, 64);
+  }
   if (tid < TPR && 4 * tid < a.d) {
-    y = sums[0][tid];
-#pragma unroll
-    for (int i = 1; i < GROUPS; ++i) y += sums[i][tid];
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = finish(y[e], lt, a.normalize);
     *reinterpret_cast<u32x2*>(a.o + (int64_t)n * a.o_t + (int64_t)hq * a.o_h + 4 * tid) =
@@ -116,14 +127,17 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t c
   return p;
 }
 
-template <int R>
-int32_t combine(const PagedArgs& a, int D, hipStream_t s) {
-  const int64_t blocks = a.N * a.Hq;
+template <int D, int R>
+int32_t combine(const PagedArgs& a, hipStream_t s) {
+  // four waves a row where the rows alone do not fill the CUs
+  const int64_t rows = a.N * a.Hq;
+  const bool wide = rows < 2048;
+  const int64_t blocks = wide ? rows : (rows + 3) / 4;
   if (!grid_fits(blocks, 256)) return CATOPT_E_UNSUPPORTED;
-  if (D == 128)
-    paged_combine<128, R><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(a);
+  if (wide)
+    paged_combine<D, R, 4><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(a);
   else
-    paged_combine<64, R><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(a);
+    paged_combine<D, R, 1><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(a);
   CATOPT_LAUNCH_CHECK();
   return CATOPT_OK;
 }
@@ -202,7 +216,12 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int D = d <= 64 ? 64 : 128;
   int32_t r = p.few ? paged_few_launch(a, D, p.tiles, st) : paged_tile_launch(a, D, p.tiles, st);
-  if (r == CATOPT_OK && p.splits > 1) r = p.few ? combine<kFewRows>(a, D, st) : combine<kTileRows>(a, D, st);
+  if (r == CATOPT_OK && p.splits > 1) {
+    if (p.few)
+      r = D == 128 ? combine<128, kFewRows>(a, st) : combine<64, kFewRows>(a, st);
+    else
+      r = D == 128 ? combine<128, kTileRows>(a, st) : combine<64, kTileRows>(a, st);
+  }
   if (r == CATOPT_OK && weights_out) r = paged_weights_launch(a, D, p.parts, ws, st);
   return r;
 }

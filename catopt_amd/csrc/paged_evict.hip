@@ -48,15 +48,19 @@ __global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {
   if (h == 0 && tid == 0) a.new_lens[b] = m;
   const int steps = (n + NT - 1) / NT, first = wave * steps * 64;  // this wave's keys: `steps` of 64
 
-  uint32_t held[HELD ? kRegs : 1];
-  if (HELD) {
+  // ranks of the U steps from step i0 on (0 behind the old keys): the loads take
+  // a valid address whatever the step, so that none waits for another
+  auto load = [&](int i0, auto& r) {
+    constexpr int U = sizeof(r) / sizeof(r[0]);
+    float x[U];
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i) {
-      const int j = first + 64 * i + lane;
-      held[i] = i < steps && j < old ? rank_of(w[j]) : 0u;
-    }
-  }
-  // f(key, rank, whether the key is one of the old ones)
+    for (int i = 0; i < U; ++i) x[i] = old > 0 ? w[min(first + 64 * (i0 + i) + lane, old - 1)] : 0.f;
+#pragma unroll
+    for (int i = 0; i < U; ++i) r[i] = first + 64 * (i0 + i) + lane < old ? rank_of(x[i]) : 0u;
+  };
+  uint32_t held[HELD ? kRegs : 1];
+  if (HELD) load(0, held);
+  // f(key, rank) for every key of the wave
   auto sweep = [&](auto f) {
     if (HELD) {
 #pragma unroll
@@ -66,11 +70,7 @@ __global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {
       constexpr int U = 8;
       for (int i0 = 0; i0 < steps; i0 += U) {
         uint32_t r[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-          const int j = first + 64 * (i0 + i) + lane;
-          r[i] = i0 + i < steps && j < old ? rank_of(w[j]) : 0u;
-        }
+        load(i0, r);
 #pragma unroll
         for (int i = 0; i < U; ++i)
           if (i0 + i < steps) f(first + 64 * (i0 + i) + lane, r[i]);
