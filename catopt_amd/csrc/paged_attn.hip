@@ -1,87 +1,11 @@
-// Paged attention: the choice of kernel, its workspace, and the combination of
-// split keys.
+// Paged attention: the choice of kernels and the workspace.
 #include "paged_attn.hpp"
 
 namespace catopt {
 namespace {
 
-// WAVES waves per row (token, query head): the carriers of its key ranges, D / 4
-// lanes to a range's numerators, so that 2 WAVES (D = 64: 4 WAVES) ranges load
-// at once.  R: the rows of the tiles they were made with.
-template <int D, int R, int WAVES>
-__global__ __launch_bounds__(256) void paged_combine(PagedArgs a) {
-  constexpr int TPR = D / 4, GROUPS = 64 * WAVES / TPR;
-  const int lane = threadIdx.x & 63, tid = WAVES == 4 ? threadIdx.x : lane;
-  const int64_t row = WAVES == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.N * a.Hq) return;
-  const int n = (int)(row / a.Hq), hq = (int)(row - (int64_t)n * a.Hq);
-  int b = -1;
-  for (int c0 = 0; c0 < a.B; c0 += 64) {  // the last sequence that starts at or before the token
-    const int i = c0 + lane;
-    const int k = __popcll(__ballot(i < a.B && min(max(a.starts[i < a.B ? i : 0], 0), (int)a.N) <= n));
-    b += k;
-    if (k < 64) break;
-  }
-  if (b < 0) return;
-  PagedTile x{};
-  x.b = b;
-  seq_rows(a.starts, b, a.N, x.row0, x.nq);
-  if (n < x.row0 || n >= x.row0 + x.nq) return;
-  x.len = min(max(a.lens[b], 0), a.cap);
-  x.r0 = ((n - x.row0) * a.G + hq % a.G) / R * R;
-  x.rows = min(R, x.nq * a.G - x.r0);
-  paged_ranges(a, x);
-  if (x.splits == 1) return;  // written by the tile
-  const float c = a.scale * kLog2e;
-  const float* ml = a.part + 2 * row * a.splits;
-  const float* num = a.part + ((2 * a.N * a.Hq * a.splits + 3) & ~(int64_t)3) + row * a.splits * D + 4 * (tid % TPR);
-  // lane s of every wave: range s (64 at most)
-  const bool mine = lane < x.splits;
-  const float ms = mine ? ml[2 * lane] : kNegInf, ls = mine ? ml[2 * lane + 1] : 0.f;
-  float mx = ms;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-  const float f = mine ? move_factor(ms, mx, c) : 0.f;
-  float lt = ls * f;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o, 64);
-  f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int U = 8;  // loads ahead of their additions
-  for (int s0 = 0; s0 < x.splits; s0 += U * GROUPS) {  // every lane stays: the factors come from lanes
-    f32x4 ys[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int s = s0 + i * GROUPS + tid / TPR;
-      ys[i] = s < x.splits ? *reinterpret_cast<const f32x4*>(num + (int64_t)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-#pragma unroll
-    for (int i = 0; i < U; ++i) y += ys[i] * __shfl(f, min(s0 + i * GROUPS + tid / TPR, 63), 64);
-  }
-  if constexpr (WAVES == 4) {
-    __shared__ f32x4 sums[GROUPS][TPR];
-    sums[tid / TPR][tid % TPR] = y;
-    __syncthreads();
-    if (tid < TPR) {
-#pragma unroll
-      for (int i = 1; i < GROUPS; ++i) y += sums[i][tid];
-    }
-  } else {
-#pragma unroll
-    for (int o = TPR; o < 64; o <<= 1)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], o, 64);
-  }
-  if (tid < TPR && 4 * tid < a.d) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = finish(y[e], lt, a.normalize);
-    *reinterpret_cast<u32x2*>(a.o + (int64_t)n * a.o_t + (int64_t)hq * a.o_h + 4 * tid) =
-        u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-  }
-  if (tid == 0) row_stats(a, row, mx, lt);
-}
-
 struct Plan {
-  bool few;
+  bool few, wide;
   int splits, min_keys, parts;
   int64_t tiles, part_floats, stat_floats, score_floats, weight_floats;
   int64_t bytes() const { return 4 * (part_floats + stat_floats + score_floats + weight_floats); }
@@ -91,6 +15,11 @@ struct Plan {
 //
 // Few rows: 32-row tiles whenever the sequences have 32 rows per key head or
 // fewer on average.
+//
+// One range, and so one launch, where the table reaches 1024 keys or fewer and
+// the CUs hold every tile at once: the wide kernel then takes 12 us at 1000
+// keys, 32 query heads on 8, and 10.7 (the host's time) at 500, where split
+// keys and their combination take 14.9.
 //
 // Ranges: few-row calls read K and V at the rate of HBM, so their ranges only
 // have to fill the CUs and even out the sequences: at most 64 to a tile and
@@ -109,7 +38,8 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t c
   int64_t s = p.few ? 16384 / groups : 512 / groups;
   const int64_t per_slot = p.few ? groups * cap / 512 : 256;
   p.min_keys = per_slot >= 4096 ? 1024 : per_slot >= 256 ? 256 : 128;
-  const int64_t most = (cap + p.min_keys - 1) / p.min_keys;
+  p.wide = p.few && groups <= 256 && cap <= 1024;
+  const int64_t most = p.wide ? 1 : (cap + p.min_keys - 1) / p.min_keys;
   if (s > kMaxSplits) s = kMaxSplits;
   if (s > most) s = most;
   p.splits = s < 1 ? 1 : (int)s;
@@ -125,21 +55,6 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t c
     }
   }
   return p;
-}
-
-template <int D, int R>
-int32_t combine(const PagedArgs& a, hipStream_t s) {
-  // four waves a row where the rows alone do not fill the CUs
-  const int64_t rows = a.N * a.Hq;
-  const bool wide = rows < 2048;
-  const int64_t blocks = wide ? rows : (rows + 3) / 4;
-  if (!grid_fits(blocks, 256)) return CATOPT_E_UNSUPPORTED;
-  if (wide)
-    paged_combine<D, R, 4><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(a);
-  else
-    paged_combine<D, R, 1><<<dim3((uint32_t)blocks), dim3(256), 0, s>>>(a);
-  CATOPT_LAUNCH_CHECK();
-  return CATOPT_OK;
 }
 
 }  // namespace
@@ -215,13 +130,8 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int D = d <= 64 ? 64 : 128;
-  int32_t r = p.few ? paged_few_launch(a, D, p.tiles, st) : paged_tile_launch(a, D, p.tiles, st);
-  if (r == CATOPT_OK && p.splits > 1) {
-    if (p.few)
-      r = D == 128 ? combine<128, kFewRows>(a, st) : combine<64, kFewRows>(a, st);
-    else
-      r = D == 128 ? combine<128, kTileRows>(a, st) : combine<64, kTileRows>(a, st);
-  }
-  if (r == CATOPT_OK && weights_out) r = paged_weights_launch(a, D, p.parts, ws, st);
+  int32_t r = p.few ? paged_few_launch(a, D, p.wide, p.tiles, st) : paged_tile_launch(a, D, p.tiles, st);
+  if (r == CATOPT_OK && p.splits > 1) r = paged_finish_launch(a, D, p.few, st);
+  if (r == CATOPT_OK && weights_out && !(a.scores && p.splits > 1)) r = paged_weights_launch(a, D, p.parts, ws, st);
   return r;
 }

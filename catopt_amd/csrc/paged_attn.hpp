@@ -41,27 +41,35 @@ struct PagedTile {
   int splits, keys;                // its key ranges and the keys of each
 };
 
+// Lane i looks at sequence i (of 64 at a time), so that the search and the
+// sequence's own numbers are one memory latency.
 template <int R>
 __device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, int t) {
   const int lane = threadIdx.x & 63;
-  int b = -1;
+  PagedTile x{};
+  x.b = -1;
+  int64_t first = 0;
   for (int c = 0; c < a.B; c += 64) {  // the last sequence whose first tile is not behind t
     const int i = c + lane;
+    int row0 = 0, nq = 0, len = 0;
     bool le = false;
     if (i < a.B) {
-      const int64_t s = min(max(a.starts[i], 0), (int)a.N);
-      le = s * a.G / R + i <= t;
+      seq_rows(a.starts, i, a.N, row0, nq);
+      len = min(max(a.lens[i], 0), a.cap);
+      le = (int64_t)row0 * a.G / R + i <= t;
     }
     const int n = __popcll(__ballot(le));
-    b += n;
+    if (n > 0) {
+      x.b = c + n - 1;
+      x.row0 = __builtin_amdgcn_readlane(row0, n - 1);
+      x.nq = __builtin_amdgcn_readlane(nq, n - 1);
+      x.len = __builtin_amdgcn_readlane(len, n - 1);
+      first = (int64_t)x.row0 * a.G / R + x.b;
+    }
     if (n < 64) break;
   }
-  PagedTile x{};
-  x.b = __builtin_amdgcn_readfirstlane(b);
   if (x.b < 0) return x;
-  seq_rows(a.starts, x.b, a.N, x.row0, x.nq);
-  x.len = min(max(a.lens[x.b], 0), a.cap);
-  const int64_t first = (int64_t)x.row0 * a.G / R + x.b, rows = (int64_t)x.nq * a.G, r0 = (t - first) * R;
+  const int64_t rows = (int64_t)x.nq * a.G, r0 = (t - first) * R;
   x.r0 = (int)r0;
   x.rows = r0 >= 0 && r0 < rows ? (int)min((int64_t)R, rows - r0) : 0;  // r0 < 0: starts that do not ascend
   return x;
@@ -96,6 +104,11 @@ __device__ __forceinline__ void row_stats(const PagedArgs& a, int64_t i, float m
   if (a.m_out) a.m_out[i] = m * a.scale;
   if (a.l_out) a.l_out[i] = l;
   if (a.row_log) a.row_log[i] = l == 0.f ? __builtin_inff() : m * (a.scale * kLog2e) + __builtin_amdgcn_logf(l);
+}
+
+__device__ __forceinline__ void add_weight(const PagedArgs& a, int b, int h, int key, int old, float w) {
+  if (a.w_in && key < old) w += a.w_in[b * a.wi_b + h * a.wi_h + key];
+  a.w_out[b * a.wo_b + h * a.wo_h + key] = w;
 }
 
 // Where 8 keys (a lane's) lie: pages hold a multiple of 8 keys, so the rows of 8
@@ -231,8 +244,10 @@ __device__ __forceinline__ void take_odd_values(bf16x8* vf, const bf16x8* p, f32
 // Host side of each kernel.
 constexpr int kFewRows = 32, kTileRows = 128;
 constexpr int kMaxSplits = 64;  // key ranges of a tile: one per lane of the wave that combines them
-int32_t paged_few_launch(const PagedArgs& a, int D, int64_t tiles, hipStream_t s);    // tiles of kFewRows
+int32_t paged_few_launch(const PagedArgs& a, int D, bool wide, int64_t tiles, hipStream_t s);  // tiles of kFewRows
 int32_t paged_tile_launch(const PagedArgs& a, int D, int64_t tiles, hipStream_t s);   // tiles of kTileRows
+int32_t paged_finish_launch(const PagedArgs& a, int D, bool few, hipStream_t s);  // split keys; and weights of scores
+int32_t paged_score_weights_launch(const PagedArgs& a, hipStream_t s);
 int paged_weight_parts(int64_t B, int64_t Hkv, int64_t cap, int64_t N, int64_t G);
 int32_t paged_weights_launch(const PagedArgs& a, int D, int parts, float* part, hipStream_t s);
 

@@ -18,16 +18,22 @@
 namespace catopt {
 namespace {
 
-template <int D>
+// Two waves (D = 64: four) of two stages fill half
+// a CU's LDS, so that two workgroups share it and one's start runs under the
+// other's loads: the form for long keys.  Eight waves of one stage (WIDE) have
+// 256 keys in flight at once: the form for one range of few keys, which spares
+// the second launch.
+template <int D, bool WIDE>
 struct Few {
-  static constexpr int WAVES = D == 128 ? 2 : 4, NT = 64 * WAVES;
+  static constexpr int WAVES = WIDE ? 8 : D == 128 ? 2 : 4, NT = 64 * WAVES, STAGES = WIDE ? 1 : 2;
   static constexpr int KEYS = 32 * WAVES;              // of a round of stages, 32 per wave
   static constexpr int HALF = 32 * AttnRow<D>::BYTES;  // a wave's K (or V) rows of a stage
-  static constexpr int STAGE = 2 * HALF, WAVE_BYTES = 2 * STAGE, BYTES = WAVES * WAVE_BYTES;
+  static constexpr int STAGE = 2 * HALF, WAVE_BYTES = STAGES * STAGE;
   static constexpr int LOADS = HALF / 1024;            // 1 KB loads of K (and of V) per stage
   static constexpr int ROWS = 32 / LOADS;              // rows of one
   static constexpr int OLD = D + 4;                    // row of the merge buffer, floats
-  static_assert(WAVES * 32 * OLD * 4 + WAVES * 64 * 4 <= BYTES, "the merge reuses the stages");
+  static constexpr int LOOP = WAVES * WAVE_BYTES, MERGE = WAVES * 32 * OLD * 4 + WAVES * 64 * 4;
+  static constexpr int BYTES = LOOP > MERGE ? LOOP : MERGE;  // the merge reuses the stages
 };
 
 // Wait for all but the newest LOADS * 2 loads (one stage's), or for all.  The
@@ -41,9 +47,9 @@ __device__ __forceinline__ void wait_stage(bool newer) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <int D>
-__global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
-  using L = Few<D>;
+template <int D, bool WIDE>
+__global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedArgs a) {
+  using L = Few<D, WIDE>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -53,6 +59,17 @@ __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
   paged_ranges(a, x);
   if (split >= x.splits) return;
   const float c = a.scale * kLog2e;
+
+  // this wave's stages: 32 keys each from key_of(i) on
+  const int k_begin = split * x.keys + 32 * wave, k_end = min(x.kend, (split + 1) * x.keys);
+  const int stages = k_end > k_begin ? (k_end - k_begin + L::KEYS - 1) / L::KEYS : 0;
+  auto key_of = [&](int i) { return k_begin + i * L::KEYS; };
+  const int32_t* table = a.table + (int64_t)x.b * a.table_ld;
+  const uint16_t *kb = a.k + (int64_t)h * a.k_h, *vb = a.v + (int64_t)h * a.v_h;
+  // the page of this lane's 8 keys of the 16 stages from stage st on; the first
+  // ones on their way before the queries are
+  auto lane_key = [&](int st) { return key_of(st + (lane >> 2)) + 8 * (lane & 3); };
+  const int first_page = group_page(a, table, lane_key(0), lane_key(0) < k_end ? x.len : 0);
 
   // this lane's query row
   const int row = x.r0 + l32, tok = (int)a.group.div(row), hq = h * a.G + row - tok * a.G;
@@ -67,12 +84,6 @@ __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
   }
   const int lim = x.off + tok;  // last key this row sees
 
-  // this wave's stages: 32 keys each from key_of(i) on
-  const int k_begin = split * x.keys + 32 * wave, k_end = min(x.kend, (split + 1) * x.keys);
-  const int stages = k_end > k_begin ? (k_end - k_begin + L::KEYS - 1) / L::KEYS : 0;
-  auto key_of = [&](int i) { return k_begin + i * L::KEYS; };
-  const int32_t* table = a.table + (int64_t)x.b * a.table_ld;
-  const uint16_t *kb = a.k + (int64_t)h * a.k_h, *vb = a.v + (int64_t)h * a.v_h;
   // a lane's 16 bytes of load k: row k ROWS + lane / CH of the stage, row & 7 of
   // its group; the swizzles depend on a row's place among 16 (K, D = 128: loads
   // k and k + 4 agree), 8 or 4 rows
@@ -89,7 +100,7 @@ __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
 #pragma unroll
     for (int k = 0; k < L::LOADS; ++k) {
       const int ln = lane0 + k * L::ROWS / 8;
-      const uint32_t to = lds0 + (i & 1) * L::STAGE + k * 1024;
+      const uint32_t to = lds0 + (i & (L::STAGES - 1)) * L::STAGE + k * 1024;
       dma_buf(k_rsrc(at, ln), koff[k & 3], to);
       dma_buf(v_rsrc(at, ln), voff[k & 1], to + L::HALF);
     }
@@ -107,23 +118,24 @@ __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
   for (int j = 0; j < D / 16; ++j)  // the queries have arrived: no wait for them below, which would wait for K and V
     asm volatile("" ::"v"(__builtin_bit_cast(u32x4, qf[j])));
 
-  KeyGroup at{};
-  uint64_t bad = 0;
+  KeyGroup at;
+  uint64_t bad;
+  auto places = [&](int st, int page) {
+    bool odd;
+    at = key_group(a, kb, vb, page, lane_key(st), lane_key(st) < k_end ? x.len : 0, odd);
+    bad = __ballot(odd);
+  };
+  places(0, first_page);
   for (int st = 0; st < stages; ++st) {
     const int in = st & 15;  // of the 16 stages whose groups the lanes hold
-    if (in == 0) {
-      const int key = key_of(st + (lane >> 2)) + 8 * (lane & 3), end = key < k_end ? x.len : 0;
-      bool odd;
-      at = key_group(a, kb, vb, group_page(a, table, key, end), key, end, odd);
-      bad = __ballot(odd);
-      issue(st, 0, at);
-    }
-    const bool newer = in < 15 && st + 1 < stages;
+    if (in == 0 && st > 0) places(st, group_page(a, table, lane_key(st), lane_key(st) < k_end ? x.len : 0));
+    if (in == 0 || L::STAGES == 1) issue(st, 4 * in, at);
+    const bool newer = L::STAGES == 2 && in < 15 && st + 1 < stages;
     if (newer) issue(st + 1, 4 * in + 4, at);
     wait_stage<2 * L::LOADS>(newer);
     const int key0 = key_of(st);
     const uint32_t bad_now = (uint32_t)(bad >> (4 * in)) & 15u;
-    const char* Ks = lds + wave * L::WAVE_BYTES + (st & 1) * L::STAGE;
+    const char* Ks = lds + wave * L::WAVE_BYTES + (st & (L::STAGES - 1)) * L::STAGE;
     const char* Vs = Ks + L::HALF;
 
     f32x16 s;
@@ -236,26 +248,28 @@ __global__ __launch_bounds__(Few<D>::NT, 2) void paged_few_kernel(PagedArgs a) {
   }
 }
 
-template <int D>
+template <int D, bool WIDE>
 int32_t launch(const PagedArgs& a, int64_t tiles, hipStream_t s) {
+  using L = Few<D, WIDE>;
   static bool attr_done = false;  // idempotent; benign race (same value written)
   if (!attr_done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_few_kernel<D>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, Few<D>::BYTES);
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_few_kernel<D, WIDE>),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
     if (e != hipSuccess) return set_hip_error(e);
     attr_done = true;
   }
   const int64_t blocks = tiles * a.splits * a.Hkv;
-  if (!grid_fits(blocks, Few<D>::NT)) return CATOPT_E_UNSUPPORTED;
-  paged_few_kernel<D><<<dim3((uint32_t)blocks), dim3(Few<D>::NT), Few<D>::BYTES, s>>>(a);
+  if (!grid_fits(blocks, L::NT)) return CATOPT_E_UNSUPPORTED;
+  paged_few_kernel<D, WIDE><<<dim3((uint32_t)blocks), dim3(L::NT), L::BYTES, s>>>(a);
   CATOPT_LAUNCH_CHECK();
   return CATOPT_OK;
 }
 
 }  // namespace
 
-int32_t paged_few_launch(const PagedArgs& a, int D, int64_t tiles, hipStream_t s) {
-  return D == 128 ? launch<128>(a, tiles, s) : launch<64>(a, tiles, s);
+int32_t paged_few_launch(const PagedArgs& a, int D, bool wide, int64_t tiles, hipStream_t s) {
+  if (D == 128) return wide ? launch<128, true>(a, tiles, s) : launch<128, false>(a, tiles, s);
+  return wide ? launch<64, true>(a, tiles, s) : launch<64, false>(a, tiles, s);
 }
 
 }  // namespace catopt

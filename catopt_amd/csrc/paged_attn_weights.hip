@@ -4,9 +4,8 @@
 //   c = scale log2 e,  o_r = m_r log2 e + log2 l_r  (PagedArgs::row_log)
 // on top of the weight so far (nothing for the new tokens' own keys).
 //
-// Few rows: the attention kernel has stored its products (4 bytes a row and
-// key, against 4 d bytes for K and V), and one thread adds four keys' rows.
-// Many rows: the products are formed again, half of the attention's.  A
+// This is the form for many rows (with few, the attention kernel stores its
+// products): they are formed again, half of the attention's work.  A
 // workgroup keeps 256 keys in registers, 64 per wave, and streams the rows by
 // 32 through LDS, each fragment of them feeding two MFMAs; the score
 // accumulator's columns are rows, so each lane adds its rows for 32 keys and
@@ -19,40 +18,6 @@ namespace catopt {
 namespace {
 
 constexpr int NT = 256;
-
-__device__ __forceinline__ void add_weight(const PagedArgs& a, int b, int h, int key, int old, float w) {
-  if (a.w_in && key < old) w += a.w_in[b * a.wi_b + h * a.wi_h + key];
-  a.w_out[b * a.wo_b + h * a.wo_h + key] = w;
-}
-
-__global__ __launch_bounds__(NT) void weights_from_scores(PagedArgs a, int blocks) {
-  const int bh = blockIdx.x / blocks, b = bh / a.Hkv, h = bh - b * a.Hkv;
-  const int key = ((blockIdx.x - bh * blocks) * NT + threadIdx.x) * 4;
-  int row0, nq;
-  seq_rows(a.starts, b, a.N, row0, nq);
-  const int len = min(max(a.lens[b], 0), a.cap);
-  if (key >= len) return;
-  const int old = len - nq;
-  const float c = a.scale * kLog2e;
-  f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int tok = 0; tok < nq; ++tok) {
-    const int seen = a.causal ? old + tok : len;  // last key
-    if (key > seen) continue;
-    for (int g = 0; g < a.G; ++g) {
-      const int64_t i = (int64_t)(row0 + tok) * a.Hq + h * a.G + g;
-      const f32x4 s = *reinterpret_cast<const f32x4*>(a.scores + i * a.cap + key);
-      const float o = a.row_log[i];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -o));
-        w[e] += key + e <= seen ? x : 0.f;
-      }
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (key + e < len) add_weight(a, b, h, key + e, old, w[e]);
-}
 
 constexpr int KB = 2;            // blocks of 32 keys per wave
 constexpr int kKeys = 128 * KB;  // of a workgroup
@@ -266,13 +231,7 @@ int paged_weight_parts(int64_t B, int64_t Hkv, int64_t cap, int64_t N, int64_t G
 int32_t paged_weights_launch(const PagedArgs& a, int D, int parts, float* part, hipStream_t s) {
   if (a.cap == 0) return CATOPT_OK;
   const int64_t heads = (int64_t)a.B * a.Hkv;
-  if (a.scores) {
-    const int64_t blocks = (a.cap + 4 * NT - 1) / (4 * NT);
-    if (!grid_fits(heads * blocks, NT)) return CATOPT_E_UNSUPPORTED;
-    weights_from_scores<<<dim3((uint32_t)(heads * blocks)), dim3(NT), 0, s>>>(a, (int)blocks);
-    CATOPT_LAUNCH_CHECK();
-    return CATOPT_OK;
-  }
+  if (a.scores) return paged_score_weights_launch(a, s);
   const int64_t blocks = (a.cap + kKeys - 1) / kKeys;
   if (!grid_fits(heads * blocks * parts, NT)) return CATOPT_E_UNSUPPORTED;
   const dim3 grid((uint32_t)(heads * blocks * parts));
