@@ -5,13 +5,16 @@
 // on top of the weight so far (nothing for the new tokens' own keys).
 //
 // This is the form for many rows (with few, the attention kernel stores its
-// products): they are formed again, half of the attention's work.  A
-// workgroup keeps 256 keys in registers, 64 per wave, and streams the rows by
-// 32 through LDS, each fragment of them feeding two MFMAs; the score
-// accumulator's columns are rows, so each lane adds its rows for 32 keys and
-// the lanes meet once at the end.  The exponentials
-// bound it.  Where the keys leave CUs idle the rows are split over workgroups
-// and the parts added in their order by another launch.
+// products): they are formed again, half of the attention's work.  A workgroup
+// keeps 128 keys in registers, 32 per wave, and streams the rows by 32 through
+// LDS; the score accumulator's columns are rows, so each lane adds its rows for
+// 16 keys and the lanes meet once at the end.  Each product's scores take an
+// exponential, a multiply-add and an addition, which costs more than the MFMA:
+// VALU issue bounds it, and the rows' addresses and offsets are kept to a few
+// additions a step.  64 keys a wave (half the LDS reads, two waves to a SIMD
+// instead of four) took 200 us where this takes 168: 2048 tokens over 8192
+// keys, 32 query heads on 8, 720 TFLOP/s.  Where the keys leave CUs idle the
+// rows are split over workgroups and the parts added in order by another launch.
 #include "paged_attn.hpp"
 
 namespace catopt {
@@ -19,13 +22,14 @@ namespace {
 
 constexpr int NT = 256;
 
-constexpr int KB = 2;            // blocks of 32 keys per wave
-constexpr int kKeys = 128 * KB;  // of a workgroup
-constexpr int RT = 1;            // blocks of 32 rows per step
+constexpr int kKeys = 128;  // of a workgroup, 32 per wave
 
 template <int D>
 __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks, int parts, float* part) {
-  __shared__ __attribute__((aligned(16))) char lds[2][32 * RT * D * 2];
+  // rows a 16-byte piece further apart than they are long: 16 rows' pieces lie
+  // in different banks, and a fragment's address is one register and a constant
+  constexpr int ROW = D * 2 + 16;
+  __shared__ __attribute__((aligned(16))) char lds[2][32 * ROW];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int u = blockIdx.x;
@@ -39,14 +43,13 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks
   const int len = min(max(a.lens[b], 0), a.cap);
   if (blk * kKeys >= len) return;
   const int old = len - nq, off = a.causal ? old : 0x3fffffff;
-  const int key0 = blk * kKeys + 32 * KB * wave;
+  const int key0 = blk * kKeys + 32 * wave;
   const float c = a.scale * kLog2e;
 
-  bf16x8 kf[KB][D / 16];
-  uint64_t ok[KB];  // keys whose page is one
-#pragma unroll
-  for (int kb = 0; kb < KB; ++kb) {
-    const int key = key0 + 32 * kb + l32;
+  bf16x8 kf[D / 16];
+  uint64_t ok;  // keys whose page is one
+  {
+    const int key = key0 + l32;
     bool valid = key < len;
     const uint32_t tp = a.page.div(valid ? key : 0);
     const int64_t page = valid ? a.table[(int64_t)b * a.table_ld + tp] : -1;
@@ -56,28 +59,28 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks
     for (int j = 0; j < D / 16; ++j) {
       u32x4 w = u32x4{0, 0, 0, 0};
       if (valid && 16 * j + 8 * g < a.d) w = *reinterpret_cast<const u32x4*>(k + 16 * j + 8 * g);
-      kf[kb][j] = __builtin_bit_cast(bf16x8, w);
+      kf[j] = __builtin_bit_cast(bf16x8, w);
     }
-    ok[kb] = __ballot(valid);
+    ok = __ballot(valid);
   }
 
-  // steps of 32 RT rows from the first that sees the block's first key; this part's share
+  // steps of 32 rows from the first that sees the block's first key; this part's share
   const int rows = nq * a.G, tok0 = max(blk * kKeys - off, 0);
-  const int ta = (int)min((int64_t)tok0 * a.G, (int64_t)rows) / (32 * RT), tb = (rows + 32 * RT - 1) / (32 * RT);
+  const int ta = (int)min((int64_t)tok0 * a.G, (int64_t)rows) / 32, tb = (rows + 31) / 32;
   const int t0 = ta + (int)((int64_t)(tb - ta) * pt / parts), t1 = ta + (int)((int64_t)(tb - ta) * (pt + 1) / parts);
 
-  constexpr int CH = AttnRow<D>::CH, LD = 32 * RT * CH / NT;  // 16-byte pieces of a step per thread
-  static_assert(LD >= 1 && LD <= 4, "the pieces' registers");
-  u32x4 qr[4];
-  float o_next[RT];
+  constexpr int CH = AttnRow<D>::CH, LD = 32 * CH / NT;  // 16-byte pieces of a step per thread
+  static_assert(LD >= 1 && LD <= 2, "the pieces' registers");
+  u32x4 qr[2];
+  float o_next = 0.f;
   // Row r of the sequence is token r / G, head r % G.  The rows that a lane
-  // reads advance by 32 RT a step, so their tokens and heads, and with them the
+  // reads advance by 32 a step, so their tokens and heads, and with them the
   // offsets of their queries and offsets o, advance by constants and a carry.
   struct Walk {
     int r, g;
     int64_t q, o;
   };
-  const int step_t = 32 * RT / a.G, step_g = 32 * RT - step_t * a.G;
+  const int step_t = 32 / a.G, step_g = 32 - step_t * a.G;
   const int64_t step_q = step_t * a.q_t + step_g * a.q_h, wrap_q = a.q_t - a.G * a.q_h;
   const int64_t step_o = (int64_t)step_t * a.Hq + step_g, wrap_o = a.Hq - a.G;
   auto walk_from = [&](int r) {
@@ -86,23 +89,27 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks
                 (int64_t)(row0 + tok) * a.Hq + h * a.G + gr};
   };
   auto advance = [&](Walk& x, bool queries) {
-    x.r += 32 * RT;
+    x.r += 32;
+    if (queries)
+      x.q += step_q;
+    else
+      x.o += step_o;
+    if (step_g == 0) return;  // G divides 32: the heads stay
     x.g += step_g;
     const bool wrap = x.g >= a.G;
     x.g -= wrap ? a.G : 0;
     if (queries)
-      x.q += step_q + (wrap ? wrap_q : 0);
+      x.q += wrap ? wrap_q : 0;
     else
-      x.o += step_o + (wrap ? wrap_o : 0);
+      x.o += wrap ? wrap_o : 0;
   };
-  Walk wq[4], wo[RT];
+  Walk wq[2];
 #pragma unroll
   for (int i = 0; i < LD; ++i) {
-    wq[i] = walk_from(32 * RT * t0 + (i * NT + tid) / CH);
+    wq[i] = walk_from(32 * t0 + (i * NT + tid) / CH);
     wq[i].q += (tid % CH) * 8;
   }
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) wo[rt] = walk_from(32 * (RT * t0 + rt) + l32);
+  Walk wo = walk_from(32 * t0 + l32);
   const bool column = (tid % CH) * 8 < a.d;
   auto fetch = [&]() {
 #pragma unroll
@@ -111,94 +118,65 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks
       if (wq[i].r < rows && column) qr[i] = *reinterpret_cast<const u32x4*>(a.q + wq[i].q);
       advance(wq[i], true);
     }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      o_next[rt] = wo[rt].r < rows ? a.row_log[wo[rt].o] : __builtin_inff();
-      advance(wo[rt], false);
-    }
+    o_next = wo.r < rows ? a.row_log[wo.o] : __builtin_inff();
+    advance(wo, false);
   };
   auto stage = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const int piece = i * NT + tid;
-      *reinterpret_cast<u32x4*>(lds[buf] + tile_off<D>(piece / CH, piece % CH)) = qr[i];
+      *reinterpret_cast<u32x4*>(lds[buf] + piece / CH * ROW + piece % CH * 16) = qr[i];
     }
   };
 
-  float w[KB][16];
+  float w[16];
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) w[kb][r] = 0.f;
+  for (int r = 0; r < 16; ++r) w[r] = 0.f;
   if (t0 < t1) {
     fetch();
     stage(0);
   }
-  // Sᵀ of the wave's keys and 32 staged rows, and the rows' terms of it
-  auto qk = [&](int buf, int rt, f32x16* s) {
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      const bf16x8 q = *reinterpret_cast<const bf16x8*>(lds[buf] + tile_off<D>(32 * rt + l32, 2 * j + g));
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) s[kb] = mfma32x32x16(kf[kb][j], q, s[kb]);
-    }
-  };
-  auto mask = [&](int r0, f32x16* s) {
-    const int lim = off + (int)a.group.div(r0 + l32);
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[kb][r] = key0 + 32 * kb + acc_row(r, g) <= lim ? s[kb][r] : kNegInf;
-  };
-  auto add = [&](const f32x16* s, float o) {
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) w[kb][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], c, -o));
-  };
-  for (int t = t0; t < t1; ++t) {
-    const int buf = (t - t0) & 1;
-    float o[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) o[rt] = o_next[rt];
+  auto step = [&](int t, int buf) {
+    const float o = o_next;
     __syncthreads();  // the step is staged, and the other buffer is free
     if (t + 1 < t1) fetch();
-    const int r0 = 32 * RT * t;
-    const int first = off + (int)a.group.div(r0);                          // last key of the step's first row
-    const int last = off + (int)a.group.div(min(r0 + 32 * RT, rows) - 1);  // and of its last row
+    const int first = off + (int)a.group.div(32 * t);                     // last key of the step's first row
+    const int last = off + (int)a.group.div(min(32 * t + 32, rows) - 1);  // and of its last row
     if (key0 <= last && key0 < len) {
-      const bool masked = key0 + 32 * KB - 1 > first;
+      f32x16 s;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        f32x16 s[KB];
-        qk(buf, rt, s);
-        if (masked) mask(r0 + 32 * rt, s);
-        add(s, o[rt]);
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+        s = mfma32x32x16(kf[j], *reinterpret_cast<const bf16x8*>(lds[buf] + l32 * ROW + (2 * j + g) * 16), s);
+      if (key0 + 31 > first) {
+        const int lim = off + (int)a.group.div(32 * t + l32);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = key0 + acc_row(r, g) <= lim ? s[r] : kNegInf;
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -o));
     }
     if (t + 1 < t1) stage(buf ^ 1);
+  };
+  for (int t = t0; t < t1; t += 2) {  // in pairs: the buffer is a constant of the addresses
+    step(t, 0);
+    if (t + 1 < t1) step(t + 1, 1);
   }
   // lane r of each half takes the key of accumulator register r
 #pragma unroll
-  for (int kb = 0; kb < KB; ++kb) {
+  for (int r = 0; r < 16; ++r) {
+    float y = w[r];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float y = w[kb][r];
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) y += __shfl_xor(y, x, 64);
-      if (l32 == r) {
-        const int in = acc_row(r, g), j = key0 + 32 * kb + in;
-        if (j < len) {
-          const float x = (ok[kb] >> in) & 1 ? y : 0.f;
-          if (parts > 1)
-            part[((int64_t)(pt * a.B + b) * a.Hkv + h) * a.cap + j] = x;
-          else
-            add_weight(a, b, h, j, old, x);
-        }
+    for (int x = 16; x > 0; x >>= 1) y += __shfl_xor(y, x, 64);
+    if (l32 == r) {
+      const int in = acc_row(r, g), j = key0 + in;
+      if (j < len) {
+        const float x = (ok >> in) & 1 ? y : 0.f;
+        if (parts > 1)
+          part[((int64_t)(pt * a.B + b) * a.Hkv + h) * a.cap + j] = x;
+        else
+          add_weight(a, b, h, j, old, x);
       }
     }
   }
@@ -223,8 +201,8 @@ __global__ __launch_bounds__(NT) void weights_add_parts(PagedArgs a, int blocks,
 int paged_weight_parts(int64_t B, int64_t Hkv, int64_t cap, int64_t N, int64_t G) {
   const int64_t groups = B * Hkv * ((cap + kKeys - 1) / kKeys);
   int64_t n = groups > 0 ? 2048 / groups : 1;
-  const int64_t steps = N * G / (32 * RT);
-  if (n > steps / 4) n = steps / 4;  // of the call: a part has a few steps at least
+  const int64_t steps = N * G / 32;
+  if (n > steps / 8) n = steps / 8;  // of the call: a part has a few steps at least
   return n < 1 ? 1 : n > 16 ? 16 : (int)n;
 }
 
