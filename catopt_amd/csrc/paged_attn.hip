@@ -11,6 +11,28 @@ struct Plan {
   int64_t bytes() const { return 4 * (part_floats + stat_floats + score_floats + weight_floats); }
 };
 
+// Key ranges of 128-row tiles by their estimated time, were every sequence as
+// long as its table.  A workgroup takes a tile of 64 keys in 1.7 us alone on
+// its CU and 2.4 beside another (D = 64: 1 and 1.5); more workgroups than the
+// 512 that the CUs hold run in rounds.  Ranges cost a launch, 5.5 us, and their
+// numerators' way through memory, at 6 TB/s.  Measured, one range against the
+// best split (us): 64 tokens over 564 keys, 32 heads on 8, 20.4 and 16.5; 512
+// new tokens 18.5 and 22.6; four chunks of 300 over up to 300, 12 heads of 64,
+// 17.0 and 23.0.
+int tile_splits(int64_t groups, int64_t rows, int64_t D, int64_t cap) {
+  const double alone = D == 128 ? 1.7 : 1.0, beside = D == 128 ? 2.4 : 1.5;
+  double best = 0;
+  int splits = 1;
+  for (int s = 1; s <= kMaxSplits; ++s) {
+    const int64_t keys = ((cap + s - 1) / s + 127) / 128 * 128, wgs = groups * s;
+    const double rounds = wgs <= 512 ? 1 : wgs / 512.0, tile = wgs <= 256 ? alone : beside;
+    const double us = rounds * (keys / 64) * tile + (s > 1 ? 5.5 + (double)rows * s * D * 8 / 6e6 : 0);
+    if (s == 1 || us < best) best = us, splits = s;
+    if (keys <= 128) break;
+  }
+  return splits;
+}
+
 // The kernel and the key ranges by sizes that the host knows.
 //
 // Few rows: 32-row tiles whenever the sequences have 32 rows per key head or
@@ -27,23 +49,29 @@ struct Plan {
 // is 256 keys at least; 128 where the table's reach is less than 256 for each
 // of the 512 workgroups that the CUs hold; 1024 where it is 4096 for each (a
 // step of 32 sequences of 300 to 16000 keys: 115 us, 124 with 256; at eight
-// sequences of 2000 to 12000 they are level).  Tiles of 128 rows are split only where they are fewer than the
-// 512 workgroups that the CUs hold, into ranges of 256 keys at least.
+// sequences of 2000 to 12000 they are level).
+//
+// 128-row tiles: see tile_splits.
 Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t cap, bool weights) {
   Plan p{};
   const int64_t G = Hq / Hkv, D = d <= 64 ? 64 : 128;
   p.few = N * G <= kFewRows * B;
   p.tiles = paged_tiles(N, G, B, p.few ? kFewRows : kTileRows);
   const int64_t groups = p.tiles * Hkv;
-  int64_t s = p.few ? 16384 / groups : 512 / groups;
-  const int64_t per_slot = p.few ? groups * cap / 512 : 256;
-  p.min_keys = per_slot >= 4096 ? 1024 : per_slot >= 256 ? 256 : 128;
-  p.wide = p.few && groups <= 256 && cap <= 1024;
-  const int64_t most = p.wide ? 1 : (cap + p.min_keys - 1) / p.min_keys;
-  if (s > kMaxSplits) s = kMaxSplits;
-  if (s > most) s = most;
-  p.splits = s < 1 ? 1 : (int)s;
   const int64_t rows = N * Hq;
+  if (p.few) {
+    int64_t s = 16384 / groups;
+    const int64_t per_slot = groups * cap / 512;
+    p.min_keys = per_slot >= 4096 ? 1024 : per_slot >= 256 ? 256 : 128;
+    p.wide = groups <= 256 && cap <= 1024;
+    const int64_t most = p.wide ? 1 : (cap + p.min_keys - 1) / p.min_keys;
+    if (s > kMaxSplits) s = kMaxSplits;
+    if (s > most) s = most;
+    p.splits = s < 1 ? 1 : (int)s;
+  } else {
+    p.min_keys = 128;
+    p.splits = tile_splits(groups, rows, D, cap);
+  }
   p.part_floats = p.splits > 1 ? ((2 * rows * p.splits + 3) & ~(int64_t)3) + rows * p.splits * D : 0;
   if (weights) {
     p.stat_floats = (rows + 3) & ~(int64_t)3;
