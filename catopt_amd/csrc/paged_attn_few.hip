@@ -11,7 +11,8 @@
 // V go global->LDS directly into two stages of its own.  A stage is loaded again
 // as soon as it has been used, and the wait for the other one leaves the new
 // loads in flight: the waves read nothing of each other's, so there is no
-// barrier in the loop.  A lane works out the place of 8 keys, the wave those of
+// barrier in the loop.  The loads carry the non-temporal hint: 32 sequences'
+// step over 131072 keys 115 -> 103 us, a step over 47000 keys 55 -> 50.  A lane works out the place of 8 keys, the wave those of
 // 16 stages at once.
 #include "paged_attn.hpp"
 
@@ -101,8 +102,8 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
     for (int k = 0; k < L::LOADS; ++k) {
       const int ln = lane0 + k * L::ROWS / 8;
       const uint32_t to = lds0 + (i & (L::STAGES - 1)) * L::STAGE + k * 1024;
-      dma_buf(k_rsrc(at, ln), koff[k & 3], to);
-      dma_buf(v_rsrc(at, ln), voff[k & 1], to + L::HALF);
+      dma_buf_once(k_rsrc(at, ln), koff[k & 3], to);
+      dma_buf_once(v_rsrc(at, ln), voff[k & 1], to + L::HALF);
     }
   };
 
