@@ -36,6 +36,20 @@ __device__ __forceinline__ void seq_rows(const int32_t* starts, int b, int64_t N
   nq = max(min(max(starts[b + 1], 0), n) - row0, 0);
 }
 
+// A kernel's dynamic LDS beyond the default, set once on each device (`done`:
+// one flag per device, idempotent; a concurrent first call sets the same).
+constexpr int kDevices = 16;
+inline int32_t allow_lds(const void* kernel, int bytes, bool* done) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return set_hip_error(e);
+  if (dev < kDevices && done[dev]) return CATOPT_OK;
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return set_hip_error(e);
+  if (dev < kDevices) done[dev] = true;
+  return CATOPT_OK;
+}
+
 inline bool strides_fit(const int64_t* s, int n, int64_t step) {
   for (int i = 0; i < n; ++i)
     if (s[i] < 0 || s[i] % step) return false;

@@ -111,11 +111,11 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
     return CATOPT_E_INVAL;
   if (normalize < 1 || normalize > 2) return CATOPT_E_INVAL;
   if (dtype != CATOPT_BF16 || d < 8 || d > 128 || d % 8 || page_size % 8) return CATOPT_E_UNSUPPORTED;
-  if (!(scale > 0.f) || !__builtin_isfinite(scale)) return CATOPT_E_UNSUPPORTED;
+  if (!(scale > 0.f) || !__builtin_isfinite(scale * kLog2e)) return CATOPT_E_UNSUPPORTED;
   const int64_t need = catopt_hip_paged_attn_workspace_bytes(B, N, Hq, Hkv, d, n_table, page_size, weights_out != nullptr);
   if (need < 0) return CATOPT_E_UNSUPPORTED;
-  if (B == 0 || N == 0) return CATOPT_OK;
-  if (!q || !o || !kv_lens || !q_starts || !strides || (n_table > 0 && !block_table)) return CATOPT_E_INVAL;
+  if (B == 0 || (N == 0 && !weights_out)) return CATOPT_OK;
+  if ((N > 0 && (!q || !o)) || !kv_lens || !q_starts || !strides || (n_table > 0 && !block_table)) return CATOPT_E_INVAL;
   if (n_pages > 0 && (!k_pages || !v_pages)) return CATOPT_E_INVAL;
   if (!strides_fit(strides, 10, 8) || !strides_fit(strides + 10, 4, 1)) return CATOPT_E_INVAL;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o)) return CATOPT_E_INVAL;
@@ -145,7 +145,7 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   a.page = FastDiv::of(page_size), a.group = FastDiv::of(Hq / Hkv);
   a.B = (int)B, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.d = (int)d, a.cap = (int)(n_table * page_size);
   a.normalize = normalize, a.causal = causal != 0, a.scale = scale;
-  const Plan p = plan_of(B, N, Hq, Hkv, d, a.cap, weights_out != nullptr);
+  const Plan p = N == 0 ? Plan{} : plan_of(B, N, Hq, Hkv, d, a.cap, weights_out != nullptr);
   float* ws = static_cast<float*>(workspace);
   a.splits = p.splits, a.min_keys = p.min_keys;
   a.part = ws;
@@ -158,6 +158,7 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int D = d <= 64 ? 64 : 128;
+  if (N == 0) return paged_weights_launch(a, D, 1, nullptr, st);  // no new tokens: the sums so far
   int32_t r = p.few ? paged_few_launch(a, D, p.wide, p.tiles, st) : paged_tile_launch(a, D, p.tiles, st);
   if (r == CATOPT_OK && p.splits > 1) r = paged_finish_launch(a, D, p.few, st);
   if (r == CATOPT_OK && weights_out && !(a.scores && p.splits > 1)) r = paged_weights_launch(a, D, p.parts, ws, st);

@@ -252,13 +252,9 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
 template <int D, bool WIDE>
 int32_t launch(const PagedArgs& a, int64_t tiles, hipStream_t s) {
   using L = Few<D, WIDE>;
-  static bool attr_done = false;  // idempotent; benign race (same value written)
-  if (!attr_done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_few_kernel<D, WIDE>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
-    if (e != hipSuccess) return set_hip_error(e);
-    attr_done = true;
-  }
+  static bool done[kDevices] = {};
+  const int32_t r = allow_lds(reinterpret_cast<const void*>(&paged_few_kernel<D, WIDE>), L::BYTES, done);
+  if (r != CATOPT_OK) return r;
   const int64_t blocks = tiles * a.splits * a.Hkv;
   if (!grid_fits(blocks, L::NT)) return CATOPT_E_UNSUPPORTED;
   paged_few_kernel<D, WIDE><<<dim3((uint32_t)blocks), dim3(L::NT), L::BYTES, s>>>(a);

@@ -291,13 +291,9 @@ __global__ __launch_bounds__(NT, 2) void paged_tile_kernel(PagedArgs a, int tile
 
 template <int D>
 int32_t launch(const PagedArgs& a, int64_t tiles, hipStream_t s) {
-  static bool attr_done = false;  // idempotent; benign race (same value written)
-  if (!attr_done) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_tile_kernel<D>),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, TileLds<D>::BYTES);
-    if (e != hipSuccess) return set_hip_error(e);
-    attr_done = true;
-  }
+  static bool done[kDevices] = {};
+  const int32_t r = allow_lds(reinterpret_cast<const void*>(&paged_tile_kernel<D>), TileLds<D>::BYTES, done);
+  if (r != CATOPT_OK) return r;
   const int64_t blocks = tiles * a.splits * a.Hkv;
   if (!grid_fits(blocks, NT)) return CATOPT_E_UNSUPPORTED;
   paged_tile_kernel<D><<<dim3((uint32_t)blocks), dim3(NT), TileLds<D>::BYTES, s>>>(a, (int)tiles);

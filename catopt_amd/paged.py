@@ -30,7 +30,6 @@ reach, keys of an invalid page count as masked, and a write to one is dropped.
 from __future__ import annotations
 
 import functools
-import math
 import struct
 
 import torch
@@ -231,7 +230,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q (N, Hq, d)`` holds the tokens of all sequences, sequence ``b``'s in
     rows ``q_starts[b]`` to ``q_starts[b + 1]`` (int32, ``B + 1`` ascending
     values); ``kv_lens (B,)`` int32 counts its cached keys, the new tokens'
-    own the last of them (write them first, :func:`qk_norm_rope_append`).
+    own the last of them (write them first, :func:`qk_norm_rope_append`); more
+    than the table reaches are cut to its reach.
     ``block_table (B, n)`` is int32.  With ``causal`` token ``i`` of ``n``
     sees keys ``j <= kv_len - n + i``, else every key.  Query head ``h`` reads
     key head ``h // (Hq // Hkv)``.  ``d`` is a multiple of 8 up to 128, the
@@ -239,8 +239,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     Returns ``o (N, Hq, d)``, written to ``out`` when given; rows behind the
     last sequence are neither read nor written.  ``return_ml`` adds the fp32
-    ``(m, l)`` om carriers of the rows, ``(N, Hq)``, so that a part of the
-    keys kept elsewhere can be combined.  A row that sees no key is NaN
+    ``(m, l)`` om carriers of the sequences' rows, ``(N, Hq)``, so that a part
+    of the keys kept elsewhere can be combined.  A row that sees no key is NaN
     (``empty_rows="nan"``) or 0 (``"zero"``), as in
     :func:`catopt_amd.kernels.attention`.
 
@@ -267,8 +267,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if page < 1 or page % 8:
         raise NotImplementedError(f"paged attention takes page sizes that are multiples of 8, got {page}")
     scale = float(scale)
-    if not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"the scale is a positive number, got {scale}")
+    if not 0 < scale < 1e38:
+        raise ValueError(f"the scale is a positive number below 1e38, got {scale}")
     kv_lens = _vector("kv_lens", kv_lens, torch.int32)
     B = kv_lens.shape[0]
     q_starts = _vector("q_starts", q_starts, torch.int32, B + 1)
@@ -296,7 +296,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if return_ml:
         m, l = (q.new_empty((N, Hq), dtype=torch.float32) for _ in range(2))
         mp, lp = m.data_ptr(), l.data_ptr()
-    if N and B:
+    if B and (N or wo is not None):
         strides = _S14(qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], so[0], so[1], wi0, wi1, wo0, wo1)
         wsb = _attn_workspace(B, N, Hq, Hkv, d, n_table, page, wo is not None)
         if wsb:

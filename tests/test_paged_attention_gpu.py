@@ -265,6 +265,55 @@ def test_pages_past_32_bit_offsets(nq):
     check_attention(small, q, [nq], [length], got, scale=0.1)
 
 
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("cap,nq,lens,Hq,Hkv", [
+    (1024, [1] * 3, [1024, 700, 1], 8, 2),        # the widest table of one range
+    (1040, [1] * 3, [1040, 700, 1], 8, 2),        # one page more: ranges
+    (512, [1] * 70, [(37 * i) % 500 + 1 for i in range(70)], 8, 4),  # more tiles than CUs
+    (1600, [1] * 150, [(97 * i) % 1600 + 1 for i in range(150)], 2, 1),  # sequences past one look of a wave
+    (1500, [1, 2, 1, 3] * 17, [(211 * i) % 1400 + 30 for i in range(68)], 32, 8),  # many rows to combine
+    (6000, [2], [6000], 64, 2),                   # every range of a tile
+])
+def test_steps_at_the_borders_of_their_kernels(cap, nq, lens, Hq, Hkv, weights):
+    cache = Cache(lens, Hkv, 128, 16, seed=cap)
+    table = torch.full((len(lens), cap // 16), -1, dtype=torch.int32, device=DEV)
+    table[:, :cache.table.shape[1]] = cache.table[:, :cap // 16]
+    q = randn(gen(2), sum(nq), Hq, 128)
+    w = torch.zeros((len(lens), Hkv, cap), device=DEV) if weights else None
+    o, m, l = P.paged_attention(q, cache.k, cache.v, table, ints(lens), starts_of(nq), 0.1, return_ml=True, weights_out=w)
+    check_attention(cache, q, nq, lens, o, scale=0.1, m=m, l=l, weights=w)
+
+
+def test_weights_of_a_step_whose_products_are_not_stored():
+    """Few rows and a table so wide that every product would take more than 1 GiB: they are formed again."""
+    B, cap = 64, 1 << 17
+    lens = [(131 * i) % 300 + 1 for i in range(B)]
+    lens[5] = 9000
+    cache = Cache(lens, 8, 64, 16, seed=3)
+    table = torch.full((B, cap // 16 + 1), -1, dtype=torch.int32, device=DEV)
+    table[:, :cache.table.shape[1]] = cache.table
+    q = randn(gen(2), B, 32, 64)
+    w = torch.zeros((B, 8, cap + 16), device=DEV)
+    o = P.paged_attention(q, cache.k, cache.v, table, ints(lens), starts_of([1] * B), 0.1, weights_out=w)
+    check_attention(cache, q, [1] * B, lens, o, scale=0.1, weights=w)
+
+
+@pytest.mark.parametrize("groups", [1, 3, 5, 7, 8, 32, 33, 40])
+def test_query_heads_that_do_not_divide_a_tile(groups):
+    _run([40, 3], [90, 300], groups * 2, 2, 64, 16, seed=groups)
+    _run([1, 1], [90, 300], groups * 2, 2, 128, 16, seed=groups)
+
+
+def test_no_new_tokens_keep_the_weights():
+    cache = Cache([50, 9], 2, 64, 16)
+    e = torch.empty((0, 4, 64), dtype=BF16, device=DEV)
+    before = torch.rand((2, 2, 80), generator=gen(1), device=DEV)
+    w = torch.full_like(before, 7.0)
+    P.paged_attention(e, cache.k, cache.v, cache.table, ints([50, 9]), ints([0, 0, 0]), 0.1, weights=before, weights_out=w)
+    for b, n in enumerate((50, 9)):
+        assert torch.equal(w[b, :, :n], before[b, :, :n]) and (w[b, :, n:] == 7).all()
+
+
 def test_nothing_to_do():
     cache = Cache([10], 2, 64, 16)
     e = torch.empty((0, 4, 64), dtype=BF16, device=DEV)

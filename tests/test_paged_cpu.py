@@ -34,14 +34,14 @@ def _attn(lib, dtype=L.BF16, B=1, N=4, Hq=4, Hkv=2, d=64, q=Q, k=KP, v=VP, n_pag
 
 def test_attention_refuses(lib):
     # nothing to do is no error, and touches nothing
-    assert _attn(lib, B=0) == L.OK and _attn(lib, N=0) == L.OK
+    assert _attn(lib, B=0) == L.OK and _attn(lib, N=0, q=None, o=None) == L.OK
     for kw in ({"B": -1}, {"N": -1}, {"Hq": 3}, {"Hkv": 0}, {"n_pages": -1}, {"n_table": -1}, {"ld": -1}, {"norm": 0},
                {"norm": 3}, {"q": None}, {"o": None}, {"k": None}, {"v": None}, {"table": None}, {"lens": None},
                {"starts": None}, {"q": Q + 8}, {"o": OUT + 2}, {"k": KP + 4}, {"v": VP + 4}, {"w_in": WIN},
                {"strides": [-256] + [64] * 13}, {"strides": [4] + [64] * 13}, {"strides": [64] * 10 + [-1] * 4}):
         assert _attn(lib, **kw) == L.E_INVAL, kw
     for kw in ({"dtype": L.F32}, {"d": 60}, {"d": 136}, {"d": 0}, {"page": 12}, {"scale": 0.0}, {"scale": float("inf")},
-               {"scale": float("nan")}, {"N": 1 << 40}, {"B": 1 << 40}, {"n_table": 1 << 30}, {"page": 1 << 40}):
+               {"scale": float("nan")}, {"scale": 3e38}, {"N": 1 << 40}, {"B": 1 << 40}, {"n_table": 1 << 30}, {"page": 1 << 40}):
         assert _attn(lib, **kw) == L.E_UNSUPPORTED, kw
     need = lib.catopt_hip_paged_attn_workspace_bytes(1, 4, 4, 2, 64, 4, 16, 1)
     assert need > 0

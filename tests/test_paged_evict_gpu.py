@@ -112,6 +112,24 @@ def test_invalid_pages_and_lengths():
     assert new.tolist() == [32, 0] and kept[0, 0].tolist() == list(range(cap - 32, cap)) and (kept[1] == -1).all()
 
 
+def test_keys_past_the_registers_of_a_workgroup():
+    """Tables of more than 16384 keys read their weights again in every sweep; in place too."""
+    lens, budget = [20000, 16385, 300], 3000
+    cache, out = Cache(lens, 1, 8, 16, seed=4), Cache([budget] * 3, 1, 8, 16, seed=2)
+    for ties in (True, False):
+        w = _weights(cache, 7, ties)
+        same = w.clone()
+        kept, new, w_to = P.paged_evict(cache.k, cache.v, cache.table, ints(lens), w, out.table, budget, 100, k_out=out.k,
+                                        v_out=out.v)
+        _check(cache, w, budget, 100, kept, new, w_to, out)
+        kept2, _, _ = P.paged_evict(cache.k, cache.v, cache.table, ints(lens), same, out.table, budget, 100, k_out=out.k,
+                                    v_out=out.v, weights_out=same)
+        assert torch.equal(kept, kept2)
+        for b, n in enumerate(lens):
+            m = min(n, budget)
+            assert torch.equal(same[b, :, :m], w_to[b, :, :m]) and torch.equal(same[b, :, m:], w[b, :, m:])
+
+
 def test_captured():
     lens = [500, 260]
     cache, out = Cache(lens, 2, 64, 16), Cache([128, 128], 2, 64, 16, seed=2)

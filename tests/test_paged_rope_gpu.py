@@ -161,6 +161,21 @@ def test_captured_and_on_a_side_stream():
         assert torch.equal(out, want) and torch.equal(kp, k2) and torch.equal(vp, v2)
 
 
+@pytest.mark.parametrize("dtype,N", [(BF16, 7000), (F32, 3500)])
+def test_rows_past_the_caches(dtype, N):
+    """More than 256 MB of rows: the same bits as in parts."""
+    q, k, v, w, cos, sin, pos = _case(N, 64, 8, 128, 128, dtype, True)
+    kp, vp = (torch.zeros((N // 16 + 1, 8, 16, 128), dtype=dtype, device=DEV) for _ in range(2))
+    slots = torch.randperm(N, generator=gen(1), device=DEV)
+    qo = P.qk_norm_rope_append(q, k, v, cos, sin, pos, kp, vp, slots, *w)
+    for a in range(0, N, 1000):
+        r = slice(a, min(a + 1000, N))
+        qe, ke = P.qk_norm_rope(q[r], k[r], cos, sin, pos[r], *w)
+        assert torch.equal(qo[r], qe) and torch.equal(kp[slots[r] // 16, :, slots[r] % 16], ke)
+        assert torch.equal(vp[slots[r] // 16, :, slots[r] % 16], v[r])
+    _near(qo[-50:], q[-50:], w[0], cos, sin, pos[-50:], False)
+
+
 def test_no_tokens():
     q, k, v, w, cos, sin, pos = _case(0, 4, 2, 64, 64, BF16, True)
     qo, ko = P.qk_norm_rope(q, k, cos, sin, pos, *w)
