@@ -1,6 +1,14 @@
 // Eviction from a paged cache by accumulated attention weight: per (sequence,
 // key head) the last `recent` keys and the largest weights of the others stay,
-// then the kept rows move to other pages.
+// and the kept rows move to other pages.
+//
+// One launch: `parts` workgroups per (sequence, head) each make the whole
+// choice, which takes 10 us at 2048 keys and 16 at 16000, and move their share
+// of the rows.  That takes 15.8 us for 2048 keys of one sequence, 8 heads, and
+// 40.5 for eight sequences of up to 16000 that keep 2048 (132 MB, so the move
+// runs at 5.4 TB/s); with a launch for the choice and one for the move they
+// took 18.4 and 41.9.  HBM bounds the move, rounds of LDS atomics and barriers
+// the choice; small calls are bound by the host.
 #include "paged.hpp"
 
 namespace catopt {
@@ -14,7 +22,8 @@ struct EvictArgs {
   int32_t *kept, *new_lens;
   int64_t table_ld, out_ld, w_b, w_h, wo_b, wo_h, n_pages, n_out_pages;
   FastDiv page, out_page;
-  int B, H, cap, budget, recent, row16;  // row16: 16-byte pieces of a row
+  FastDiv row16;                      // 16-byte pieces of a row
+  int B, H, cap, budget, recent, parts;
 };
 
 constexpr int NT = 1024;
@@ -29,23 +38,62 @@ __device__ __forceinline__ uint32_t rank_of(float w) {
 constexpr int kWaves = NT / 64, kRegs = 16;  // weights per lane held in registers: NT * kRegs keys
 constexpr int kBins = 2048;
 
-// One workgroup per (sequence, head); wave i takes the i-th of 16 runs of the
-// keys.  A radix select by 11, 11 and 10 bits of the rank finds the rank of the
+// 16 bytes of each of U pieces of kept rows (of k and of v) per thread.  They
+// are read for the last time, so the loads leave the caches alone.  (Two pieces:
+// 40.5 us in the case above, 42.0 with four, 44.0 with eight.)
+template <int U>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, const int32_t* kept, int b, int h, int lo, int hi) {
+  const int32_t *table = a.table + b * a.table_ld, *out_table = a.out_table + b * a.out_ld;
+  const uint32_t pieces = (uint32_t)(hi - lo) * a.row16.d;
+  for (uint32_t at0 = threadIdx.x; at0 < pieces; at0 += U * NT) {
+    u32x4 k[U], v[U];
+    int64_t to_k[U], to_v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t at = at0 + u * NT, r = a.row16.div(min(at, pieces - 1)), piece = min(at, pieces - 1) - r * a.row16.d;
+      const int i = lo + (int)r, j = kept[i];
+      const uint32_t tp = a.out_page.div(i), sp = a.page.div(j);
+      const int64_t to = out_table[tp], from = table[sp];
+      const int64_t ti = i - (int)(tp * a.out_page.d), si = j - (int)(sp * a.page.d);
+      k[u] = v[u] = u32x4{0, 0, 0, 0};
+      if (from >= 0 && from < a.n_pages) {  // strides in 16-byte pieces
+        k[u] = __builtin_nontemporal_load(static_cast<const u32x4*>(a.k.p) +
+                                          (from * a.k.s_page + h * a.k.s_head + si * a.k.s_slot + piece));
+        v[u] = __builtin_nontemporal_load(static_cast<const u32x4*>(a.v.p) +
+                                          (from * a.v.s_page + h * a.v.s_head + si * a.v.s_slot + piece));
+      }
+      const bool ok = at < pieces && to >= 0 && to < a.n_out_pages;
+      to_k[u] = ok ? to * a.ko.s_page + h * a.ko.s_head + ti * a.ko.s_slot + piece : -1;
+      to_v[u] = to * a.vo.s_page + h * a.vo.s_head + ti * a.vo.s_slot + piece;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (to_k[u] < 0) continue;
+      static_cast<u32x4*>(const_cast<void*>(a.ko.p))[to_k[u]] = k[u];
+      static_cast<u32x4*>(const_cast<void*>(a.vo.p))[to_v[u]] = v[u];
+    }
+  }
+}
+
+// Wave i of a workgroup takes the i-th of 16 runs of the keys.  A radix select by 11, 11 and 10 bits of the rank finds the rank of the
 // last key that stays and how many of its equals do (the first ones); each wave
 // then counts its keys above and at that rank, one exchange of the counts gives
 // every wave its place, and a second sweep lists the kept keys in order.
 // HELD: a lane's weights stay in registers over the five sweeps (they cover
 // tables of up to 16384 keys); else each sweep reads them again, from L2.
 template <bool HELD>
-__global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {
-  __shared__ uint32_t hist[kBins], wave_sum[kWaves], sh_bin, sh_left, cnt_above[kWaves], cnt_equal[kWaves];
-  const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, tid = threadIdx.x, lane = tid & 63;
+__global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
+  __shared__ uint32_t hist[kBins], wave_sum[kWaves], sh_bin, sh_left, sh_all, cnt_above[kWaves], cnt_equal[kWaves];
+  const int bh = blockIdx.x / a.parts, part = blockIdx.x - bh * a.parts;
+  const int b = bh / a.H, h = bh - b * a.H, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = min(max(a.lens[b], 0), a.cap), m = min(n, a.budget);
   const int old = n - min(a.recent, m);  // keys from here on stay
   const float* w = a.w + b * a.w_b + h * a.w_h;
-  int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
-  if (h == 0 && tid == 0) a.new_lens[b] = m;
+  int32_t* kept = a.kept + (int64_t)bh * a.budget;
+  if (h == 0 && part == 0 && tid == 0) a.new_lens[b] = m;
+  // this workgroup's kept keys
+  const int lo = (int)((int64_t)m * part / a.parts), hi = (int)((int64_t)m * (part + 1) / a.parts);
   const int steps = (n + NT - 1) / NT, first = wave * steps * 64;  // this wave's keys: `steps` of 64
 
   // weights of the U steps from step i0 on: the loads take a valid address
@@ -92,8 +140,8 @@ __global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {
       });
       __syncthreads();
       // keys in this thread's two bins and in all bins above them
-      const uint32_t hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
-      uint32_t sum = hi + lo;
+      const uint32_t upper = hist[kBins - 1 - 2 * tid], lower = hist[kBins - 2 - 2 * tid];
+      uint32_t sum = upper + lower;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const uint32_t x = __shfl_up(sum, o, 64);
@@ -101,16 +149,21 @@ __global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {
       }
       if (lane == 63) wave_sum[wave] = sum;
       __syncthreads();
-      uint32_t above = sum - hi - lo;
+      uint32_t above = sum - upper - lower;
       for (int i = 0; i < wave; ++i) above += wave_sum[i];
-      if (above < equals && equals <= above + hi + lo) {  // one thread
-        const bool in_hi = equals <= above + hi;
-        sh_bin = kBins - 1 - 2 * tid - (in_hi ? 0 : 1);
-        sh_left = equals - above - (in_hi ? 0u : hi);
+      if (above < equals && equals <= above + upper + lower) {  // one thread
+        const bool in_upper = equals <= above + upper;
+        sh_bin = kBins - 1 - 2 * tid - (in_upper ? 0 : 1);
+        sh_left = equals - above - (in_upper ? 0u : upper);
+        sh_all = sh_left == (in_upper ? upper : lower);
       }
       __syncthreads();
       limit |= sh_bin << shift;
       equals = sh_left;
+      if (sh_all) {  // the whole bin stays: all ranks from its first on, which is not 0 as need < old
+        limit -= 1, equals = 0;
+        break;
+      }
     }
   } else if (need == 0) {
     limit = 0xffffffffu, equals = 0;  // none of them stays
@@ -137,49 +190,29 @@ __global__ __launch_bounds__(NT) void evict_select(EvictArgs a) {
     const bool stay = j < n && (!is_old || r > limit || (r == limit && eq + __popcll(be & below) < equals));
     const uint64_t bs = __ballot(stay);
     const uint32_t to = at + __popcll(bs & below);
-    if (stay && to < (uint32_t)m) {
+    if (stay && to >= (uint32_t)lo && to < (uint32_t)hi) {
       kept[to] = j;
-      if (HELD && w_out) w_out[to] = x;  // every wave holds its own: they may lie where the weights did
+      // (one part alone may write where the weights are: its waves hold theirs)
+      if (HELD && w_out) w_out[to] = x;
     }
     at += __popcll(bs);
     eq += __popcll(be);
   });
-  for (int j = m + tid; j < a.budget; j += NT) kept[j] = -1;
-  if (HELD || !w_out) return;
-  // the kept weights, which may go where the weights are: a kept key's place is
-  // never behind it, so a step's writes lie before every later step's reads
-  __syncthreads();
-  for (int i0 = 0; i0 < m; i0 += NT) {
-    const int i = i0 + tid;
-    const float x = i < m ? w[kept[i]] : 0.f;
-    __syncthreads();
-    if (i < m) w_out[i] = x;
+  if (part == 0)
+    for (int j = m + tid; j < a.budget; j += NT) kept[j] = -1;
+  __syncthreads();  // the list is written
+  if (!HELD && w_out) {
+    // the kept weights, which one part alone may write where the weights are: a
+    // kept key's place is never behind it, so a step's writes lie before every
+    // later step's reads
+    for (int i0 = lo; i0 < hi; i0 += NT) {
+      const int i = i0 + tid;
+      const float x = i < hi ? w[kept[i]] : 0.f;
+      __syncthreads();
+      if (i < hi) w_out[i] = x;
+    }
   }
-}
-
-// 16 bytes of one kept row of k and of v per thread.  They are read for the last
-// time, so the loads leave the caches alone (8 x 8 heads, 2048 keys each: 48 -> 43 us
-// for the whole call).
-__global__ __launch_bounds__(256) void evict_move(EvictArgs a) {
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = at / a.row16;
-  const int piece = (int)(at - row * a.row16);
-  if (row >= (int64_t)a.B * a.H * a.budget) return;
-  const int64_t bh = row / a.budget;
-  const int i = (int)(row - bh * a.budget), b = (int)(bh / a.H), h = (int)(bh - (int64_t)b * a.H);
-  const int j = a.kept[row];
-  if (j < 0) return;
-  const uint32_t tp = a.out_page.div(i), sp = a.page.div(j);
-  const int64_t to = a.out_table[b * a.out_ld + tp], from = a.table[b * a.table_ld + sp];
-  if (to < 0 || to >= a.n_out_pages) return;
-  const uint32_t ti = i - tp * a.out_page.d, si = j - sp * a.page.d;
-  u32x4 k = u32x4{0, 0, 0, 0}, v = u32x4{0, 0, 0, 0};
-  if (from >= 0 && from < a.n_pages) {  // strides in 16-byte pieces
-    k = __builtin_nontemporal_load(static_cast<const u32x4*>(a.k.p) + (from * a.k.s_page + h * a.k.s_head + si * a.k.s_slot + piece));
-    v = __builtin_nontemporal_load(static_cast<const u32x4*>(a.v.p) + (from * a.v.s_page + h * a.v.s_head + si * a.v.s_slot + piece));
-  }
-  static_cast<u32x4*>(const_cast<void*>(a.ko.p))[to * a.ko.s_page + h * a.ko.s_head + ti * a.ko.s_slot + piece] = k;
-  static_cast<u32x4*>(const_cast<void*>(a.vo.p))[to * a.vo.s_page + h * a.vo.s_head + ti * a.vo.s_slot + piece] = v;
+  move_rows<2>(a, kept, b, h, lo, hi);
 }
 
 }  // namespace
@@ -206,6 +239,8 @@ extern "C" int32_t catopt_hip_paged_evict(int32_t dtype, int64_t B, int64_t Hkv,
     return CATOPT_E_UNSUPPORTED;
   if (n_table * page_size > lim || !grid_fits(B * Hkv, NT)) return CATOPT_E_UNSUPPORTED;  // B Hkv < 2^22
   if (n_out_table * out_page_size < budget) return CATOPT_E_INVAL;
+  // a head's kept rows are counted in 16-byte pieces, in 31 bits
+  if ((budget < n_table * page_size ? budget : n_table * page_size) * (row / 16) > lim) return CATOPT_E_UNSUPPORTED;
   if (B == 0) return CATOPT_OK;
   const int64_t step = 16 / (dtype == CATOPT_BF16 ? 2 : 4);
   if (!strides || !strides_fit(strides, 12, step) || !strides_fit(strides + 12, 4, 1)) return CATOPT_E_INVAL;
@@ -242,16 +277,20 @@ extern "C" int32_t catopt_hip_paged_evict(int32_t dtype, int64_t B, int64_t Hkv,
   a.n_pages = n_pages, a.n_out_pages = n_out_pages;
   a.page = FastDiv::of(page_size), a.out_page = FastDiv::of(out_page_size);
   a.B = (int)B, a.H = (int)Hkv, a.cap = (int)(n_table * page_size), a.budget = (int)budget, a.recent = (int)recent;
-  a.row16 = (int)(row / 16);
-  const int64_t blocks = (B * Hkv * budget * a.row16 + 255) / 256;  // the product is below 2^62
-  if (!grid_fits(blocks, 256)) return CATOPT_E_UNSUPPORTED;
+  a.row16 = FastDiv::of(row / 16);
+  // parts that together fill the CUs once, of 64 rows at least (with 512 in all the
+  // larger case above takes 48 us: a second choice for every CU); one where the
+  // weights move in place, as the others would still be reading them
+  int64_t parts = 256 / (B * Hkv);
+  if (parts > (budget + 63) / 64) parts = (budget + 63) / 64;
+  if (parts < 1 || (weights_out && weights_out == weights)) parts = 1;
+  a.parts = (int)parts;
+  const dim3 grid((uint32_t)(B * Hkv * parts));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.cap <= NT * kRegs)
-    evict_select<true><<<dim3((uint32_t)(B * Hkv)), dim3(NT), 0, st>>>(a);
+    evict_kernel<true><<<grid, dim3(NT), 0, st>>>(a);
   else
-    evict_select<false><<<dim3((uint32_t)(B * Hkv)), dim3(NT), 0, st>>>(a);
-  CATOPT_LAUNCH_CHECK();
-  evict_move<<<dim3((uint32_t)blocks), dim3(256), 0, st>>>(a);
+    evict_kernel<false><<<grid, dim3(NT), 0, st>>>(a);
   CATOPT_LAUNCH_CHECK();
   return CATOPT_OK;
 }
