@@ -1,5 +1,7 @@
 // What the kernels of the paged cache share: the page arithmetic.
 #pragma once
+#include <initializer_list>
+
 #include "common.hpp"
 
 namespace catopt {
@@ -50,11 +52,20 @@ inline int32_t allow_lds(const void* kernel, int bytes, bool* done) {
   return CATOPT_OK;
 }
 
-inline bool strides_fit(const int64_t* s, int n, int64_t step) {
-  for (int i = 0; i < n; ++i)
-    if (s[i] < 0 || s[i] % step) return false;
-  return true;
-}
+// Strides as the kernels take them: none negative, multiples of `step`; that of
+// an axis of one entry, which may be anything, as 0.
+struct Strides {
+  int64_t s[16];
+  bool fit = true;
+  Strides(const int64_t* in, std::initializer_list<int64_t> extents, int64_t step) {
+    int i = 0;
+    for (const int64_t n : extents) {
+      s[i] = n > 1 ? in[i] : 0;
+      if (s[i] < 0 || s[i] % step) fit = false;
+      ++i;
+    }
+  }
+};
 
 // A tensor's layout for the checks of what may overlap what: up to four axes,
 // extents and strides in elements, and the size of one.

@@ -117,29 +117,31 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   if (B == 0 || (N == 0 && !weights_out)) return CATOPT_OK;
   if ((N > 0 && (!q || !o)) || !kv_lens || !q_starts || !strides || (n_table > 0 && !block_table)) return CATOPT_E_INVAL;
   if (n_pages > 0 && (!k_pages || !v_pages)) return CATOPT_E_INVAL;
-  if (!strides_fit(strides, 10, 8) || !strides_fit(strides + 10, 4, 1)) return CATOPT_E_INVAL;
+  const Strides rows(strides, {N, Hq, n_pages, Hkv, page_size, n_pages, Hkv, page_size, N, Hq}, 8);
+  const Strides sums(strides + 10, {B, Hkv, B, Hkv}, 1);
+  if (!rows.fit || !sums.fit) return CATOPT_E_INVAL;
+  const int64_t *s = rows.s, *w = sums.s;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o)) return CATOPT_E_INVAL;
   if (weights_in && !weights_out) return CATOPT_E_INVAL;
-  const Layout out = layout3(o, 2, N, strides[8], Hq, strides[9], d), lq = layout3(q, 2, N, strides[0], Hq, strides[1], d);
-  const Layout lk = layout_pages(k_pages, 2, n_pages, Hkv, page_size, d, strides + 2);
-  const Layout lv = layout_pages(v_pages, 2, n_pages, Hkv, page_size, d, strides + 5);
+  const Layout out = layout3(o, 2, N, s[8], Hq, s[9], d), lq = layout3(q, 2, N, s[0], Hq, s[1], d);
+  const Layout lk = layout_pages(k_pages, 2, n_pages, Hkv, page_size, d, s + 2);
+  const Layout lv = layout_pages(v_pages, 2, n_pages, Hkv, page_size, d, s + 5);
   if (out.folded() || out.overlaps(lq) || out.overlaps(lk) || out.overlaps(lv)) return CATOPT_E_INVAL;
   if (weights_out) {
     const int64_t cap = n_table * page_size;
-    const Layout wo = layout3(weights_out, 4, B, strides[12], Hkv, strides[13], cap);
-    const Layout wi = layout3(weights_in, 4, B, strides[10], Hkv, strides[11], cap);
+    const Layout wo = layout3(weights_out, 4, B, w[2], Hkv, w[3], cap);
+    const Layout wi = layout3(weights_in, 4, B, w[0], Hkv, w[1], cap);
     if (wo.folded() || wo.overlaps(lq) || wo.overlaps(lk) || wo.overlaps(lv) || wo.overlaps(out)) return CATOPT_E_INVAL;
     if (weights_in && ((wo.overlaps(wi) && !wo.same(wi)) || out.overlaps(wi))) return CATOPT_E_INVAL;
   }
   // the rows of one load lie within 31 bits of its resource's base
-  if (strides[4] > (1 << 26) || strides[7] > (1 << 26)) return CATOPT_E_UNSUPPORTED;
+  if (s[4] > (1 << 26) || s[7] > (1 << 26)) return CATOPT_E_UNSUPPORTED;
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return CATOPT_E_WORKSPACE;
   PagedArgs a{};
-  const int64_t* s = strides;
   a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k_pages);
   a.v = static_cast<const uint16_t*>(v_pages), a.o = static_cast<uint16_t*>(o);
   a.q_t = s[0], a.q_h = s[1], a.k_p = s[2], a.k_h = s[3], a.k_s = s[4], a.v_p = s[5], a.v_h = s[6], a.v_s = s[7];
-  a.o_t = s[8], a.o_h = s[9], a.wi_b = s[10], a.wi_h = s[11], a.wo_b = s[12], a.wo_h = s[13];
+  a.o_t = s[8], a.o_h = s[9], a.wi_b = w[0], a.wi_h = w[1], a.wo_b = w[2], a.wo_h = w[3];
   a.table = block_table, a.lens = kv_lens, a.starts = q_starts, a.table_ld = table_ld, a.n_pages = n_pages, a.N = N;
   a.m_out = m_out, a.l_out = l_out, a.w_in = weights_in, a.w_out = weights_out;
   a.page = FastDiv::of(page_size), a.group = FastDiv::of(Hq / Hkv);

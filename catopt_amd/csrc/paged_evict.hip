@@ -243,18 +243,22 @@ extern "C" int32_t catopt_hip_paged_evict(int32_t dtype, int64_t B, int64_t Hkv,
   if ((budget < n_table * page_size ? budget : n_table * page_size) * (row / 16) > lim) return CATOPT_E_UNSUPPORTED;
   if (B == 0) return CATOPT_OK;
   const int64_t step = 16 / (dtype == CATOPT_BF16 ? 2 : 4);
-  if (!strides || !strides_fit(strides, 12, step) || !strides_fit(strides + 12, 4, 1)) return CATOPT_E_INVAL;
+  if (!strides) return CATOPT_E_INVAL;
+  const Strides rows(strides, {n_pages, Hkv, page_size, n_pages, Hkv, page_size, n_out_pages, Hkv, out_page_size,
+                               n_out_pages, Hkv, out_page_size}, step);
+  const Strides sums(strides + 12, {B, Hkv, B, Hkv}, 1);
+  if (!rows.fit || !sums.fit) return CATOPT_E_INVAL;
   if (!kv_lens || !kept || !new_lens || !out_table || (n_table > 0 && (!block_table || !weights))) return CATOPT_E_INVAL;
   if ((n_pages > 0 && (!k_pages || !v_pages)) || (n_out_pages > 0 && (!k_out || !v_out))) return CATOPT_E_INVAL;
   if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(k_out) || !aligned16(v_out)) return CATOPT_E_INVAL;
-  const int64_t* s = strides;
+  const int64_t *s = rows.s, *sw = sums.s;
   const int64_t size = 16 / step;
   const Layout lk = layout_pages(k_pages, size, n_pages, Hkv, page_size, d, s);
   const Layout lv = layout_pages(v_pages, size, n_pages, Hkv, page_size, d, s + 3);
   const Layout ko = layout_pages(k_out, size, n_out_pages, Hkv, out_page_size, d, s + 6);
   const Layout vo = layout_pages(v_out, size, n_out_pages, Hkv, out_page_size, d, s + 9);
-  const Layout w = layout3(weights, 4, B, s[12], Hkv, s[13], n_table * page_size);
-  const Layout wo = layout3(weights_out, 4, B, s[14], Hkv, s[15], budget);
+  const Layout w = layout3(weights, 4, B, sw[0], Hkv, sw[1], n_table * page_size);
+  const Layout wo = layout3(weights_out, 4, B, sw[2], Hkv, sw[3], budget);
   // the same pool keeps its place in both roles; keys and values may be parts
   // of one storage, so only their beginnings tell them apart
   const bool pool = k_out == k_pages;
@@ -272,7 +276,7 @@ extern "C" int32_t catopt_hip_paged_evict(int32_t dtype, int64_t B, int64_t Hkv,
   a.ko = Pages{k_out, s[6] / step, s[7] / step, s[8] / step};
   a.vo = Pages{v_out, s[9] / step, s[10] / step, s[11] / step};
   a.w = weights, a.w_out = weights_out, a.kept = kept, a.new_lens = new_lens;
-  a.w_b = s[12], a.w_h = s[13], a.wo_b = s[14], a.wo_h = s[15];
+  a.w_b = sw[0], a.w_h = sw[1], a.wo_b = sw[2], a.wo_h = sw[3];
   a.table = block_table, a.out_table = out_table, a.lens = kv_lens, a.table_ld = table_ld, a.out_ld = out_table_ld;
   a.n_pages = n_pages, a.n_out_pages = n_out_pages;
   a.page = FastDiv::of(page_size), a.out_page = FastDiv::of(out_page_size);

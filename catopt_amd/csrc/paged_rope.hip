@@ -325,18 +325,20 @@ extern "C" int32_t catopt_hip_qk_norm_rope(int32_t dtype, int64_t N, int64_t Hq,
   if (dtype != CATOPT_F32 && dtype != CATOPT_BF16) return CATOPT_E_UNSUPPORTED;
   if (d > kMaxD || Hq > (1 << 20) || Hkv > (1 << 20) || N > (1LL << 40)) return CATOPT_E_UNSUPPORTED;
   if (N == 0 || Hq + Hkv == 0) return CATOPT_OK;
-  if (!strides || !positions || (Hq && (!q || !q_out)) || (Hkv && (!k || !k_out))) return CATOPT_E_INVAL;
+  if (!strides || !positions || (Hq && (!q || !q_out)) || (Hkv && (!k || (!k_out && !(slots && n_pages == 0)))))
+    return CATOPT_E_INVAL;
   if (rot > 0 && n_pos > 0 && (!cos || !sin || ld_table < rot / 2)) return CATOPT_E_INVAL;
-  const int n_strides = slots ? 12 : 4;
-  if (!strides_fit(strides, n_strides, 1)) return CATOPT_E_INVAL;
-  if (slots && ((Hkv && (!v || !v_out)) || n_pages < 0 || page_size < 1)) return CATOPT_E_INVAL;
+  if (slots && ((Hkv && (!v || (n_pages > 0 && !v_out))) || n_pages < 0 || page_size < 1)) return CATOPT_E_INVAL;
+  const int64_t np = slots ? n_pages : 0, ns = slots ? page_size : 0, nv = slots ? N : 0;
+  const Strides st(strides, {N, Hq, N, Hkv, nv, Hkv, np, Hkv, ns, np, Hkv, ns}, 1);
+  if (!st.fit) return CATOPT_E_INVAL;
   if (slots) {
     if (n_pages > (1LL << 31) || page_size > (1LL << 31) || n_pages * page_size >= (1LL << 31)) return CATOPT_E_UNSUPPORTED;
     const int64_t size = dtype == CATOPT_BF16 ? 2 : 4;
-    const Layout lk = layout_pages(k_out, size, n_pages, Hkv, page_size, d, strides + 6);
-    const Layout lv = layout_pages(v_out, size, n_pages, Hkv, page_size, d, strides + 9);
-    const Layout in[3] = {layout3(q, size, N, strides[0], Hq, strides[1], d), layout3(k, size, N, strides[2], Hkv, strides[3], d),
-                          layout3(v, size, N, strides[4], Hkv, strides[5], d)};
+    const Layout lk = layout_pages(k_out, size, n_pages, Hkv, page_size, d, st.s + 6);
+    const Layout lv = layout_pages(v_out, size, n_pages, Hkv, page_size, d, st.s + 9);
+    const Layout in[3] = {layout3(q, size, N, st.s[0], Hq, st.s[1], d), layout3(k, size, N, st.s[2], Hkv, st.s[3], d),
+                          layout3(v, size, N, st.s[4], Hkv, st.s[5], d)};
     // keys and values may be parts of one storage, so their ranges may interleave
     if (lk.folded() || lv.folded() || (k_out == v_out && !lk.empty())) return CATOPT_E_INVAL;
     for (const Layout& x : in)
@@ -346,11 +348,11 @@ extern "C" int32_t catopt_hip_qk_norm_rope(int32_t dtype, int64_t N, int64_t Hq,
   a.q = q, a.k = k, a.v = v, a.qw = q_weight, a.kw = k_weight;
   a.cos = cos, a.sin = sin, a.pos = positions, a.slots = slots;
   a.q_out = q_out, a.k_out = k_out, a.v_out = v_out;
-  a.q_st = strides[0], a.q_sh = strides[1], a.k_st = strides[2], a.k_sh = strides[3];
+  a.q_st = st.s[0], a.q_sh = st.s[1], a.k_st = st.s[2], a.k_sh = st.s[3];
   if (slots) {
-    a.v_st = strides[4], a.v_sh = strides[5];
-    a.ko_p = strides[6], a.ko_h = strides[7], a.ko_s = strides[8];
-    a.vo_p = strides[9], a.vo_h = strides[10], a.vo_s = strides[11];
+    a.v_st = st.s[4], a.v_sh = st.s[5];
+    a.ko_p = st.s[6], a.ko_h = st.s[7], a.ko_s = st.s[8];
+    a.vo_p = st.s[9], a.vo_h = st.s[10], a.vo_s = st.s[11];
   }
   a.N = N, a.n_pos = n_pos, a.ld_table = ld_table;
   a.n_slots = slots ? n_pages * page_size : 0;

@@ -71,7 +71,8 @@ def _launch(dev: int, fn, *args) -> int:
 
 
 def _heads(name: str, t: torch.Tensor) -> tuple[torch.Tensor, torch.Size, tuple]:
-    """``(N, H, d)`` with a contiguous last axis, rows readable in 16-byte pieces; its shape and strides."""
+    """``(N, H, d)`` with a contiguous last axis, rows readable in 16-byte pieces where a copy makes them so; its shape
+    and strides."""
     if t.dim() != 3:
         raise ValueError(f"{name} is (tokens, heads, head dim), got {tuple(t.shape)}")
     s = t.stride()
@@ -134,8 +135,9 @@ def _norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleave
     rot = 2 * half
     if rot > d:
         raise ValueError(f"the tables rotate {rot} dims of a head of {d}")
-    if rot and (cos.stride() != sin.stride() or cos.stride(1) != 1):
-        cos, sin = cos.contiguous(), sin.contiguous()
+    ld = cos.stride(0)
+    if rot and (cos.stride() != sin.stride() or cos.stride(1) != 1 or ld < half):
+        cos, sin, ld = cos.contiguous(), sin.contiguous(), half
     qw = kw = vp = slots_p = None
     if q_weight is not None:
         q_weight = _norm_weight(q_weight, q, d)
@@ -161,7 +163,7 @@ def _norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleave
         k_out, v_out = q.new_empty((N, Hkv, d)), None
         strides = _S12(qs[0], qs[1], ks[0], ks[1], 0, 0, 0, 0, 0, 0, 0, 0)
     st = _launch(dev, lib.catopt_hip_qk_norm_rope, dt, N, Hq, Hkv, d, rot, 1 if interleaved else 0, q.data_ptr(),
-                 k.data_ptr(), vp, qw, kw, eps, cos.data_ptr(), sin.data_ptr(), n_pos, cos.stride(0) if rot else 0,
+                 k.data_ptr(), vp, qw, kw, eps, cos.data_ptr(), sin.data_ptr(), n_pos, ld,
                  positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), v_out, strides, slots_p, n_pages, page,
                  _stream(q))
     _check("qk_norm_rope", st)
@@ -237,7 +239,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     key head ``h // (Hq // Hkv)``.  ``d`` is a multiple of 8 up to 128, the
     page size a multiple of 8.
 
-    Returns ``o (N, Hq, d)``, written to ``out`` when given; rows behind the
+    Returns ``o (N, Hq, d)``, written to ``out`` when given (memory of its
+    own: not between the operands' first and last rows); rows behind the
     last sequence are neither read nor written.  ``return_ml`` adds the fp32
     ``(m, l)`` om carriers of the sequences' rows, ``(N, Hq)``, so that a part
     of the keys kept elsewhere can be combined.  A row that sees no key is NaN
@@ -257,6 +260,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if q.dtype != torch.bfloat16 or k_pages.dtype != q.dtype:
         raise NotImplementedError(f"paged attention runs on bf16 operands, got {q.dtype} and {k_pages.dtype} pages")
     q, (N, Hq, d), qs = _heads("q", q)
+    if q.data_ptr() % 16:
+        q = q.clone()
     (n_pages, Hkv, page, pd), ks, vs = _pages(k_pages, v_pages)
     if pd != d or Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"q has {Hq} heads of {d}, the pages {Hkv} heads of {pd}: the head dims agree and the query "
@@ -324,7 +329,8 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     in ``k_out, v_out (n_out_pages, Hkv, out_page_size, d)``, a cache of its
     own (say of a fixed size for generation) or, by default, ``k_pages,
     v_pages``.  In that case the pages of ``out_table`` are free ones: none
-    may be in ``block_table``, whose pages can be given back afterwards.
+    may be in ``block_table``, whose pages can be given back afterwards.  No
+    page is in ``out_table`` twice.
     Rows behind the last kept key are left as they were.
 
     Returns ``kept (B, Hkv, budget)`` int32 (the keys' indices, -1 behind the

@@ -314,6 +314,28 @@ def test_no_new_tokens_keep_the_weights():
         assert torch.equal(w[b, :, :n], before[b, :, :n]) and (w[b, :, n:] == 7).all()
 
 
+@pytest.mark.parametrize("nq", [1, 40])
+def test_axes_of_one_entry_and_queries_off_alignment(nq):
+    """The stride of an axis of one entry is no stride; queries that start between 16-byte pieces are copied."""
+    cache = Cache([100], 1, 64, 128, seed=3)
+    table, st = cache.table, ints([0, nq])
+    q = randn(gen(2), nq, 4, 64)
+    want = P.paged_attention(q, cache.k, cache.v, table, ints([100]), st, 0.1)
+    w = torch.zeros((1, 1, table.shape[1] * 128), device=DEV)
+    off = torch.empty((nq * 256 + 3,), dtype=BF16, device=DEV)[3:].view(nq, 4, 64)
+    off.copy_(q)
+    k, v = (t.as_strided(t.shape, (t.stride(0), 77, t.stride(2), 1)) for t in (cache.k, cache.v))  # one key head
+    w1 = w.as_strided(w.shape, (5, 3, 1))
+    assert torch.equal(P.paged_attention(off, k, v, table, ints([100]), st, 0.1, weights_out=w1), want)
+    page = int(table[0, 0])
+    k, v = (t[page:page + 1].as_strided((1, 1, 128, 64), (13, 77, 64, 1)) for t in (cache.k, cache.v))  # and one page
+    assert torch.equal(P.paged_attention(q, k, v, torch.zeros_like(table), ints([100]), st, 0.1), want)
+    if nq == 1:
+        q1 = q.as_strided(q.shape, (101, 64, 1))
+        out = torch.empty_like(q).as_strided(q.shape, (7, 64, 1))
+        assert torch.equal(P.paged_attention(q1, k, v, torch.zeros_like(table), ints([100]), st, 0.1, out=out), want)
+
+
 def test_nothing_to_do():
     cache = Cache([10], 2, 64, 16)
     e = torch.empty((0, 4, 64), dtype=BF16, device=DEV)

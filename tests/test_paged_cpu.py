@@ -61,8 +61,9 @@ def test_attention_refuses_overlaps(lib):
         return ok[:at] + list(v) + ok[at + len(v):]
 
     # q: 4 x 256 elements; pages: 8 x 2048; weights: 1 x 2 x 64 of 4 bytes
-    for kw in ({}, {"o": Q + 2048}, {"o": KP + 2 * 8 * 2048}, {"v": KP}, {"w_in": WIN}, {"w_in": WOUT},
-               {"w_out": Q + 2048}, {"w_in": WOUT + 512}, {"strides": strides(8, 512, 64)},
+    odd = [100, 1] + ok[2:8] + [3, 5, 7, 128, 9, 128]  # axes of one entry may have any stride
+    for kw in ({}, {"N": 1, "Hq": 1, "Hkv": 1, "strides": odd}, {"o": Q + 2048},
+               {"o": KP + 2 * 8 * 2048}, {"v": KP}, {"w_in": WIN}, {"w_in": WOUT}, {"w_out": Q + 2048}, {"w_in": WOUT + 512}, {"strides": strides(8, 512, 64)},
                {"strides": strides(8, 64, 256)}, {"N": 1, "strides": strides(8, 0, 64)}):
         assert ask(**kw) == L.E_WORKSPACE, kw
     for kw in ({"o": Q}, {"o": Q + 2032}, {"o": Q - 2032}, {"o": KP + 64}, {"o": VP + 2 * 8 * 2048 - 16}, {"w_out": Q + 2044},
@@ -126,7 +127,8 @@ def test_evict_refuses(lib):
                {"strides": [2048, 1024, 64] * 4 + [128, 64, 0, 64], "wo": WOUT, "B": 2}):
         assert _evict(lib, **kw) == L.E_INVAL, kw
     for kw in ({"dtype": 2}, {"d": 4}, {"d": 1 << 14}, {"B": 1 << 21}, {"H": 1 << 21}, {"B": 1 << 11, "H": 1 << 11},
-               {"n_table": 1 << 27}, {"budget": 1 << 31, "n_to": 1 << 28}):
+               {"n_table": 1 << 27}, {"budget": 1 << 31, "n_to": 1 << 28},
+               {"d": 1 << 12, "page": 1 << 20, "n_table": 4, "budget": 1 << 22, "n_to": 1 << 18}):
         assert _evict(lib, **kw) == L.E_UNSUPPORTED, kw
 
 

@@ -130,6 +130,24 @@ def test_keys_past_the_registers_of_a_workgroup():
             assert torch.equal(same[b, :, :m], w_to[b, :, :m]) and torch.equal(same[b, :, m:], w[b, :, m:])
 
 
+@pytest.mark.parametrize("lens,Hkv,budget", [([900], 1, 64), ([900], 1, 65), ([3000, 20], 3, 1000), ([600] * 200, 2, 130),
+                                             ([17000], 2, 4000)])
+def test_parts_of_a_head(lens, Hkv, budget):
+    """Heads whose kept rows one workgroup moves, and several; the weights apart and in place."""
+    cache, out = Cache(lens, Hkv, 16, 16, seed=budget), Cache([budget] * len(lens), Hkv, 16, 16, seed=2)
+    w = _weights(cache, 5)
+    same = w.clone()
+    args = (cache.k, cache.v, cache.table, ints(lens))
+    kept, new, w_to = P.paged_evict(*args, w, out.table, budget, 7, k_out=out.k, v_out=out.v)
+    _check(cache, w, budget, 7, kept, new, w_to, out)
+    ko, vo = torch.zeros_like(out.k), torch.zeros_like(out.v)
+    P.paged_evict(*args, same, out.table, budget, 7, k_out=ko, v_out=vo, weights_out=same)
+    for b, n in enumerate(lens):
+        m = min(n, budget)
+        assert torch.equal(same[b, :, :m], w_to[b, :, :m])
+        assert torch.equal(out.rows(ko, b, m), out.rows(out.k, b, m)) and torch.equal(out.rows(vo, b, m), out.rows(out.v, b, m))
+
+
 def test_captured():
     lens = [500, 260]
     cache, out = Cache(lens, 2, 64, 16), Cache([128, 128], 2, 64, 16, seed=2)

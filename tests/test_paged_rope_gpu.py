@@ -176,6 +176,26 @@ def test_rows_past_the_caches(dtype, N):
     _near(qo[-50:], q[-50:], w[0], cos, sin, pos[-50:], False)
 
 
+def test_one_row_of_the_tables_for_every_position_and_axes_of_one_entry():
+    q, k, v, w, cos, sin, _ = _case(6, 4, 1, 64, 64, BF16, True)
+    pos = torch.arange(6, device=DEV)
+    c, s = (t[5:6].expand(6, -1) for t in (cos, sin))
+    qo, ko = P.qk_norm_rope(q, k, c, s, pos, *w)
+    wq, wk = P.qk_norm_rope(q, k, cos, sin, torch.full_like(pos, 5), *w)
+    assert torch.equal(qo, wq) and torch.equal(ko, wk)
+    one = (t[5:6].as_strided((1, 32), (3, 1)) for t in (cos, sin))
+    k1 = k.as_strided(k.shape, (k.stride(0), 19, 1))  # one key head
+    qo, ko = P.qk_norm_rope(q, k1, *one, torch.zeros_like(pos), *w)
+    assert torch.equal(qo, wq) and torch.equal(ko, wk)
+
+
+def test_no_pages():
+    q, k, v, w, cos, sin, pos = _case(6, 4, 2, 64, 64, BF16, True)
+    none = torch.empty((0, 2, 16, 64), dtype=BF16, device=DEV)
+    qo = P.qk_norm_rope_append(q, k, v, cos, sin, pos, none, none.clone(), torch.full_like(pos, -1), *w)
+    _near(qo, q, w[0], cos, sin, pos, False)
+
+
 def test_no_tokens():
     q, k, v, w, cos, sin, pos = _case(0, 4, 2, 64, 64, BF16, True)
     qo, ko = P.qk_norm_rope(q, k, cos, sin, pos, *w)
