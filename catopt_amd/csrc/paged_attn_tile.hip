@@ -41,7 +41,7 @@ __device__ __forceinline__ void pin(const bf16x8& x) { asm volatile("" ::"v"(__b
 __device__ __forceinline__ void pin(float x) { asm volatile("" ::"v"(x)); }
 
 template <int D>
-__global__ __launch_bounds__(NT, 2) void paged_tile_kernel(PagedArgs a, int tiles) {
+__global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(PagedArgs a, int tiles) {
   using L = TileLds<D>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
