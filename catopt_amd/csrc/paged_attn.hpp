@@ -241,6 +241,19 @@ __device__ __forceinline__ void take_odd_values(bf16x8* vf, const bf16x8* p, f32
   }
 }
 
+// -inf for the scores of the keys from `first` + `room` + 1 on, and of the groups
+// of 8 from `first` on whose bit in `bad` is set.  One comparison a score: the
+// row's limit and the keys' end come as one number.
+__device__ __forceinline__ void mask_scores(f32x16& s, int room, uint32_t bad) {
+  const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = acc_row(r, 0) <= room - 4 * g ? s[r] : kNegInf;
+  if (bad) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = (bad >> (r >> 2)) & 1 ? kNegInf : s[r];
+  }
+}
+
 // Host side of each kernel.
 constexpr int kFewRows = 32, kTileRows = 128;
 constexpr int kMaxSplits = 64;  // key ranges of a tile: one per lane of the wave that combines them

@@ -83,7 +83,7 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
     if (live && 16 * j + 8 * g < a.d) w = *reinterpret_cast<const u32x4*>(q + 16 * j + 8 * g);
     qf[j] = __builtin_bit_cast(bf16x8, w);
   }
-  const int lim = x.off + tok;  // last key this row sees
+  const int lim = min(x.off + tok, x.len - 1);  // last key this row sees
 
   // a lane's 16 bytes of load k: row k ROWS + lane / CH of the stage, row & 7 of
   // its group; the swizzles depend on a row's place among 16 (K, D = 128: loads
@@ -147,14 +147,7 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
       s = mfma32x32x16(*reinterpret_cast<const bf16x8*>(Ks + tile_off<D>(l32, 2 * j + g)), qf[j], s);
     // some row does not see some key: the first row sees the fewest
     const bool masked = key0 + 32 > x.len || key0 + 31 > x.off + x.r0 / a.G || bad_now;
-    if (masked) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = key0 + acc_row(r, g);
-        const bool keep = key < x.len && key <= lim && !((bad_now >> (acc_row(r, g) >> 3)) & 1);
-        s[r] = keep ? s[r] : kNegInf;
-      }
-    }
+    if (masked) mask_scores(s, lim - key0, bad_now);
     if (srow && live) {
 #pragma unroll
       for (int rg = 0; rg < 4; ++rg) {

@@ -63,7 +63,7 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
     if (live && 16 * j + 8 * g < a.d) w = *reinterpret_cast<const u32x4*>(q + 16 * j + 8 * g);
     qf[j] = __builtin_bit_cast(bf16x8, w);
   }
-  const int lim = x.off + tok;  // last key this row sees
+  const int lim = min(x.off + tok, x.len - 1);  // last key this row sees
   // of the wave's rows the first sees the fewest keys, the last the most
   const int w0 = x.r0 + 32 * wave, w1 = min(w0 + 31, x.r0 + x.rows - 1);
   const int lim0 = __builtin_amdgcn_readfirstlane(x.off + (int)a.group.div(w0));
@@ -153,14 +153,7 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
 #pragma unroll
           for (int u = 0; u < 2; ++u) acc[db] = mfma32x32x16(vf[kb2][2 * db + u], p[u], acc[db]);
       };
-      auto apply_mask = [&](int kb2, f32x16& s) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int in = 32 * kb2 + acc_row(r, g), key = kv0 + in;
-          const bool keep = key < x.len && key <= lim && !((bad >> (in >> 3)) & 1);
-          s[r] = keep ? s[r] : kNegInf;
-        }
-      };
+      auto apply_mask = [&](int kb2, f32x16& s) { mask_scores(s, lim - kv0 - 32 * kb2, (bad >> (4 * kb2)) & 15u); };
       // row max of a half over both lane halves, the true max, and the lazy
       // move of the reference max; returns the factor for O^T (1: no move)
       auto half_max = [&](const f32x16& s) -> float {
