@@ -55,14 +55,6 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
 
   const int row = x.r0 + 32 * wave + l32, tok = (int)a.group.div(row), hq = h * a.G + row - tok * a.G;
   const bool live = 32 * wave + l32 < x.rows;
-  const uint16_t* q = a.q + (int64_t)(x.row0 + tok) * a.q_t + (int64_t)hq * a.q_h;
-  bf16x8 qf[D / 16];
-#pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
-    u32x4 w = u32x4{0, 0, 0, 0};
-    if (live && 16 * j + 8 * g < a.d) w = *reinterpret_cast<const u32x4*>(q + 16 * j + 8 * g);
-    qf[j] = __builtin_bit_cast(bf16x8, w);
-  }
   const int lim = min(x.off + tok, x.len - 1);  // last key this row sees
   // of the wave's rows the first sees the fewest keys, the last the most
   const int w0 = x.r0 + 32 * wave, w1 = min(w0 + 31, x.r0 + x.rows - 1);
@@ -111,11 +103,30 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
   };
 
   uint32_t bad = 0, bad_next = 0;  // a bit for each 8 keys of the tile whose page is invalid
+  bf16x8 qf[D / 16];
   if (t0 < t1) {
+    // the first pages' ids, the queries and the first tile are on their way
+    // together; the queries as whole rows through the second stage, four times
+    // fewer lines a load than as fragments
     next_page = group_page(a, table, key_of(t0), x.len);
+    const uint64_t q = reinterpret_cast<uint64_t>(a.q + (int64_t)(x.row0 + tok) * a.q_t + (int64_t)hq * a.q_h);
+    u32x4 qr[2 * L::LOADS];
+#pragma unroll
+    for (int i = 0; i < 2 * L::LOADS; ++i) {
+      const int r = i * L::ROWS + sub;
+      const uint32_t lo = __shfl((uint32_t)q, r, 64), hi = __shfl((uint32_t)(q >> 32), r, 64);
+      qr[i] = u32x4{0, 0, 0, 0};
+      if (32 * wave + r < x.rows && 8 * cp < a.d)
+        qr[i] = *reinterpret_cast<const u32x4*>((((uint64_t)hi << 32) | lo) + 16 * cp);
+    }
     places(t0);
     bad = (uint32_t)bads & 0xffu;
     issue(t0, 0);
+    char* Qs = lds + L::STAGE + wave * 32 * AttnRow<D>::BYTES;
+#pragma unroll
+    for (int i = 0; i < 2 * L::LOADS; ++i) *reinterpret_cast<u32x4*>(Qs + tile_off<D>(i * L::ROWS + sub, cp)) = qr[i];
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) qf[j] = *reinterpret_cast<const bf16x8*>(Qs + tile_off<D>(l32, 2 * j + g));
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
   }
@@ -250,9 +261,9 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
   // ---- epilogue: back to the true max, then the row or its range's carrier
   const float fix = m_true != kNegInf && m_run != kNegInf ? __builtin_amdgcn_exp2f((m_run - m_true) * c) : 1.f;
   const float l_sum = l_run + __shfl_xor(l_run, 32, 64);
-  if (!live) return;
   const int64_t i = (int64_t)(x.row0 + tok) * a.Hq + hq;
   if (x.splits > 1) {
+    if (!live) return;
     const int64_t rows = a.N * a.Hq, at = i * a.splits + split;
     if (g == 0) {
       a.part[2 * at] = m_true;
@@ -267,19 +278,28 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
             f32x4{acc[db][4 * rg] * fix, acc[db][4 * rg + 1] * fix, acc[db][4 * rg + 2] * fix, acc[db][4 * rg + 3] * fix};
     return;
   }
+  // the lane halves swap words, so that each stores 16 bytes: 8 columns of an
+  // even (g = 0) or odd eighth of every 32
   uint16_t* orow = a.o + (int64_t)(x.row0 + tok) * a.o_t + (int64_t)hq * a.o_h;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) {
 #pragma unroll
-    for (int rg = 0; rg < 4; ++rg) {
-      const int d = 32 * db + 8 * rg + 4 * g;
-      if (d < a.d)
-        *reinterpret_cast<u32x2*>(orow + d) =
-            u32x2{pack_bf16x2(finish(acc[db][4 * rg], l_sum, a.normalize), finish(acc[db][4 * rg + 1], l_sum, a.normalize)),
-                  pack_bf16x2(finish(acc[db][4 * rg + 2], l_sum, a.normalize), finish(acc[db][4 * rg + 3], l_sum, a.normalize))};
+    for (int rg = 0; rg < 4; rg += 2) {
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const f32x16& y = acc[db];
+        const int r = 4 * rg + 2 * e;
+        const auto sw = __builtin_amdgcn_permlane32_swap(
+            pack_bf16x2(finish(y[r], l_sum, a.normalize), finish(y[r + 1], l_sum, a.normalize)),
+            pack_bf16x2(finish(y[r + 4], l_sum, a.normalize), finish(y[r + 5], l_sum, a.normalize)), false, false);
+        w[e] = sw[0], w[2 + e] = sw[1];
+      }
+      const int d = 32 * db + 8 * (rg + g);
+      if (live && d < a.d) *reinterpret_cast<u32x4*>(orow + d) = w;
     }
   }
-  if (g == 0) row_stats(a, i, m_true, l_sum * fix);
+  if (live && g == 0) row_stats(a, i, m_true, l_sum * fix);
 }
 
 template <int D>
