@@ -11,19 +11,20 @@
 // V go global->LDS directly into two stages of its own.  A stage is loaded again
 // as soon as it has been used, and the wait for the other one leaves the new
 // loads in flight: the waves read nothing of each other's, so there is no
-// barrier in the loop.  The loads carry the non-temporal hint: 32 sequences'
-// step over 131072 keys 115 -> 103 us, a step over 47000 keys 55 -> 50.  A lane works out the place of 8 keys, the wave those of
-// 16 stages at once.
+// barrier in the loop.  The loads carry the non-temporal hint: a step of 32
+// sequences over 131072 keys 115 -> 102 us with the combination, 536 MB and so 5.4
+// TB/s; a step over 47000 keys with their weights 55 -> 50.  A lane works out the
+// place of 8 keys, the wave those of 16 stages at once.
 #include "paged_attn.hpp"
 
 namespace catopt {
 namespace {
 
-// Two waves (D = 64: four) of two stages fill half
-// a CU's LDS, so that two workgroups share it and one's start runs under the
-// other's loads: the form for long keys.  Eight waves of one stage (WIDE) have
-// 256 keys in flight at once: the form for one range of few keys, which spares
-// the second launch.
+// Two waves (D = 64: four) of two stages fill at most half a CU's LDS, so that
+// two workgroups share it and one's start runs under the other's loads: the form
+// for long keys.  Four waves at D = 128 took 182 us for the step above.  Eight
+// waves of one stage (WIDE) have 256 keys in flight at once: the form for one
+// range of few keys, which spares the second launch.
 template <int D, bool WIDE>
 struct Few {
   static constexpr int WAVES = WIDE ? 8 : D == 128 ? 2 : 4, NT = 64 * WAVES, STAGES = WIDE ? 1 : 2;

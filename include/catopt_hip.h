@@ -563,7 +563,8 @@ int32_t catopt_hip_silu_mul(int32_t dtype, int64_t n, const void* g,
  * The cache of one layer is two tensors of pages, k_pages and v_pages, each
  * [n_pages, Hkv, page_size, d] with a contiguous last axis and explicit
  * strides (element counts, order page, head, slot; multiples of 16 bytes, so
- * that a (n_pages, page_size, Hkv, d) storage is the same call).  Key j of
+ * that a (n_pages, page_size, Hkv, d) storage is the same call; that of an axis
+ * of one entry may be anything, here and in every strides array).  Key j of
  * sequence b lies in slot j % page_size of page block_table[b, j / page_size]
  * (int32, rows table_ld apart, n_table entries each); entries behind a
  * sequence's last page are never read.  A page index outside [0, n_pages) is
@@ -613,9 +614,10 @@ int32_t catopt_hip_qk_norm_rope(
  * A row that sees no key is NaN (normalize 1) or 0 (normalize 2).  m_out,
  * l_out (fp32 [N, Hq], optional): the row's om carrier, max s and sum of
  * exp(s - m); (-inf, 0) for an empty row.
- * weights_out (fp32 [B, Hkv, >= n_table * page_size], optional) receives each key's attention weight summed over the tokens and
- * the query heads of its group, on top of weights_in (the same layout; NULL:
- * zeros), which is not read for the new tokens' own keys:
+ * weights_out (fp32 [B, Hkv, >= n_table * page_size], optional) receives each
+ * key's attention weight summed over the tokens and the query heads of its
+ * group, on top of weights_in (the same layout; NULL: zeros), which is not read
+ * for the new tokens' own keys:
  *   weights_out[b, h, j] = (j < kv_len - n ? weights_in[b, h, j] : 0)
  *                          + sum_rows exp(s - m) / l,      j < kv_len
  * Entries from kv_len on are left as they were.  weights_out may be
@@ -651,8 +653,9 @@ int32_t catopt_hip_paged_attn_fwd(
  * count and size are their own (n_out_table * out_page_size >= budget).
  * kept (int32 [B, Hkv, budget]) holds their indices, then -1; new_lens
  * (int32 [B]) the counts; weights_out (fp32 [B, Hkv, >= budget], optional)
- * their weights.  The row of a key whose page index is invalid moves as zeros.  k_out / v_out may be k_pages / v_pages where no
- * page of out_table is one of block_table's; weights_out may be weights.
+ * their weights.  The row of a key whose page index is invalid moves as zeros.
+ * k_out / v_out may be k_pages / v_pages where no page of out_table is one of
+ * block_table's; no page is in out_table twice; weights_out may be weights.
  * F32 or BF16 rows of a multiple of 16 bytes; 1 <= budget.
  * strides (host, 16 values): k_pages, v_pages, k_out, v_out (page, head,
  * slot); weights, weights_out (sequence, head).
