@@ -117,7 +117,7 @@ SIGNATURES: dict[str, tuple] = {
     "catopt_hip_paged_evict": (
         _i32,
         [_i32, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64,
-         _i64, _p, _p, _p, _p, _p],
+         _i64, _p, _p, _p, _i32, _p, _p],
     ),
 }
 

@@ -23,7 +23,7 @@ struct EvictArgs {
   int64_t table_ld, out_ld, w_b, w_h, wo_b, wo_h, n_pages, n_out_pages;
   FastDiv page, out_page;
   FastDiv row16;                      // 16-byte pieces of a row
-  int B, H, cap, budget, recent, parts;
+  int B, H, cap, budget, recent, parts, clear;
 };
 
 constexpr int NT = 1024;
@@ -199,7 +199,10 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
     eq += __popcll(be);
   });
   if (part == 0)
-    for (int j = m + tid; j < a.budget; j += NT) kept[j] = -1;
+    for (int j = m + tid; j < a.budget; j += NT) {
+      kept[j] = -1;
+      if (w_out && a.clear) w_out[j] = 0.f;
+    }
   __syncthreads();  // the list is written
   if (!HELD && w_out) {
     // the kept weights, which one part alone may write where the weights are: a
@@ -227,7 +230,7 @@ extern "C" int32_t catopt_hip_paged_evict(int32_t dtype, int64_t B, int64_t Hkv,
                                           void* k_out, void* v_out, int64_t n_out_pages, int64_t out_page_size,
                                           const int32_t* out_table, int64_t out_table_ld, int64_t n_out_table,
                                           int32_t* kept, int32_t* new_lens, float* weights_out,
-                                          const int64_t* strides, void* stream) {
+                                          int32_t clear_behind, const int64_t* strides, void* stream) {
   if (dtype != CATOPT_F32 && dtype != CATOPT_BF16) return CATOPT_E_UNSUPPORTED;
   if (B < 0 || Hkv < 1 || d < 1 || n_pages < 0 || page_size < 1 || n_table < 0 || table_ld < 0)
     return CATOPT_E_INVAL;
@@ -288,7 +291,7 @@ extern "C" int32_t catopt_hip_paged_evict(int32_t dtype, int64_t B, int64_t Hkv,
   int64_t parts = 256 / (B * Hkv);
   if (parts > (budget + 63) / 64) parts = (budget + 63) / 64;
   if (parts < 1 || (weights_out && weights_out == weights)) parts = 1;
-  a.parts = (int)parts;
+  a.parts = (int)parts, a.clear = clear_behind != 0;
   const dim3 grid((uint32_t)(B * Hkv * parts));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.cap <= NT * kRegs)

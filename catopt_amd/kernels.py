@@ -30,10 +30,14 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _stream(t: torch.Tensor) -> int:
+def _stream_of(dev: int) -> int:
     if _raw_stream is not None:
-        return _raw_stream(t.get_device())
-    return torch.cuda.current_stream(t.device).cuda_stream
+        return _raw_stream(dev)
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _stream(t: torch.Tensor) -> int:
+    return _stream_of(t.get_device())
 
 
 def _need_device(*ts: torch.Tensor | None) -> int:

@@ -35,7 +35,7 @@ import struct
 import torch
 
 from . import _lib as L
-from .kernels import _DT, _need_device, _stream
+from .kernels import _DT, _need_device, _stream_of
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_append", "paged_attention", "paged_evict", "PAGED_ATTENTION_MAX_HEAD_DIM",
            "QK_NORM_ROPE_MAX_HEAD_DIM"]
@@ -47,40 +47,40 @@ QK_NORM_ROPE_MAX_HEAD_DIM = 256
 _S12, _S14, _S16 = (struct.Struct(f"{n}q").pack for n in (12, 14, 16))
 
 
-def _device(*ts: torch.Tensor | None) -> int:
+_get_device = torch.Tensor.get_device
+
+
+def _device(ts: tuple) -> int:
     """The device index that all operands share; raises as ``kernels`` does where they do not."""
     try:
-        dev = ts[0].get_device()
-        for t in ts:
-            if t is not None and t.get_device() != dev:
-                break
-        else:
+        devs = {*map(_get_device, ts)}
+        if len(devs) == 1:
+            dev = devs.pop()
             if dev >= 0:
                 return dev
-    except AttributeError:
+    except TypeError:  # not a tensor
         pass
     return _need_device(*ts)
 
 
 def _launch(dev: int, fn, *args) -> int:
-    """``fn(*args)`` with the operands' device as the current one."""
+    """``fn(*args, stream)`` with the operands' device as the current one."""
     if torch._C._cuda_getDevice() == dev:
-        return fn(*args)
+        return fn(*args, _stream_of(dev))
     with torch.cuda.device(dev):
-        return fn(*args)
+        return fn(*args, _stream_of(dev))
 
 
-def _heads(name: str, t: torch.Tensor) -> tuple[torch.Tensor, torch.Size, tuple]:
-    """``(N, H, d)`` with a contiguous last axis, rows readable in 16-byte pieces where a copy makes them so; its shape
-    and strides."""
-    if t.dim() != 3:
+def _heads(name: str, t: torch.Tensor, step: int) -> tuple[torch.Tensor, torch.Size, tuple, int]:
+    """``(N, H, d)`` with a contiguous last axis, rows readable in 16-byte pieces (``step`` elements) where a copy makes
+    them so; its shape, strides and address."""
+    s, at = t.stride(), t.data_ptr()
+    if len(s) != 3:
         raise ValueError(f"{name} is (tokens, heads, head dim), got {tuple(t.shape)}")
-    s = t.stride()
-    step = 16 // t.element_size()
-    if s[2] != 1 or s[0] % step or s[1] % step or t.data_ptr() % 16:
+    if s[2] != 1 or s[0] % step or s[1] % step or at % 16:
         t = t.contiguous()
-        s = t.stride()
-    return t, t.shape, s
+        s, at = t.stride(), t.data_ptr()
+    return t, t.shape, s, at
 
 
 def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, what: str = "") -> tuple[torch.Size, tuple, tuple]:
@@ -94,16 +94,21 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, what: str = "") -> tupl
     return shape, ks, vs
 
 
-def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, n: int | None = None) -> torch.Tensor:
-    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name} is an {dtype} vector{'' if n is None else f' of {n}'}, got {t.dtype} {tuple(t.shape)}")
+def _vector(name: str, t: torch.Tensor, dtype: torch.dtype, n: int) -> torch.Tensor:
+    if t.dtype is not dtype or t.shape != (n,):
+        raise ValueError(f"{name} is an {dtype} vector of {n}, got {t.dtype} {tuple(t.shape)}")
     return t.contiguous()
 
 
-def _table(name: str, t: torch.Tensor, B: int) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B:
-        raise ValueError(f"{name} is an int32 ({B}, pages of a sequence) tensor, got {t.dtype} {tuple(t.shape)}")
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+def _table(name: str, t: torch.Tensor, B: int) -> tuple[torch.Tensor, int, int]:
+    """An int32 table of B rows, its entries a row and the rows' distance."""
+    shape, s = t.shape, t.stride()
+    if t.dtype is not torch.int32 or len(shape) != 2 or shape[0] != B:
+        raise ValueError(f"{name} is an int32 ({B}, pages of a sequence) tensor, got {t.dtype} {tuple(shape)}")
+    if s[1] != 1 and shape[1] > 1:
+        t = t.contiguous()
+        s = t.stride()
+    return t, shape[1], s[0]
 
 
 def _check(fn: str, status: int) -> None:
@@ -116,62 +121,68 @@ def _check(fn: str, status: int) -> None:
 
 
 def _norm_rope(q, k, v, cos, sin, positions, q_weight, k_weight, eps, interleaved, k_pages, v_pages, slots):
-    append = slots is not None
-    dev = _device(q, k, v, cos, sin, positions, q_weight, k_weight, k_pages, v_pages, slots)
-    lib = L.load()
-    dt = _DT.get(q.dtype)
+    ts = (q, k, cos, sin, positions) if slots is None else (q, k, cos, sin, positions, v, k_pages, v_pages, slots)
+    if q_weight is not None:
+        ts += (q_weight,)
+    if k_weight is not None:
+        ts += (k_weight,)
+    dev = _device(ts)
+    dtype = q.dtype
+    dt = _DT.get(dtype)
     if dt is None:
-        raise NotImplementedError(f"qk_norm_rope runs on fp32 and bf16 operands, got {q.dtype}")
-    q, (N, Hq, d), qs = _heads("q", q)
-    k, (kn, Hkv, kd), ks = _heads("k", k)
-    if k.dtype != q.dtype or kn != N or kd != d:
-        raise ValueError(f"q and k share tokens, head dim and type: {tuple(q.shape)} {q.dtype}, "
-                         f"{tuple(k.shape)} {k.dtype}")
+        raise NotImplementedError(f"qk_norm_rope runs on fp32 and bf16 operands, got {dtype}")
+    step = 8 if dt == L.BF16 else 4
+    q, qshape, (q0, q1, _), q_at = _heads("q", q, step)
+    k, kshape, (k0, k1, _), k_at = _heads("k", k, step)
+    N, Hq, d = qshape
+    kn, Hkv, kd = kshape
+    if k.dtype is not dtype or kn != N or kd != d:
+        raise ValueError(f"q and k share tokens, head dim and type: {tuple(qshape)} {dtype}, {tuple(kshape)} {k.dtype}")
     if not 1 <= d <= QK_NORM_ROPE_MAX_HEAD_DIM:
         raise NotImplementedError(f"qk_norm_rope takes head dims up to {QK_NORM_ROPE_MAX_HEAD_DIM}, got {d}")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    table, cs = cos.shape, cos.stride()
+    if len(table) != 2 or sin.shape != table or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise ValueError("cos and sin are fp32 tables (positions, rotated dims / 2) of one shape")
-    n_pos, half = cos.shape
-    rot = 2 * half
+    n_pos, half = table
+    rot, ld = 2 * half, cs[0]
     if rot > d:
         raise ValueError(f"the tables rotate {rot} dims of a head of {d}")
-    ld = cos.stride(0)
-    if rot and (cos.stride() != sin.stride() or cos.stride(1) != 1 or ld < half):
+    if rot and (cs[1] != 1 or ld < half or sin.stride() != cs):
         cos, sin, ld = cos.contiguous(), sin.contiguous(), half
-    qw = kw = vp = slots_p = None
+    qw = kw = None
     if q_weight is not None:
-        q_weight = _norm_weight(q_weight, q, d)
+        q_weight = _norm_weight(q_weight, dtype, d)
         qw = q_weight.data_ptr()
     if k_weight is not None:
-        k_weight = _norm_weight(k_weight, q, d)
+        k_weight = _norm_weight(k_weight, dtype, d)
         kw = k_weight.data_ptr()
     positions = _vector("positions", positions, torch.int64, N)
-    q_out = q.new_empty((N, Hq, d))
-    n_pages = page = 0
-    if append:
-        v, vshape, vs = _heads("v", v)
-        if vshape != k.shape or v.dtype != q.dtype:
-            raise ValueError(f"v has k's shape and type: {tuple(v.shape)} {v.dtype}, {tuple(k.shape)} {k.dtype}")
-        (n_pages, ph, page, pd), ko, vo = _pages(k_pages, v_pages)
-        if ph != Hkv or pd != d or k_pages.dtype != q.dtype:
-            raise ValueError(f"the pages hold {ph} heads of {pd} {k_pages.dtype}, k has {Hkv} of {d} {q.dtype}")
-        slots = _vector("slots", slots, torch.int64, N)
-        slots_p, vp = slots.data_ptr(), v.data_ptr()
-        k_out, v_out = k_pages, v_pages.data_ptr()
-        strides = _S12(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], ko[0], ko[1], ko[2], vo[0], vo[1], vo[2])
+    q_out = q.new_empty(qshape)
+    if slots is None:
+        k_out = q.new_empty(kshape)
+        v_at = slots_at = v_out = None
+        k_to, n_pages, page = k_out.data_ptr(), 0, 0
+        strides = _S12(q0, q1, k0, k1, 0, 0, 0, 0, 0, 0, 0, 0)
     else:
-        k_out, v_out = q.new_empty((N, Hkv, d)), None
-        strides = _S12(qs[0], qs[1], ks[0], ks[1], 0, 0, 0, 0, 0, 0, 0, 0)
-    st = _launch(dev, lib.catopt_hip_qk_norm_rope, dt, N, Hq, Hkv, d, rot, 1 if interleaved else 0, q.data_ptr(),
-                 k.data_ptr(), vp, qw, kw, eps, cos.data_ptr(), sin.data_ptr(), n_pos, ld,
-                 positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), v_out, strides, slots_p, n_pages, page,
-                 _stream(q))
-    _check("qk_norm_rope", st)
+        v, vshape, (v0, v1, _), v_at = _heads("v", v, step)
+        if vshape != kshape or v.dtype is not dtype:
+            raise ValueError(f"v has k's shape and type: {tuple(vshape)} {v.dtype}, {tuple(kshape)} {dtype}")
+        (n_pages, ph, page, pd), (ko0, ko1, ko2, _), (vo0, vo1, vo2, _) = _pages(k_pages, v_pages)
+        if ph != Hkv or pd != d or k_pages.dtype is not dtype:
+            raise ValueError(f"the pages hold {ph} heads of {pd} {k_pages.dtype}, k has {Hkv} of {d} {dtype}")
+        slots = _vector("slots", slots, torch.int64, N)
+        k_out, slots_at, k_to, v_out = None, slots.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
+        strides = _S12(q0, q1, k0, k1, v0, v1, ko0, ko1, ko2, vo0, vo1, vo2)
+    st = _launch(dev, L.load().catopt_hip_qk_norm_rope, dt, N, Hq, Hkv, d, rot, 1 if interleaved else 0, q_at, k_at,
+                 v_at, qw, kw, eps, cos.data_ptr(), sin.data_ptr(), n_pos, ld, positions.data_ptr(), q_out.data_ptr(),
+                 k_to, v_out, strides, slots_at, n_pages, page)
+    if st:
+        _check("qk_norm_rope", st)
     return q_out, k_out
 
 
-def _norm_weight(w: torch.Tensor, x: torch.Tensor, d: int) -> torch.Tensor:
-    if w.dtype != x.dtype or w.numel() != d:
+def _norm_weight(w: torch.Tensor, dtype: torch.dtype, d: int) -> torch.Tensor:
+    if w.dtype is not dtype or w.numel() != d:
         raise ValueError(f"a norm weight holds one value of q's type for each head dim, got {tuple(w.shape)} {w.dtype}")
     return w.contiguous()
 
@@ -216,11 +227,12 @@ def _attn_workspace(B: int, N: int, Hq: int, Hkv: int, d: int, n_table: int, pag
 
 
 def _weight_rows(name: str, w: torch.Tensor, B: int, H: int, width: int) -> tuple[int, int]:
-    if w.dtype != torch.float32 or w.dim() != 3 or w.shape[0] != B or w.shape[1] != H or w.shape[2] < width:
-        raise ValueError(f"{name} is an fp32 ({B}, {H}, at least {width}) tensor, got {w.dtype} {tuple(w.shape)}")
-    if w.shape[2] > 1 and w.stride(2) != 1:
-        raise ValueError(f"{name} needs a contiguous last axis, got strides {w.stride()}")
-    return w.stride(0), w.stride(1)
+    shape, s = w.shape, w.stride()
+    if w.dtype is not torch.float32 or len(shape) != 3 or shape[0] != B or shape[1] != H or shape[2] < width:
+        raise ValueError(f"{name} is an fp32 ({B}, {H}, at least {width}) tensor, got {w.dtype} {tuple(shape)}")
+    if s[2] != 1 and shape[2] > 1:
+        raise ValueError(f"{name} needs a contiguous last axis, got strides {s}")
+    return s[0], s[1]
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -255,14 +267,22 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``weights``."""
     if empty_rows not in ("nan", "zero"):
         raise ValueError(f"empty_rows is 'nan' or 'zero', got {empty_rows!r}")
-    dev = _device(q, k_pages, v_pages, block_table, kv_lens, q_starts, weights, weights_out, out)
-    lib = L.load()
-    if q.dtype != torch.bfloat16 or k_pages.dtype != q.dtype:
+    ts = (q, k_pages, v_pages, block_table, kv_lens, q_starts)
+    if out is not None:
+        ts += (out,)
+    if weights_out is not None:
+        ts += (weights_out,) if weights is None else (weights_out, weights)
+    elif weights is not None:
+        raise ValueError("weights need a weights_out to go to")
+    dev = _device(ts)
+    if q.dtype is not torch.bfloat16 or k_pages.dtype is not torch.bfloat16:
         raise NotImplementedError(f"paged attention runs on bf16 operands, got {q.dtype} and {k_pages.dtype} pages")
-    q, (N, Hq, d), qs = _heads("q", q)
-    if q.data_ptr() % 16:
+    q, qshape, (q0, q1, _), q_at = _heads("q", q, 8)
+    if q_at % 16:
         q = q.clone()
-    (n_pages, Hkv, page, pd), ks, vs = _pages(k_pages, v_pages)
+        q_at = q.data_ptr()
+    N, Hq, d = qshape
+    (n_pages, Hkv, page, pd), (k0, k1, k2, _), (v0, v1, v2, _) = _pages(k_pages, v_pages)
     if pd != d or Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"q has {Hq} heads of {d}, the pages {Hkv} heads of {pd}: the head dims agree and the query "
                          "heads are a multiple of the key heads")
@@ -274,44 +294,40 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     scale = float(scale)
     if not 0 < scale < 1e38:
         raise ValueError(f"the scale is a positive number below 1e38, got {scale}")
-    kv_lens = _vector("kv_lens", kv_lens, torch.int32)
-    B = kv_lens.shape[0]
+    B = q_starts.numel() - 1
+    kv_lens = _vector("kv_lens", kv_lens, torch.int32, B)
     q_starts = _vector("q_starts", q_starts, torch.int32, B + 1)
-    table = _table("block_table", block_table, B)
-    n_table = table.shape[1]
+    table, n_table, table_ld = _table("block_table", block_table, B)
     if out is None:
-        o = q.new_empty((N, Hq, d))
-    else:
-        o = out
-        if o.shape != q.shape or o.dtype != q.dtype:
-            raise ValueError(f"out has q's shape and type, got {tuple(o.shape)} {o.dtype}")
-    so = o.stride()
-    if so[2] != 1:
-        raise ValueError(f"out needs a contiguous head dim, got strides {so}")
+        out = q.new_empty(qshape)
+    elif out.shape != qshape or out.dtype is not torch.bfloat16:
+        raise ValueError(f"out has q's shape and type, got {tuple(out.shape)} {out.dtype}")
+    o0, o1, o2 = out.stride()
+    if o2 != 1:
+        raise ValueError(f"out needs a contiguous head dim, got strides {out.stride()}")
     wi0 = wi1 = wo0 = wo1 = 0
-    wi = wo = m = l = mp = lp = ws = None
+    wi = wo = m = l = mp = lp = ws_at = None
     if weights_out is not None:
         wo0, wo1 = _weight_rows("weights_out", weights_out, B, Hkv, n_table * page)
         wo = weights_out.data_ptr()
         if weights is not None:
             wi0, wi1 = _weight_rows("weights", weights, B, Hkv, n_table * page)
             wi = weights.data_ptr()
-    elif weights is not None:
-        raise ValueError("weights need a weights_out to go to")
     if return_ml:
-        m, l = (q.new_empty((N, Hq), dtype=torch.float32) for _ in range(2))
+        m, l = q.new_empty((N, Hq), dtype=torch.float32), q.new_empty((N, Hq), dtype=torch.float32)
         mp, lp = m.data_ptr(), l.data_ptr()
     if B and (N or wo is not None):
-        strides = _S14(qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], so[0], so[1], wi0, wi1, wo0, wo1)
         wsb = _attn_workspace(B, N, Hq, Hkv, d, n_table, page, wo is not None)
         if wsb:
             ws = q.new_empty(wsb // 2)
-        st = _launch(dev, lib.catopt_hip_paged_attn_fwd, L.BF16, B, N, Hq, Hkv, d, q.data_ptr(), k_pages.data_ptr(),
-                     v_pages.data_ptr(), n_pages, page, table.data_ptr(), table.stride(0), n_table, kv_lens.data_ptr(),
-                     q_starts.data_ptr(), scale, 1 if causal else 0, 2 if empty_rows == "zero" else 1, o.data_ptr(),
-                     mp, lp, wi, wo, strides, None if ws is None else ws.data_ptr(), wsb, _stream(q))
-        _check("paged_attention", st)
-    return (o, m, l) if return_ml else o
+            ws_at = ws.data_ptr()
+        st = _launch(dev, L.load().catopt_hip_paged_attn_fwd, L.BF16, B, N, Hq, Hkv, d, q_at, k_pages.data_ptr(),
+                     v_pages.data_ptr(), n_pages, page, table.data_ptr(), table_ld, n_table, kv_lens.data_ptr(),
+                     q_starts.data_ptr(), scale, 1 if causal else 0, 2 if empty_rows == "zero" else 1, out.data_ptr(),
+                     mp, lp, wi, wo, _S14(q0, q1, k0, k1, k2, v0, v1, v2, o0, o1, wi0, wi1, wo0, wo1), ws_at, wsb)
+        if st:
+            _check("paged_attention", st)
+    return (out, m, l) if return_ml else out
 
 
 def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -339,39 +355,46 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
     tensor whose entries behind the last kept key are 0."""
     if (k_out is None) != (v_out is None):
         raise ValueError("give both k_out and v_out, or neither")
-    dev = _device(k_pages, v_pages, block_table, kv_lens, weights, out_table, k_out, v_out, weights_out)
-    lib = L.load()
-    dt = _DT.get(k_pages.dtype)
+    ts = (k_pages, v_pages, block_table, kv_lens, weights, out_table)
+    if k_out is not None:
+        ts += (k_out, v_out)
+    if weights_out is not None:
+        ts += (weights_out,)
+    dev = _device(ts)
+    dtype = k_pages.dtype
+    dt = _DT.get(dtype)
     if dt is None:
-        raise NotImplementedError(f"eviction runs on fp32 and bf16 pages, got {k_pages.dtype}")
-    (n_pages, Hkv, page, d), ks, vs = _pages(k_pages, v_pages)
-    k_to, v_to = (k_pages, v_pages) if k_out is None else (k_out, v_out)
-    (n_out, ho, page_out, do), kt, vt = _pages(k_to, v_to, "output ")
-    if ho != Hkv or do != d or k_to.dtype != k_pages.dtype:
-        raise ValueError(f"the output pages hold {ho} heads of {do} {k_to.dtype}, the cache {Hkv} of {d} {k_pages.dtype}")
-    if d < 1 or Hkv < 1 or page < 1 or page_out < 1 or d * k_pages.element_size() % 16:
-        raise NotImplementedError(f"eviction takes rows of a multiple of 16 bytes, got {d} of {k_pages.dtype}")
+        raise NotImplementedError(f"eviction runs on fp32 and bf16 pages, got {dtype}")
+    (n_pages, Hkv, page, d), (k0, k1, k2, _), (v0, v1, v2, _) = _pages(k_pages, v_pages)
+    if k_out is None:
+        k_out, v_out = k_pages, v_pages
+    (n_out, ho, page_out, do), (ko0, ko1, ko2, _), (vo0, vo1, vo2, _) = _pages(k_out, v_out, "output ")
+    if ho != Hkv or do != d or k_out.dtype is not dtype:
+        raise ValueError(f"the output pages hold {ho} heads of {do} {k_out.dtype}, the cache {Hkv} of {d} {dtype}")
+    if d < 1 or Hkv < 1 or page < 1 or page_out < 1 or d % (8 if dt == L.BF16 else 4):
+        raise NotImplementedError(f"eviction takes rows of a multiple of 16 bytes, got {d} of {dtype}")
     budget, recent = int(budget), int(recent)
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"a budget of at least 1 with 0 <= recent <= budget, got {budget} and {recent}")
-    kv_lens = _vector("kv_lens", kv_lens, torch.int32)
-    B = kv_lens.shape[0]
-    table, to = _table("block_table", block_table, B), _table("out_table", out_table, B)
-    n_table, n_to = table.shape[1], to.shape[1]
+    B = kv_lens.numel()
+    kv_lens = _vector("kv_lens", kv_lens, torch.int32, B)
+    table, n_table, table_ld = _table("block_table", block_table, B)
+    to, n_to, to_ld = _table("out_table", out_table, B)
     if n_to * page_out < budget:
         raise ValueError(f"out_table reaches {n_to * page_out} keys, the budget is {budget}")
     wi0, wi1 = _weight_rows("weights", weights, B, Hkv, n_table * page)
-    if weights_out is None:
-        weights_out = torch.zeros((B, Hkv, budget), dtype=torch.float32, device=weights.device)
+    fresh = weights_out is None
+    if fresh:
+        weights_out = weights.new_empty((B, Hkv, budget))
     wo0, wo1 = _weight_rows("weights_out", weights_out, B, Hkv, budget)
     kept = kv_lens.new_empty((B, Hkv, budget))
     new_lens = kv_lens.new_empty((B,))
     if B:
-        strides = _S16(ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kt[0], kt[1], kt[2], vt[0], vt[1], vt[2],
-                       wi0, wi1, wo0, wo1)
-        st = _launch(dev, lib.catopt_hip_paged_evict, dt, B, Hkv, d, k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
-                     page, table.data_ptr(), table.stride(0), n_table, kv_lens.data_ptr(), weights.data_ptr(), budget,
-                     recent, k_to.data_ptr(), v_to.data_ptr(), n_out, page_out, to.data_ptr(), to.stride(0), n_to,
-                     kept.data_ptr(), new_lens.data_ptr(), weights_out.data_ptr(), strides, _stream(k_pages))
-        _check("paged_evict", st)
+        st = _launch(dev, L.load().catopt_hip_paged_evict, dt, B, Hkv, d, k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
+                     page, table.data_ptr(), table_ld, n_table, kv_lens.data_ptr(), weights.data_ptr(), budget, recent,
+                     k_out.data_ptr(), v_out.data_ptr(), n_out, page_out, to.data_ptr(), to_ld, n_to, kept.data_ptr(),
+                     new_lens.data_ptr(), weights_out.data_ptr(), 1 if fresh else 0,
+                     _S16(k0, k1, k2, v0, v1, v2, ko0, ko1, ko2, vo0, vo1, vo2, wi0, wi1, wo0, wo1))
+        if st:
+            _check("paged_evict", st)
     return kept, new_lens, weights_out

@@ -653,7 +653,8 @@ int32_t catopt_hip_paged_attn_fwd(
  * count and size are their own (n_out_table * out_page_size >= budget).
  * kept (int32 [B, Hkv, budget]) holds their indices, then -1; new_lens
  * (int32 [B]) the counts; weights_out (fp32 [B, Hkv, >= budget], optional)
- * their weights.  The row of a key whose page index is invalid moves as zeros.
+ * their weights, with zeros behind the last up to budget where clear_behind is
+ * not 0.  The row of a key whose page index is invalid moves as zeros.
  * k_out / v_out may be k_pages / v_pages where no page of out_table is one of
  * block_table's; no page is in out_table twice; weights_out may be weights.
  * F32 or BF16 rows of a multiple of 16 bytes; 1 <= budget.
@@ -668,7 +669,7 @@ int32_t catopt_hip_paged_evict(
     int64_t recent, void* k_out, void* v_out, int64_t n_out_pages,
     int64_t out_page_size, const int32_t* out_table, int64_t out_table_ld,
     int64_t n_out_table, int32_t* kept, int32_t* new_lens, float* weights_out,
-    const int64_t* strides, void* stream);
+    int32_t clear_behind, const int64_t* strides, void* stream);
 
 #ifdef __cplusplus
 }

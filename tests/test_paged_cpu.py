@@ -111,7 +111,7 @@ def _evict(lib, dtype=L.BF16, B=1, H=2, d=64, k=KP, v=VP, n_pages=8, page=16, ta
            new=FAKE, wo=None, strides=None):
     st = (C.c_int64 * 16)(*(strides or [2048, 1024, 64] * 4 + [128, 64] * 2))
     return lib.catopt_hip_paged_evict(dtype, B, H, d, k, v, n_pages, page, table, ld, n_table, lens, w, budget, recent,
-                                      ko, vo, n_out, page_out, to, to_ld, n_to, kept, new, wo, st, None)
+                                      ko, vo, n_out, page_out, to, to_ld, n_to, kept, new, wo, 0, st, None)
 
 
 def test_evict_refuses(lib):
@@ -148,10 +148,10 @@ def test_host_tensors_are_refused():
 
 def test_layout_checks():
     u = torch.zeros((3, 4, 12))
-    assert P._heads("t", u[..., :7])[0].data_ptr() == u.data_ptr()  # rows of 48 bytes: read in place
-    t, shape, strides = P._heads("t", u[..., 1:8])
-    assert t.is_contiguous() and shape == (3, 4, 7) and strides == (28, 7, 1)  # misaligned: copied
+    assert P._heads("t", u[..., :7], 4)[3] == u.data_ptr()  # rows of 48 bytes: read in place
+    t, shape, strides, at = P._heads("t", u[..., 1:8], 4)
+    assert t.is_contiguous() and shape == (3, 4, 7) and strides == (28, 7, 1) and at == t.data_ptr()  # misaligned: copied
     with pytest.raises(ValueError):
-        P._heads("t", u[0])
+        P._heads("t", u[0], 4)
     with pytest.raises(ValueError):
         P._pages(u, u)
