@@ -145,11 +145,12 @@ extern "C" int32_t catopt_hip_paged_attn_fwd(
   a.table = block_table, a.lens = kv_lens, a.starts = q_starts, a.table_ld = table_ld, a.n_pages = n_pages, a.N = N;
   a.m_out = m_out, a.l_out = l_out, a.w_in = weights_in, a.w_out = weights_out;
   a.page = FastDiv::of(page_size), a.group = FastDiv::of(Hq / Hkv);
+  a.q_heads = FastDiv::of(Hq), a.k_heads = FastDiv::of(Hkv);
   a.B = (int)B, a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.d = (int)d, a.cap = (int)(n_table * page_size);
   a.normalize = normalize, a.causal = causal != 0, a.scale = scale;
   const Plan p = N == 0 ? Plan{} : plan_of(B, N, Hq, Hkv, d, a.cap, weights_out != nullptr);
   float* ws = static_cast<float*>(workspace);
-  a.splits = p.splits, a.min_keys = p.min_keys;
+  a.splits = p.splits, a.min_keys = p.min_keys, a.ranges = FastDiv::of(p.splits < 1 ? 1 : p.splits);
   a.part = ws;
   ws += p.part_floats;
   if (weights_out) {

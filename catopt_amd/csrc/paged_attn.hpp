@@ -22,6 +22,7 @@ struct PagedArgs {
   const float* w_in;
   float* w_out;
   FastDiv page, group;  // by the page size, by the query heads of a key head
+  FastDiv q_heads, k_heads, ranges;  // by Hq, Hkv, splits
   int B, Hq, Hkv, G, d, cap, normalize, causal;
   int splits, min_keys;  // key ranges per tile at most, keys of one at least
   float scale;
@@ -38,7 +39,8 @@ struct PagedTile {
   int b, row0, nq, len, r0, rows;  // sequence, its tokens and keys; the tile's first row and its rows (0: no such tile)
   int off;                         // token i sees keys <= off + i
   int kend;                        // keys that some row of the tile sees
-  int splits, keys;                // its key ranges and the keys of each
+  int keys;                        // of each of its key ranges
+  bool split;                      // it has several
 };
 
 // Lane i looks at sequence i (of 64 at a time), so that the search and the
@@ -80,12 +82,23 @@ __device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, int t) {
 // kernel).
 __device__ __forceinline__ void paged_ranges(const PagedArgs& a, PagedTile& x) {
   x.off = a.causal ? x.len - x.nq : 0x3fffffff;
-  const int64_t last = (int64_t)x.off + (x.r0 + x.rows - 1) / a.G;
-  x.kend = last < 0 ? 0 : (int)min((int64_t)x.len, last + 1);
-  int keys = (x.kend + a.splits - 1) / a.splits;
-  keys = (max(keys, a.min_keys) + 127) & ~127;
-  x.keys = keys;
-  x.splits = max((x.kend + keys - 1) / keys, 1);
+  const int last = x.off + (int)a.group.div(x.r0 + x.rows - 1);  // below 2^31: both are below 2^30
+  x.kend = last < 0 ? 0 : min(x.len, last + 1);
+  x.keys = (max((int)a.ranges.div(x.kend + a.splits - 1), a.min_keys) + 127) & ~127;
+  x.split = x.kend > x.keys;
+}
+// Whether range s of a tile has keys (the first is there in any case).
+__device__ __forceinline__ bool has_range(const PagedTile& x, int s) { return s == 0 || (int64_t)s * x.keys < x.kend; }
+// The ranges of a tile: 64 at most, so lane s looks at range s.
+__device__ __forceinline__ int count_ranges(const PagedTile& x) { return __popcll(__ballot(has_range(x, threadIdx.x & 63))); }
+
+// A workgroup's key head, its tile and key range: the heads next to each other,
+// then the ranges.
+__device__ __forceinline__ void decode_block(const PagedArgs& a, int& h, int& tile, int& range) {
+  const uint32_t ts = a.k_heads.div(blockIdx.x);
+  h = (int)(blockIdx.x - ts * a.k_heads.d);
+  tile = (int)a.ranges.div(ts);
+  range = (int)(ts - (uint32_t)tile * a.ranges.d);
 }
 
 // exp2((from - to) c), 0 for an empty `from`.

@@ -55,11 +55,12 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = blockIdx.x % a.Hkv, ts = blockIdx.x / a.Hkv, t = ts / a.splits, split = ts - t * a.splits;
+  int h, t, split;
+  decode_block(a, h, t, split);
   PagedTile x = paged_tile<kFewRows>(a, t);
   if (x.rows == 0) return;
   paged_ranges(a, x);
-  if (split >= x.splits) return;
+  if (!has_range(x, split)) return;
   const float c = a.scale * kLog2e;
 
   // this wave's stages: 32 keys each from key_of(i) on
@@ -85,6 +86,7 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
     qf[j] = __builtin_bit_cast(bf16x8, w);
   }
   const int lim = min(x.off + tok, x.len - 1);  // last key this row sees
+  const int lim0 = x.off + (int)a.group.div(x.r0);  // and the tile's first
 
   // a lane's 16 bytes of load k: row k ROWS + lane / CH of the stage, row & 7 of
   // its group; the swizzles depend on a row's place among 16 (K, D = 128: loads
@@ -147,7 +149,7 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
     for (int j = 0; j < D / 16; ++j)
       s = mfma32x32x16(*reinterpret_cast<const bf16x8*>(Ks + tile_off<D>(l32, 2 * j + g)), qf[j], s);
     // some row does not see some key: the first row sees the fewest
-    const bool masked = key0 + 32 > x.len || key0 + 31 > x.off + x.r0 / a.G || bad_now;
+    const bool masked = key0 + 32 > x.len || key0 + 31 > lim0 || bad_now;
     if (masked) mask_scores(s, lim - key0, bad_now);
     if (srow && live) {
 #pragma unroll
@@ -226,7 +228,7 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
     }
     const int tk = (int)a.group.div(x.r0 + r), hr = h * a.G + x.r0 + r - tk * a.G;
     const int64_t i = (int64_t)(x.row0 + tk) * a.Hq + hr;
-    if (x.splits > 1) {
+    if (x.split) {
       const int64_t rows = a.N * a.Hq;
       if (d == 0) {
         a.part[2 * (i * a.splits + split)] = mx;

@@ -18,9 +18,9 @@ template <int D, int R, int WAVES>
 __device__ __forceinline__ void combine_rows(const PagedArgs& a, int block) {
   constexpr int TPR = D / 4, GROUPS = 64 * WAVES / TPR;
   const int lane = threadIdx.x & 63, tid = WAVES == 4 ? threadIdx.x : lane;
-  const int64_t row = WAVES == 4 ? block : (int64_t)block * 4 + (threadIdx.x >> 6);
+  const int row = WAVES == 4 ? block : block * 4 + (int)(threadIdx.x >> 6);  // N Hq < 2^30
   if (row >= a.N * a.Hq) return;
-  const int n = (int)(row / a.Hq), hq = (int)(row - (int64_t)n * a.Hq);
+  const int n = (int)a.q_heads.div(row), hq = row - n * a.Hq;
   int b = -1;
   for (int c0 = 0; c0 < a.B; c0 += 64) {  // the last sequence that starts at or before the token
     const int i = c0 + lane;
@@ -34,15 +34,17 @@ __device__ __forceinline__ void combine_rows(const PagedArgs& a, int block) {
   seq_rows(a.starts, b, a.N, x.row0, x.nq);
   if (n < x.row0 || n >= x.row0 + x.nq) return;
   x.len = min(max(a.lens[b], 0), a.cap);
-  x.r0 = ((n - x.row0) * a.G + hq % a.G) / R * R;
+  x.r0 = ((n - x.row0) * a.G + hq - (int)a.group.div(hq) * a.G) / R * R;
   x.rows = min(R, x.nq * a.G - x.r0);
   paged_ranges(a, x);
-  if (x.splits == 1) return;  // written by the tile
+  if (!x.split) return;  // written by the tile
+  const int splits = count_ranges(x);
   const float c = a.scale * kLog2e;
-  const float* ml = a.part + 2 * row * a.splits;
-  const float* num = a.part + ((2 * a.N * a.Hq * a.splits + 3) & ~(int64_t)3) + row * a.splits * D + 4 * (tid % TPR);
+  const float* ml = a.part + (int64_t)2 * row * a.splits;
+  const float* num =
+      a.part + ((2 * a.N * a.Hq * a.splits + 3) & ~(int64_t)3) + (int64_t)row * a.splits * D + 4 * (tid % TPR);
   // lane s of every wave: range s (64 at most)
-  const bool mine = lane < x.splits;
+  const bool mine = lane < splits;
   const float ms = mine ? ml[2 * lane] : kNegInf, ls = mine ? ml[2 * lane + 1] : 0.f;
   float mx = ms;
 #pragma unroll
@@ -53,12 +55,12 @@ __device__ __forceinline__ void combine_rows(const PagedArgs& a, int block) {
   for (int o = 32; o > 0; o >>= 1) lt += __shfl_xor(lt, o, 64);
   f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr int U = 8;  // loads ahead of their additions
-  for (int s0 = 0; s0 < x.splits; s0 += U * GROUPS) {  // every lane stays: the factors come from lanes
+  for (int s0 = 0; s0 < splits; s0 += U * GROUPS) {  // every lane stays: the factors come from lanes
     f32x4 ys[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int s = s0 + i * GROUPS + tid / TPR;
-      ys[i] = s < x.splits ? *reinterpret_cast<const f32x4*>(num + (int64_t)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+      ys[i] = s < splits ? *reinterpret_cast<const f32x4*>(num + (int64_t)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) y += ys[i] * __shfl(f, min(s0 + i * GROUPS + tid / TPR, 63), 64);
@@ -106,7 +108,7 @@ constexpr int kLogRows = 64;  // rows whose statistics are in LDS at a time
 // Four keys per thread: their stored products of every row that sees them.
 __device__ __forceinline__ void weights_of_scores(const PagedArgs& a, int block, int blocks) {
   __shared__ float logs[kLogRows];
-  const int bh = block / blocks, b = bh / a.Hkv, h = bh - b * a.Hkv, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int bh = block / blocks, b = (int)a.k_heads.div(bh), h = bh - b * a.Hkv, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int key0 = (block - bh * blocks) * NT * 4, key = key0 + 4 * threadIdx.x;
   PagedTile x{};
   x.b = b;
@@ -125,7 +127,7 @@ __device__ __forceinline__ void weights_of_scores(const PagedArgs& a, int block,
       x.r0 = (r0 + r) / kFewRows * kFewRows;
       x.rows = min(kFewRows, rows - x.r0);
       paged_ranges(a, x);
-      const float o = x.splits > 1 ? ranges_log(a, i, x.splits) : a.row_log[i];
+      const float o = x.split ? ranges_log(a, i, count_ranges(x)) : a.row_log[i];
       if (lane == 0) logs[r] = o;
     }
     __syncthreads();

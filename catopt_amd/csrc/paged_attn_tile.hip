@@ -52,11 +52,12 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int h = blockIdx.x % a.Hkv, ts = blockIdx.x / a.Hkv, tr = ts / a.splits, split = ts - tr * a.splits;
+  int h, tr, split;
+  decode_block(a, h, tr, split);
   PagedTile x = paged_tile<kTileRows>(a, tiles - 1 - tr);
   if (x.rows == 0) return;
   paged_ranges(a, x);
-  if (split >= x.splits) return;
+  if (!has_range(x, split)) return;
   const float c = a.scale * kLog2e;
 
   const int row = x.r0 + 32 * wave + l32, tok = (int)a.group.div(row), hq = h * a.G + row - tok * a.G;
@@ -268,7 +269,7 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
   const float fix = m_true != kNegInf && m_run != kNegInf ? __builtin_amdgcn_exp2f((m_run - m_true) * c) : 1.f;
   const float l_sum = l_run + __shfl_xor(l_run, 32, 64);
   const int64_t i = (int64_t)(x.row0 + tok) * a.Hq + hq;
-  if (x.splits > 1) {
+  if (x.split) {
     if (!live) return;
     const int64_t rows = a.N * a.Hq, at = i * a.splits + split;
     if (g == 0) {

@@ -25,19 +25,16 @@ constexpr int NT = 256;
 constexpr int kKeys = 128;  // of a workgroup, 32 per wave
 
 template <int D>
-__global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks, int parts, float* part) {
+__global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, FastDiv blocks, FastDiv parts, float* part) {
   // rows a 16-byte piece further apart than they are long: 16 rows' pieces lie
   // in different banks, and a fragment's address is one register and a constant
   constexpr int ROW = D * 2 + 16;
   __shared__ __attribute__((aligned(16))) char lds[2][32 * ROW];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int u = blockIdx.x;
-  const int h = u % a.Hkv;
-  u /= a.Hkv;
-  const int pt = u % parts;
-  u /= parts;
-  const int blk = u % blocks, b = u / blocks;
+  const uint32_t hs = a.k_heads.div(blockIdx.x), ps = parts.div(hs);
+  const int h = (int)(blockIdx.x - hs * a.k_heads.d), pt = (int)(hs - ps * parts.d);
+  const int b = (int)blocks.div(ps), blk = (int)(ps - (uint32_t)b * blocks.d);
   int row0, nq;
   seq_rows(a.starts, b, a.N, row0, nq);
   const int len = min(max(a.lens[b], 0), a.cap);
@@ -67,7 +64,7 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks
   // steps of 32 rows from the first that sees the block's first key; this part's share
   const int rows = nq * a.G, tok0 = max(blk * kKeys - off, 0);
   const int ta = (int)min((int64_t)tok0 * a.G, (int64_t)rows) / 32, tb = (rows + 31) / 32;
-  const int t0 = ta + (int)((int64_t)(tb - ta) * pt / parts), t1 = ta + (int)((int64_t)(tb - ta) * (pt + 1) / parts);
+  const int t0 = ta + (int)parts.div((tb - ta) * pt), t1 = ta + (int)parts.div((tb - ta) * (pt + 1));  // below 2^30
 
   constexpr int CH = AttnRow<D>::CH, LD = 32 * CH / NT;  // 16-byte pieces of a step per thread
   static_assert(LD >= 1 && LD <= 2, "the pieces' registers");
@@ -163,23 +160,27 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, int blocks
     step(t, 0);
     if (t + 1 < t1) step(t + 1, 1);
   }
-  // lane r of each half takes the key of accumulator register r
+  // The halves' 32 lanes meet: in each step a lane hands half of its keys' sums to
+  // the lane whose index differs in one bit and takes that one's of the others, so
+  // that two neighbours end with the key of register l32 / 2.  16 exchanges, where
+  // summing each key over all lanes takes 80.
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    float y = w[r];
+  for (int x = 16, n = 8; n > 0; x >>= 1, n >>= 1) {
+    const bool upper = l32 & x;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) y += __shfl_xor(y, x, 64);
-    if (l32 == r) {
-      const int in = acc_row(r, g), j = key0 + in;
-      if (j < len) {
-        const float x = (ok >> in) & 1 ? y : 0.f;
-        if (parts > 1)
-          part[((int64_t)(pt * a.B + b) * a.Hkv + h) * a.cap + j] = x;
-        else
-          add_weight(a, b, h, j, old, x);
-      }
+    for (int i = 0; i < n; ++i) {
+      const float keep = upper ? w[i + n] : w[i], give = upper ? w[i] : w[i + n];
+      w[i] = keep + __shfl_xor(give, x, 64);
     }
   }
+  w[0] += __shfl_xor(w[0], 1, 64);
+  const int in = 8 * (l32 >> 3) + 4 * g + ((l32 >> 1) & 3), j = key0 + in;  // acc_row(l32 / 2, g)
+  if (l32 & 1 || j >= len) return;
+  const float y = (ok >> in) & 1 ? w[0] : 0.f;
+  if (parts.d > 1)
+    part[((int64_t)(pt * a.B + b) * a.Hkv + h) * a.cap + j] = y;
+  else
+    add_weight(a, b, h, j, old, y);
 }
 
 __global__ __launch_bounds__(NT) void weights_add_parts(PagedArgs a, int blocks, int parts, const float* part) {
@@ -214,9 +215,9 @@ int32_t paged_weights_launch(const PagedArgs& a, int D, int parts, float* part, 
   if (!grid_fits(heads * blocks * parts, NT)) return CATOPT_E_UNSUPPORTED;
   const dim3 grid((uint32_t)(heads * blocks * parts));
   if (D == 128)
-    weights_of_rows<128><<<grid, dim3(NT), 0, s>>>(a, (int)blocks, parts, part);
+    weights_of_rows<128><<<grid, dim3(NT), 0, s>>>(a, FastDiv::of(blocks), FastDiv::of(parts), part);
   else
-    weights_of_rows<64><<<grid, dim3(NT), 0, s>>>(a, (int)blocks, parts, part);
+    weights_of_rows<64><<<grid, dim3(NT), 0, s>>>(a, FastDiv::of(blocks), FastDiv::of(parts), part);
   CATOPT_LAUNCH_CHECK();
   if (parts > 1) {
     const int64_t n = (a.cap + NT - 1) / NT;

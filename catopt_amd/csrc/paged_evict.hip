@@ -93,7 +93,7 @@ __global__ __launch_bounds__(NT) void evict_kernel(EvictArgs a) {
   int32_t* kept = a.kept + (int64_t)bh * a.budget;
   if (h == 0 && part == 0 && tid == 0) a.new_lens[b] = m;
   // this workgroup's kept keys
-  const int lo = (int)((int64_t)m * part / a.parts), hi = (int)((int64_t)m * (part + 1) / a.parts);
+  const int share = (m + a.parts - 1) / a.parts, lo = min(part * share, m), hi = min(lo + share, m);
   const int steps = (n + NT - 1) / NT, first = wave * steps * 64;  // this wave's keys: `steps` of 64
 
   // weights of the U steps from step i0 on: the loads take a valid address
