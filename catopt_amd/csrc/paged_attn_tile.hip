@@ -15,8 +15,8 @@
 // until then p <= 2^kLazy, exact in range for fp32 and bf16.
 //
 // MFMAs, softmax VALU and LDS reads bound it together: four prompts of 4096, 32
-// heads of 128, 619 us, 888 TFLOP/s at a MFMA-throttled clock; 2048 tokens over
-// 8192 keys, 32 heads on 8, 256 us.  Two workgroups a CU at D = 128 (registers),
+// heads of 128, 620 us, 887 TFLOP/s at a MFMA-throttled clock; 2048 tokens over
+// 8192 keys, 32 heads on 8, 259 us.  Two workgroups a CU at D = 128 (registers),
 // three at 64 (two: 77 us where three take 70, four prompts of 2048, 16 heads;
 // four spill).  Further stages of tiles in flight measured level.
 //

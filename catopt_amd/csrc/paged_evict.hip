@@ -4,11 +4,10 @@
 //
 // One launch: `parts` workgroups per (sequence, head) each make the whole
 // choice, which takes 10 us at 2048 keys and 16 at 16000, and move their share
-// of the rows.  That takes 15.8 us for 2048 keys of one sequence, 8 heads, and
-// 40.5 for eight sequences of up to 16000 that keep 2048 (132 MB, so the move
-// runs at 5.4 TB/s); with a launch for the choice and one for the move they
-// took 18.4 and 41.9.  HBM bounds the move, rounds of LDS atomics and barriers
-// the choice; small calls are bound by the host.
+// of the rows.  That takes 12 us for 2048 keys of one sequence, 8 heads, and 40
+// for eight sequences of up to 16000 that keep 2048 (132 MB, so the move runs at
+// 5.5 TB/s); a launch for the choice and one for the move take 2.6 and 1.4 more.
+// HBM bounds the move, rounds of LDS atomics and barriers the choice.
 #include "paged.hpp"
 
 namespace catopt {
