@@ -298,7 +298,7 @@ def test_weights_of_a_step_whose_products_are_not_stored():
     check_attention(cache, q, [1] * B, lens, o, scale=0.1, weights=w)
 
 
-@pytest.mark.parametrize("groups", [1, 3, 5, 7, 8, 32, 33, 40])
+@pytest.mark.parametrize("groups", [1, 3, 5, 7, 8, 32, 33, 40, 130])
 def test_query_heads_that_do_not_divide_a_tile(groups):
     _run([40, 3], [90, 300], groups * 2, 2, 64, 16, seed=groups)
     _run([1, 1], [90, 300], groups * 2, 2, 128, 16, seed=groups)
