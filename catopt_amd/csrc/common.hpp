@@ -120,13 +120,6 @@ __device__ __forceinline__ void dma_buf(u32x4 rsrc, uint32_t voff, uint32_t lds)
                :: "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds)) : "m0", "memory");
 }
 
-// dma_buf for bytes that are read once: the non-temporal hint keeps them from
-// passing through the caches as if they were to be read again.
-__device__ __forceinline__ void dma_buf_once(u32x4 rsrc, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
-               :: "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds)) : "m0", "memory");
-}
-
 // Buffer resource (raw, stride 0) over `bytes` bytes from `base`.
 __device__ __forceinline__ u32x4 make_rsrc(const void* base, uint32_t bytes) {
   const uint64_t b = reinterpret_cast<uint64_t>(base);

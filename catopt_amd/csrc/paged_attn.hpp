@@ -164,6 +164,35 @@ __device__ __forceinline__ u32x4 lane_rsrc(uint32_t lo, uint32_t hi, uint32_t by
 __device__ __forceinline__ u32x4 k_rsrc(const KeyGroup& x, int lane) { return lane_rsrc(x.k_lo, x.k_hi, x.k_bytes, lane); }
 __device__ __forceinline__ u32x4 v_rsrc(const KeyGroup& x, int lane) { return lane_rsrc(x.v_lo, x.v_hi, x.v_bytes, lane); }
 
+// Two direct loads of 1 KB of rows, to `lds` and `step` bytes behind, as dma_buf
+// makes one, with the non-temporal hint: for rows that are read once.  The
+// resources come out of lanes just before, and an SGPR that a lane read has
+// written must not be read by a memory instruction for five wait states, which
+// the compiler does not see in here: the move and s_nop 3 are those five for all.
+__device__ __forceinline__ void dma_rows_once(u32x4 rsrc0, uint32_t off0, u32x4 rsrc1, uint32_t off1, uint32_t lds,
+                                              uint32_t step) {
+  const uint32_t to0 = __builtin_amdgcn_readfirstlane(lds), to1 = __builtin_amdgcn_readfirstlane(lds + step);
+  asm volatile(
+      "s_mov_b32 m0, %4\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds\n\t"
+      "s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen nt lds" ::"v"(off0),
+      "s"(rsrc0), "v"(off1), "s"(rsrc1), "s"(to0), "s"(to1)
+      : "m0", "memory");
+}
+
+// The same for two loads of K (to `k_lds` and `step` behind) and two of V, for rows
+// that are read again.
+__device__ __forceinline__ void dma_rows4(u32x4 k0, u32x4 k1, uint32_t k_off, uint32_t k_lds, u32x4 v0, u32x4 v1,
+                                          uint32_t v_off, uint32_t v_lds, uint32_t step) {
+  const uint32_t to = __builtin_amdgcn_readfirstlane(k_lds), vto = __builtin_amdgcn_readfirstlane(v_lds);
+  asm volatile(
+      "s_mov_b32 m0, %6\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds\n\t"
+      "s_add_u32 m0, m0, %8\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %3, 0 offen lds\n\t"
+      "s_mov_b32 m0, %7\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %4, 0 offen lds\n\t"
+      "s_add_u32 m0, m0, %8\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds" ::"v"(k_off),
+      "v"(v_off), "s"(k0), "s"(k1), "s"(v0), "s"(v1), "s"(to), "s"(vto), "s"(step)
+      : "m0", "scc", "memory");
+}
+
 // A lane's byte offset from its group's first row: row `row` of the 8, 16-byte
 // piece `piece` of it; pieces past d lie outside every resource.
 __device__ __forceinline__ uint32_t group_offset(int64_t s_slot, int row, int piece, int d) {

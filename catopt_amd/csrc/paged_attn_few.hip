@@ -105,8 +105,7 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
     for (int k = 0; k < L::LOADS; ++k) {
       const int ln = lane0 + k * L::ROWS / 8;
       const uint32_t to = lds0 + (i & (L::STAGES - 1)) * L::STAGE + k * 1024;
-      dma_buf_once(k_rsrc(at, ln), koff[k & 3], to);
-      dma_buf_once(v_rsrc(at, ln), voff[k & 1], to + L::HALF);
+      dma_rows_once(k_rsrc(at, ln), koff[k & 3], v_rsrc(at, ln), voff[k & 1], to, L::HALF);
     }
   };
 

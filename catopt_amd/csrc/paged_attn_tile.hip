@@ -101,11 +101,10 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
   auto issue = [&](int t, int stage) {
     const int lane0 = 8 * ((t - t0) & 7);
 #pragma unroll
-    for (int i = 0; i < L::LOADS; ++i) {
-      const int ln = lane0 + ((4 * i + wave) * L::ROWS >> 3);
+    for (int i = 0; i < L::LOADS; i += 2) {
+      const int l0 = lane0 + ((4 * i + wave) * L::ROWS >> 3), l1 = lane0 + ((4 * i + 4 + wave) * L::ROWS >> 3);
       const uint32_t to = lds0 + stage * L::STAGE + i * 4096;
-      dma_buf(k_rsrc(at, ln), koff, to);
-      dma_buf(v_rsrc(at, ln), voff, to + L::TILE);
+      dma_rows4(k_rsrc(at, l0), k_rsrc(at, l1), koff, to, v_rsrc(at, l0), v_rsrc(at, l1), voff, to + L::TILE, 4096);
     }
   };
 
