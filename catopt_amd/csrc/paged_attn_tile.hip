@@ -42,6 +42,11 @@ struct TileLds {
   static constexpr int ROWS = 1024 / AttnRow<D>::BYTES;  // rows of one
 };
 
+// Masks, odd values and moves of the maximum leave the loop's straight line: 1500
+// new tokens over 4500 keys, 32 heads on 8, 142 -> 134 us; prompts of 4 x 4096 612
+// -> 597.  (A macro: the hint does not survive a function's inlining.)
+#define UNLIKELY(x) __builtin_expect(!!(x), 0)
+
 // An empty asm use: the value is computed before this point.
 __device__ __forceinline__ void pin(const bf16x8& x) { asm volatile("" ::"v"(__builtin_bit_cast(u32x4, x))); }
 __device__ __forceinline__ void pin(float x) { asm volatile("" ::"v"(x)); }
@@ -184,7 +189,7 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
         }
         m_true = fmaxf(m_true, mt);
         float alpha = 1.f;
-        if (__builtin_amdgcn_ballot_w64((mt - m_run) * c > kLazy) != 0) {
+        if (UNLIKELY(__builtin_amdgcn_ballot_w64((mt - m_run) * c > kLazy) != 0)) {
           const float m_new = fmaxf(m_run, mt);
           alpha = move_factor(m_run, m_new, c);
           l_run *= alpha;
@@ -215,9 +220,9 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
       read_k(0);
       read_k(1);
       qk(0, s0);
-      if (masked) apply_mask(0, s0);
+      if (UNLIKELY(masked)) apply_mask(0, s0);
       const float a0 = half_max(s0);
-      if (__builtin_amdgcn_ballot_w64(a0 != 1.f) != 0) rescale(a0);
+      if (UNLIKELY(__builtin_amdgcn_ballot_w64(a0 != 1.f) != 0)) rescale(a0);
       __builtin_amdgcn_sched_barrier(0);
       qk(1, s1);
       half_exp(s0, p0);
@@ -232,9 +237,9 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
       pin(p0[1]);
       pin(l_run);
       __builtin_amdgcn_sched_barrier(0);
-      if (masked) apply_mask(1, s1);
+      if (UNLIKELY(masked)) apply_mask(1, s1);
       const float a1 = half_max(s1);
-      if (masked && odd_values<D>(vf[0])) take_odd_values<D>(vf[0], p0, acc);
+      if (UNLIKELY(masked) && UNLIKELY(odd_values<D>(vf[0]))) take_odd_values<D>(vf[0], p0, acc);
       __builtin_amdgcn_sched_barrier(0);
       pv(0, p0);
       half_exp(s1, p1);
@@ -249,8 +254,8 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
       pin(p1[1]);
       pin(l_run);
       __builtin_amdgcn_sched_barrier(0);
-      if (__builtin_amdgcn_ballot_w64(a1 != 1.f) != 0) rescale(a1);
-      if (masked && odd_values<D>(vf[1])) take_odd_values<D>(vf[1], p1, acc);
+      if (UNLIKELY(__builtin_amdgcn_ballot_w64(a1 != 1.f) != 0)) rescale(a1);
+      if (UNLIKELY(masked) && UNLIKELY(odd_values<D>(vf[1]))) take_odd_values<D>(vf[1], p1, acc);
       pv(1, p1);
     }
     bad = bad_next;
