@@ -13,12 +13,13 @@ struct Plan {
 
 // Key ranges of 128-row tiles by their estimated time, were every sequence as
 // long as its table.  A workgroup takes a tile of 64 keys in 1.7 us alone on
-// its CU and 2.4 beside another (D = 64: 1 and 1.5); more workgroups than the
-// 512 that the CUs hold run in rounds.  Ranges cost a launch, 5.5 us, and their
-// numerators' way through memory, at 6 TB/s.  Measured, one range against the
-// best split (us): 64 tokens over 564 keys, 32 heads on 8, 20.4 and 16.5; 512
-// new tokens 18.5 and 22.6; four chunks of 300 over up to 300, 12 heads of 64,
-// 17.0 and 23.0.
+// its CU and 2.4 beside another (D = 64: 1 and 1.5), its start and masked tiles
+// shared out (1.35 and 2.3 without, which chose worse: 150 tokens each of two
+// sequences over 1650 keys 32.6 us for 29.1); more workgroups than 512 run in
+// rounds.  Ranges cost a launch, 5.5 us, and their numerators' way through
+// memory, at 6 TB/s.  Measured, one range against the ranges chosen (us): 64
+// tokens over 564 keys, 32 heads on 8, 18.0 and 14.2; 512 new tokens 16.5 and
+// 20 (one chosen); 33 to 171 tokens of five sequences, 12 heads of 64, 40 and 21.
 int tile_splits(int64_t groups, int64_t rows, int64_t D, int64_t cap) {
   const double alone = D == 128 ? 1.7 : 1.0, beside = D == 128 ? 2.4 : 1.5;
   double best = 0;
