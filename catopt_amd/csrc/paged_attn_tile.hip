@@ -14,9 +14,9 @@
 // reference max moves only when a half exceeds it by kLazy (log2 units);
 // until then p <= 2^kLazy, exact in range for fp32 and bf16.
 //
-// MFMAs, softmax VALU and LDS reads bound it together: four prompts of 4096, 32
-// heads of 128, 620 us, 887 TFLOP/s at a MFMA-throttled clock; 2048 tokens over
-// 8192 keys, 32 heads on 8, 259 us.  Two workgroups a CU at D = 128 (registers),
+// MFMAs and softmax VALU bound it together (0.4 and 0.55 of the cycles): four
+// prompts of 4096, 32 heads of 128, 598 us, 919 TFLOP/s at a clock of 1.9 GHz; 2048
+// tokens over 8192 keys, 32 heads on 8, 257 us.  Two workgroups a CU at D = 128 (registers),
 // three at 64 (two: 77 us where three take 70, four prompts of 2048, 16 heads;
 // four spill).  Further stages of tiles in flight measured level.
 //
