@@ -146,8 +146,10 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, FastDiv bl
 #pragma unroll
       for (int j = 0; j < D / 16; ++j)
         s = mfma32x32x16(kf[j], *reinterpret_cast<const bf16x8*>(lds[buf] + l32 * ROW + (2 * j + g) * 16), s);
-      if (key0 + 31 > first) {
-        const int lim = off + (int)a.group.div(32 * t + l32);
+      // a row behind the last (staged as zeros) sees no key: against an infinite one
+      // its score is NaN
+      if (key0 + 31 > first || 32 * t + 32 > rows) {
+        const int lim = 32 * t + l32 < rows ? off + (int)a.group.div(32 * t + l32) : -1;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = key0 + acc_row(r, g) <= lim ? s[r] : kNegInf;
       }
