@@ -146,15 +146,18 @@ __global__ __launch_bounds__(NT, 2) void weights_of_rows(PagedArgs a, FastDiv bl
 #pragma unroll
       for (int j = 0; j < D / 16; ++j)
         s = mfma32x32x16(kf[j], *reinterpret_cast<const bf16x8*>(lds[buf] + l32 * ROW + (2 * j + g) * 16), s);
-      // a row behind the last (staged as zeros) sees no key: against an infinite one
-      // its score is NaN
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], c, -o);
+      // The mask is for the exponents: a row whose o is NaN adds nothing to keys that
+      // it does not see.  One behind the last (staged as zeros) sees none: against an
+      // infinite key its score is NaN.
       if (key0 + 31 > first || 32 * t + 32 > rows) {
         const int lim = 32 * t + l32 < rows ? off + (int)a.group.div(32 * t + l32) : -1;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = key0 + acc_row(r, g) <= lim ? s[r] : kNegInf;
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) w[r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -o));
+      for (int r = 0; r < 16; ++r) w[r] += __builtin_amdgcn_exp2f(s[r]);
     }
     if (t + 1 < t1) stage(buf ^ 1);
   };

@@ -50,3 +50,26 @@ def test_keys_whose_scores_are_all_minus_infinity_get_nothing(nq, lens, Hkv, Hq,
     before = _sums(cache, 5)
     o, m, l, w = _call(cache, q, nq, lens, before, causal)
     check_attention(cache, q, nq, lens, o, scale=0.1, causal=causal, m=m, l=l, weights=w, before=before, keep=keep)
+
+
+# new tokens, keys, key and query heads, the token whose query is not finite
+@pytest.mark.parametrize("x", [float("nan"), INF])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nq,length,Hkv,Hq,token", [(5, 70, 2, 4, 2), (12, 900, 2, 4, 0), (150, 400, 2, 2, 70),
+                                                    (150, 150, 1, 3, 40), (64, 1000, 2, 4, 33), (90, 91, 1, 1, 0)])
+def test_a_query_that_is_not_finite_reaches_only_the_keys_it_sees(nq, length, Hkv, Hq, token, d, x):
+    """The sums of later tokens' keys, and of the other key heads, are the same bits as without it."""
+    cache = Cache([length], Hkv, d, 16, seed=nq + d)
+    q = randn(gen(2), nq, Hq, d)
+    before = _sums(cache, 5)
+    o, m, l, w = _call(cache, q, [nq], [length], before)
+    check_attention(cache, q, [nq], [length], o, scale=0.1, m=m, l=l, weights=w, before=before)
+    q[token, Hq // Hkv - 1] = x  # the last query head of the first key head: every score is NaN or infinite
+    o2, m2, l2, w2 = _call(cache, q, [nq], [length], before)
+    seen = length - nq + token + 1
+    assert torch.isnan(o2[token, Hq // Hkv - 1]).all() and torch.isnan(w2[0, 0, :seen]).all()
+    assert torch.equal(w2[0, 0, seen:], w[0, 0, seen:]) and torch.equal(w2[0, 1:], w[0, 1:])
+    rest = torch.ones((nq, Hq), dtype=torch.bool, device=DEV)
+    rest[token, Hq // Hkv - 1] = False
+    for a, b in ((o2, o), (m2, m), (l2, l)):
+        assert torch.equal(a[rest], b[rest])
