@@ -117,6 +117,9 @@ __device__ __forceinline__ void weights_of_scores(const PagedArgs& a, int block,
   if (key0 >= x.len) return;
   const int old = x.len - x.nq, rows = x.nq * a.G;
   const float c = a.scale * kLog2e;
+  // the page of the four keys; of an invalid one they count as masked, whatever the
+  // rows hold (a NaN would pass their stored -inf)
+  const int page = group_page(a, a.table + (int64_t)b * a.table_ld, key, x.len);
   f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int r0 = 0; r0 < rows; r0 += kLogRows) {
     const int n = min(rows - r0, kLogRows);
@@ -145,7 +148,7 @@ __device__ __forceinline__ void weights_of_scores(const PagedArgs& a, int block,
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (key + e < x.len) add_weight(a, b, h, key + e, old, w[e]);
+    if (key + e < x.len) add_weight(a, b, h, key + e, old, page >= 0 && page < a.n_pages ? w[e] : 0.f);
 }
 
 template <int D, int R, int WAVES>

@@ -73,3 +73,22 @@ def test_a_query_that_is_not_finite_reaches_only_the_keys_it_sees(nq, length, Hk
     rest[token, Hq // Hkv - 1] = False
     for a, b in ((o2, o), (m2, m), (l2, l)):
         assert torch.equal(a[rest], b[rest])
+
+
+@pytest.mark.parametrize("bad", [-1, 2 ** 31 - 1])
+@pytest.mark.parametrize("nq,length", [(1, 200), (2, 3000), (90, 200)])
+def test_keys_of_an_invalid_page_get_nothing_from_any_row(nq, length, bad):
+    """Also from a row whose query is NaN: such keys count as masked."""
+    cache = Cache([length], 2, 128, 16, seed=4)
+    good = ints([0, 5, 6])  # pages, none of a new token's key
+    q = randn(gen(1), nq, 4, 128)
+    q[nq // 2, 1] = float("nan")
+    before = _sums(cache, 5)
+    keys = (16 * good[:, None] + torch.arange(16, device=DEV)).flatten()
+    keys = keys[keys < length - nq]
+    cache.table[0, good.long()] = bad
+    *_, w = _call(cache, q, [nq], [length], before)
+    assert torch.equal(w[0][:, keys], before[0][:, keys])
+    rest = torch.ones(length - nq, dtype=torch.bool, device=DEV)
+    rest[keys] = False
+    assert torch.isnan(w[0, 0, :length - nq][rest]).all() and torch.isfinite(w[0, 1, :length]).all()
