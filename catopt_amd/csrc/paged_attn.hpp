@@ -244,9 +244,12 @@ __device__ __forceinline__ bool odd_values(const bf16x8* vf) {
 // For a product O^T += V^T P^T in which a row may not see a key whose value is
 // infinite or NaN: 0 times that value is NaN, so the fragments are left with
 // finite values only, and products of ones count, for each row and column, the
-// seen keys (weight not 0) that hold +inf, -inf or NaN, and add those.
+// seen keys that hold +inf, -inf or NaN, and add those: the keys up to `room` of
+// groups of 8 not in `bad`, as mask_scores has them, whose weight may have
+// underflowed to 0.
 template <int D>
-__device__ __forceinline__ void take_odd_values(bf16x8* vf, const bf16x8* p, f32x16* acc) {
+__device__ __forceinline__ void take_odd_values(bf16x8* vf, int room, uint32_t bad, f32x16* acc) {
+  const int g = (threadIdx.x & 63) >> 5;
 #pragma unroll 1
   for (int kind = 0; kind < 3; ++kind) {
     const float add = kind == 0 ? __builtin_inff() : kind == 1 ? kNegInf : __builtin_nanf("");
@@ -257,15 +260,18 @@ __device__ __forceinline__ void take_odd_values(bf16x8* vf, const bf16x8* p, f32
       for (int r = 0; r < 16; ++r) cnt[r] = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        u32x4 v = __builtin_bit_cast(u32x4, vf[2 * db + u]), w = __builtin_bit_cast(u32x4, p[u]), x, y;
+        u32x4 v = __builtin_bit_cast(u32x4, vf[2 * db + u]), x, y;
+        int last = room - 4 * g;
         // opaque: nothing of this is worked out for all blocks before the loop,
         // which would cost the attention loop its registers
-        asm volatile("" : "+v"(v), "+v"(w));
+        asm volatile("" : "+v"(v), "+v"(last));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t inf = halves_set(v[e] ^ (kind == 0 ? 0x7f807f80u : 0xff80ff80u)) ^ 0x80008000u;
           x[e] = ((kind < 2 ? inf : halves_nan(v[e])) >> 15) * 0x3f80u;  // 1.0
-          y[e] = (halves_set(w[e]) >> 15) * 0x3f80u;
+          const int r = 8 * u + 2 * e;  // the scores' registers of this word: two keys of one group
+          const uint32_t ones = (acc_row(r, 0) <= last ? 0x3f80u : 0u) | (acc_row(r + 1, 0) <= last ? 0x3f800000u : 0u);
+          y[e] = (bad >> (r >> 2)) & 1 ? 0u : ones;
         }
         cnt = mfma32x32x16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), cnt);
       }

@@ -183,7 +183,7 @@ __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedA
     }
     bf16x8 vf[D / 16];
     read_v<D>(Vs, 0, vf);
-    if (masked && odd_values<D>(vf)) take_odd_values<D>(vf, p, acc);
+    if (masked && odd_values<D>(vf)) take_odd_values<D>(vf, lim - key0, bad_now, acc);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll

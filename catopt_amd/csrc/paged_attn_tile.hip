@@ -239,7 +239,7 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
       __builtin_amdgcn_sched_barrier(0);
       if (UNLIKELY(masked)) apply_mask(1, s1);
       const float a1 = half_max(s1);
-      if (UNLIKELY(masked) && UNLIKELY(odd_values<D>(vf[0]))) take_odd_values<D>(vf[0], p0, acc);
+      if (UNLIKELY(masked) && UNLIKELY(odd_values<D>(vf[0]))) take_odd_values<D>(vf[0], lim - kv0, bad & 15u, acc);
       __builtin_amdgcn_sched_barrier(0);
       pv(0, p0);
       half_exp(s1, p1);
@@ -255,7 +255,7 @@ __global__ __launch_bounds__((NT), (D == 64 ? 3 : 2)) void paged_tile_kernel(Pag
       pin(l_run);
       __builtin_amdgcn_sched_barrier(0);
       if (UNLIKELY(__builtin_amdgcn_ballot_w64(a1 != 1.f) != 0)) rescale(a1);
-      if (UNLIKELY(masked) && UNLIKELY(odd_values<D>(vf[1]))) take_odd_values<D>(vf[1], p1, acc);
+      if (UNLIKELY(masked) && UNLIKELY(odd_values<D>(vf[1]))) take_odd_values<D>(vf[1], lim - kv0 - 32, (bad >> 4) & 15u, acc);
       pv(1, p1);
     }
     bad = bad_next;
