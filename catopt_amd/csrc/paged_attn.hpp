@@ -112,9 +112,12 @@ __device__ __forceinline__ float finish(float x, float l, int normalize) {
   return x * (1.0f / l);
 }
 
-// A finished row's statistics: max m (units of q . k) and sum l.
+// A finished row's statistics: max m (units of q . k) and sum l.  The max of the
+// kernels passes a NaN score by, the sum does not (but it is NaN with +inf, too):
+// the carrier's m is NaN then, or a part whose only scores are NaN would compose as
+// an empty one.
 __device__ __forceinline__ void row_stats(const PagedArgs& a, int64_t i, float m, float l) {
-  if (a.m_out) a.m_out[i] = m * a.scale;
+  if (a.m_out) a.m_out[i] = l != l && m < __builtin_inff() ? l : m * a.scale;
   if (a.l_out) a.l_out[i] = l;
   if (a.row_log) a.row_log[i] = l == 0.f ? __builtin_inff() : m * (a.scale * kLog2e) + __builtin_amdgcn_logf(l);
 }

@@ -613,7 +613,7 @@ int32_t catopt_hip_qk_norm_rope(
  *   o = softmax(s) v                    (o: [N, Hq, d])
  * A row that sees no key is NaN (normalize 1) or 0 (normalize 2).  m_out,
  * l_out (fp32 [N, Hq], optional): the row's om carrier, max s and sum of
- * exp(s - m); (-inf, 0) for an empty row.
+ * exp(s - m); (-inf, 0) for an empty row, NaN where a seen score is NaN.
  * weights_out (fp32 [B, Hkv, >= n_table * page_size], optional) receives each
  * key's attention weight summed over the tokens and the query heads of its
  * group, on top of weights_in (the same layout; NULL: zeros), which is not read
