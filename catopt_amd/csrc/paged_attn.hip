@@ -15,11 +15,14 @@ struct Plan {
 // long as its table.  A workgroup takes a tile of 64 keys in 1.7 us alone on
 // its CU and 2.4 beside another (D = 64: 1 and 1.5), its start and masked tiles
 // shared out (1.35 and 2.3 without, which chose worse: 150 tokens each of two
-// sequences over 1650 keys 32.6 us for 29.1); more workgroups than 512 run in
-// rounds.  Ranges cost a launch, 5.5 us, and their numerators' way through
-// memory, at 6 TB/s.  Measured, one range against the ranges chosen (us): 64
-// tokens over 564 keys, 32 heads on 8, 18.0 and 14.2; 512 new tokens 16.5 and
-// 20 (one chosen); 33 to 171 tokens of five sequences, 12 heads of 64, 40 and 21.
+// sequences over 1650 keys 32.6 us for 29.1); more workgroups than 512 are
+// priced as rounds (at D = 64, where three fit a CU, 513 to 768 are priced a
+// round that they do not run).  Ranges cost a launch, 5.5 us, and their
+// numerators' way through memory, at 6 TB/s.  Measured, one range against the
+// ranges chosen (us): 64 tokens over 564 keys, 32 heads on 8, 18.0 and 14.2; 33 to
+// 171 tokens of five sequences, 12 heads of 64, 40 and 21; a prompt of 512 tokens
+// and a table as long 17 and 20 (one chosen), but against a table of 2048 keys or
+// more it gets four ranges and takes 21.
 int tile_splits(int64_t groups, int64_t rows, int64_t D, int64_t cap) {
   const double alone = D == 128 ? 1.7 : 1.0, beside = D == 128 ? 2.4 : 1.5;
   double best = 0;
@@ -49,10 +52,17 @@ int tile_splits(int64_t groups, int64_t rows, int64_t D, int64_t cap) {
 // 16384 workgroups in all (those behind a sequence's keys end at once).  A range
 // is 256 keys at least; 128 where the table's reach is less than 256 for each
 // of the 512 workgroups that the CUs hold; 1024 where it is 4096 for each (a
-// step of 32 sequences of 300 to 16000 keys: 115 us, 124 with 256; at eight
+// step of 32 sequences of 300 to 16000 keys: 100.6 us, 106.6 with 256; at eight
 // sequences of 2000 to 12000 they are level).
 //
 // 128-row tiles: see tile_splits.
+//
+// All of this goes by the tables' reach and the average of the rows, so it is at
+// its best where tables are about as wide as the longest sequence and no entry is
+// idle.  Eight steps of 2000 keys take 17 us, against tables of 32768 keys 33; of
+// 500 keys 10 and 21.  A chunk of 2048 tokens takes 56 us alone and 195 beside 255
+// idle entries, which put it on 32-row tiles.  32 steps of 16000 keys and a chunk
+// of 512 tokens over 4096 keys take 394 us in one call, 330 and 55 in two.
 Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t cap, bool weights) {
   Plan p{};
   const int64_t G = Hq / Hkv, D = d <= 64 ? 64 : 128;

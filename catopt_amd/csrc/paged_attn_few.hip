@@ -12,9 +12,14 @@
 // as soon as it has been used, and the wait for the other one leaves the new
 // loads in flight: the waves read nothing of each other's, so there is no
 // barrier in the loop.  The loads carry the non-temporal hint: a step of 32
-// sequences over 131072 keys 115 -> 102 us with the combination, 536 MB and so 5.4
-// TB/s; a step over 47000 keys with their weights 55 -> 50.  A lane works out the
+// sequences over 131072 keys 115 -> 101 us with the combination, 536 MB and so 5.3
+// TB/s; a step over 47000 keys with their weights 55 -> 49.  A lane works out the
 // place of 8 keys, the wave those of 16 stages at once.
+//
+// The softmax terms are summed in fp32 and rounded to bf16 for the product with V,
+// as in the 128-row kernel, so that both are as exact whichever of them a call takes:
+// off by 0.0021 to 0.0022 of the result's size on random inputs, where the result's
+// own rounding gives 0.0017.
 #include "paged_attn.hpp"
 
 namespace catopt {

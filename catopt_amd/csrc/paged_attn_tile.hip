@@ -12,11 +12,15 @@
 // A tile runs as two key halves of 32, each its own online-softmax step, so
 // that the exponentials of one half issue between the MFMAs of the other.  The
 // reference max moves only when a half exceeds it by kLazy (log2 units);
-// until then p <= 2^kLazy, exact in range for fp32 and bf16.
+// until then p <= 2^kLazy, exact in range for fp32 and bf16.  The row's sum takes p
+// in fp32; the product with V takes it rounded to bf16, which MFMA at this rate
+// asks for: each term is off by half a step at most, and the result by 0.0021 to
+// 0.0023 of its size on random inputs where its own rounding alone gives 0.0017.
 //
-// MFMAs and softmax VALU bound it together (0.4 and 0.55 of the cycles): four
-// prompts of 4096, 32 heads of 128, 598 us, 919 TFLOP/s at a clock of 1.9 GHz; 2048
-// tokens over 8192 keys, 32 heads on 8, 257 us.  Two workgroups a CU at D = 128 (registers),
+// MFMAs and softmax VALU bound it together (0.39 and 0.48 of the cycles): four
+// prompts of 4096, 32 heads of 128, 621 us, 886 TFLOP/s at a clock of 1.9 GHz (598
+// to 657 from one card to another); 2048 tokens over 8192 keys, 32 heads on 8, 263 us
+// (257 to 287).  Two workgroups a CU at D = 128 (registers),
 // three at 64 (two: 77 us where three take 70, four prompts of 2048, 16 heads;
 // four spill).  Further stages of tiles in flight measured level.
 //

@@ -9,12 +9,15 @@
 // keeps 128 keys in registers, 32 per wave, and streams the rows by 32 through
 // LDS; the score accumulator's columns are rows, so each lane adds its rows for
 // 16 keys and the lanes meet once at the end.  Each product's scores take an
-// exponential, a multiply-add and an addition, which costs more than the MFMA:
-// VALU issue bounds it, and the rows' addresses and offsets are kept to a few
-// additions a step.  64 keys a wave (half the LDS reads, two waves to a SIMD
-// instead of four) took 200 us where this took 168, now 164: 2048 tokens over 8192
-// keys, 32 query heads on 8, 730 TFLOP/s.  Where the keys leave CUs idle the
-// rows are split over workgroups and the parts added in order by another launch.
+// exponential, a multiply-add and an addition, which costs more than the MFMA, so
+// the rows' addresses and offsets are kept to a few additions a step.  64 keys a
+// wave (half the LDS reads, two waves to a SIMD instead of four) took 200 us where
+// this took 168, now 164: 2048 tokens over 8192 keys, 32 query heads on 8, 730
+// TFLOP/s.  There VALU and MFMA fill the SIMDs (0.55 and 0.35 of the cycles).  Two
+// chunks of 700 and 1100 tokens over 2200 and 4600 keys take 81 us with 0.43 and
+// 0.26: 1296 workgroups of 1 to 46 steps on 1024 places.  Where the keys leave
+// CUs idle the rows are split over workgroups and the parts added in order by
+// another launch.
 #include "paged_attn.hpp"
 
 namespace catopt {

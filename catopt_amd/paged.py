@@ -1,8 +1,9 @@
 """Operators of a key/value cache kept in pages, for serving.
 
 The cache of one layer is two tensors of pages ``k_pages`` and ``v_pages``,
-each ``(n_pages, Hkv, page_size, d)`` with a contiguous last axis (any other
-strides: pass a ``(n_pages, page_size, Hkv, d)`` storage transposed).  Key
+each ``(n_pages, Hkv, page_size, d)`` with a contiguous last axis (other
+strides as they are, for attention and eviction multiples of 16 bytes: pass a
+``(n_pages, page_size, Hkv, d)`` storage transposed).  Key
 ``j`` of sequence ``b`` lies in slot ``j % page_size`` of page
 ``block_table[b, j // page_size]``; one table serves every layer.  Lengths,
 tables, positions and slots are device tensors that no call reads back, so a
@@ -25,6 +26,10 @@ allocator, and work is enqueued on torch's current stream of the operands'
 device.  What only the device knows (a length past the table, a page index
 outside the pages) never leads out of bounds: lengths are cut to the table's
 reach, keys of an invalid page count as masked, and a write to one is dropped.
+
+What the host knows chooses the kernels: tokens, sequences and the table's width.
+So a call is fastest with tables about as wide as its longest sequence and
+without idle sequences beside a long chunk.
 """
 
 from __future__ import annotations
@@ -255,16 +260,21 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     own: not between the operands' first and last rows); rows behind the
     last sequence are neither read nor written.  ``return_ml`` adds the fp32
     ``(m, l)`` om carriers of the sequences' rows, ``(N, Hq)``, so that a part
-    of the keys kept elsewhere can be combined.  A row that sees no key is NaN
-    (``empty_rows="nan"``) or 0 (``"zero"``), as in
-    :func:`catopt_amd.kernels.attention`.
+    of the keys kept elsewhere can be combined: ``(m, l, o.float() * l[...,
+    None])`` is what :func:`catopt_amd.kernels.om_compose` takes.  A row that
+    sees no key is NaN (``empty_rows="nan"``) or 0 (``"zero"``), as in
+    :func:`catopt_amd.kernels.attention`; its carrier is ``(-inf, 0)``, that of
+    a row with a NaN score NaN.  Scores, statistics and sums are fp32; the
+    softmax terms are rounded to bf16 for the product with the values, and the
+    result once more.
 
     ``weights_out (B, Hkv, L)`` fp32, ``L`` at least the table's reach,
     receives the sum over the new tokens and the key head's query heads of
     each key's softmax weight, on top of ``weights`` (the sums so far; none:
     zeros), which is not read for the new tokens' own keys.  Entries from
     ``kv_lens[b]`` on are left as they were.  ``weights_out`` may be
-    ``weights``."""
+    ``weights``.  With few new tokens the products are kept in between, 4 bytes
+    for each token, query head and key of the table's reach, up to 1 GiB."""
     if empty_rows not in ("nan", "zero"):
         raise ValueError(f"empty_rows is 'nan' or 'zero', got {empty_rows!r}")
     ts = (q, k_pages, v_pages, block_table, kv_lens, q_starts)

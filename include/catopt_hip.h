@@ -621,12 +621,19 @@ int32_t catopt_hip_qk_norm_rope(
  *   weights_out[b, h, j] = (j < kv_len - n ? weights_in[b, h, j] : 0)
  *                          + sum_rows exp(s - m) / l,      j < kv_len
  * Entries from kv_len on are left as they were.  weights_out may be
- * weights_in.  bf16; d a multiple of 8 up to 128; page_size a multiple of 8;
- * q, pages and o 16-byte aligned.
+ * weights_in.  A row adds to the keys that it sees and to no other, whatever it
+ * holds; a value that is infinite or NaN reaches the rows that see its key.
+ * bf16, scores, statistics and sums in fp32, the softmax terms rounded to bf16
+ * for the product with v; d a multiple of 8 up to 128; page_size a multiple of
+ * 8; q, pages and o 16-byte aligned.
  * strides (host, 14 values): q (token, head); k_pages, v_pages (page, head,
  * slot); o (token, head); weights_in, weights_out (sequence, head).
  * Workspace: catopt_hip_paged_attn_workspace_bytes(...) bytes, 16-byte
- * aligned, any contents (-1: invalid arguments).
+ * aligned, any contents (-1: invalid arguments).  It goes by the table's reach,
+ * not by the lengths: with weights_out and 32 rows (N Hq / Hkv) a sequence or
+ * fewer it holds N Hq n_table page_size products of 4 bytes where those take 1
+ * GiB at most.  Beyond, they are formed again (64 sequences of 2000 keys, 32
+ * heads: 223 us with the 1 GiB of a reach of 131072, 267 without).
  */
 int64_t catopt_hip_paged_attn_workspace_bytes(int64_t B, int64_t N, int64_t Hq,
                                               int64_t Hkv, int64_t d,
