@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from catopt_amd import paged as P
-from paged_ref import BF16, DEV, Cache, check_attention, gen, ints, randn, starts_of
+from paged_ref import DEV, Cache, check_attention, gen, ints, randn, starts_of
 
 pytestmark = pytest.mark.gpu
 
