@@ -119,6 +119,15 @@ SIGNATURES: dict[str, tuple] = {
         [_i32, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64,
          _i64, _p, _p, _p, _i32, _p, _p],
     ),
+    "catopt_hip_paged_extend": (
+        _i32,
+        [_i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p],
+    ),
+    "catopt_hip_paged_release_workspace_bytes": (_i64, [_i64]),
+    "catopt_hip_paged_release": (
+        _i32,
+        [_i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _i64, _p],
+    ),
 }
 
 

@@ -9,7 +9,9 @@ strides as they are, for attention and eviction multiples of 16 bytes: pass a
 tables, positions and slots are device tensors that no call reads back, so a
 step recorded into a hipGraph replays with new ones.
 
-A layer's step over new tokens:
+Before a step :func:`paged_extend` makes its starts, positions, slots and new
+table entries out of the requests' lengths, and :func:`paged_release` gives the
+pages of finished requests back.  A layer's step over new tokens:
 
 * :func:`qk_norm_rope_append` norms and rotates their queries and keys and
   writes keys and values into the cache (:func:`qk_norm_rope` returns them
@@ -36,14 +38,15 @@ from __future__ import annotations
 
 import functools
 import struct
+from typing import NamedTuple
 
 import torch
 
 from . import _lib as L
 from .kernels import _DT, _need_device, _stream_of
 
-__all__ = ["qk_norm_rope", "qk_norm_rope_append", "paged_attention", "paged_evict", "PAGED_ATTENTION_MAX_HEAD_DIM",
-           "QK_NORM_ROPE_MAX_HEAD_DIM"]
+__all__ = ["qk_norm_rope", "qk_norm_rope_append", "paged_attention", "paged_evict", "paged_extend", "paged_release",
+           "PagedStep", "PAGED_ATTENTION_MAX_HEAD_DIM", "QK_NORM_ROPE_MAX_HEAD_DIM"]
 
 PAGED_ATTENTION_MAX_HEAD_DIM = 128
 QK_NORM_ROPE_MAX_HEAD_DIM = 256
@@ -408,3 +411,123 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch
         if st:
             _check("paged_evict", st)
     return kept, new_lens, weights_out
+
+
+class PagedStep(NamedTuple):
+    """What :func:`paged_extend` returns: a step's operands for the other calls."""
+
+    q_starts: torch.Tensor  # (B + 1,) int32
+    positions: torch.Tensor  # (n_tokens,) int64
+    slots: torch.Tensor  # (n_tokens,) int64
+    kv_lens: torch.Tensor  # (B,) int32, the new tokens included
+    free_count: torch.Tensor  # (1,) int32
+
+
+def _in_place(name: str, t: torch.Tensor, n: int) -> torch.Tensor:
+    """An int32 vector that a call writes: taken as it is, never a copy of it."""
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} is a contiguous int32 vector of {n}, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+    return t
+
+
+def _pool(free_pages: torch.Tensor, free_count: torch.Tensor) -> int:
+    if free_pages.dim() != 1:
+        raise ValueError(f"free_pages is an int32 vector, got {tuple(free_pages.shape)}")
+    _in_place("free_pages", free_pages, free_pages.numel())
+    _in_place("free_count", free_count, 1)
+    return free_pages.numel()
+
+
+def _page_size(page_size: int) -> int:
+    page_size = int(page_size)
+    if page_size < 1:
+        raise ValueError(f"a page holds at least one key, got {page_size}")
+    return page_size
+
+
+def paged_extend(block_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
+                 free_count: torch.Tensor, n_tokens: int, page_size: int, *, offsets: torch.Tensor | None = None,
+                 kv_lens_out: torch.Tensor | None = None, free_count_out: torch.Tensor | None = None) -> PagedStep:
+    """A step's starts, positions, slots and new pages from its requests'
+    lengths (all int32 on the device).
+
+    Sequence ``b`` has ``kv_lens[b]`` cached keys and ``new_lens[b]`` new
+    tokens; a negative number counts as 0.  Its rows among the ``n_tokens`` of
+    the step begin at ``q_starts[b]``, its ``i``-th new token is key
+    ``kv_lens[b] + i``, at position ``kv_lens[b] + i + offsets[b]`` (none: 0; a
+    shared prefix's length, say) and in ``slots``' place of the cache.  Rows
+    behind the last token are padding: position 0, slot -1; tokens for which
+    there is no row are cut off, from the last sequences.
+
+    Pages beyond those that hold ``kv_lens[b]`` keys come out of the pool
+    ``free_pages[:free_count]`` (``free_count (1,)``), the last one first,
+    sequence by sequence, and go into ``block_table (B, n)`` in place.  A pool
+    that runs out gives -1, whose keys are not written and count as masked.
+    Keys past the table's reach get no page either, and lengths end there.
+
+    The lengths with the new tokens and the pages left are returned as new
+    tensors, or written to ``kv_lens_out`` and ``free_count_out``, which may be
+    ``kv_lens`` and ``free_count``: a step recorded into a hipGraph then goes on
+    where its last replay ended."""
+    ts = (block_table, kv_lens, new_lens, free_pages, free_count)
+    ts += tuple(t for t in (offsets, kv_lens_out, free_count_out) if t is not None)
+    dev = _device(ts)
+    B = kv_lens.numel()
+    n_tokens, page_size = int(n_tokens), _page_size(page_size)
+    if n_tokens < 0:
+        raise ValueError(f"a step has at least 0 tokens, got {n_tokens}")
+    kv_lens, new_lens = _vector("kv_lens", kv_lens, torch.int32, B), _vector("new_lens", new_lens, torch.int32, B)
+    offsets_at = None
+    if offsets is not None:
+        offsets = _vector("offsets", offsets, torch.int32, B)
+        offsets_at = offsets.data_ptr()
+    table, n_table, table_ld = _table("block_table", block_table, B)
+    if table is not block_table:
+        raise ValueError(f"block_table is written in place and needs a contiguous last axis, got strides {block_table.stride()}")
+    n_free = _pool(free_pages, free_count)
+    lens_out = kv_lens.new_empty((B,)) if kv_lens_out is None else _in_place("kv_lens_out", kv_lens_out, B)
+    count_out = kv_lens.new_empty((1,)) if free_count_out is None else _in_place("free_count_out", free_count_out, 1)
+    starts = kv_lens.new_empty((B + 1,))
+    positions = kv_lens.new_empty((n_tokens,), dtype=torch.int64)
+    slots = kv_lens.new_empty((n_tokens,), dtype=torch.int64)
+    st = _launch(dev, L.load().catopt_hip_paged_extend, B, n_tokens, page_size, table.data_ptr(), table_ld, n_table,
+                 kv_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), n_free, free_count.data_ptr(), offsets_at,
+                 starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), lens_out.data_ptr(), count_out.data_ptr())
+    if st:
+        _check("paged_extend", st)
+    return PagedStep(starts, positions, slots, lens_out, count_out)
+
+
+def paged_release(block_table: torch.Tensor, kv_lens: torch.Tensor, released: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, page_size: int, *, kv_lens_out: torch.Tensor | None = None,
+                  free_count_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Give the pages of finished sequences back to the pool.
+
+    For each sequence with ``released[b]`` (bool), in order, the pages of its
+    ``kv_lens[b]`` keys (those of ``block_table`` that are not negative) go to
+    ``free_pages`` from ``free_count`` on; what does not fit is dropped.  The
+    table stays as it is.  Returns the lengths, 0 for the released, and the new
+    count, in new tensors or in ``kv_lens_out`` and ``free_count_out``, which
+    may be ``kv_lens`` and ``free_count``."""
+    ts = (block_table, kv_lens, released, free_pages, free_count)
+    ts += tuple(t for t in (kv_lens_out, free_count_out) if t is not None)
+    dev = _device(ts)
+    B = kv_lens.numel()
+    page_size = _page_size(page_size)
+    kv_lens, released = _vector("kv_lens", kv_lens, torch.int32, B), _vector("released", released, torch.bool, B)
+    table, n_table, table_ld = _table("block_table", block_table, B)
+    n_free = _pool(free_pages, free_count)
+    lens_out = kv_lens.new_empty((B,)) if kv_lens_out is None else _in_place("kv_lens_out", kv_lens_out, B)
+    count_out = kv_lens.new_empty((1,)) if free_count_out is None else _in_place("free_count_out", free_count_out, 1)
+    lib = L.load()
+    wsb = lib.catopt_hip_paged_release_workspace_bytes(B)
+    ws_at = None
+    if wsb > 0:
+        ws = kv_lens.new_empty((wsb // 4,))
+        ws_at = ws.data_ptr()
+    st = _launch(dev, lib.catopt_hip_paged_release, B, page_size, table.data_ptr(), table_ld, n_table, kv_lens.data_ptr(),
+                 released.data_ptr(), free_pages.data_ptr(), n_free, free_count.data_ptr(), lens_out.data_ptr(),
+                 count_out.data_ptr(), ws_at, max(wsb, 0))
+    if st:
+        _check("paged_release", st)
+    return lens_out, count_out

@@ -678,6 +678,51 @@ int32_t catopt_hip_paged_evict(
     int64_t n_out_table, int32_t* kept, int32_t* new_lens, float* weights_out,
     int32_t clear_behind, const int64_t* strides, void* stream);
 
+/*
+ * A step's tables, slots and positions from its requests' lengths.  Sequence b
+ * (of B) has kv_lens[b] cached keys and new_lens[b] new tokens (int32; below 0
+ * counts as 0), all tokens together at most N rows (what is more is cut off,
+ * from the last sequences):
+ *   q_starts (int32 [B + 1])   each one's first row, and the end
+ *   positions (int64 [N])      kv_lens[b] + i, + offsets[b] (int32 [B], optional)
+ *   slots (int64 [N])          page * page_size + slot of key kv_lens[b] + i
+ *   kv_lens_out (int32 [B])    the lengths with the new tokens
+ *   free_count_out (int32 [1]) the pages left
+ * Rows behind the last token get position 0 and slot -1.  A sequence's pages
+ * beyond those that hold its keys are taken from the pool, free_pages[0 ..
+ * free_count) (int32), the last one first, sequence by sequence, and written
+ * into block_table (int32 [B, n_table], rows table_ld apart); where the pool
+ * has none, -1 is written and the slots are -1.  Keys past the table's reach
+ * (n_table * page_size) get no page and the slot -1, and lengths end there.
+ * kv_lens_out may be kv_lens and free_count_out free_count (then the call takes
+ * two launches where N > 0); no other output may overlap an operand.
+ */
+int32_t catopt_hip_paged_extend(
+    int64_t B, int64_t N, int64_t page_size, int32_t* block_table,
+    int64_t table_ld, int64_t n_table, const int32_t* kv_lens,
+    const int32_t* new_lens, const int32_t* free_pages, int64_t n_free,
+    const int32_t* free_count, const int32_t* offsets, int32_t* q_starts,
+    int64_t* positions, int64_t* slots, int32_t* kv_lens_out,
+    int32_t* free_count_out, void* stream);
+
+/*
+ * The pages of finished sequences back to the pool: for each b with
+ * released[b] != 0, in order, the valid ones (>= 0) of the ceil(kv_lens[b] /
+ * page_size) pages that block_table names go to free_pages from free_count on
+ * (what does not fit into its n_free entries is dropped).  kv_lens_out: 0 for
+ * those, else kv_lens; free_count_out: the new count.  Both may be in place.
+ * The table is left as it is.
+ * Workspace: catopt_hip_paged_release_workspace_bytes(B) bytes, any contents
+ * (-1: invalid arguments).
+ */
+int64_t catopt_hip_paged_release_workspace_bytes(int64_t B);
+int32_t catopt_hip_paged_release(
+    int64_t B, int64_t page_size, const int32_t* block_table, int64_t table_ld,
+    int64_t n_table, const int32_t* kv_lens, const uint8_t* released,
+    int32_t* free_pages, int64_t n_free, const int32_t* free_count,
+    int32_t* kv_lens_out, int32_t* free_count_out, void* workspace,
+    int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
