@@ -21,7 +21,7 @@ EPI_NONE, EPI_BIAS, EPI_BIAS_ADD2, EPI_SILU_MUL, EPI_GLU = 0, 1, 2, 3, 4
 MASK_NONE, MASK_CAUSAL, MASK_BOOL, MASK_BIAS = 0, 1, 2, 3
 SCAN_AUTO, SCAN_STREAM, SCAN_CHUNKED = 0, 1, 2
 
-_i32, _i64, _f32, _p = C.c_int32, C.c_int64, C.c_float, C.c_void_p
+_i32, _i64, _f32, _f64, _p = C.c_int32, C.c_int64, C.c_float, C.c_double, C.c_void_p
 _pi64 = C.POINTER(C.c_int64)
 
 #: name -> (restype, argtypes); the exported surface of the header.
@@ -127,6 +127,11 @@ SIGNATURES: dict[str, tuple] = {
     "catopt_hip_paged_release": (
         _i32,
         [_i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _i64, _p],
+    ),
+    "catopt_hip_sample_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32]),
+    "catopt_hip_sample": (
+        _i32,
+        [_i32, _i64, _i64, _p, _i64, _p, _p, _f64, _p, _i64, _p, _f64, _p, _f64, _p, _p, _p, _i64, _p, _i64, _p],
     ),
 }
 

@@ -1,0 +1,148 @@
+// What the kernels of token sampling share: a call's arguments, a row's settings
+// and the fixed-point weights.
+#pragma once
+#include "common.hpp"
+
+namespace catopt {
+
+// Weights exp((x - max) / T) lie on a grid of 16 steps to a factor of 2: with y =
+// x 16 log2(e) / T and n = rint(y), a logit belongs to the bin n and weighs
+// 2^(n / 16) 2^((y - n) / 16).  The second factor, between 0.978 and 1.022, is
+// rounded to 42 bits behind the point: a bin's weight is then a sum of integers,
+// the same in every order, whichever chunk of the row a logit lies in.  A bin 768
+// steps below the largest logit's weighs 2^-48 of it or less and counts as nothing.
+constexpr int kBins = 768;
+constexpr int kPoint = 42;
+constexpr int64_t kMaxVocab = 1LL << 21;  // a bin's sum stays below 2^(21 + 42.04)
+
+struct SampleArgs {
+  const void* x;
+  int64_t ld, ld_probs;
+  int V, B, chunks;
+  // a row's own setting, else the call's
+  const float *t_row, *p_row, *low_row;
+  const int32_t* k_row;
+  double t, p, low;
+  int64_t k;
+  const float* u;
+  int64_t* tokens;
+  float *logprobs, *probs;
+  struct ChunkHead* heads;  // [B][chunks]
+  uint64_t* weights;        // [B][chunks][kBins]
+  uint32_t* counts;         // the same, of rows with a top-k
+  struct RowState* rows;    // [B], for the probabilities
+};
+
+struct ChunkHead {
+  float max;
+  int32_t first;  // greedy rows: where the largest logit is first
+  int32_t nan, pad;
+};
+
+// What the probabilities of a row are worked out from.
+struct RowState {
+  double c, ref, low, log2_total;  // y = c x; the largest logit's n; the least y; log2 of the kept weights
+  uint64_t cut_at;                 // in the cut's bin the last place that is kept
+  int32_t cut, token;              // the last bin that is kept (some of it); kOneHot, kNone: the token alone, NaN
+};
+constexpr int kOneHot = -1, kNone = -2;
+
+struct Settings {
+  double t, p, low;
+  int64_t k;
+  bool greedy, valid;
+};
+
+__device__ __forceinline__ Settings settings(const SampleArgs& a, int row) {
+  Settings s;
+  s.t = a.t_row ? (double)a.t_row[row] : a.t;
+  s.p = a.p_row ? (double)a.p_row[row] : a.p;
+  s.low = a.low_row ? (double)a.low_row[row] : a.low;
+  s.k = a.k_row ? (int64_t)a.k_row[row] : a.k;
+  s.valid = s.t >= 0;
+  s.greedy = s.t == 0 || s.k == 1;
+  if (s.k <= 0 || s.k >= a.V) s.k = 0;  // all
+  return s;
+}
+
+// y's factor: at most 2^40 for the largest logit, where all that is not equal to it
+// lies far behind the last bin, so that n is exact.
+__device__ __forceinline__ double factor(double t, float max) {
+  return fmin(16 * 1.4426950408889634 / t, 0x1p40 / fmax(fabs((double)max), 0x1p-120));
+}
+
+// A logit's n; and its place in the bin, y - n.
+__device__ __forceinline__ double grid(float x, double c, double& rest) {
+  const double magic = 0x1.8p52;
+  const double n = __builtin_fma((double)x, c, magic) - magic;
+  rest = __builtin_fma((double)x, c, -n);
+  return n;
+}
+
+// 2^(rest / 16) in fixed point, |rest| <= 1/2: the series to the fifth power, off by
+// less than 1.5e-13, with the sum's last addend 2^52 making the mantissa an integer.
+__device__ __forceinline__ uint64_t fixed(double rest) {
+  constexpr double l = 0.6931471805599453 / 16, one = 1LL << kPoint;
+  double s = one * (l * l * l * l * l / 120);
+  s = __builtin_fma(s, rest, one * (l * l * l * l / 24));
+  s = __builtin_fma(s, rest, one * (l * l * l / 6));
+  s = __builtin_fma(s, rest, one * (l * l / 2));
+  s = __builtin_fma(s, rest, one * l);
+  s = __builtin_fma(s, rest, one + 0x1p52);
+  return __builtin_bit_cast(uint64_t, s) & 0xfffffffffffffull;
+}
+
+// The order of a row, as ascending numbers: the largest logit first, the lowest
+// index first among equals (-0 as 0).
+__device__ __forceinline__ uint64_t place(float x, int i) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
+  const uint32_t key = b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+  return (uint64_t)~key << 32 | (uint32_t)i;
+}
+__device__ __forceinline__ float logit_of(uint64_t place) {
+  const uint32_t key = ~(uint32_t)(place >> 32);
+  return __builtin_bit_cast(float, key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
+// A row in pieces of 16 bytes from the aligned address at or before its first
+// logit: piece i holds logits W i - shift on.  Pieces at the row's ends are read
+// logit by logit; what is not in the row reads as -inf.
+template <typename T>
+struct RowReader {
+  static constexpr int W = 16 / sizeof(T);
+  const T* row;
+  int V, shift;
+
+  __device__ __forceinline__ RowReader(const SampleArgs& a, int r)
+      : row(static_cast<const T*>(a.x) + (int64_t)r * a.ld), V(a.V) {
+    shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+  }
+  __device__ __forceinline__ int pieces() const { return (V + shift + W - 1) / W; }
+  __device__ __forceinline__ int first(int piece) const { return piece * W - shift; }
+  __device__ __forceinline__ u32x4 load(int piece) const {
+    const int i = first(piece);
+    if (i >= 0 && i + W <= V) return *reinterpret_cast<const u32x4*>(row + i);
+    const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+    u32x4 w = {none, none, none, none};
+    if (i + W <= 0 || i >= V) return w;
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      if (i + e < 0 || i + e >= V) continue;
+      if constexpr (sizeof(T) == 4)
+        w[e] = __builtin_bit_cast(uint32_t, row[i + e]);
+      else
+        w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | (uint32_t)row[i + e] << 16 : (w[e / 2] & 0xffff0000u) | row[i + e];
+    }
+    return w;
+  }
+  // Logit e of a piece.
+  static __device__ __forceinline__ float at(const u32x4& w, int e) {
+    const uint32_t word = sizeof(T) == 4 ? w[e] : w[e / 2];
+    return __builtin_bit_cast(float, sizeof(T) == 4 ? word : e & 1 ? word & 0xffff0000u : word << 16);
+  }
+};
+
+// +inf as the largest finite number.
+__device__ __forceinline__ float finite_top(float x) { return __builtin_fminf(x, 0x1.fffffep127f); }
+
+}  // namespace catopt

@@ -1,0 +1,106 @@
+"""The next tokens of a generation step, from logits and given random numbers.
+
+As in :mod:`catopt_amd.paged`, operands are device tensors checked on the host
+before any launch, outputs and workspace come from torch's caching allocator,
+and work is enqueued on torch's current stream of the operands' device.  Nothing
+is read back, so a step records into a hipGraph and replays on new logits,
+numbers and settings.
+"""
+
+from __future__ import annotations
+
+import functools
+
+import torch
+
+from . import _lib as L
+from .kernels import _DT
+from .paged import _device, _launch
+
+__all__ = ["sample", "SAMPLE_MAX_VOCAB"]
+
+SAMPLE_MAX_VOCAB = 1 << 21
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(B: int, V: int, counted: bool, probs: bool) -> int:
+    n = L.load().catopt_hip_sample_workspace_bytes(B, V, counted, probs)
+    if n < 0:
+        raise NotImplementedError(f"sample takes vocabularies of up to {SAMPLE_MAX_VOCAB}, got {B} rows of {V}")
+    return n
+
+
+def _setting(name: str, v, dtype: torch.dtype, B: int, ok) -> tuple[torch.Tensor | None, float]:
+    """A setting of every row's own (a tensor), or one number for all of them."""
+    if isinstance(v, torch.Tensor):
+        if v.dtype is not dtype or v.shape != (B,):
+            raise ValueError(f"{name} is a number or a {dtype} vector of {B}, got {v.dtype} {tuple(v.shape)}")
+        return v.contiguous(), 0
+    if not ok(v):
+        raise ValueError(f"{name} is out of range: {v!r}")
+    return None, v
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: float | torch.Tensor = 1.0,
+           top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0, *,
+           return_probs: bool = False):
+    """The next token of each row of ``logits (B, V)`` (fp32 or bf16) by
+    temperature, top-k, top-p, min-p and ``uniforms (B,)``, fp32 numbers in
+    ``[0, 1)``.
+
+    A token's weight is ``exp((x - max) / temperature)``.  In the order that
+    takes the largest logit first and the lowest index first among equals, what
+    is left are the first ``top_k`` (0: all), of those as many as it takes for a
+    share ``top_p`` of their weight (1: all; one at least), of those the ones
+    whose weight is ``min_p`` times the largest or more.  The token is the first
+    of them at which the running sum of weights exceeds ``uniforms`` times the
+    whole; a temperature of 0 takes the first largest logit.
+
+    Each setting is a number or a vector of one for each row (fp32, ``top_k``
+    int32).  In a vector a ``top_k`` below 1, a ``top_p`` of 1 or more or NaN and
+    a ``min_p`` of 0 or below or NaN mean all; a ``top_p`` of 0 or below the
+    first, a ``min_p`` above 1 as much as 1.  A number outside ``[0, 1)`` counts
+    as the nearest inside it, a NaN as 0.
+
+    Returns ``tokens (B,)`` int64 and ``logprobs (B,)`` fp32, the log
+    probability of each among those that were left, and with ``return_probs``
+    their probabilities ``(B, V)`` fp32, 0 for the others.  Masked logits are
+    ``-inf``; one of ``+inf`` counts as the largest finite number.  A row with a
+    NaN, with nothing above ``-inf`` or with a temperature that is negative or
+    NaN gives token -1 and NaN.
+
+    Weights are in 64 bits, each off by 2^-42 of itself at most, and added up as
+    integers, so the outcome does not depend on the run; those below 2^-42 of the
+    largest count as nothing."""
+    ts = (logits, uniforms) + tuple(v for v in (temperature, top_k, top_p, min_p) if isinstance(v, torch.Tensor))
+    dev = _device(ts)
+    dt = _DT.get(logits.dtype)
+    if dt is None:
+        raise NotImplementedError(f"sample runs on fp32 and bf16 logits, got {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits is (rows, at least one token), got {tuple(logits.shape)}")
+    B, V = logits.shape
+    if uniforms.dtype is not torch.float32 or uniforms.shape != (B,):
+        raise ValueError(f"uniforms is an fp32 vector of {B}, got {uniforms.dtype} {tuple(uniforms.shape)}")
+    t, t_all = _setting("temperature", temperature, torch.float32, B, lambda v: v >= 0)
+    k, k_all = _setting("top_k", top_k, torch.int32, B, lambda v: isinstance(v, int) and v >= 0)
+    p, p_all = _setting("top_p", top_p, torch.float32, B, lambda v: 0 <= v <= 1)
+    low, low_all = _setting("min_p", min_p, torch.float32, B, lambda v: 0 <= v <= 1)
+    if (logits.stride(1) != 1 and V > 1) or (B > 1 and logits.stride(0) < 0):
+        logits = logits.contiguous()
+    uniforms = uniforms.contiguous()
+    tokens = uniforms.new_empty((B,), dtype=torch.int64)
+    logprobs = uniforms.new_empty((B,))
+    probs = uniforms.new_empty((B, V)) if return_probs else None
+    if B:
+        k_all = min(int(k_all), V)
+        wsb = _workspace(B, V, k is not None or k_all > 1, return_probs)
+        ws = uniforms.new_empty(wsb // 4 + 1)
+        st = _launch(dev, L.load().catopt_hip_sample, dt, B, V, logits.data_ptr(), logits.stride(0), uniforms.data_ptr(),
+                     t if t is None else t.data_ptr(), t_all, k if k is None else k.data_ptr(), k_all,
+                     p if p is None else p.data_ptr(), p_all, low if low is None else low.data_ptr(), low_all,
+                     tokens.data_ptr(), logprobs.data_ptr(), None if probs is None else probs.data_ptr(), V, ws.data_ptr(),
+                     wsb)
+        if st:
+            L.check("sample", st)
+    return (tokens, logprobs, probs) if return_probs else (tokens, logprobs)

@@ -723,6 +723,35 @@ int32_t catopt_hip_paged_release(
     int32_t* kv_lens_out, int32_t* free_count_out, void* workspace,
     int64_t workspace_bytes, void* stream);
 
+/*
+ * The next token of each of B rows of V logits (F32 or BF16, rows ld apart) by
+ * temperature T, top-k, top-p, min-p and a number u in [0, 1).  With w =
+ * exp((x - max x) / T) and the order that takes the largest logit first, the
+ * lowest index first among equals, the first k are left (k <= 0: all), of those
+ * as many as it takes for a share p of their weight (p >= 1: all; one at
+ * least), of those the ones with w >= min_p.  The token is the first of them at
+ * which the running sum of w exceeds u times the whole; logprobs its log
+ * probability among them; probs (fp32 [B, V], rows ld_probs apart, optional)
+ * everyone's, 0 for the others.  T = 0 takes the first largest logit.  A row
+ * with a NaN, with nothing above -inf or with T < 0 gives -1 and NaN.  A logit
+ * of +inf counts as the largest finite number.
+ * Weights have an error of 2^-42 of themselves and those below 2^-42 of the
+ * largest count as nothing; sums are of integers, the same on every run.
+ * temperature, top_k, top_p, min_p ([B], device, optional) hold each row's own
+ * settings; NULL: the *_all value for all rows.  V <= 2^21.
+ * Workspace: catopt_hip_sample_workspace_bytes(B, V, counted, with probs) bytes,
+ * 16-byte aligned, any contents; counted where top_k is given or top_k_all > 1.
+ */
+int64_t catopt_hip_sample_workspace_bytes(int64_t B, int64_t V,
+                                          int32_t counted, int32_t probs);
+int32_t catopt_hip_sample(
+    int32_t dtype, int64_t B, int64_t V, const void* logits, int64_t ld,
+    const float* u, const float* temperature, double temperature_all,
+    const int32_t* top_k, int64_t top_k_all, const float* top_p,
+    double top_p_all, const float* min_p, double min_p_all, int64_t* tokens,
+    float* logprobs, float* probs, int64_t ld_probs, void* workspace,
+    int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,58 @@
+"""What token sampling refuses on the host, before any launch (the addresses are never read)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from catopt_amd import _lib as L
+from catopt_amd import sampling as S
+
+A = [1 << 20 | i << 32 for i in range(16)]  # far apart
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not L.LIB_PATH.exists():
+        from catopt_amd import build
+
+        build.build()
+    return L.load()
+
+
+def _call(lib, dtype=L.F32, B=4, V=100, x=A[0], ld=100, u=A[1], t=None, t_all=1.0, k=None, k_all=0, p=None, p_all=1.0, low=None,
+          low_all=0.0, tokens=A[2], logprobs=A[3], probs=None, ld_probs=100, ws=A[4], wsb=1 << 30):
+    return lib.catopt_hip_sample(dtype, B, V, x, ld, u, t, t_all, k, k_all, p, p_all, low, low_all, tokens, logprobs, probs,
+                                 ld_probs, ws, wsb, None)
+
+
+def test_refusals(lib):
+    assert _call(lib, B=0) == L.OK
+    for kw in ({"B": -1}, {"V": 0}, {"x": None}, {"u": None}, {"tokens": None}, {"logprobs": None}, {"ld": -1},
+               {"x": A[0] + 2}, {"probs": A[5], "ld_probs": 99}, {"tokens": A[1]}, {"logprobs": A[0] + 1596}, {"probs": A[0]},
+               {"tokens": A[3] + 8}, {"probs": A[2] - 1596}, {"t": A[2]}, {"k": A[3] + 12}, {"p": A[5], "probs": A[5]}, {"low": A[2] + 28}):
+        assert _call(lib, **kw) == L.E_INVAL, kw
+    for kw in ({"dtype": 2}, {"V": (1 << 21) + 1}, {"B": 1 << 21}, {"B": 1 << 20, "V": 1 << 20}):
+        assert _call(lib, **kw) == L.E_UNSUPPORTED, kw
+    f = lib.catopt_hip_sample_workspace_bytes
+    need = f(4, 100, 1, 0)
+    assert 0 < f(4, 100, 0, 0) < need < f(4, 100, 1, 1)
+    assert f(-1, 100, 0, 0) == -1 and f(4, 0, 0, 0) == -1 and f(4, (1 << 21) + 1, 0, 0) == -1
+    for kw in ({"ws": None}, {"wsb": need - 1}, {"ws": A[4] + 8}):
+        assert _call(lib, k_all=5, **kw) == L.E_WORKSPACE, kw
+
+
+def test_python_checks(monkeypatch):
+    x, u = torch.zeros((3, 10)), torch.zeros((3,))
+    with pytest.raises(ValueError, match="ROCm device"):
+        S.sample(x, u)
+    monkeypatch.setattr(S, "_device", lambda ts: 0)  # the checks behind it, which end before the launch
+    for a in ((x[0], u), (x[:, :0], u), (x, u[:2]), (x, u.double()), (x, u, -0.5), (x, u, float("nan")), (x, u, 1.0, -1),
+              (x, u, 1.0, 2.5), (x, u, 1.0, 0, 1.5), (x, u, 1.0, 0, -0.1), (x, u, 1.0, 0, float("nan")), (x, u, 1.0, 0, 1.0, 2.0),
+              (x, u, u.double()), (x, u, u[:2]), (x, u, 1.0, u), (x, u, 1.0, 0, u.int()), (x, u, 1.0, 0, 1.0, u[None])):
+        with pytest.raises(ValueError):
+            S.sample(*a)
+    with pytest.raises(NotImplementedError):
+        S.sample(x.half(), u)
+    with pytest.raises(NotImplementedError):
+        S.sample(torch.zeros((1,)).expand(1, (1 << 21) + 1), u[:1])

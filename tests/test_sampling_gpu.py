@@ -1,0 +1,274 @@
+"""Token sampling against its definition in float64 (numpy's argsort, cumsum and searchsorted)."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from catopt_amd import sampling as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def row_ref(x, u, t, k, p, low):
+    """(token, log probability, probabilities, how near u and the borders come to a sum, how far off sums may be), the
+    last two relative to the whole.  A weight is rounded to 2^-42 of itself (half of it off at most) and its series is
+    off by 2^-42.6, so a sum is off by less than 2^-41 of itself; each of 768 bins' sums is rounded to 2^-42 of the
+    largest weight, which is at most the whole; and weights below 2^-41 of the largest may count as nothing."""
+    V = len(x)
+    if np.isnan(x).any() or not (x > -np.inf).any() or not t >= 0:
+        return -1, math.nan, np.full(V, np.nan), 1.0, 0.0
+    x = np.minimum(x, np.finfo(np.float32).max)
+    order = np.argsort(-x, kind="stable")
+    order = order[x[order] > -np.inf]
+    if k > 0:
+        order = order[:k]
+    if t == 0:
+        order, w = order[:1], np.ones(1)
+    else:
+        w = np.exp((x[order] - x[order[0]]) / t)
+    off = 2.0 ** -40 + 768 * 2.0 ** -43 + w[w < 2.0 ** -41].sum()  # in both sums that are compared
+    near = 1.0
+    if p < 1:
+        cum = np.cumsum(w)
+        near = min(near, float(np.abs(cum / cum[-1] - p).min()))
+        n = 1 + int(np.searchsorted(cum, p * cum[-1], side="left"))
+        order, w = order[:n], w[:n]
+    if low > 0:
+        near = min(near, float(np.abs(w - min(low, 1.0))[w < 1].min(initial=1.0)))
+        keep = w >= min(low, 1.0)
+        order, w = order[keep], w[keep]
+    cum = np.cumsum(w)
+    u = min(max(u if u == u else 0.0, 0.0), 1 - 2.0 ** -25)
+    i = min(int(np.searchsorted(cum, u * cum[-1], side="right")), len(w) - 1)
+    if u > 0:
+        near = min(near, float(np.abs(cum / cum[-1] - u).min()))
+    probs = np.zeros(V)
+    probs[order] = w / cum[-1]
+    return int(order[i]), math.log(w[i] / cum[-1]), probs, near, off
+
+
+def check(x, u, t=1.0, k=0, p=1.0, low=0.0, probs=True, ties=False):
+    """The token must be the reference's unless a border or u is as near to a sum as sums may be off, which no seed here
+    comes to."""
+    r = S.sample(x, u, t, k, p, low, return_probs=probs)
+    B, V = x.shape
+    xs, us = x.double().cpu().numpy(), u.double().cpu().numpy()
+    rows = [np.broadcast_to(v.double().cpu().numpy() if isinstance(v, torch.Tensor) else float(v), (B,)) for v in (t, k, p, low)]
+    tokens, logs = r[0].tolist(), r[1].tolist()
+    for b in range(B):
+        tb, kb, pb, lb = (v[b] for v in rows)
+        token, log, pr, near, off = row_ref(xs[b], us[b], tb, int(kb), pb, lb)
+        assert ties or near > off, "the inputs are too near to a border to tell"
+        assert tokens[b] == token, (b, tokens[b], token)
+        if math.isnan(log):
+            assert math.isnan(logs[b])
+        else:
+            # rounded to fp32 once; the sum and the weight off as above
+            assert abs(logs[b] - log) <= 2.0 ** -24 * abs(log) + off, (b, logs[b], log)
+        if probs:
+            got = r[2][b].double().cpu().numpy()
+            if math.isnan(log):
+                assert np.isnan(got).all()
+                continue
+            # an exponential of one step (2^-23), its argument's rounding (2^-25 log 2) and a division's: below 2^-22
+            assert (np.abs(got - pr) <= (2.0 ** -22 + off) * pr + 2.0 ** -40).all(), (b, np.abs(got - pr).max())
+            assert ((got > 0) == (pr > 2.0 ** -39))[(pr > 2.0 ** -39) | (pr == 0)].all()
+    return r
+
+
+def logits(g, B, V, dtype=torch.float32, spread=2.0, peaks=True):
+    x = torch.randn((B, V), generator=g, device=DEV) * spread * (0.5 + torch.rand((B, 1), generator=g, device=DEV))
+    if peaks and V > 8:
+        at = torch.randint(0, V, (B, 8), generator=g, device=DEV)
+        x.scatter_add_(1, at, 3 + 6 * torch.rand((B, 8), generator=g, device=DEV))
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,V", [(1, 1), (3, 2), (5, 3), (4, 64), (3, 1000), (2, 4089), (2, 4095), (2, 4096), (2, 4097), (3, 16391),
+                                 (2, 50021), (1, 131072), (260, 70001)])
+@pytest.mark.parametrize("setting", [(1.0, 0, 1.0, 0.0), (0.7, 40, 1.0, 0.0), (1.2, 0, 0.9, 0.0), (0.9, 0, 1.0, 0.05),
+                                     (0.8, 100, 0.8, 0.02), (0.0, 0, 0.9, 0.0), (1.0, 1, 1.0, 0.0)])
+def test_settings(B, V, dtype, setting):
+    if B * V > 1 << 22 and (setting[1] != 0 or dtype is torch.bfloat16):
+        B = 20  # the reference's time
+    g = gen(B * 7 + V)
+    check(logits(g, B, V, dtype), torch.rand((B,), generator=g, device=DEV), *setting, ties=dtype is torch.bfloat16 or V < 4)
+
+
+@pytest.mark.parametrize("V", [37, 5000, 40000])
+def test_every_row_its_own_settings(V):
+    g, B = gen(V), 64
+    x, u = logits(g, B, V), torch.rand((B,), generator=g, device=DEV)
+    t = torch.rand((B,), generator=g, device=DEV) * 2
+    t[::9] = 0
+    k = torch.randint(-2, 2 * V, (B,), generator=g, device=DEV, dtype=torch.int32)
+    k[::3] = torch.randint(0, 30, (len(k[::3]),), generator=g, device=DEV, dtype=torch.int32)
+    p = torch.rand((B,), generator=g, device=DEV) * 1.3
+    low = torch.rand((B,), generator=g, device=DEV).pow(4) - 0.1
+    check(x, u, t, k, p, low)
+    # a setting of all rows as a vector is as the number (both exact in fp32)
+    one = torch.ones((B,), device=DEV)
+    a = S.sample(x, u, 0.75, 20, 0.5, 0.125, return_probs=True)
+    b = S.sample(x, u, 0.75 * one, (20 * one).int(), 0.5 * one, 0.125 * one, return_probs=True)
+    assert all(torch.equal(m, n) for m, n in zip(a, b))
+
+
+@pytest.mark.parametrize("V", [9, 5000, 131072])
+@pytest.mark.parametrize("setting", [(1.0, 0, 1.0, 0.0), (1.0, 0, 0.5, 0.0), (1.0, 3, 1.0, 0.0), (2.0, 0, 0.3, 0.5), (1.0, 0, 1.0, 1.0)])
+def test_equal_logits_go_by_index(V, setting):
+    """More equal logits than the list in LDS holds: what is left is the first of them, the token by index alone."""
+    x = torch.full((4, V), -3.25, device=DEV)
+    x[3, V // 2] = -1e30
+    u = torch.tensor([0.0, 0.3751, 0.99, 0.7], device=DEV)
+    t, k, p, low = setting
+    r = S.sample(x, u, t, k, p, low, return_probs=True)
+    for b in range(4):
+        n = V - (b == 3)
+        n = min(n, k) if k else n
+        n = math.ceil(p * n) if p < 1 else n
+        i = int(u[b].double().item() * n)
+        want = i + (b == 3 and i >= V // 2)
+        assert r[0][b].item() == want
+        assert abs(r[1][b].item() + math.log(n)) <= 2.0 ** -23 * max(math.log(n), 1)
+        assert (r[2][b] > 0).sum().item() == n
+
+
+@pytest.mark.parametrize("V", [300, 30000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_few_different_logits(V, dtype):
+    """Whole numbers, in whose sums many borders nearly meet: the order among equals is the index's."""
+    g = gen(V)
+    x = torch.randint(-6, 4, (6, V), generator=g, device=DEV).to(dtype)
+    u = torch.rand((6,), generator=g, device=DEV)
+    for setting in ((1.0, 0, 1.0, 0.0), (1.5, 7, 1.0, 0.0), (1.0, V // 3, 0.77, 0.0), (1.0, 0, 0.913, 0.01)):
+        check(x, u, *setting, ties=True)
+
+
+@pytest.mark.parametrize("spread", [0.0, 1e-6, 0.02, 30.0, 1e4, 1e30])
+def test_flat_and_steep_rows(spread):
+    g = gen(5)
+    x = torch.randn((3, 60000), generator=g, device=DEV) * spread
+    u = torch.rand((3,), generator=g, device=DEV)
+    for setting in ((1.0, 0, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.0, 5000, 0.99, 0.0)):
+        check(x, u, *setting, ties=spread < 1e-3)
+
+
+@pytest.mark.parametrize("t", [1e-38, 1e-30, 1e-6, 1e-3, 0.05, 50.0, 1e30, float("inf")])
+def test_temperatures(t):
+    g = gen(6)
+    x = logits(g, 4, 9000)
+    x[1, ::2] = -math.inf
+    x[2] = 0
+    x[2, 7:9] = 1e-20
+    check(x, torch.rand((4,), generator=g, device=DEV), t, 0, 0.9, ties=True)
+    check(x, torch.rand((4,), generator=g, device=DEV), t, 50, 1.0, ties=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("setting", [(1.0, 0, 1.0, 0.0), (0.8, 5, 0.9, 0.01), (0.0, 0, 1.0, 0.0)])
+def test_infinities_and_nan(dtype, setting):
+    g, V, inf = gen(7), 6001, math.inf
+    x = logits(g, 10, V, dtype)
+    x[0] = -inf  # nothing left
+    x[1, 17] = math.nan
+    x[2], x[2, 4444] = -inf, -55.0  # one left
+    x[3, 3000] = inf
+    x[4, 10], x[4, 5000] = inf, torch.finfo(torch.float32).max if dtype is torch.float32 else inf
+    x[5] = inf
+    x[6] = math.nan
+    x[7, 1:] = -inf
+    x[8, ::2], x[8, 1::2] = -inf, -1e30
+    x[9], x[9, V - 1] = -inf, 3.0
+    check(x, torch.rand((10,), generator=g, device=DEV), *setting, ties=True)
+
+
+def test_settings_out_of_range():
+    g, V, nan = gen(8), 700, math.nan
+    x = logits(g, 6, V)
+    u = torch.tensor([0.2, 0.4, 0.6, -1.0, 1.0, nan], device=DEV)
+    t = torch.tensor([-1.0, nan, 1.0, 1.0, 1.0, 1.0], device=DEV)
+    p = torch.tensor([0.5, 0.5, nan, -2.0, 7.0, 0.9], device=DEV)
+    low = torch.tensor([0.0, 0.0, nan, -1.0, 0.0, 9.0], device=DEV)
+    k = torch.tensor([0, 0, -(2 ** 31), 2 ** 31 - 1, 0, 0], dtype=torch.int32, device=DEV)
+    check(x, u, t, k, p, low)
+
+
+def test_numbers_over_the_whole_range_give_the_distribution():
+    """One row of logits for 4096 numbers: every kept token as often as its probability says, in order."""
+    g, n = gen(9), 4096
+    x = logits(g, 1, 3000).expand(n, 3000)
+    u = (torch.arange(n, device=DEV) + 0.5) / n
+    r = S.sample(x, u, 0.9, 60, 0.97, return_probs=True)
+    pr = r[2][0].double()
+    count = torch.bincount(r[0], minlength=3000)
+    assert ((count / n - pr).abs() <= 1.0 / n).all() and (r[2] == r[2][:1]).all()
+    at = x[0][r[0]]
+    assert (at[1:] <= at[:-1]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_views(dtype):
+    g = gen(10)
+    wide = logits(g, 5, 5013, dtype)
+    u = torch.rand((10,), generator=g, device=DEV)[::2]
+    for x in (wide[:, 1:], wide[:, 3:5000], wide[1:, 7:8], wide[:, ::2], wide.t().contiguous().t(), wide[2:3, 5:], wide[:, :4096]):
+        n = x.shape[0]
+        assert all(torch.equal(a, b) for a, b in zip(S.sample(x, u[:n], 0.9, 30, 0.9, return_probs=True),
+                                                     S.sample(x.clone(), u[:n].clone(), 0.9, 30, 0.9, return_probs=True)))
+        check(x, u[:n], 0.9, 30, 0.9, ties=True)
+
+
+def test_the_same_on_every_run():
+    g = gen(11)
+    x, u = logits(g, 32, 65536, peaks=False), torch.rand((32,), generator=g, device=DEV)
+    first = S.sample(x, u, 1.0, 0, 0.95, return_probs=True)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, S.sample(x, u, 1.0, 0, 0.95, return_probs=True)))
+
+
+def test_nothing_to_do():
+    r = S.sample(torch.zeros((0, 5), device=DEV), torch.zeros((0,), device=DEV), return_probs=True)
+    assert [tuple(t.shape) for t in r] == [(0,), (0,), (0, 5)]
+
+
+def test_two_captured_steps_and_an_eager_one():
+    """Two graphs of other settings replayed in turn on new logits, with an eager call on another stream between them."""
+    g, B, V = gen(12), 6, 20000
+    x, u = logits(g, B, V), torch.rand((B,), generator=g, device=DEV)
+    k = torch.full((B,), 50, dtype=torch.int32, device=DEV)
+    calls = [lambda: S.sample(x, u, 0.8, k, 0.9, return_probs=True), lambda: S.sample(x, u, 1.1, 0, 0.95)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for f in calls:
+            f()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for f in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(f())
+    for step in range(4):
+        x.copy_(logits(g, B, V))
+        u.copy_(torch.rand((B,), generator=g, device=DEV))
+        k.fill_(5 + 20 * step)
+        side.wait_stream(torch.cuda.current_stream())
+        for h in graphs:
+            h.replay()
+        with torch.cuda.stream(side):
+            eager = calls[1]()
+        torch.cuda.synchronize()
+        for f, o in zip(calls, outs):
+            assert all(torch.equal(a, b) for a, b in zip(f(), o))
+        assert all(torch.equal(a, b) for a, b in zip(eager, outs[1]))
+        check(x, u, 0.8, k, 0.9)
