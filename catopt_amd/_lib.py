@@ -128,6 +128,12 @@ SIGNATURES: dict[str, tuple] = {
         _i32,
         [_i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _i64, _p],
     ),
+    "catopt_hip_paged_prefix_attn_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "catopt_hip_paged_prefix_attn_fwd": (
+        _i32,
+        [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _p,
+         _p, _f32, _i32, _i32, _p, _p, _p, _p, _p, _i64, _p],
+    ),
     "catopt_hip_sample_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32]),
     "catopt_hip_sample": (
         _i32,

@@ -26,6 +26,10 @@ struct PagedArgs {
   int B, Hq, Hkv, G, d, cap, normalize, causal;
   int splits, min_keys;  // key ranges per tile at most, keys of one at least
   float scale;
+  // Of the calls that combine carriers of two sets of keys (CARRIERS), a set's part:
+  const int32_t* groups;  // the set's sequences are groups of the call's (NULL: they are those), their first ones
+  int n_seq;              // the call's sequences
+  int part_ld, part_first;  // of a row's carriers: all, and the set's first
 };
 
 // Query rows of one key head are its G query heads of every token, a token's
@@ -43,9 +47,18 @@ struct PagedTile {
   bool split;                      // it has several
 };
 
+// The rows of sequence b, or of group b of them.
+template <bool CARRIERS>
+__device__ __forceinline__ void set_rows(const PagedArgs& a, int b, int& row0, int& nq) {
+  if (!CARRIERS || !a.groups) return seq_rows(a.starts, b, a.N, row0, nq);
+  const int n = (int)a.N;
+  row0 = min(max(a.starts[min(max(a.groups[b], 0), a.n_seq)], 0), n);
+  nq = max(min(max(a.starts[min(max(a.groups[b + 1], 0), a.n_seq)], 0), n) - row0, 0);
+}
+
 // Lane i looks at sequence i (of 64 at a time), so that the search and the
 // sequence's own numbers are one memory latency.
-template <int R>
+template <int R, bool CARRIERS>
 __device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, int t) {
   const int lane = threadIdx.x & 63;
   PagedTile x{};
@@ -56,7 +69,7 @@ __device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, int t) {
     int row0 = 0, nq = 0, len = 0;
     bool le = false;
     if (i < a.B) {
-      seq_rows(a.starts, i, a.N, row0, nq);
+      set_rows<CARRIERS>(a, i, row0, nq);
       len = min(max(a.lens[i], 0), a.cap);
       le = (int64_t)row0 * a.G / R + i <= t;
     }
@@ -94,11 +107,22 @@ __device__ __forceinline__ int count_ranges(const PagedTile& x) { return __popcl
 
 // A workgroup's key head, its tile and key range: the heads next to each other,
 // then the ranges.
-__device__ __forceinline__ void decode_block(const PagedArgs& a, int& h, int& tile, int& range) {
-  const uint32_t ts = a.k_heads.div(blockIdx.x);
-  h = (int)(blockIdx.x - ts * a.k_heads.d);
+__device__ __forceinline__ void decode_block(const PagedArgs& a, uint32_t block, int& h, int& tile, int& range) {
+  const uint32_t ts = a.k_heads.div(block);
+  h = (int)(block - ts * a.k_heads.d);
   tile = (int)a.ranges.div(ts);
   range = (int)(ts - (uint32_t)tile * a.ranges.d);
+}
+
+// Where range `split` of row i has its carrier, counted in carriers; and where
+// their numerators begin.
+template <bool CARRIERS>
+__device__ __forceinline__ int64_t part_at(const PagedArgs& a, int64_t i, int split) {
+  return CARRIERS ? i * a.part_ld + a.part_first + split : i * a.splits + split;
+}
+template <bool CARRIERS>
+__device__ __forceinline__ float* part_numerators(const PagedArgs& a) {
+  return a.part + ((2 * a.N * a.Hq * (CARRIERS ? a.part_ld : a.splits) + 3) & ~(int64_t)3);
 }
 
 // exp2((from - to) c), 0 for an empty `from`.

@@ -1,0 +1,273 @@
+// Paged attention of sequences that share the keys before their own: the first
+// part's K and V are read for all of a group's rows together, not once for each
+// sequence.
+//
+// The keys are two sets, each attended as paged attention has it (32-row or
+// 128-row tiles, key ranges): the prefixes', whose "sequences" are the groups with
+// the rows of all their members and no mask, and the sequences' own.  One launch
+// takes the tiles of both: the prefix' are bound by MFMA, a step's own keys by HBM
+// and latency, so they share the CUs.  Each tile and range leaves a carrier (m, l,
+// numerator); a second launch combines a row's.
+#include "paged_attn_few.hpp"
+#include "paged_attn_tile.hpp"
+
+namespace catopt {
+namespace {
+
+constexpr int NT = kTileThreads;
+
+// The few-row form of four waves, as many as the 128-row kernel has.
+template <int D>
+using FewFour = FewShape<D, 4, D == 128 ? 1 : 2>;
+
+template <int D, bool FEW>
+constexpr int lds_of() {
+  return FEW ? FewFour<D>::BYTES : TileLds<D>::BYTES;
+}
+
+template <int D, bool FEW>
+__device__ __forceinline__ void attend(const PagedArgs& a, uint32_t block, int tiles) {
+  if constexpr (FEW)
+    paged_few<D, FewFour<D>, true>(a, block);
+  else
+    paged_tile_rows<D, true>(a, block, tiles);
+}
+
+// p: the prefixes, o: the sequences' own keys.
+template <int D, bool PFEW, bool OFEW>
+__global__ __launch_bounds__(NT, 2) void paged_prefix_kernel(PagedArgs p, PagedArgs o, uint32_t p_blocks, int p_tiles,
+                                                              int o_tiles) {
+  if (blockIdx.x < p_blocks)
+    attend<D, PFEW>(p, blockIdx.x, p_tiles);
+  else
+    attend<D, OFEW>(o, blockIdx.x - p_blocks, o_tiles);
+}
+
+// The last of n ascending starts that is not above x; -1 where none is.
+__device__ __forceinline__ int last_start(const int32_t* starts, int n, int most, int x) {
+  const int lane = threadIdx.x & 63;
+  int at = -1;
+  for (int c = 0; c < n; c += 64) {
+    const int i = c + lane;
+    const int k = __popcll(__ballot(i < n && min(max(starts[min(i, n - 1)], 0), most) <= x));
+    at += k;
+    if (k < 64) break;
+  }
+  return at;
+}
+
+// WAVES waves a row, D / 4 lanes to a carrier's numerators.
+template <int D, int WAVES>
+__global__ __launch_bounds__(NT) void paged_prefix_combine(PagedArgs p, PagedArgs o, int p_rows, int o_rows) {
+  constexpr int TPR = D / 4, GROUPS = 64 * WAVES / TPR;
+  const int lane = threadIdx.x & 63, tid = WAVES == 4 ? threadIdx.x : lane;
+  const int row = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + (int)(threadIdx.x >> 6);  // N Hq < 2^30
+  if (row >= o.N * o.Hq) return;
+  const int n = (int)o.q_heads.div(row), hq = row - n * o.Hq;
+  const int b = last_start(o.starts, o.B, (int)o.N, n);
+  if (b < 0) return;
+  // the ranges of the row's tiles: the own keys' behind the prefix'
+  uint64_t ranges = 0;
+  auto add = [&](const PagedArgs& a, int i, int tile_rows) {
+    PagedTile x{};
+    x.b = i;
+    set_rows<true>(a, i, x.row0, x.nq);
+    if (n < x.row0 || n >= x.row0 + x.nq) return false;
+    x.len = min(max(a.lens[i], 0), a.cap);
+    x.r0 = ((n - x.row0) * a.G + hq - (int)a.group.div(hq) * a.G) / tile_rows * tile_rows;
+    x.rows = min(tile_rows, x.nq * a.G - x.r0);
+    paged_ranges(a, x);
+    ranges |= __ballot(lane < a.splits && has_range(x, lane)) << a.part_first;
+    return true;
+  };
+  if (!add(o, b, o_rows)) return;
+  const int group = p.B > 0 ? last_start(p.groups, p.B, p.n_seq, b) : -1;
+  if (group >= 0) add(p, group, p_rows);
+  const int slots = o.part_ld;
+  const float c = o.scale * kLog2e;
+  const float* ml = o.part + (int64_t)2 * row * slots;
+  const float* num = part_numerators<true>(o) + (int64_t)row * slots * D + 4 * (tid % TPR);
+  const bool mine = (ranges >> lane) & 1;
+  const float ms = mine ? ml[2 * lane] : kNegInf, ls = mine ? ml[2 * lane + 1] : 0.f;
+  float mx = ms;
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s, 64));
+  const float f = mine ? move_factor(ms, mx, c) : 0.f;
+  float lt = mine ? ls * f : 0.f;
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) lt += __shfl_xor(lt, s, 64);
+  f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 8;  // loads ahead of their additions
+  for (int s0 = 0; s0 < slots; s0 += U * GROUPS) {  // every lane stays: the factors come from lanes
+    f32x4 ys[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int s = s0 + i * GROUPS + tid / TPR;
+      ys[i] = s < slots && (ranges >> s) & 1 ? *reinterpret_cast<const f32x4*>(num + (int64_t)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) y += ys[i] * __shfl(f, min(s0 + i * GROUPS + tid / TPR, 63), 64);
+  }
+  if constexpr (WAVES == 4) {
+    __shared__ f32x4 sums[GROUPS][TPR];
+    sums[tid / TPR][tid % TPR] = y;
+    __syncthreads();
+    if (tid < TPR) {
+#pragma unroll
+      for (int i = 1; i < GROUPS; ++i) y += sums[i][tid];
+    }
+  } else {
+#pragma unroll
+    for (int s = TPR; s < 64; s <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], s, 64);
+  }
+  if (tid < TPR && 4 * tid < o.d) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = finish(y[e], lt, o.normalize);
+    *reinterpret_cast<u32x2*>(o.o + (int64_t)n * o.o_t + (int64_t)hq * o.o_h + 4 * tid) =
+        u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+  }
+  if (tid == 0) row_stats(o, row, mx, lt);
+}
+
+// ------------------------------------------------------------------ host
+
+// One set's kernel and key ranges.
+struct Set {
+  bool few;
+  int splits, min_keys;
+  int64_t tiles, blocks;
+};
+
+Set set_of(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t cap, bool few) {
+  Set s{};
+  s.few = few;
+  s.splits = 0, s.min_keys = 128;
+  if (B == 0 || cap == 0) return s;
+  s.tiles = paged_tiles(N, G, B, few ? kFewRows : kTileRows);
+  const int64_t groups = s.tiles * Hkv;
+  int64_t n = (512 + groups - 1) / groups;
+  const int64_t most = (cap + 255) / 256;
+  if (n > most) n = most;
+  if (n > kMaxSplits / 2) n = kMaxSplits / 2;
+  s.splits = n < 1 ? 1 : (int)n;
+  s.blocks = groups * s.splits;
+  return s;
+}
+
+struct Plan {
+  Set p, o;
+  int64_t carriers;
+  int64_t bytes(int64_t rows, int64_t D) const { return 4 * (((2 * rows * carriers + 3) & ~(int64_t)3) + rows * carriers * D); }
+};
+
+Plan plan_of(int64_t P, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t p_cap, int64_t cap) {
+  Plan x;
+  const int64_t G = Hq / Hkv;
+  const bool o_few = N * G <= kFewRows * B, p_few = o_few && N * G <= kFewRows * P;
+  x.p = set_of(P, N, G, Hkv, p_cap, p_few);
+  x.o = set_of(B, N, G, Hkv, cap < 1 ? 1 : cap, o_few);  // without own keys its empty carriers
+  x.carriers = x.p.splits + x.o.splits;
+  return x;
+}
+
+template <int D, bool PFEW, bool OFEW>
+int32_t launch(const PagedArgs& p, const PagedArgs& o, const Plan& x, hipStream_t s) {
+  static bool done[kDevices] = {};
+  constexpr int a = lds_of<D, PFEW>(), b = lds_of<D, OFEW>(), bytes = a > b ? a : b;
+  const auto kernel = &paged_prefix_kernel<D, PFEW, OFEW>;
+  const int32_t r = allow_lds(reinterpret_cast<const void*>(kernel), bytes, done);
+  if (r != CATOPT_OK) return r;
+  const int64_t blocks = x.p.blocks + x.o.blocks, rows = o.N * o.Hq;
+  const bool wide = rows < 2048;  // four waves a row where the rows alone do not fill the CUs
+  const int64_t nc = wide ? rows : (rows + 3) / 4;
+  if (!grid_fits(blocks, NT) || !grid_fits(nc, NT)) return CATOPT_E_UNSUPPORTED;
+  kernel<<<dim3((uint32_t)blocks), dim3(NT), bytes, s>>>(p, o, (uint32_t)x.p.blocks, (int)x.p.tiles, (int)x.o.tiles);
+  CATOPT_LAUNCH_CHECK();
+  const int p_rows = PFEW ? kFewRows : kTileRows, o_rows = OFEW ? kFewRows : kTileRows;
+  if (wide)
+    paged_prefix_combine<D, 4><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
+  else
+    paged_prefix_combine<D, 1><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
+  CATOPT_LAUNCH_CHECK();
+  return CATOPT_OK;
+}
+
+template <int D>
+int32_t launch_form(const PagedArgs& p, const PagedArgs& o, const Plan& x, hipStream_t s) {
+  if (x.p.few) return launch<D, true, true>(p, o, x, s);
+  return x.o.few ? launch<D, false, true>(p, o, x, s) : launch<D, false, false>(p, o, x, s);
+}
+
+}  // namespace
+}  // namespace catopt
+
+using namespace catopt;
+
+extern "C" int64_t catopt_hip_paged_prefix_attn_workspace_bytes(int64_t P, int64_t B, int64_t N, int64_t Hq, int64_t Hkv,
+                                                                int64_t d, int64_t n_prefix_table, int64_t n_table,
+                                                                int64_t page_size) {
+  const int64_t lim = 1LL << 30;
+  if (P < 0 || B < 0 || N < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || d < 8 || d > 128 || d % 8) return -1;
+  if (n_prefix_table < 0 || n_table < 0 || page_size < 8 || page_size % 8) return -1;
+  if (P > (1 << 20) || B > (1 << 20) || N >= lim || Hq > 65535 || N * Hq >= lim || B * Hkv >= lim || P * Hkv >= lim) return -1;
+  if (n_table > lim || n_prefix_table > lim || page_size > lim || n_table * page_size >= lim || n_prefix_table * page_size >= lim)
+    return -1;
+  if (B == 0 || N == 0) return 0;
+  return plan_of(P, B, N, Hq, Hkv, n_prefix_table * page_size, n_table * page_size).bytes(N * Hq, d <= 64 ? 64 : 128);
+}
+
+extern "C" int32_t catopt_hip_paged_prefix_attn_fwd(
+    int32_t dtype, int64_t P, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, const void* q, const void* k_pages,
+    const void* v_pages, int64_t n_pages, int64_t page_size, const int32_t* prefix_table, int64_t prefix_ld,
+    int64_t n_prefix_table, const int32_t* prefix_lens, const int32_t* prefix_starts, const int32_t* block_table,
+    int64_t table_ld, int64_t n_table, const int32_t* kv_lens, const int32_t* q_starts, float scale, int32_t causal,
+    int32_t normalize, void* o, float* m_out, float* l_out, const int64_t* strides, void* workspace,
+    int64_t workspace_bytes, void* stream) {
+  if (P < 0 || B < 0 || N < 0 || Hq < 1 || Hkv < 1 || Hq % Hkv || n_pages < 0 || n_table < 0 || n_prefix_table < 0 ||
+      page_size < 1 || table_ld < 0 || prefix_ld < 0)
+    return CATOPT_E_INVAL;
+  if (normalize < 1 || normalize > 2) return CATOPT_E_INVAL;
+  if (dtype != CATOPT_BF16 || d < 8 || d > 128 || d % 8 || page_size % 8) return CATOPT_E_UNSUPPORTED;
+  if (!(scale > 0.f) || !__builtin_isfinite(scale * kLog2e)) return CATOPT_E_UNSUPPORTED;
+  const int64_t need = catopt_hip_paged_prefix_attn_workspace_bytes(P, B, N, Hq, Hkv, d, n_prefix_table, n_table, page_size);
+  if (need < 0) return CATOPT_E_UNSUPPORTED;
+  if (B == 0 || N == 0) return CATOPT_OK;
+  if (!q || !o || !kv_lens || !q_starts || !strides || (n_table > 0 && !block_table)) return CATOPT_E_INVAL;
+  if (P > 0 && (!prefix_lens || !prefix_starts || (n_prefix_table > 0 && !prefix_table))) return CATOPT_E_INVAL;
+  if (n_pages > 0 && (!k_pages || !v_pages)) return CATOPT_E_INVAL;
+  const Strides rows(strides, {N, Hq, n_pages, Hkv, page_size, n_pages, Hkv, page_size, N, Hq}, 8);
+  if (!rows.fit) return CATOPT_E_INVAL;
+  const int64_t* s = rows.s;
+  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o)) return CATOPT_E_INVAL;
+  const Layout out = layout3(o, 2, N, s[8], Hq, s[9], d);
+  if (out.folded() || out.overlaps(layout3(q, 2, N, s[0], Hq, s[1], d)) ||
+      out.overlaps(layout_pages(k_pages, 2, n_pages, Hkv, page_size, d, s + 2)) ||
+      out.overlaps(layout_pages(v_pages, 2, n_pages, Hkv, page_size, d, s + 5)))
+    return CATOPT_E_INVAL;
+  // the rows of one load lie within 31 bits of its resource's base
+  if (s[4] > (1 << 26) || s[7] > (1 << 26)) return CATOPT_E_UNSUPPORTED;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need) return CATOPT_E_WORKSPACE;
+  const Plan x = plan_of(P, B, N, Hq, Hkv, n_prefix_table * page_size, n_table * page_size);
+  PagedArgs a{};
+  a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k_pages);
+  a.v = static_cast<const uint16_t*>(v_pages), a.o = static_cast<uint16_t*>(o);
+  a.q_t = s[0], a.q_h = s[1], a.k_p = s[2], a.k_h = s[3], a.k_s = s[4], a.v_p = s[5], a.v_h = s[6], a.v_s = s[7];
+  a.o_t = s[8], a.o_h = s[9];
+  a.starts = q_starts, a.n_pages = n_pages, a.N = N, a.m_out = m_out, a.l_out = l_out;
+  a.page = FastDiv::of(page_size), a.group = FastDiv::of(Hq / Hkv);
+  a.q_heads = FastDiv::of(Hq), a.k_heads = FastDiv::of(Hkv);
+  a.Hq = (int)Hq, a.Hkv = (int)Hkv, a.G = (int)(Hq / Hkv), a.d = (int)d, a.normalize = normalize, a.scale = scale;
+  a.part = static_cast<float*>(workspace), a.part_ld = (int)x.carriers, a.n_seq = (int)B;
+  PagedArgs p = a, own = a;
+  auto set = [](PagedArgs& y, const Set& z, int64_t n, const int32_t* table, int64_t ld, int64_t reach, const int32_t* lens) {
+    y.B = z.splits ? (int)n : 0, y.table = table, y.table_ld = ld, y.cap = (int)reach, y.lens = lens;
+    y.splits = z.splits, y.min_keys = z.min_keys, y.ranges = FastDiv::of(z.splits < 1 ? 1 : z.splits);
+  };
+  set(p, x.p, P, prefix_table, prefix_ld, n_prefix_table * page_size, prefix_lens);
+  set(own, x.o, B, block_table, table_ld, n_table * page_size, kv_lens);
+  p.groups = prefix_starts, own.causal = causal != 0, own.part_first = x.p.splits;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return d <= 64 ? launch_form<64>(p, own, x, st) : launch_form<128>(p, own, x, st);
+}

@@ -18,7 +18,9 @@ pages of finished requests back.  A layer's step over new tokens:
   instead);
 * :func:`paged_attention` attends from each sequence's new tokens to its
   cached keys, a prompt, a chunk of one or a single token alike, and can add
-  up every key's attention weight;
+  up every key's attention weight; :func:`paged_prefix_attention` does where
+  sequences share the keys before their own (an instruction, a document), which
+  are in the cache and read once for all of them;
 * :func:`paged_evict` moves each head's most attended and most recent keys
   into a smaller cache.
 
@@ -46,13 +48,13 @@ from . import _lib as L
 from .kernels import _DT, _need_device, _stream_of
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_append", "paged_attention", "paged_evict", "paged_extend", "paged_release",
-           "PagedStep", "PAGED_ATTENTION_MAX_HEAD_DIM", "QK_NORM_ROPE_MAX_HEAD_DIM"]
+           "paged_prefix_attention", "PagedStep", "PAGED_ATTENTION_MAX_HEAD_DIM", "QK_NORM_ROPE_MAX_HEAD_DIM"]
 
 PAGED_ATTENTION_MAX_HEAD_DIM = 128
 QK_NORM_ROPE_MAX_HEAD_DIM = 256
 
 # host arrays of strides, as the C entries take them
-_S12, _S14, _S16 = (struct.Struct(f"{n}q").pack for n in (12, 14, 16))
+_S10, _S12, _S14, _S16 = (struct.Struct(f"{n}q").pack for n in (10, 12, 14, 16))
 
 
 _get_device = torch.Tensor.get_device
@@ -243,6 +245,42 @@ def _weight_rows(name: str, w: torch.Tensor, B: int, H: int, width: int) -> tupl
     return s[0], s[1]
 
 
+def _attention_operands(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, scale: float) -> tuple:
+    """What attention takes of its queries and cache: q with its shape, strides and address, the pages' and the scale."""
+    if q.dtype is not torch.bfloat16 or k_pages.dtype is not torch.bfloat16:
+        raise NotImplementedError(f"paged attention runs on bf16 operands, got {q.dtype} and {k_pages.dtype} pages")
+    q, qshape, (q0, q1, _), q_at = _heads("q", q, 8)
+    if q_at % 16:
+        q = q.clone()
+        q_at = q.data_ptr()
+    N, Hq, d = qshape
+    (n_pages, Hkv, page, pd), (k0, k1, k2, _), (v0, v1, v2, _) = _pages(k_pages, v_pages)
+    if pd != d or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"q has {Hq} heads of {d}, the pages {Hkv} heads of {pd}: the head dims agree and the query "
+                         "heads are a multiple of the key heads")
+    if d % 8 or not 8 <= d <= PAGED_ATTENTION_MAX_HEAD_DIM:
+        raise NotImplementedError(f"paged attention takes head dims that are multiples of 8 up to "
+                                  f"{PAGED_ATTENTION_MAX_HEAD_DIM}, got {d}")
+    if page < 1 or page % 8:
+        raise NotImplementedError(f"paged attention takes page sizes that are multiples of 8, got {page}")
+    scale = float(scale)
+    if not 0 < scale < 1e38:
+        raise ValueError(f"the scale is a positive number below 1e38, got {scale}")
+    return q, qshape, (q0, q1), q_at, (n_pages, Hkv, page), (k0, k1, k2), (v0, v1, v2), scale
+
+
+def _attention_out(q: torch.Tensor, out: torch.Tensor | None) -> tuple[torch.Tensor, int, int]:
+    """The result's tensor and strides."""
+    if out is None:
+        out = q.new_empty(q.shape)
+    elif out.shape != q.shape or out.dtype is not torch.bfloat16:
+        raise ValueError(f"out has q's shape and type, got {tuple(out.shape)} {out.dtype}")
+    o0, o1, o2 = out.stride()
+    if o2 != 1:
+        raise ValueError(f"out needs a contiguous head dim, got strides {out.stride()}")
+    return out, o0, o1
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                     kv_lens: torch.Tensor, q_starts: torch.Tensor, scale: float, *, causal: bool = True,
                     weights: torch.Tensor | None = None, weights_out: torch.Tensor | None = None,
@@ -288,36 +326,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     elif weights is not None:
         raise ValueError("weights need a weights_out to go to")
     dev = _device(ts)
-    if q.dtype is not torch.bfloat16 or k_pages.dtype is not torch.bfloat16:
-        raise NotImplementedError(f"paged attention runs on bf16 operands, got {q.dtype} and {k_pages.dtype} pages")
-    q, qshape, (q0, q1, _), q_at = _heads("q", q, 8)
-    if q_at % 16:
-        q = q.clone()
-        q_at = q.data_ptr()
-    N, Hq, d = qshape
-    (n_pages, Hkv, page, pd), (k0, k1, k2, _), (v0, v1, v2, _) = _pages(k_pages, v_pages)
-    if pd != d or Hkv < 1 or Hq < 1 or Hq % Hkv:
-        raise ValueError(f"q has {Hq} heads of {d}, the pages {Hkv} heads of {pd}: the head dims agree and the query "
-                         "heads are a multiple of the key heads")
-    if d % 8 or not 8 <= d <= PAGED_ATTENTION_MAX_HEAD_DIM:
-        raise NotImplementedError(f"paged attention takes head dims that are multiples of 8 up to "
-                                  f"{PAGED_ATTENTION_MAX_HEAD_DIM}, got {d}")
-    if page < 1 or page % 8:
-        raise NotImplementedError(f"paged attention takes page sizes that are multiples of 8, got {page}")
-    scale = float(scale)
-    if not 0 < scale < 1e38:
-        raise ValueError(f"the scale is a positive number below 1e38, got {scale}")
+    q, (N, Hq, d), (q0, q1), q_at, (n_pages, Hkv, page), (k0, k1, k2), (v0, v1, v2), scale = _attention_operands(
+        q, k_pages, v_pages, scale)
     B = q_starts.numel() - 1
     kv_lens = _vector("kv_lens", kv_lens, torch.int32, B)
     q_starts = _vector("q_starts", q_starts, torch.int32, B + 1)
     table, n_table, table_ld = _table("block_table", block_table, B)
-    if out is None:
-        out = q.new_empty(qshape)
-    elif out.shape != qshape or out.dtype is not torch.bfloat16:
-        raise ValueError(f"out has q's shape and type, got {tuple(out.shape)} {out.dtype}")
-    o0, o1, o2 = out.stride()
-    if o2 != 1:
-        raise ValueError(f"out needs a contiguous head dim, got strides {out.stride()}")
+    out, o0, o1 = _attention_out(q, out)
     wi0 = wi1 = wo0 = wo1 = 0
     wi = wo = m = l = mp = lp = ws_at = None
     if weights_out is not None:
@@ -340,6 +355,63 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                      mp, lp, wi, wo, _S14(q0, q1, k0, k1, k2, v0, v1, v2, o0, o1, wi0, wi1, wo0, wo1), ws_at, wsb)
         if st:
             _check("paged_attention", st)
+    return (out, m, l) if return_ml else out
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_workspace(P: int, B: int, N: int, Hq: int, Hkv: int, d: int, n_prefix: int, n_table: int, page: int) -> int:
+    n = L.load().catopt_hip_paged_prefix_attn_workspace_bytes(P, B, N, Hq, Hkv, d, n_prefix, n_table, page)
+    if n < 0:
+        raise NotImplementedError("paged prefix attention: the call is beyond what one launch takes")
+    return n
+
+
+def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, prefix_table: torch.Tensor,
+                           prefix_lens: torch.Tensor, prefix_starts: torch.Tensor, block_table: torch.Tensor,
+                           kv_lens: torch.Tensor, q_starts: torch.Tensor, scale: float, *, causal: bool = True,
+                           return_ml: bool = False, empty_rows: str = "nan", out: torch.Tensor | None = None):
+    """:func:`paged_attention` of sequences that share the keys before their
+    own (bf16).
+
+    Group ``p`` of ``P`` is the sequences ``prefix_starts[p]`` to
+    ``prefix_starts[p + 1]`` (int32, ``P + 1`` ascending values).  Their tokens
+    see the first ``prefix_lens[p]`` (int32) keys of the pages
+    ``prefix_table[p]`` (int32 ``(P, n')``), all of them, and then their own
+    sequence's keys, of which ``kv_lens``, ``block_table`` and ``causal`` speak
+    as they do there.  A prefix may end inside a page; a sequence's own keys begin
+    a page of their own.  A sequence outside the groups has no prefix.
+
+    The prefix of a group is read once for all its rows, up to 128 query rows of
+    a key head together: worth it for prefixes of some hundred keys and groups of
+    several sequences.  Results and the remaining arguments are as in
+    :func:`paged_attention`, ``(m, l)`` over both sets of keys."""
+    if empty_rows not in ("nan", "zero"):
+        raise ValueError(f"empty_rows is 'nan' or 'zero', got {empty_rows!r}")
+    ts = (q, k_pages, v_pages, prefix_table, prefix_lens, prefix_starts, block_table, kv_lens, q_starts)
+    dev = _device(ts if out is None else ts + (out,))
+    q, (N, Hq, d), (q0, q1), q_at, (n_pages, Hkv, page), ks, vs, scale = _attention_operands(q, k_pages, v_pages, scale)
+    B, P = q_starts.numel() - 1, prefix_starts.numel() - 1
+    kv_lens = _vector("kv_lens", kv_lens, torch.int32, B)
+    q_starts = _vector("q_starts", q_starts, torch.int32, B + 1)
+    table, n_table, table_ld = _table("block_table", block_table, B)
+    prefix_lens = _vector("prefix_lens", prefix_lens, torch.int32, P)
+    prefix_starts = _vector("prefix_starts", prefix_starts, torch.int32, P + 1)
+    p_table, n_prefix, p_ld = _table("prefix_table", prefix_table, P)
+    out, o0, o1 = _attention_out(q, out)
+    m = l = mp = lp = ws_at = None
+    if return_ml:
+        m, l = q.new_empty((N, Hq), dtype=torch.float32), q.new_empty((N, Hq), dtype=torch.float32)
+        mp, lp = m.data_ptr(), l.data_ptr()
+    if B and N:
+        wsb = _prefix_workspace(P, B, N, Hq, Hkv, d, n_prefix, n_table, page)
+        ws = q.new_empty(wsb // 2)
+        st = _launch(dev, L.load().catopt_hip_paged_prefix_attn_fwd, L.BF16, P, B, N, Hq, Hkv, d, q_at, k_pages.data_ptr(),
+                     v_pages.data_ptr(), n_pages, page, p_table.data_ptr(), p_ld, n_prefix, prefix_lens.data_ptr(),
+                     prefix_starts.data_ptr(), table.data_ptr(), table_ld, n_table, kv_lens.data_ptr(), q_starts.data_ptr(),
+                     scale, 1 if causal else 0, 2 if empty_rows == "zero" else 1, out.data_ptr(), mp, lp,
+                     _S10(q0, q1, *ks, *vs, o0, o1), ws.data_ptr(), wsb)
+        if st:
+            _check("paged_prefix_attention", st)
     return (out, m, l) if return_ml else out
 
 

@@ -724,6 +724,35 @@ int32_t catopt_hip_paged_release(
     int64_t workspace_bytes, void* stream);
 
 /*
+ * catopt_hip_paged_attn_fwd (without weights) for sequences that share the keys
+ * before their own.  Group p is the sequences prefix_starts[p] ..
+ * prefix_starts[p + 1] (int32 [P + 1], ascending); each of their tokens sees the
+ * prefix_lens[p] (int32 [P]) keys of the pages prefix_table[p, :] (int32 [P,
+ * n_prefix_table], rows prefix_ld apart) and then, as there, the sequence's own
+ * keys: kv_lens and block_table count and name those alone.  A sequence outside
+ * the groups has no prefix.  What the prefixes hold is read once for each 128 (or
+ * 32) rows of a group, not once for each sequence.
+ * strides (host, 10 values): q (token, head); k_pages, v_pages (page, head,
+ * slot); o (token, head).
+ * Workspace: catopt_hip_paged_prefix_attn_workspace_bytes(...) bytes, 16-byte
+ * aligned, any contents (-1: invalid arguments); a row's carriers, one for each
+ * range of its keys.
+ */
+int64_t catopt_hip_paged_prefix_attn_workspace_bytes(
+    int64_t P, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d,
+    int64_t n_prefix_table, int64_t n_table, int64_t page_size);
+int32_t catopt_hip_paged_prefix_attn_fwd(
+    int32_t dtype, int64_t P, int64_t B, int64_t N, int64_t Hq, int64_t Hkv,
+    int64_t d, const void* q, const void* k_pages, const void* v_pages,
+    int64_t n_pages, int64_t page_size, const int32_t* prefix_table,
+    int64_t prefix_ld, int64_t n_prefix_table, const int32_t* prefix_lens,
+    const int32_t* prefix_starts, const int32_t* block_table, int64_t table_ld,
+    int64_t n_table, const int32_t* kv_lens, const int32_t* q_starts,
+    float scale, int32_t causal, int32_t normalize, void* o, float* m_out,
+    float* l_out, const int64_t* strides, void* workspace,
+    int64_t workspace_bytes, void* stream);
+
+/*
  * The next token of each of B rows of V logits (F32 or BF16, rows ld apart) by
  * temperature T, top-k, top-p, min-p and a number u in [0, 1).  With w =
  * exp((x - max x) / T) and the order that takes the largest logit first, the

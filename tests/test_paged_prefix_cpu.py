@@ -1,0 +1,90 @@
+"""What attention over shared prefixes refuses on the host, before any launch (the addresses are never read)."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+import torch
+
+from catopt_amd import _lib as L
+from catopt_amd import paged as P
+
+A = [1 << 20 | i << 32 for i in range(16)]  # far apart
+Q, KP, VP, OUT = A[:4]
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not L.LIB_PATH.exists():
+        from catopt_amd import build
+
+        build.build()
+    return L.load()
+
+
+OK = [256, 64, 2048, 1024, 64, 2048, 1024, 64, 256, 64]
+
+
+def _call(lib, dtype=L.BF16, groups=1, B=2, N=4, Hq=4, Hkv=2, d=64, q=Q, k=KP, v=VP, n_pages=8, page=16, p_table=A[4], p_ld=4,
+          n_p=4, p_lens=A[5], p_starts=A[6], table=A[7], ld=4, n_table=4, lens=A[8], starts=A[9], scale=1.0, causal=1, norm=1,
+          o=OUT, strides=None, ws=A[10], wsb=1 << 40):
+    st = (C.c_int64 * 10)(*(strides or OK))
+    return lib.catopt_hip_paged_prefix_attn_fwd(dtype, groups, B, N, Hq, Hkv, d, q, k, v, n_pages, page, p_table, p_ld, n_p, p_lens,
+                                                p_starts, table, ld, n_table, lens, starts, scale, causal, norm, o, None, None,
+                                                st, ws, wsb, None)
+
+
+def test_refusals(lib):
+    assert _call(lib, B=0) == L.OK and _call(lib, N=0, q=None, o=None) == L.OK
+    for kw in ({"groups": -1}, {"B": -1}, {"N": -1}, {"Hq": 3}, {"Hkv": 0}, {"n_pages": -1}, {"n_table": -1}, {"n_p": -1},
+               {"ld": -1}, {"p_ld": -1}, {"norm": 0}, {"norm": 3}, {"q": None}, {"o": None}, {"k": None}, {"v": None},
+               {"table": None}, {"lens": None}, {"starts": None}, {"p_table": None}, {"p_lens": None}, {"p_starts": None},
+               {"q": Q + 8}, {"o": OUT + 2}, {"k": KP + 4}, {"v": VP + 4}, {"strides": [-256] + [64] * 9},
+               {"strides": [4] + [64] * 9}, {"o": Q}, {"o": Q + 2032}, {"o": KP + 64}, {"o": VP + 2 * 8 * 2048 - 16},
+               {"strides": OK[:8] + [0, 64]}, {"strides": OK[:8] + [256, 0]}):
+        assert _call(lib, **kw) == L.E_INVAL, kw
+    for kw in ({"dtype": L.F32}, {"d": 60}, {"d": 136}, {"d": 0}, {"page": 12}, {"scale": 0.0}, {"scale": float("inf")},
+               {"scale": float("nan")}, {"scale": 3e38}, {"N": 1 << 40}, {"B": 1 << 40}, {"groups": 1 << 40}, {"n_table": 1 << 30},
+               {"n_p": 1 << 30}, {"page": 1 << 40}):
+        assert _call(lib, **kw) == L.E_UNSUPPORTED, kw
+    need = lib.catopt_hip_paged_prefix_attn_workspace_bytes(1, 2, 4, 4, 2, 64, 4, 4, 16)
+    assert need > 0
+    for kw in ({"ws": None}, {"wsb": need - 1}, {"ws": A[10] + 8}):
+        assert _call(lib, **kw) == L.E_WORKSPACE, kw
+    # asked with too small a workspace: what is not refused before ends at that check
+    for kw in ({}, {"groups": 0, "p_table": None, "p_lens": None, "p_starts": None}, {"n_table": 0, "table": None},
+               {"n_p": 0, "p_table": None}, {"v": KP}, {"o": Q + 2048}):
+        assert _call(lib, wsb=0, **kw) == L.E_WORKSPACE, kw
+
+
+def test_workspace_query(lib):
+    f = lib.catopt_hip_paged_prefix_attn_workspace_bytes
+    ok = [1, 2, 4, 4, 2, 64, 4, 4, 16]
+    assert f(*ok) > 0 and f(*(ok[:1] + [0] + ok[2:])) == 0 and f(0, *ok[1:]) > 0
+    for i, x in ((0, -1), (1, -1), (2, -1), (3, 3), (4, 0), (5, 0), (5, 132), (5, 60), (6, -1), (7, -1), (8, 0), (8, 12),
+                 (0, 1 << 31), (2, 1 << 31), (3, 1 << 20), (6, 1 << 31), (7, 1 << 31), (8, 1 << 31)):
+        bad = list(ok)
+        bad[i] = x
+        assert f(*bad) == -1, bad
+
+
+def test_python_checks(monkeypatch):
+    q, p = torch.zeros((4, 4, 64), dtype=torch.bfloat16), torch.zeros((2, 2, 16, 64), dtype=torch.bfloat16)
+    i = lambda *n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    good = dict(q=q, k_pages=p, v_pages=p.clone(), prefix_table=i(1, 4), prefix_lens=i(1), prefix_starts=i(2), block_table=i(3, 4),
+                kv_lens=i(3), q_starts=i(4), scale=1.0)
+    with pytest.raises(ValueError, match="ROCm device"):
+        P.paged_prefix_attention(**good)
+    monkeypatch.setattr(P, "_device", lambda ts: 0)  # the checks behind it, which end before the launch
+    for kw in (dict(prefix_lens=i(2)), dict(prefix_lens=i(1).long()), dict(prefix_starts=i(1)), dict(prefix_starts=i(0)),
+               dict(prefix_table=i(2, 4)), dict(prefix_table=i(4)), dict(prefix_table=i(1, 4).long()), dict(kv_lens=i(2)),
+               dict(q_starts=i(3)), dict(block_table=i(2, 4)), dict(scale=0.0), dict(scale=float("nan")), dict(empty_rows="no"),
+               dict(q=q[0]), dict(q=q[:, :3]), dict(v_pages=p[:1]), dict(out=q[:2]), dict(out=q.float()),
+               dict(out=torch.zeros((4, 64, 4), dtype=torch.bfloat16).transpose(1, 2))):
+        with pytest.raises(ValueError):
+            P.paged_prefix_attention(**(good | kw))
+    for kw in (dict(q=q.float()), dict(k_pages=p.float(), v_pages=p.float()), dict(q=q[..., :60], k_pages=p[..., :60], v_pages=p[..., :60]),
+               dict(k_pages=p[:, :, :12], v_pages=p[:, :, :12])):
+        with pytest.raises(NotImplementedError):
+            P.paged_prefix_attention(**(good | kw))

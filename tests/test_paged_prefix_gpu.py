@@ -1,0 +1,271 @@
+"""Attention over a prefix that sequences share and their own keys, against float64 over both sets of keys."""
+
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from catopt_amd import kernels as K
+from catopt_amd import paged as P
+from paged_ref import BF16, DEV, Cache, attention, check_attention, gen, ints, randn, starts_of
+
+pytestmark = pytest.mark.gpu
+
+
+class Both:
+    """A cache whose first sequences are the prefixes and the rest the sequences; ``rows`` are a sequence's keys with its
+    prefix's before them."""
+
+    def __init__(self, pre, groups, own, Hkv, d, page, seed=0, **kw):
+        self.cache = Cache(list(pre) + list(own), Hkv, d, page, seed, **kw)
+        self.pre, self.groups, self.own, self.Hkv = list(pre), list(groups), list(own), Hkv
+        self.k, self.v = self.cache.k, self.cache.v
+        self.pre_table, self.table = self.cache.table[:len(pre)], self.cache.table[len(pre):]
+
+    def group(self, b):
+        at = [p for p in range(len(self.pre)) if self.groups[p] <= b < self.groups[p + 1]]
+        return at[0] if at else None
+
+    def lens(self):
+        return [n + (self.pre[self.group(b)] if self.group(b) is not None else 0) for b, n in enumerate(self.own)]
+
+    def rows(self, pages, b, n):
+        p, own = self.group(b), self.cache.rows(pages, len(self.pre) + b)
+        return own if p is None else torch.cat([self.cache.rows(pages, p), own], 1)
+
+    def call(self, q, nq, scale, **kw):
+        args = dict(pre_lens=ints(self.pre), groups=ints(self.groups), lens=ints(self.own), starts=starts_of(nq))
+        args.update({k: kw.pop(k) for k in list(kw) if k in args})
+        return P.paged_prefix_attention(q, self.k, self.v, self.pre_table, args["pre_lens"], args["groups"], self.table,
+                                        args["lens"], args["starts"], scale, **kw)
+
+
+def _run(pre, groups, nq, own, Hq, Hkv, d, page, seed=0, q_scale=1.0, causal=True, slot_major=False, empty="nan", keep=None):
+    c = Both(pre, groups, own, Hkv, d, page, seed, slot_major=slot_major)
+    q = randn(gen(seed), sum(nq), Hq, d, scale=q_scale)
+    o, m, l = c.call(q, nq, d ** -0.5, causal=causal, return_ml=True, empty_rows=empty)
+    check_attention(c, q, nq, c.lens(), o, scale=d ** -0.5, causal=causal, m=m, l=l, empty=empty)
+    assert torch.equal(torch.nan_to_num(o), torch.nan_to_num(c.call(q, nq, d ** -0.5, causal=causal, empty_rows=empty)))
+    return c, q, o
+
+
+# prefix lengths, the groups' first sequences; new tokens, own keys; query and key heads, head dim, page
+CASES = [
+    ([1], [0, 1], [1], [1], 1, 1, 8, 8),
+    ([5], [0, 2], [1, 1], [1, 9], 4, 2, 64, 8),
+    ([64], [0, 3], [1, 1, 1], [1, 17, 64], 8, 2, 128, 16),
+    ([500], [0, 4], [1] * 4, [10, 33, 128, 700], 32, 8, 128, 16),
+    ([1000, 77], [0, 20, 40], [1] * 40, [1 + 13 * i for i in range(40)], 8, 2, 128, 16),
+    ([2000], [0, 150], [1] * 150, [1 + i % 40 for i in range(150)], 4, 1, 64, 32),
+    ([333, 65, 1200], [0, 2, 5, 9], [3, 17, 1, 40, 0, 2, 9, 1, 77], [3, 50, 1, 40, 5, 30, 9, 300, 100], 6, 2, 96, 24),
+    ([3000], [0, 5], [33, 64, 5, 130, 200], [33, 64, 5, 130, 200], 8, 8, 128, 64),
+    ([700], [0, 2], [300, 150], [900, 150], 12, 4, 64, 16),
+    ([128], [0, 64], [2] * 64, [2 + i for i in range(64)], 16, 2, 128, 8),
+    ([4096], [0, 1], [1], [5], 8, 1, 128, 64),
+    ([900, 900], [0, 1, 2], [260, 1], [260, 40], 14, 2, 40, 16),
+]
+
+
+@pytest.mark.parametrize("pre,groups,nq,own,Hq,Hkv,d,page", CASES)
+def test_both_sets(pre, groups, nq, own, Hq, Hkv, d, page):
+    _run(pre, groups, nq, own, Hq, Hkv, d, page, seed=sum(own) + d)
+
+
+@pytest.mark.parametrize("pre,groups,nq,own,Hq,Hkv,d,page", CASES[2::4])
+def test_all_own_keys_seen(pre, groups, nq, own, Hq, Hkv, d, page):
+    _run(pre, groups, nq, own, Hq, Hkv, d, page, seed=d, causal=False, slot_major=True)
+
+
+@pytest.mark.parametrize("q_scale", [30.0, 0.0])
+@pytest.mark.parametrize("nq", [1, 40])
+def test_large_and_equal_scores(nq, q_scale):
+    _run([600], [0, 3], [nq] * 3, [nq, nq + 70, nq + 300], 8, 2, 128, 16, q_scale=q_scale)
+
+
+@pytest.mark.parametrize("groups", [[1, 3], [0, 0], [3, 3], [0, 2], [2, 4], [0, 4], [0, 9], [-5, 2]])
+@pytest.mark.parametrize("nq", [[1, 1, 1, 1], [40, 9, 0, 64]])
+def test_sequences_outside_the_group(groups, nq):
+    c = Both([260], groups, [40, 40, 3, 100], 2, 64, 16, seed=7)
+    q = randn(gen(7), sum(nq), 8, 64)
+    o, m, l = c.call(q, nq, 0.125, return_ml=True)
+    check_attention(c, q, nq, c.lens(), o, scale=0.125, m=m, l=l)
+
+
+@pytest.mark.parametrize("pre,groups", [([0], [0, 3]), ([0, 50], [0, 1, 3]), ([30, 0, 0, 70], [0, 0, 1, 1, 3]), ([], [0])])
+@pytest.mark.parametrize("nq", [1, 50])
+def test_empty_prefixes_and_groups(pre, groups, nq):
+    _run(pre, groups, [nq] * 3, [nq, nq + 5, nq + 200], 4, 2, 128, 16)
+
+
+def test_no_own_keys_at_all():
+    # all keys are the prefix', as for one more pass over it
+    c, q, _ = _run([300], [0, 2], [3, 5], [0, 0], 4, 2, 64, 16, causal=False)
+    o = P.paged_prefix_attention(q, c.k, c.v, c.pre_table, ints([300]), ints([0, 2]), c.table[:, :0], ints([0, 0]),
+                                 starts_of([3, 5]), 0.125)
+    want = P.paged_attention(q, c.k, c.v, c.pre_table, ints([300]), starts_of([8]), 0.125, causal=False)
+    check_attention(c, q, [3, 5], [300, 300], o, scale=0.125, causal=False)
+    check_attention(c, q, [3, 5], [300, 300], want, scale=0.125, causal=False)
+
+
+@pytest.mark.parametrize("nq", [[5, 1], [60, 40]])
+def test_rows_that_see_no_own_key_see_the_prefix(nq):
+    """More new tokens than own keys: the first of them see the prefix alone."""
+    own = [2, 0]
+    c = Both([90], [0, 2], own, 2, 128, 16, seed=3)
+    q = randn(gen(4), sum(nq), 4, 128)
+    o = c.call(q, nq, 0.1)
+    at = 0
+    for b, n in enumerate(nq):
+        few = n - own[b]
+        one = SimpleNamespace(k=c.k, v=c.v, Hkv=2, rows=lambda pages, i, length: c.cache.rows(pages, 0))
+        check_attention(one, q[at:at + few], [few], [90], o[at:at + few], scale=0.1, causal=False)
+        if own[b]:
+            two = SimpleNamespace(k=c.k, v=c.v, Hkv=2, rows=lambda pages, i, length, b=b: c.rows(pages, b, length))
+            check_attention(two, q[at + few:at + n], [own[b]], [90 + own[b]], o[at + few:at + n], scale=0.1)
+        at += n
+
+
+@pytest.mark.parametrize("empty", ["nan", "zero"])
+@pytest.mark.parametrize("nq", [[1, 2], [70, 3]])
+def test_rows_that_see_nothing(empty, nq):
+    _run([0], [0, 2], nq, [0, 1], 4, 2, 64, 16, empty=empty)
+
+
+@pytest.mark.parametrize("nq", [1, 50])
+def test_infinities_and_nan(nq):
+    """A value of a prefix key reaches every row of the group, one of an own key the rows that see it."""
+    c = Both([100, 40], [0, 2, 3], [nq + 30, nq, nq + 9], 2, 64, 16, seed=nq)
+    cache = c.cache
+    for b, j, x in ((0, 33, float("inf")), (2, 10, float("nan")), (4, nq + 8, float("-inf"))):
+        p, s = (t[j] for t in cache.where(b, cache.lens[b]))
+        cache.v[p, 0, s, 5] = x
+    q = randn(gen(5), 3 * nq, 4, 64)
+    o, m, l = c.call(q, [nq] * 3, 0.125, return_ml=True)
+    check_attention(c, q, [nq] * 3, c.lens(), o, scale=0.125, m=m, l=l)
+    # a prefix key of NaN: its group's rows alone
+    p, s = (t[0] for t in cache.where(0, 100))
+    cache.k[p, :, s] = float("nan")
+    o2, m2, l2 = c.call(q, [nq] * 3, 0.125, return_ml=True)
+    assert torch.isnan(o2[:2 * nq]).all() and torch.isnan(m2[:2 * nq]).all() and torch.isnan(l2[:2 * nq]).all()
+    assert torch.equal(torch.nan_to_num(o2[2 * nq:]), torch.nan_to_num(o[2 * nq:]))
+
+
+@pytest.mark.parametrize("nq", [1, 50])
+def test_invalid_pages_and_lengths_past_the_tables(nq):
+    c = Both([80, 48], [0, 1, 3], [nq + 40, nq + 3, nq + 17], 2, 128, 16, seed=2, table_extra=0)
+    q = randn(gen(2), 3 * nq, 4, 128)
+    good = c.cache.table.clone()
+    for bad in (-1, c.cache.n_pages, 2 ** 31 - 1, -(2 ** 31)):
+        c.cache.table[0, 2] = bad  # 16 keys of the first prefix
+        c.cache.table[2, 1] = bad  # and 16 of the first sequence
+        o, m, l = c.call(q, [nq] * 3, 0.1, return_ml=True)
+        c.cache.table.copy_(good)
+        keep = [torch.ones(n, dtype=torch.bool, device=DEV) for n in c.lens()]
+        keep[0][32:48] = False
+        keep[0][80 + 16:80 + 32] = False
+        check_attention(c, q, [nq] * 3, c.lens(), o, scale=0.1, m=m, l=l, keep=keep)
+    # cut to the tables' reach: both tables are as wide as the longest entry
+    width = c.cache.table.shape[1] * 16
+    full = Both([width], [0, 2], [width, width], 2, 128, 16, seed=3, table_extra=0)
+    q = randn(gen(2), 2 * nq, 4, 128)
+    want = full.call(q, [nq] * 2, 0.1)
+    got = full.call(q, [nq] * 2, 0.1, pre_lens=ints([2 ** 31 - 1]), lens=ints([width, 2 ** 31 - 1]))
+    assert torch.equal(got, want)
+    none = full.call(q, [nq] * 2, 0.1, pre_lens=ints([-3]), lens=ints([-1, -(2 ** 31)]), empty_rows="zero")
+    assert (none == 0).all()
+
+
+def test_padded_rows_are_left_alone():
+    c = Both([200], [0, 2], [9, 70, 0], 2, 64, 16, seed=1)
+    q = torch.full((12, 4, 64), float("nan"), device=DEV, dtype=BF16)
+    q[:6] = randn(gen(1), 6, 4, 64)
+    out = torch.full((12, 4, 64), 9.0, device=DEV, dtype=BF16)
+    r = c.call(q, [2, 4, 0], 0.125, out=out)
+    assert r is out and (out[6:] == 9).all()
+    check_attention(c, q[:6], [2, 4, 0], c.lens(), out[:6], scale=0.125)
+
+
+@pytest.mark.parametrize("nq", [1, 33])
+def test_views_and_another_stream(nq):
+    c = Both([130], [0, 3], [nq, nq + 20, nq + 90], 2, 64, 16, seed=9)
+    qkv = randn(gen(9), 3 * nq, 12 * 64)
+    q = qkv[:, 128:128 + 512].unflatten(1, (8, 64))
+    wide = torch.zeros((3 * nq, 8, 72), device=DEV, dtype=BF16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.call(q, [nq] * 3, 0.125, out=wide[..., :64])
+    side.synchronize()
+    check_attention(c, q, [nq] * 3, c.lens(), wide[..., :64], scale=0.125)
+    assert (wide[..., 64:] == 0).all()
+    assert torch.equal(c.call(q.clone(), [nq] * 3, 0.125), wide[..., :64].contiguous())
+
+
+def test_as_two_calls_and_their_composition():
+    nq = [1, 7, 20]
+    c = Both([400], [0, 3], [30, 7, 100], 4, 128, 16, seed=11)
+    q = randn(gen(11), sum(nq), 8, 128)
+    o, m, l = c.call(q, nq, 0.09, return_ml=True)
+    parts = []
+    for table, lens, starts, causal in ((c.pre_table, [400], [0, 28], False), (c.table, c.own, [0, 1, 8, 28], True)):
+        o1, m1, l1 = P.paged_attention(q, c.k, c.v, table, ints(lens), ints(starts), 0.09, causal=causal, return_ml=True)
+        parts.append((m1, l1, o1.float() * l1[..., None]))
+    m2, l2, a2 = K.om_compose(*parts)
+    check_attention(c, q, nq, c.lens(), o, scale=0.09, m=m, l=l)
+    at = 0
+    for b, n in enumerate(nq):
+        rows, length = slice(at, at + n), c.lens()[b]
+        at += n
+        r = attention(q[rows], c.rows(c.k, b, length), c.rows(c.v, b, length), 0.09)
+        es = torch.expm1(2 * r["es"]) + (length + 64) * 2.0 ** -24
+        # the softmax terms and the parts' results are rounded to bf16, each off by 2^-8 of what it weighs at most
+        err = ((a2 / l2[..., None])[rows].double().transpose(0, 1) - r["o"]).abs()
+        assert (err <= (2 * 2.0 ** -8 + es)[..., None] * r["mag"] * 1.01).all(), b
+        assert ((m2[rows].double().t() - r["m"]).abs() <= r["es"] + 1e-37).all()
+        assert ((l2[rows].double().t() - r["l"]).abs() <= es * r["l"] * 1.01).all()
+
+
+@pytest.mark.parametrize("nq", [1, 40])
+def test_a_captured_step_replays_on_other_lengths(nq):
+    c = Both([500, 300], [0, 3, 6], [nq + 100] * 6, 2, 128, 16, seed=13)
+    q = randn(gen(13), 6 * nq, 8, 128)
+    pre, groups, lens, starts = ints([500, 300]), ints([0, 3, 6]), ints(c.own), starts_of([nq] * 6)
+    def run(scale=0.1):
+        return P.paged_prefix_attention(q, c.k, c.v, c.pre_table, pre, groups, c.table, lens, starts, scale, return_ml=True)
+
+    calls = [run, lambda: run(0.2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for f in calls:
+            f()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for f in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(f())
+    for step in range(4):
+        c.pre, c.groups = [500 - 99 * step, 7 + 40 * step], [0, 3 - step % 3, 6 - step % 2]
+        c.own = [nq + 13 * step + i for i in range(6)]
+        c.cache.lens = c.pre + c.own
+        pre.copy_(ints(c.pre)), groups.copy_(ints(c.groups)), lens.copy_(ints(c.own))
+        q.copy_(randn(gen(step), 6 * nq, 8, 128))
+        for g in graphs:
+            g.replay()
+        for f, out in zip(calls, outs):
+            assert all(torch.equal(x, y) for x, y in zip(f(), out))
+        o, m, l = outs[0]
+        check_attention(c, q, [nq] * 6, c.lens(), o, scale=0.1, m=m, l=l)
+
+
+def test_nothing_to_do():
+    c = Both([40], [0, 1], [4], 2, 64, 16)
+    o, m, l = c.call(randn(gen(0), 0, 4, 64), [0], 0.1, return_ml=True)
+    assert o.shape == (0, 4, 64) and m.shape == l.shape == (0, 4)
+    q = randn(gen(0), 3, 4, 64)
+    out = torch.full_like(q, 5.0)
+    P.paged_prefix_attention(q, c.k, c.v, c.pre_table, ints([40]), ints([0, 0]), c.table[:0], ints([]), ints([0]), 0.1, out=out)
+    assert (out == 5).all()
