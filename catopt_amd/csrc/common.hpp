@@ -24,6 +24,20 @@ int32_t set_hip_error(hipError_t e);
     if (e_ != hipSuccess) return ::catopt::set_hip_error(e_);   \
   } while (0)
 
+// A kernel's dynamic LDS beyond the default, set once on each device (`done`:
+// one flag per device, idempotent; a concurrent first call sets the same).
+constexpr int kDevices = 16;
+inline int32_t allow_lds(const void* kernel, int bytes, bool* done) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return set_hip_error(e);
+  if (dev < kDevices && done[dev]) return CATOPT_OK;
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return set_hip_error(e);
+  if (dev < kDevices) done[dev] = true;
+  return CATOPT_OK;
+}
+
 __device__ __forceinline__ float bf16_to_f32(uint16_t h) {
   return __uint_as_float(static_cast<uint32_t>(h) << 16);
 }

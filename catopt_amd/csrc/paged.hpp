@@ -38,20 +38,6 @@ __device__ __forceinline__ void seq_rows(const int32_t* starts, int b, int64_t N
   nq = max(min(max(starts[b + 1], 0), n) - row0, 0);
 }
 
-// A kernel's dynamic LDS beyond the default, set once on each device (`done`:
-// one flag per device, idempotent; a concurrent first call sets the same).
-constexpr int kDevices = 16;
-inline int32_t allow_lds(const void* kernel, int bytes, bool* done) {
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
-  if (e != hipSuccess) return set_hip_error(e);
-  if (dev < kDevices && done[dev]) return CATOPT_OK;
-  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != hipSuccess) return set_hip_error(e);
-  if (dev < kDevices) done[dev] = true;
-  return CATOPT_OK;
-}
-
 // Strides as the kernels take them: none negative, multiples of `step`; that of
 // an axis of one entry, which may be anything, as 0.
 struct Strides {

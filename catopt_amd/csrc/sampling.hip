@@ -99,33 +99,38 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
 // ------------------------------------------------------------------ rows
 
 constexpr int RT = 1024, WAVES = RT / 64;
-constexpr int kList = 4096;    // logits of a row that are kept in LDS
-constexpr int kSubs = 256;     // parts of a range
+constexpr int kList = 8192;   // logits of a row that are kept in LDS
+constexpr int kParts = 256;   // of a range
 constexpr int kMaxChunks = 520;
+
+// What one step of a search adds up.  Three of them take turns: a step clears the
+// next one's, which was last read before the barrier that ended the step before,
+// so that a step is one barrier.
+struct Step {
+  uint64_t weight[kParts];
+  uint64_t last[64];
+  uint32_t n[kParts];
+  uint32_t count;
+};
 
 struct RowLds {
   uint64_t cum[kBins];  // weights up to a bin's end, in units of 2^-42 of bin 0's
   uint64_t list[kList];
-  uint64_t sub[kSubs];
-  uint64_t last[64];
+  Step steps[3];
   uint64_t wave_sums[WAVES];
-  uint64_t lo, hi, found, found_sum;
   uint32_t cum_n[kBins];  // logits up to it: exactly with a top-k, else at most
-  uint32_t sub_n[kSubs];
   uint32_t wave_counts[WAVES];
   int off[kMaxChunks];  // a chunk's first bin among the row's
-  uint32_t n;
-  int bin;
 };
 
 // (min and max of the headers take 64-bit integers as doubles.)
 __device__ __forceinline__ uint64_t least_of(uint64_t a, uint64_t b) { return a < b ? a : b; }
-__device__ __forceinline__ uint64_t most_of(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 __device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
   return (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane, 64) << 32 | (uint32_t)__shfl((int)(uint32_t)v, lane, 64);
 }
-__device__ __forceinline__ uint64_t scan_u64(uint64_t v) {  // inclusive, over the wave
+// Inclusive sums over the wave.
+__device__ __forceinline__ uint64_t scan_u64(uint64_t v) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -143,6 +148,25 @@ __device__ __forceinline__ uint32_t scan_u32(uint32_t v) {
   }
   return v;
 }
+__device__ __forceinline__ double scan_f64(double v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// The wave's places (~0 behind the last) in ascending order, lane by lane.
+__device__ __forceinline__ uint64_t sorted(uint64_t mine, int n) {
+  int rank = 0;
+  for (int j = 0; j < n; ++j) rank += shfl_u64(mine, j) < mine;
+  if ((int)(threadIdx.x & 63) >= n) rank = threadIdx.x & 63;
+  const uint32_t hi = __builtin_amdgcn_ds_permute(4 * rank, (int)(mine >> 32));
+  const uint32_t lo = __builtin_amdgcn_ds_permute(4 * rank, (int)(uint32_t)mine);
+  return (uint64_t)hi << 32 | lo;
+}
 
 // What a border or the token is looked for by: the logit at a rank, or the first
 // whose running sum of weights reaches or passes a number.
@@ -151,208 +175,198 @@ __device__ __forceinline__ bool meets(Find f, double target, uint64_t sum, uint3
   return f == kRank ? (double)n > target : f == kReaches ? (double)sum >= target : (double)sum > target;
 }
 
-// A row's search.  The source of its passes is the row or, once the logits in
-// question fit, the list in LDS.
+// Bin b's weight to bin 0's.
+__device__ __forceinline__ double scale_of(int b) { return exp2(-(double)b / 16); }
+
+struct Bins {
+  int first, last;
+  __device__ __forceinline__ bool has(int b) const { return b >= first && b <= last; }
+};
+constexpr Bins kNoBins{1, 0};
+
+// A row's search.  Every wave comes to the same decisions, from what is in LDS.
 template <typename T>
 struct Search {
   RowLds& s;
   const RowReader<T> r;
   double c, ref;
-  bool listed;  // the list holds all logits of bins up to list_end
-  int list_end;
+  int step = 0;
+  uint32_t n_list = 0;
+  Bins listed = kNoBins, listed2 = kNoBins;  // the list holds all their logits
 
   __device__ __forceinline__ int bin_of(float x, double& rest) const {
     const double d = ref - grid(x, c, rest);
     return d < kBins ? (int)d : kBins;
   }
 
-  // f(logit, place) for every logit of bins [b0, b1] that are not empty.
+  // Numbers that no logit of bins up to b is below, or from b on above.
+  __device__ __forceinline__ float floor_of(int b) const {
+    const float f = (float)((ref - b - 0.5) / c);
+    return f - fabsf(f) * 0x1p-22f - 0x1p-140f;
+  }
+  __device__ __forceinline__ float top_of(int b) const {
+    const float f = (float)((ref - b + 0.5) / c);
+    return f + fabsf(f) * 0x1p-22f + 0x1p-140f;
+  }
+
+  __device__ __forceinline__ Step& begin() {
+    Step& next = s.steps[(step + 1) % 3];
+    if (threadIdx.x < kParts) next.weight[threadIdx.x] = 0, next.n[threadIdx.x] = 0;
+    if (threadIdx.x == 0) next.count = 0;
+    return s.steps[step++ % 3];
+  }
+
+  // f(place, rest) for the row's logits in either of the bins.
   template <typename F>
-  __device__ __forceinline__ void pass(bool list, uint32_t n_list, int b0, int b1, F f) const {
-    if (list) {
-      for (uint32_t i = threadIdx.x; i < n_list; i += RT) {
-        const uint64_t at = s.list[i];
-        const float x = logit_of(at);
-        double rest;
-        const int b = bin_of(x, rest);
-        if (b >= b0 && b <= b1) f(x, at, rest);
-      }
-      return;
-    }
-    constexpr int U = sizeof(T) == 4 ? 2 : 1;
+  __device__ __forceinline__ void scan_row(Bins a, Bins b, F f) const {
+    constexpr int U = 4;
+    // most logits fall out by two comparisons; the others' bins are worked out
+    const float lo = floor_of(a.last), hi = top_of(a.first), lo2 = floor_of(b.last), hi2 = top_of(b.first);
+    const bool two = b.first <= b.last;
     const int n = r.pieces();
+#pragma unroll 1
     for (int p0 = threadIdx.x; p0 < n; p0 += U * RT) {
       u32x4 w[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) w[j] = r.load(p0 + j * RT);
 #pragma unroll
-      for (int j = 0; j < U; ++j)
+      for (int j = 0; j < U; ++j) {
+        uint32_t some = 0;
 #pragma unroll
         for (int e = 0; e < RowReader<T>::W; ++e) {
-          const float x = finite_top(r.at(w[j], e));
-          double rest;
-          const int b = bin_of(x, rest);
-          if (b >= b0 && b <= b1) f(x, place(x, r.first(p0 + j * RT) + e), rest);
+          const float x = r.at(w[j], e);
+          some |= ((x >= lo && x <= hi) || (two && x >= lo2 && x <= hi2)) ? 1u << e : 0u;
         }
+        while (some) {
+          const int e = __builtin_ctz(some);
+          some &= some - 1;
+          float x = r.at(w[j], 0);
+#pragma unroll
+          for (int i = 1; i < RowReader<T>::W; ++i) x = i == e ? r.at(w[j], i) : x;
+          x = finite_top(x);
+          double rest;
+          const int bin = bin_of(x, rest);
+          if (a.has(bin) || b.has(bin)) f(place(x, r.first(p0 + j * RT) + e), rest);
+        }
+      }
     }
   }
 
-  // The logits of a range of places into the list, as far as it holds them; their
-  // number.
-  __device__ __forceinline__ uint32_t gather(int b0, int b1, uint64_t lo, uint64_t hi) {
-    __syncthreads();
-    if (threadIdx.x == 0) s.n = 0;
-    __syncthreads();
-    pass(false, 0, b0, b1, [&](float, uint64_t at, double) {
-      if (at >= lo && at <= hi) {
-        const uint32_t i = atomicAdd(&s.n, 1u);
-        if (i < kList) s.list[i] = at;
-      }
+  // The logits of a range of places of those bins into the list, as far as it
+  // holds them; their number.
+  __device__ __forceinline__ uint32_t gather(Bins a, Bins b, uint64_t lo, uint64_t hi) {
+    Step& t = begin();
+    scan_row(a, b, [&](uint64_t at, double) {
+      if (at < lo || at > hi) return;
+      const uint32_t i = atomicAdd(&t.count, 1u);
+      if (i < kList) s.list[i] = at;
     });
     __syncthreads();
-    return s.n;
+    return t.count;
+  }
+
+  // The same to be searched in afterwards, if it holds them.
+  __device__ __forceinline__ void list_bins(Bins a, Bins b) {
+    n_list = gather(a, b, 0, ~0ull);
+    const bool all = n_list <= kList;
+    listed = all ? a : kNoBins, listed2 = all ? b : kNoBins;
+  }
+
+  // The first bin whose running sum (or count) meets the target, kBins - 1 where none does.
+  __device__ __forceinline__ int find_bin(Find find, double target) const {
+    const int lane = threadIdx.x & 63, group = 64 * min(lane, kBins / 64 - 1);
+    const uint64_t ends = __ballot(lane < kBins / 64 && meets(find, target, s.cum[group + 63], s.cum_n[group + 63]));
+    if (!ends) return kBins - 1;
+    const int first = 64 * __builtin_ctzll(ends);
+    return first + __builtin_ctzll(__ballot(meets(find, target, s.cum[first + lane], s.cum_n[first + lane])));
   }
 
   // Of bin b, the logit that `find` names by `target` (a rank or a sum within the
   // bin): its place and the sum up to it; the last one where none does.
   __device__ __forceinline__ uint64_t resolve(int b, Find find, double target, uint64_t& sum) {
-    const int tid = threadIdx.x, lane = tid & 63;
-    bool list = listed && b <= list_end;
-    uint32_t n_list = s.n, n = 0;
-    uint64_t lo = 0, hi = ~0ull, before = 0;
-    uint32_t n_before = 0;
-    if (!list) {
-      listed = false;  // it is overwritten
-      n = n_list = gather(b, b, 0, ~0ull);
-      list = n <= kList;
-    }
-    // the range that the bin's places take
-    __syncthreads();
-    if (tid == 0) s.lo = ~0ull, s.hi = 0, s.bin = 0;
-    __syncthreads();
-    {
-      uint64_t least = ~0ull, most = 0;
-      uint32_t mine = 0;
-      pass(list, n_list, b, b, [&](float, uint64_t at, double) {
-        least = least_of(least, at), most = most_of(most, at);
-        ++mine;
-      });
-      if (mine) {
-        atomicMin(reinterpret_cast<unsigned long long*>(&s.lo), (unsigned long long)least);
-        atomicMax(reinterpret_cast<unsigned long long*>(&s.hi), (unsigned long long)most);
-        atomicAdd(reinterpret_cast<uint32_t*>(&s.bin), mine);
+    const int lane = threadIdx.x & 63;
+    const Bins one{b, b};
+    uint64_t lo = place(top_of(b), 0), hi = place(floor_of(b), -1), before = 0;
+    uint32_t n_before = 0, n = s.cum_n[b] - (b ? s.cum_n[b - 1] : 0);
+    bool list = listed.has(b) || listed2.has(b), own = false;  // own: the list is this call's, and holds the range alone
+    for (;;) {
+      if (!list && n <= kList) {
+        listed = listed2 = kNoBins;
+        n = n_list = gather(one, kNoBins, lo, hi);
+        list = own = true;
       }
-      __syncthreads();
-      lo = s.lo, hi = s.hi, n = (uint32_t)s.bin;
-    }
-    while (n > 64) {
-      // 256 parts of the range; the one that the logit is in
+      // one key alone: its indexes end with the row
+      if (lo >> 32 == hi >> 32) hi = least_of(hi, (hi & ~0xffffffffull) | (uint32_t)(r.V - 1));
+      const bool few = n <= 64;
       const int bits = 64 - __builtin_clzll((hi - lo) | 1), shift = max(bits - 8, 0);
-      __syncthreads();
-      if (tid < kSubs) s.sub[tid] = 0, s.sub_n[tid] = 0;
-      __syncthreads();
-      pass(list, n_list, b, b, [&](float, uint64_t at, double rest) {
+      Step& t = begin();
+      auto take = [&](uint64_t at, double rest) {
         if (at < lo || at > hi) return;
-        const int i = (int)((at - lo) >> shift);
-        atomicAdd(reinterpret_cast<unsigned long long*>(s.sub + i), (unsigned long long)fixed(rest));
-        atomicAdd(s.sub_n + i, 1u);
-      });
-      __syncthreads();
-      if (tid < 64) {  // four parts a lane
-        uint64_t w[4], all = 0;
-        uint32_t k[4], all_n = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = s.sub[4 * lane + i], k[i] = s.sub_n[4 * lane + i];
-          all += w[i], all_n += k[i];
+        if (few) {
+          t.last[atomicAdd(&t.count, 1u) & 63] = at;
+        } else {
+          const int i = (int)((at - lo) >> shift);
+          atomicAdd(reinterpret_cast<unsigned long long*>(t.weight + i), (unsigned long long)fixed(rest));
+          atomicAdd(t.n + i, 1u);
         }
-        uint64_t upto = scan_u64(all) - all + before;
-        uint32_t upto_n = scan_u32(all_n) - all_n + n_before;
-        int at = -1;
-        uint64_t at_sum = 0;
-        uint32_t at_n = 0, here = 0;
-        int at_last = -1;  // the last part that holds one
-        uint64_t last_sum = 0;
-        uint32_t last_n = 0, last_here = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (k[i]) {
-            if (at < 0 && meets(find, target, upto + w[i], upto_n + k[i])) at = 4 * lane + i, at_sum = upto, at_n = upto_n, here = k[i];
-            at_last = 4 * lane + i, last_sum = upto, last_n = upto_n, last_here = k[i];
-          }
-          upto += w[i], upto_n += k[i];
+      };
+      if (list) {
+#pragma unroll 1
+        for (uint32_t i = threadIdx.x; i < n_list; i += RT) {
+          const uint64_t at = s.list[i];
+          double rest;
+          if (bin_of(logit_of(at), rest) == b) take(at, rest);
         }
-        const uint64_t some = __ballot(at >= 0), held = __ballot(at_last >= 0);
-        const bool none = some == 0;
-        const int from = none ? 63 - __builtin_clzll(held) : __builtin_ctzll(some);
-        if (lane == from) {
-          s.bin = none ? at_last : at;
-          s.found_sum = none ? last_sum : at_sum;
-          s.sub_n[0] = none ? last_n : at_n;
-          s.n = none ? last_here : here;
-        }
+      } else {
+        scan_row(one, kNoBins, take);
       }
       __syncthreads();
-      lo += (uint64_t)s.bin << shift;
-      hi = least_of(hi, lo + ((1ull << shift) - 1));
-      before = s.found_sum, n_before = s.sub_n[0], n = s.n;
-      if (!list && n <= kList) n_list = gather(b, b, lo, hi), list = true;
-    }
-    // at most 64: a wave puts them in order
-    __syncthreads();
-    if (tid == 0) s.bin = 0;
-    __syncthreads();
-    pass(list, n_list, b, b, [&](float, uint64_t at, double) {
-      if (at >= lo && at <= hi) s.last[atomicAdd(&s.bin, 1) & 63] = at;
-    });
-    __syncthreads();
-    if (tid < 64) {
-      const int m = min(s.bin, 64);
-      const uint64_t mine = lane < m ? s.last[lane] : ~0ull;
-      int rank = 0;
-      for (int j = 0; j < m; ++j) rank += shfl_u64(mine, j) < mine;
-      if (lane < m) s.last[rank] = mine;
-      __builtin_amdgcn_wave_barrier();
-      const uint64_t at = lane < m ? s.last[lane] : ~0ull;
-      double rest = 0;
-      uint64_t w = 0;
-      if (lane < m) {
+      if (few) {  // a wave puts them in order
+        const int m = min((int)t.count, 64);
+        const uint64_t at = sorted(lane < m ? t.last[lane] : ~0ull, m);
+        double rest;
         bin_of(logit_of(at), rest);
-        w = fixed(rest);
+        const uint64_t upto = scan_u64(lane < m ? fixed(rest) : 0) + before;
+        const uint64_t some = __ballot(lane < m && meets(find, target, upto, n_before + lane + 1));
+        const int from = some ? __builtin_ctzll(some) : max(m - 1, 0);
+        sum = shfl_u64(upto, from);
+        if (own) listed = listed2 = kNoBins;
+        return shfl_u64(at, from);
       }
-      const uint64_t upto = scan_u64(w) + before;
-      const uint64_t some = __ballot(lane < m && meets(find, target, upto, n_before + lane + 1));
-      const int from = some ? __builtin_ctzll(some) : max(m - 1, 0);
-      if (lane == from) s.found = at, s.found_sum = upto;
+      // four parts a lane: the part that the logit is in, the last that holds one where none meets the target
+      uint64_t w[4], all = 0;
+      uint32_t k[4], all_n = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = t.weight[4 * lane + i], k[i] = t.n[4 * lane + i];
+        all += w[i], all_n += k[i];
+      }
+      uint64_t upto = scan_u64(all) - all + before, at_sum = 0;
+      uint32_t upto_n = scan_u32(all_n) - all_n + n_before, at_n = 0, here = 0;
+      int at = -1;
+      bool met = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (k[i] && !met) {
+          at = 4 * lane + i, at_sum = upto, at_n = upto_n, here = k[i];
+          met = meets(find, target, upto + w[i], upto_n + k[i]);
+        }
+        upto += w[i], upto_n += k[i];
+      }
+      const uint64_t some = __ballot(met), held = __ballot(at >= 0);
+      const int from = some ? __builtin_ctzll(some) : 63 - __builtin_clzll(held | 1);
+      const int part = max(__shfl(at, from, 64), 0);
+      lo += (uint64_t)part << shift;
+      hi = least_of(hi, lo + ((1ull << shift) - 1));
+      before = shfl_u64(at_sum, from), n_before = __shfl(at_n, from, 64), n = __shfl(here, from, 64);
     }
-    __syncthreads();
-    if (listed) s.n = n_list;  // the list is as it was
-    sum = s.found_sum;
-    const uint64_t at = s.found;
-    __syncthreads();
-    return at;
-  }
-
-  // The first bin whose running sum (or count) meets the target, kBins - 1 where none does.
-  __device__ __forceinline__ int find_bin(Find find, double target) {
-    const int tid = threadIdx.x;
-    __syncthreads();
-    if (tid == 0) s.bin = kBins - 1;
-    __syncthreads();
-    if (tid < kBins && meets(find, target, s.cum[tid], s.cum_n[tid]) &&
-        (tid == 0 || !meets(find, target, s.cum[tid - 1], s.cum_n[tid - 1])))
-      s.bin = tid;
-    __syncthreads();
-    return s.bin;
   }
 };
 
-// Bin b's weight to bin 0's.
-__device__ __forceinline__ double scale_of(int b) { return exp2(-(double)b / 16); }
-
 template <typename T>
 __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
-  __shared__ RowLds s;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  RowLds& s = *reinterpret_cast<RowLds*>(lds);
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Settings set = settings(a, row);
   const ChunkHead* heads = a.heads + (int64_t)row * a.chunks;
@@ -363,6 +377,7 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     m = fmaxf(m, h.max);
     nan |= h.nan;
   }
+  const float u_row = a.u[row];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const bool valid = set.valid && __ballot(nan != 0) == 0 && m != -__builtin_inff();
@@ -382,7 +397,7 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   const double c = factor(set.t, m);
   double rest;
   const double ref = grid(m, c, rest);
-  Search<T> find{s, RowReader<T>(a, row), c, ref, false, -1};
+  Search<T> find{s, RowReader<T>(a, row), c, ref};
   // ---- the row's bins from the chunks'
   for (int i = tid; i < a.chunks; i += RT) {
     const float cm = heads[i].max;
@@ -390,18 +405,21 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     const double d = cm == -__builtin_inff() ? kBins : ref - grid(cm, c, rest);
     s.off[i] = d < kBins ? max((int)d, 0) : kBins;
   }
+  if (tid < kParts) s.steps[0].weight[tid] = 0, s.steps[0].n[tid] = 0;
+  if (tid == 0) s.steps[0].count = 0;
   __syncthreads();
   const bool counted = set.k != 0;
   uint64_t w = 0;
   uint32_t n = 0;
   if (tid < kBins) {
-    const int64_t at = (int64_t)row * a.chunks * kBins;
+    const uint64_t* ws = a.weights + (int64_t)row * a.chunks * kBins + tid;
+    const uint32_t* ns = a.counts + (int64_t)row * a.chunks * kBins + tid;
+#pragma unroll 4
     for (int i = 0; i < a.chunks; ++i) {
-      const int b = tid - s.off[i];
-      if (b >= 0) {
-        w += a.weights[at + (int64_t)i * kBins + b];
-        if (counted) n += a.counts[at + (int64_t)i * kBins + b];
-      }
+      const int o = s.off[i];
+      const bool in = tid >= o;
+      w += in ? ws[(int64_t)i * kBins - o] : 0;
+      if (counted) n += in ? ns[(int64_t)i * kBins - o] : 0;
     }
     // a logit weighs at least 0.978 in its bin
     if (!counted) n = (uint32_t)((double)w * (1.0 / (0.978 * (1LL << kPoint)))) + (w != 0);
@@ -419,12 +437,15 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   }
   __syncthreads();
   // ---- the kept prefix: up to `cut_at` in bin `cut`, `total` in all
+  // below 1 by half a step of fp32 at least, so that the product stays below the total; a NaN counts as 0
+  const double u = fmin(fmax((double)u_row, 0.0), 1 - 0x1p-25);
   int cut = kBins - 1;
   uint64_t cut_at = ~0ull, total = s.cum[kBins - 1];
   bool by_rank = counted && s.cum_n[kBins - 1] > set.k, by_sum = set.p < 1, by_low = set.low > 0;
   const double low = by_low ? (double)m * c + 16 * log2(fmin(set.low, 1.0)) : -__builtin_inf();
   const double low_bin = by_low ? ref - rint(low) : kBins;
   auto before = [&](int b) { return b > 0 ? s.cum[b - 1] : 0ull; };
+  auto before_n = [&](int b) { return b > 0 ? s.cum_n[b - 1] : 0u; };
   auto within = [&](int b, uint64_t sum) { return before(b) + (uint64_t)rint((double)sum * scale_of(b)); };
   if (by_rank || by_sum || by_low) {
     if (by_rank) cut = find.find_bin(kRank, (double)(set.k - 1));
@@ -433,16 +454,46 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     by_low = low_bin <= end;
     if (low_bin < end && !(by_rank && by_sum)) by_rank = by_sum = false, end = (int)low_bin;
     if (s.cum_n[end] <= kList) {
-      find.gather(0, end, 0, ~0ull);
-      find.listed = true, find.list_end = end;
+      find.list_bins({0, end}, kNoBins);
+      if (find.n_list <= 64) {
+        // all that may be kept is in one wave: the definition, lane by lane
+        const int n_all = (int)find.n_list;
+        const uint64_t at = sorted(lane < n_all ? s.list[lane] : ~0ull, n_all);
+        const int bin = find.bin_of(logit_of(at), rest);
+        const double sums = scan_f64(lane < n_all ? (double)fixed(rest) * scale_of(bin) : 0);
+        const double whole = by_rank ? __shfl(sums, (int)set.k - 1, 64) : (double)total;
+        bool kept = lane < (by_rank ? (int)set.k : n_all);
+        if (by_sum) {
+          const uint64_t reach = __ballot(kept && sums >= set.p * whole);
+          if (reach) kept = lane <= __builtin_ctzll(reach);
+        }
+        if (by_low) kept = kept && (double)logit_of(at) * c >= low;
+        const int last = 63 - __builtin_clzll(__ballot(kept) | 1);
+        const double kept_sum = __shfl(sums, last, 64);
+        const uint64_t pass = __ballot(lane <= last && sums > u * kept_sum);
+        const int from = pass ? __builtin_ctzll(pass) : last;
+        const double log2_total = log2(kept_sum) - kPoint;
+        if (wave == 0 && lane == from) {
+          a.tokens[row] = (int64_t)(uint32_t)at;
+          a.logprobs[row] = (float)(((rest - bin) / 16 - log2_total) * 0.6931471805599453);
+        }
+        if (wave == 0 && lane == last && a.rows) a.rows[row] = RowState{c, ref, low, log2_total, at, bin, 0};
+        return;
+      }
+    } else if (!by_rank) {
+      // the border lies in bin `end`, the token where u says for a whole between the sums before and behind it: both
+      // are read at once if they fit
+      const Bins pick{find.find_bin(kPasses, u * (double)before(end)), min(find.find_bin(kPasses, u * (double)s.cum[end]), end - 1)};
+      const uint32_t here = s.cum_n[end] - before_n(end);
+      const uint32_t there = pick.first <= pick.last ? s.cum_n[pick.last] - before_n(pick.first) : 0;
+      if (here + there <= kList) find.list_bins({end, end}, pick);
     }
     uint64_t sum;
     if (by_rank) {
-      const uint32_t n_before = cut > 0 ? s.cum_n[cut - 1] : 0;
       if (s.cum_n[cut] == set.k) {
         total = s.cum[cut];
       } else {
-        cut_at = find.resolve(cut, kRank, (double)(set.k - 1 - n_before), sum);
+        cut_at = find.resolve(cut, kRank, (double)(set.k - 1 - before_n(cut)), sum);
         total = within(cut, sum);
       }
     }
@@ -455,22 +506,27 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     if (by_low && low_bin <= cut) {
       // of the border's bin those whose y is not below it
       const int b = (int)low_bin;
-      __syncthreads();
-      if (tid == 0) s.lo = 0;
-      __syncthreads();
+      if (!find.listed.has(b)) find.list_bins({b, b}, kNoBins);
+      Step& t = find.begin();
       uint64_t mine = 0;
-      find.pass(find.listed && b <= find.list_end, s.n, b, b, [&](float x, uint64_t at, double rs) {
+      auto take = [&](float x, uint64_t at, double rs) {
         if ((double)x * c >= low && (b < cut || at <= cut_at)) mine += fixed(rs);
-      });
-      if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(&s.lo), (unsigned long long)mine);
+      };
+      if (find.listed.has(b)) {
+        for (uint32_t i = tid; i < find.n_list; i += RT) {
+          const float x = logit_of(s.list[i]);
+          if (find.bin_of(x, rest) == b) take(x, s.list[i], rest);
+        }
+      } else {
+        find.scan_row({b, b}, kNoBins, [&](uint64_t at, double rs) { take(logit_of(at), at, rs); });
+      }
+      if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(t.weight), (unsigned long long)mine);
       __syncthreads();
-      total = least_of(total, within(b, s.lo));
+      total = least_of(total, within(b, t.weight[0]));
       if (b < cut) cut = b, cut_at = ~0ull;
     }
   }
   // ---- the token
-  // below 1 by half a step of fp32 at least, so that the product stays below the total; a NaN counts as 0
-  const double u = fmin(fmax((double)a.u[row], 0.0), 1 - 0x1p-25);
   const double target = u * (double)total;
   const int b = min(find.find_bin(kPasses, target), cut);
   uint64_t sum, at = find.resolve(b, kPasses, (target - (double)before(b)) / scale_of(b), sum);
@@ -547,7 +603,10 @@ int32_t launch(const SampleArgs& a, const Plan& p, hipStream_t st) {
   else
     sample_chunks<T, 8><<<grid, dim3(CT), 0, st>>>(a);
   CATOPT_LAUNCH_CHECK();
-  sample_rows<T><<<dim3((uint32_t)a.B), dim3(RT), 0, st>>>(a);
+  static bool done[kDevices] = {};
+  const int32_t r = allow_lds(reinterpret_cast<const void*>(&sample_rows<T>), sizeof(RowLds), done);
+  if (r != CATOPT_OK) return r;
+  sample_rows<T><<<dim3((uint32_t)a.B), dim3(RT), sizeof(RowLds), st>>>(a);
   CATOPT_LAUNCH_CHECK();
   if (a.probs) {
     constexpr int64_t per = PT * PIECES * RowReader<T>::W;
