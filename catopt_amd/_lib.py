@@ -134,7 +134,7 @@ SIGNATURES: dict[str, tuple] = {
         [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _p,
          _p, _f32, _i32, _i32, _p, _p, _p, _p, _p, _i64, _p],
     ),
-    "catopt_hip_sample_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32]),
+    "catopt_hip_sample_workspace_bytes": (_i64, [_i64, _i64, _i32]),
     "catopt_hip_sample": (
         _i32,
         [_i32, _i64, _i64, _p, _i64, _p, _p, _f64, _p, _i64, _p, _f64, _p, _f64, _p, _p, _p, _i64, _p, _i64, _p],

@@ -19,8 +19,7 @@ constexpr int CT = 512;
 template <typename T, int EPT>
 __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
   constexpr int W = RowReader<T>::W, P = EPT / W;
-  __shared__ uint64_t weights[kBins];
-  __shared__ uint32_t counts[kBins];
+  __shared__ uint64_t bins[kBins];
   __shared__ float maxima[CT / 64];
   __shared__ int firsts[CT / 64], nans[CT / 64];
   const int row = (int)(blockIdx.x / (uint32_t)a.chunks), chunk = (int)(blockIdx.x - (uint32_t)row * a.chunks);
@@ -31,9 +30,9 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
 #pragma unroll
   for (int j = 0; j < P; ++j) w[j] = r.load(piece0 + j * CT);
   const Settings s = settings(a, row);
-  const bool binned = s.valid && !s.greedy, counted = binned && s.k;
+  const bool binned = s.valid && !s.greedy;
   if (binned)
-    for (int i = tid; i < kBins; i += CT) weights[i] = 0, counts[i] = 0;
+    for (int i = tid; i < kBins; i += CT) bins[i] = 0;
   float m = -__builtin_inff();
   bool nan = false;
 #pragma unroll
@@ -74,26 +73,21 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
     *head = h;
   }
   if (!binned || m == -__builtin_inff()) return;
-  const double c = factor(s.t, m);
-  double rest;
-  const double ref = grid(m, c, rest);
+  const Grid g(s.t, m);
 #pragma unroll
   for (int j = 0; j < P; ++j)
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      const double d = ref - grid(finite_top(r.at(w[j], e)), c, rest);
-      if (d < kBins) {  // not so for -inf, nor where T is infinite and that a NaN
-        const int bin = (int)d;
-        atomicAdd(reinterpret_cast<unsigned long long*>(weights + bin), (unsigned long long)fixed(rest));
-        if (counted) atomicAdd(counts + bin, 1u);
-      }
+      const float x = finite_top(r.at(w[j], e));
+      const double on = g.on(x);
+      const uint64_t bin = g.below(on);
+      if (bin < kBins)
+        atomicAdd(reinterpret_cast<unsigned long long*>(bins + bin),
+                  (unsigned long long)(g.weight(g.rest(x, on)) | 1ull << kCount));
     }
   __syncthreads();
   const int64_t at = ((int64_t)row * a.chunks + chunk) * kBins;
-  for (int i = tid; i < kBins; i += CT) {
-    a.weights[at + i] = weights[i];
-    if (counted) a.counts[at + i] = counts[i];
-  }
+  for (int i = tid; i < kBins; i += CT) a.bins[at + i] = bins[i];
 }
 
 // ------------------------------------------------------------------ rows
@@ -104,8 +98,7 @@ constexpr int kParts = 256;   // of a range
 constexpr int kMaxChunks = 520;
 
 // What one step of a search adds up.  Three of them take turns: a step clears the
-// next one's, which was last read before the barrier that ended the step before,
-// so that a step is one barrier.
+// next one's, which was last read before the barriers of the step before.
 struct Step {
   uint64_t weight[kParts];
   uint64_t last[64];
@@ -117,8 +110,12 @@ struct RowLds {
   uint64_t cum[kBins];  // weights up to a bin's end, in units of 2^-42 of bin 0's
   uint64_t list[kList];
   Step steps[3];
+  struct {
+    uint64_t lo, sum;
+    uint32_t n_before, n;
+  } found[2];  // what the first wave has decided, in turn
   uint64_t wave_sums[WAVES];
-  uint32_t cum_n[kBins];  // logits up to it: exactly with a top-k, else at most
+  uint32_t cum_n[kBins];  // logits up to it
   uint32_t wave_counts[WAVES];
   int off[kMaxChunks];  // a chunk's first bin among the row's
 };
@@ -126,43 +123,46 @@ struct RowLds {
 // (min and max of the headers take 64-bit integers as doubles.)
 __device__ __forceinline__ uint64_t least_of(uint64_t a, uint64_t b) { return a < b ? a : b; }
 
-__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int lane) {
-  return (uint64_t)(uint32_t)__shfl((int)(v >> 32), lane, 64) << 32 | (uint32_t)__shfl((int)(uint32_t)v, lane, 64);
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {  // of a lane that is the same for the wave
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+  return __builtin_bit_cast(double, lane_u64(__builtin_bit_cast(uint64_t, v), lane));
+}
+// The value of the lane that a DPP control names, 0 where there is none (row_shr
+// by 1 to 8 within 16 lanes, then the ends of 16 and of 32 lanes to those behind).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t from_lane(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t from_lane(uint64_t v) {
+  return (uint64_t)from_lane<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | from_lane<CTRL, ROWS>((uint32_t)v);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lane(double v) {
+  return __builtin_bit_cast(double, from_lane<CTRL, ROWS>(__builtin_bit_cast(uint64_t, v)));
 }
 // Inclusive sums over the wave.
-__device__ __forceinline__ uint64_t scan_u64(uint64_t v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t u = shfl_u64(v, max(lane - o, 0));
-    if (lane >= o) v += u;
-  }
-  return v;
-}
-__device__ __forceinline__ uint32_t scan_u32(uint32_t v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
-  return v;
-}
-__device__ __forceinline__ double scan_f64(double v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {
+  v += from_lane<0x111, 0xf>(v);
+  v += from_lane<0x112, 0xf>(v);
+  v += from_lane<0x114, 0xf>(v);
+  v += from_lane<0x118, 0xf>(v);
+  v += from_lane<0x142, 0xa>(v);
+  v += from_lane<0x143, 0xc>(v);
   return v;
 }
 
 // The wave's places (~0 behind the last) in ascending order, lane by lane.
 __device__ __forceinline__ uint64_t sorted(uint64_t mine, int n) {
+  const int lane = threadIdx.x & 63;
   int rank = 0;
-  for (int j = 0; j < n; ++j) rank += shfl_u64(mine, j) < mine;
-  if ((int)(threadIdx.x & 63) >= n) rank = threadIdx.x & 63;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) rank += lane_u64(mine, j) < mine;
+  if (lane >= n) rank = lane;
   const uint32_t hi = __builtin_amdgcn_ds_permute(4 * rank, (int)(mine >> 32));
   const uint32_t lo = __builtin_amdgcn_ds_permute(4 * rank, (int)(uint32_t)mine);
   return (uint64_t)hi << 32 | lo;
@@ -175,8 +175,13 @@ __device__ __forceinline__ bool meets(Find f, double target, uint64_t sum, uint3
   return f == kRank ? (double)n > target : f == kReaches ? (double)sum >= target : (double)sum > target;
 }
 
-// Bin b's weight to bin 0's.
-__device__ __forceinline__ double scale_of(int b) { return exp2(-(double)b / 16); }
+// What a sum of bin b counts in units: 2^(-b / 16), a factor for each of the last
+// four bits.
+__device__ __forceinline__ double scale_of(int b) {
+  const double x = (b & 1 ? 0.9576032806985737 : 1.0) * (b & 2 ? 0.9170040432046712 : 1.0);
+  const double y = (b & 4 ? 0.8408964152537145 : 1.0) * (b & 8 ? 0.7071067811865476 : 1.0);
+  return ldexp(x * y, kUnits - kPoint - (b >> 4));
+}
 
 struct Bins {
   int first, last;
@@ -184,28 +189,31 @@ struct Bins {
 };
 constexpr Bins kNoBins{1, 0};
 
-// A row's search.  Every wave comes to the same decisions, from what is in LDS.
+// A row's search: all waves add up, the first one decides.
 template <typename T>
 struct Search {
   RowLds& s;
   const RowReader<T> r;
-  double c, ref;
+  const Grid g;
+  static constexpr int U = 4;  // pieces at a time
   int step = 0;
   uint32_t n_list = 0;
   Bins listed = kNoBins, listed2 = kNoBins;  // the list holds all their logits
 
   __device__ __forceinline__ int bin_of(float x, double& rest) const {
-    const double d = ref - grid(x, c, rest);
-    return d < kBins ? (int)d : kBins;
+    const double on = g.on(x);
+    rest = g.rest(x, on);
+    const uint64_t bin = g.below(on);
+    return bin < kBins ? (int)bin : kBins;
   }
 
-  // Numbers that no logit of bins up to b is below, or from b on above.
+  // Finite numbers that no logit of bins up to b is below, or from b on above.
   __device__ __forceinline__ float floor_of(int b) const {
-    const float f = (float)((ref - b - 0.5) / c);
-    return f - fabsf(f) * 0x1p-22f - 0x1p-140f;
+    const float f = (float)((g.ref - kGrid - b - 0.5) / g.c);
+    return fmaxf(f - fabsf(f) * 0x1p-22f - 0x1p-140f, -0x1.fffffep127f);
   }
   __device__ __forceinline__ float top_of(int b) const {
-    const float f = (float)((ref - b + 0.5) / c);
+    const float f = (float)((g.ref - kGrid - b + 0.5) / g.c);
     return f + fabsf(f) * 0x1p-22f + 0x1p-140f;
   }
 
@@ -216,58 +224,71 @@ struct Search {
     return s.steps[step++ % 3];
   }
 
-  // f(place, rest) for the row's logits in either of the bins.
+  // f(first piece, a bit for each logit of four pieces that may be in either of the
+  // bins), by whole waves.  Two comparisons a logit; a bin's neighbours' edges come
+  // along.
   template <typename F>
   __device__ __forceinline__ void scan_row(Bins a, Bins b, F f) const {
-    constexpr int U = 4;
-    // most logits fall out by two comparisons; the others' bins are worked out
-    const float lo = floor_of(a.last), hi = top_of(a.first), lo2 = floor_of(b.last), hi2 = top_of(b.first);
+    const float lo = floor_of(a.last), hi = top_of(a.first);
     const bool two = b.first <= b.last;
+    const float lo2 = two ? floor_of(b.last) : __builtin_inff(), hi2 = two ? top_of(b.first) : -__builtin_inff();
     const int n = r.pieces();
 #pragma unroll 1
-    for (int p0 = threadIdx.x; p0 < n; p0 += U * RT) {
+    for (int p0 = threadIdx.x; p0 - (int)(threadIdx.x & 63) < n; p0 += U * RT) {
       u32x4 w[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) w[j] = r.load(p0 + j * RT);
+      uint32_t some = 0;
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        uint32_t some = 0;
+      for (int j = 0; j < U; ++j)
 #pragma unroll
         for (int e = 0; e < RowReader<T>::W; ++e) {
           const float x = r.at(w[j], e);
-          some |= ((x >= lo && x <= hi) || (two && x >= lo2 && x <= hi2)) ? 1u << e : 0u;
+          some |= ((x >= lo && x <= hi) || (x >= lo2 && x <= hi2)) ? 1u << (j * RowReader<T>::W + e) : 0u;
         }
-        while (some) {
-          const int e = __builtin_ctz(some);
-          some &= some - 1;
-          float x = r.at(w[j], 0);
-#pragma unroll
-          for (int i = 1; i < RowReader<T>::W; ++i) x = i == e ? r.at(w[j], i) : x;
-          x = finite_top(x);
-          double rest;
-          const int bin = bin_of(x, rest);
-          if (a.has(bin) || b.has(bin)) f(place(x, r.first(p0 + j * RT) + e), rest);
-        }
-      }
+      if (__ballot(some != 0)) f(p0, some);
     }
   }
+  // The index of bit i, and the place of the logit with an index.
+  __device__ __forceinline__ int index_of(int p0, int i) const {
+    return r.first(p0 + i / RowReader<T>::W * RT) + i % RowReader<T>::W;
+  }
+  __device__ __forceinline__ uint64_t place_of(int i) const { return place(finite_top(r.value(i)), i); }
 
-  // The logits of a range of places of those bins into the list, as far as it
-  // holds them; their number.
-  __device__ __forceinline__ uint32_t gather(Bins a, Bins b, uint64_t lo, uint64_t hi) {
+  // f(place, rest) for the row's logits in a bin.
+  template <typename F>
+  __device__ __forceinline__ void each_in_row(int b, F f) const {
+    scan_row(Bins{b, b}, kNoBins, [&](int p0, uint32_t some) {
+      for (; some; some &= some - 1) {
+        const uint64_t at = place_of(index_of(p0, __builtin_ctz(some)));
+        double rest;
+        if (bin_of(logit_of(at), rest) == b) f(at, rest);
+      }
+    });
+  }
+
+  // The logits that may be in those bins into the list, as far as it holds them;
+  // their number.  The indexes come first, by a sum over each wave, then the places.
+  __device__ __forceinline__ uint32_t gather(Bins a, Bins b) {
     Step& t = begin();
-    scan_row(a, b, [&](uint64_t at, double) {
-      if (at < lo || at > hi) return;
-      const uint32_t i = atomicAdd(&t.count, 1u);
-      if (i < kList) s.list[i] = at;
+    scan_row(a, b, [&](int p0, uint32_t some) {
+      const uint32_t mine = __builtin_popcount(some), upto = wave_scan(mine);
+      uint32_t base = 0;
+      if ((threadIdx.x & 63) == 63) base = atomicAdd(&t.count, upto);
+      uint32_t i = (uint32_t)__builtin_amdgcn_readlane((int)base, 63) + upto - mine;
+      for (; some; some &= some - 1, ++i)
+        if (i < kList) s.list[i] = (uint32_t)index_of(p0, __builtin_ctz(some));
     });
     __syncthreads();
-    return t.count;
+    const uint32_t n = t.count;
+    for (uint32_t i = threadIdx.x; i < n && i < kList; i += RT) s.list[i] = place_of((int)(uint32_t)s.list[i]);
+    __syncthreads();
+    return n;
   }
 
   // The same to be searched in afterwards, if it holds them.
   __device__ __forceinline__ void list_bins(Bins a, Bins b) {
-    n_list = gather(a, b, 0, ~0ull);
+    n_list = gather(a, b);
     const bool all = n_list <= kList;
     listed = all ? a : kNoBins, listed2 = all ? b : kNoBins;
   }
@@ -285,15 +306,15 @@ struct Search {
   // bin): its place and the sum up to it; the last one where none does.
   __device__ __forceinline__ uint64_t resolve(int b, Find find, double target, uint64_t& sum) {
     const int lane = threadIdx.x & 63;
-    const Bins one{b, b};
     uint64_t lo = place(top_of(b), 0), hi = place(floor_of(b), -1), before = 0;
     uint32_t n_before = 0, n = s.cum_n[b] - (b ? s.cum_n[b - 1] : 0);
-    bool list = listed.has(b) || listed2.has(b), own = false;  // own: the list is this call's, and holds the range alone
+    bool list = listed.has(b) || listed2.has(b), own = false;  // own: the list is this call's
+    bool narrowed = false;  // more logits than the list holds: the row is read for each step
     for (;;) {
-      if (!list && n <= kList) {
+      if (!list && n <= kList && !narrowed) {
         listed = listed2 = kNoBins;
-        n = n_list = gather(one, kNoBins, lo, hi);
-        list = own = true;
+        n = n_list = gather(Bins{b, b}, kNoBins);
+        list = own = n <= kList;  // not so where the neighbours' edges were too many
       }
       // one key alone: its indexes end with the row
       if (lo >> 32 == hi >> 32) hi = least_of(hi, (hi & ~0xffffffffull) | (uint32_t)(r.V - 1));
@@ -306,7 +327,7 @@ struct Search {
           t.last[atomicAdd(&t.count, 1u) & 63] = at;
         } else {
           const int i = (int)((at - lo) >> shift);
-          atomicAdd(reinterpret_cast<unsigned long long*>(t.weight + i), (unsigned long long)fixed(rest));
+          atomicAdd(reinterpret_cast<unsigned long long*>(t.weight + i), (unsigned long long)g.weight(rest));
           atomicAdd(t.n + i, 1u);
         }
       };
@@ -318,47 +339,56 @@ struct Search {
           if (bin_of(logit_of(at), rest) == b) take(at, rest);
         }
       } else {
-        scan_row(one, kNoBins, take);
+        each_in_row(b, take);
       }
       __syncthreads();
-      if (few) {  // a wave puts them in order
+      auto& found = s.found[step & 1];
+      if (threadIdx.x < 64 && few) {  // in order
         const int m = min((int)t.count, 64);
         const uint64_t at = sorted(lane < m ? t.last[lane] : ~0ull, m);
         double rest;
         bin_of(logit_of(at), rest);
-        const uint64_t upto = scan_u64(lane < m ? fixed(rest) : 0) + before;
+        const uint64_t upto = wave_scan(lane < m ? g.weight(rest) : 0) + before;
         const uint64_t some = __ballot(lane < m && meets(find, target, upto, n_before + lane + 1));
         const int from = some ? __builtin_ctzll(some) : max(m - 1, 0);
-        sum = shfl_u64(upto, from);
-        if (own) listed = listed2 = kNoBins;
-        return shfl_u64(at, from);
+        if (lane == from) found.lo = at, found.sum = upto;
       }
-      // four parts a lane: the part that the logit is in, the last that holds one where none meets the target
-      uint64_t w[4], all = 0;
-      uint32_t k[4], all_n = 0;
+      if (threadIdx.x < 64 && !few) {
+        // four parts a lane: the part that the logit is in, the last that holds one where none meets the target
+        uint64_t w[4], all = 0;
+        uint32_t k[4], all_n = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = t.weight[4 * lane + i], k[i] = t.n[4 * lane + i];
-        all += w[i], all_n += k[i];
-      }
-      uint64_t upto = scan_u64(all) - all + before, at_sum = 0;
-      uint32_t upto_n = scan_u32(all_n) - all_n + n_before, at_n = 0, here = 0;
-      int at = -1;
-      bool met = false;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (k[i] && !met) {
-          at = 4 * lane + i, at_sum = upto, at_n = upto_n, here = k[i];
-          met = meets(find, target, upto + w[i], upto_n + k[i]);
+        for (int i = 0; i < 4; ++i) {
+          w[i] = t.weight[4 * lane + i], k[i] = t.n[4 * lane + i];
+          all += w[i], all_n += k[i];
         }
-        upto += w[i], upto_n += k[i];
+        uint64_t upto = wave_scan(all) - all + before, at_sum = 0;
+        uint32_t upto_n = wave_scan(all_n) - all_n + n_before, at_n = 0, here = 0;
+        int at = -1;
+        bool met = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (k[i] && !met) {
+            at = 4 * lane + i, at_sum = upto, at_n = upto_n, here = k[i];
+            met = meets(find, target, upto + w[i], upto_n + k[i]);
+          }
+          upto += w[i], upto_n += k[i];
+        }
+        const uint64_t some = __ballot(met), held = __ballot(at >= 0);
+        if (lane == (some ? __builtin_ctzll(some) : 63 - __builtin_clzll(held | 1))) {
+          found.lo = lo + ((uint64_t)max(at, 0) << shift);
+          found.sum = at_sum, found.n_before = at_n, found.n = here;
+        }
       }
-      const uint64_t some = __ballot(met), held = __ballot(at >= 0);
-      const int from = some ? __builtin_ctzll(some) : 63 - __builtin_clzll(held | 1);
-      const int part = max(__shfl(at, from, 64), 0);
-      lo += (uint64_t)part << shift;
+      __syncthreads();
+      if (few) {
+        if (own) listed = listed2 = kNoBins;
+        sum = found.sum;
+        return found.lo;
+      }
+      narrowed = true;
+      lo = found.lo, before = found.sum, n_before = found.n_before, n = found.n;
       hi = least_of(hi, lo + ((1ull << shift) - 1));
-      before = shfl_u64(at_sum, from), n_before = __shfl(at_n, from, 64), n = __shfl(here, from, 64);
     }
   }
 };
@@ -394,40 +424,34 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     }
     return;
   }
-  const double c = factor(set.t, m);
   double rest;
-  const double ref = grid(m, c, rest);
-  Search<T> find{s, RowReader<T>(a, row), c, ref};
+  Search<T> find{s, RowReader<T>(a, row), Grid(set.t, m)};
+  const double c = find.g.c, ref = find.g.ref;
   // ---- the row's bins from the chunks'
   for (int i = tid; i < a.chunks; i += RT) {
     const float cm = heads[i].max;
     // by the row's factor: it is the chunk's too wherever the chunk has a bin of the row's
-    const double d = cm == -__builtin_inff() ? kBins : ref - grid(cm, c, rest);
-    s.off[i] = d < kBins ? max((int)d, 0) : kBins;
+    s.off[i] = find.bin_of(cm, rest);
   }
   if (tid < kParts) s.steps[0].weight[tid] = 0, s.steps[0].n[tid] = 0;
   if (tid == 0) s.steps[0].count = 0;
   __syncthreads();
-  const bool counted = set.k != 0;
   uint64_t w = 0;
   uint32_t n = 0;
   if (tid < kBins) {
-    const uint64_t* ws = a.weights + (int64_t)row * a.chunks * kBins + tid;
-    const uint32_t* ns = a.counts + (int64_t)row * a.chunks * kBins + tid;
+    const uint64_t* bins = a.bins + (int64_t)row * a.chunks * kBins + tid;
 #pragma unroll 4
     for (int i = 0; i < a.chunks; ++i) {
       const int o = s.off[i];
-      const bool in = tid >= o;
-      w += in ? ws[(int64_t)i * kBins - o] : 0;
-      if (counted) n += in ? ns[(int64_t)i * kBins - o] : 0;
+      const uint64_t v = tid >= o ? bins[(int64_t)i * kBins - o] : 0;
+      w += v & ((1ull << kCount) - 1);
+      n += (uint32_t)(v >> kCount);
     }
-    // a logit weighs at least 0.978 in its bin
-    if (!counted) n = (uint32_t)((double)w * (1.0 / (0.978 * (1LL << kPoint)))) + (w != 0);
     w = (uint64_t)rint((double)w * scale_of(tid));
   }
   {
-    const uint64_t sw = scan_u64(w);
-    const uint32_t sn = scan_u32(n);
+    const uint64_t sw = wave_scan(w);
+    const uint32_t sn = wave_scan(n);
     if (lane == 63) s.wave_sums[wave] = sw, s.wave_counts[wave] = sn;
     __syncthreads();
     uint64_t bw = 0;
@@ -441,12 +465,13 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   const double u = fmin(fmax((double)u_row, 0.0), 1 - 0x1p-25);
   int cut = kBins - 1;
   uint64_t cut_at = ~0ull, total = s.cum[kBins - 1];
-  bool by_rank = counted && s.cum_n[kBins - 1] > set.k, by_sum = set.p < 1, by_low = set.low > 0;
+  bool by_rank = set.k && s.cum_n[kBins - 1] > set.k, by_sum = set.p < 1, by_low = set.low > 0;
   const double low = by_low ? (double)m * c + 16 * log2(fmin(set.low, 1.0)) : -__builtin_inf();
-  const double low_bin = by_low ? ref - rint(low) : kBins;
+  const double low_bin = by_low ? ref - kGrid - rint(low) : kBins;
   auto before = [&](int b) { return b > 0 ? s.cum[b - 1] : 0ull; };
   auto before_n = [&](int b) { return b > 0 ? s.cum_n[b - 1] : 0u; };
   auto within = [&](int b, uint64_t sum) { return before(b) + (uint64_t)rint((double)sum * scale_of(b)); };
+  Bins list = kNoBins, list2 = kNoBins;
   if (by_rank || by_sum || by_low) {
     if (by_rank) cut = find.find_bin(kRank, (double)(set.k - 1));
     int end = by_rank || !by_sum ? cut : find.find_bin(kReaches, set.p * (double)total);
@@ -454,88 +479,92 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     by_low = low_bin <= end;
     if (low_bin < end && !(by_rank && by_sum)) by_rank = by_sum = false, end = (int)low_bin;
     if (s.cum_n[end] <= kList) {
-      find.list_bins({0, end}, kNoBins);
-      if (find.n_list <= 64) {
-        // all that may be kept is in one wave: the definition, lane by lane
-        const int n_all = (int)find.n_list;
-        const uint64_t at = sorted(lane < n_all ? s.list[lane] : ~0ull, n_all);
-        const int bin = find.bin_of(logit_of(at), rest);
-        const double sums = scan_f64(lane < n_all ? (double)fixed(rest) * scale_of(bin) : 0);
-        const double whole = by_rank ? __shfl(sums, (int)set.k - 1, 64) : (double)total;
-        bool kept = lane < (by_rank ? (int)set.k : n_all);
-        if (by_sum) {
-          const uint64_t reach = __ballot(kept && sums >= set.p * whole);
-          if (reach) kept = lane <= __builtin_ctzll(reach);
-        }
-        if (by_low) kept = kept && (double)logit_of(at) * c >= low;
-        const int last = 63 - __builtin_clzll(__ballot(kept) | 1);
-        const double kept_sum = __shfl(sums, last, 64);
-        const uint64_t pass = __ballot(lane <= last && sums > u * kept_sum);
-        const int from = pass ? __builtin_ctzll(pass) : last;
-        const double log2_total = log2(kept_sum) - kPoint;
-        if (wave == 0 && lane == from) {
-          a.tokens[row] = (int64_t)(uint32_t)at;
-          a.logprobs[row] = (float)(((rest - bin) / 16 - log2_total) * 0.6931471805599453);
-        }
-        if (wave == 0 && lane == last && a.rows) a.rows[row] = RowState{c, ref, low, log2_total, at, bin, 0};
-        return;
-      }
+      list = Bins{0, end};
     } else if (!by_rank) {
       // the border lies in bin `end`, the token where u says for a whole between the sums before and behind it: both
       // are read at once if they fit
       const Bins pick{find.find_bin(kPasses, u * (double)before(end)), min(find.find_bin(kPasses, u * (double)s.cum[end]), end - 1)};
       const uint32_t here = s.cum_n[end] - before_n(end);
       const uint32_t there = pick.first <= pick.last ? s.cum_n[pick.last] - before_n(pick.first) : 0;
-      if (here + there <= kList) find.list_bins({end, end}, pick);
+      if (here + there <= kList) list = Bins{end, end}, list2 = pick;
     }
-    uint64_t sum;
-    if (by_rank) {
-      if (s.cum_n[cut] == set.k) {
-        total = s.cum[cut];
-      } else {
-        cut_at = find.resolve(cut, kRank, (double)(set.k - 1 - before_n(cut)), sum);
-        total = within(cut, sum);
+    if (list.has(end)) find.list_bins(list, list2);
+    if (find.listed.first == 0 && find.n_list <= 64) {
+      // all that may be kept is in one wave: the definition, lane by lane
+      if (wave > 0) return;
+      const uint64_t at = sorted(lane < (int)find.n_list ? s.list[lane] : ~0ull, (int)find.n_list);
+      const int bin = find.bin_of(logit_of(at), rest);
+      const int n_all = __builtin_popcountll(__ballot(lane < (int)find.n_list && bin <= end));
+      const double sums = wave_scan(lane < n_all ? (double)find.g.weight(rest) * scale_of(bin) : 0);
+      const double whole = by_rank ? lane_f64(sums, (int)set.k - 1) : (double)total;
+      bool kept = lane < (by_rank ? (int)set.k : n_all);
+      if (by_sum) {
+        const uint64_t reach = __ballot(kept && sums >= set.p * whole);
+        if (reach) kept = lane <= __builtin_ctzll(reach);
       }
-    }
-    if (by_sum) {
-      const double target = set.p * (double)total;
-      const int b = min(find.find_bin(kReaches, target), cut);
-      const uint64_t at = find.resolve(b, kReaches, (target - (double)before(b)) / scale_of(b), sum);
-      if (b < cut || at < cut_at) cut = b, cut_at = at, total = within(b, sum);
-    }
-    if (by_low && low_bin <= cut) {
-      // of the border's bin those whose y is not below it
-      const int b = (int)low_bin;
-      if (!find.listed.has(b)) find.list_bins({b, b}, kNoBins);
-      Step& t = find.begin();
-      uint64_t mine = 0;
-      auto take = [&](float x, uint64_t at, double rs) {
-        if ((double)x * c >= low && (b < cut || at <= cut_at)) mine += fixed(rs);
-      };
-      if (find.listed.has(b)) {
-        for (uint32_t i = tid; i < find.n_list; i += RT) {
-          const float x = logit_of(s.list[i]);
-          if (find.bin_of(x, rest) == b) take(x, s.list[i], rest);
-        }
-      } else {
-        find.scan_row({b, b}, kNoBins, [&](uint64_t at, double rs) { take(logit_of(at), at, rs); });
+      if (by_low) kept = kept && (double)logit_of(at) * c >= low;
+      const int last = 63 - __builtin_clzll(__ballot(kept) | 1);
+      const double kept_sum = lane_f64(sums, last);
+      const uint64_t pass = __ballot(lane <= last && sums > u * kept_sum);
+      const int from = pass ? __builtin_ctzll(pass) : last;
+      const double log2_total = log2(kept_sum) - kUnits;
+      if (lane == from) {
+        a.tokens[row] = (int64_t)(uint32_t)at;
+        a.logprobs[row] = (float)(((rest - bin) / 16 - log2_total) * 0.6931471805599453);
       }
-      if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(t.weight), (unsigned long long)mine);
-      __syncthreads();
-      total = least_of(total, within(b, t.weight[0]));
-      if (b < cut) cut = b, cut_at = ~0ull;
+      if (lane == last && a.rows) a.rows[row] = RowState{c, ref, low, log2_total, at, bin, 0};
+      return;
     }
   }
-  // ---- the token
-  const double target = u * (double)total;
-  const int b = min(find.find_bin(kPasses, target), cut);
-  uint64_t sum, at = find.resolve(b, kPasses, (target - (double)before(b)) / scale_of(b), sum);
-  if (b == cut && at > cut_at) at = cut_at;
+  uint64_t at = 0;
+#pragma unroll 1
+  for (int look = 0; look < 3; ++look) {  // for top-k's border, for top-p's, for the token
+    Find by = kRank;
+    double target = 0;
+    int b = cut;
+    if (look == 0) {
+      if (!by_rank) continue;
+      if (s.cum_n[cut] == set.k) {
+        total = s.cum[cut];
+        continue;
+      }
+      target = (double)(set.k - 1 - before_n(cut));
+    } else {
+      if (look == 1 && !by_sum) continue;
+      if (look == 2 && by_low && low_bin <= cut) {
+        // of the border's bin those whose y is not below it
+        b = (int)low_bin;
+        Step& t = find.begin();
+        uint64_t mine = 0;
+        auto take = [&](uint64_t place, double rs) {
+          if ((double)logit_of(place) * c >= low && (b < cut || place <= cut_at)) mine += find.g.weight(rs);
+        };
+        if (find.listed.has(b)) {
+          for (uint32_t i = tid; i < find.n_list; i += RT)
+            if (find.bin_of(logit_of(s.list[i]), rest) == b) take(s.list[i], rest);
+        } else {
+          find.each_in_row(b, take);
+        }
+        if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(t.weight), (unsigned long long)mine);
+        __syncthreads();
+        total = least_of(total, within(b, t.weight[0]));
+        if (b < cut) cut = b, cut_at = ~0ull;
+      }
+      by = look == 1 ? kReaches : kPasses;
+      target = (look == 1 ? set.p : u) * (double)total;
+      b = min(find.find_bin(by, target), cut);
+      target = (target - (double)before(b)) / scale_of(b);
+    }
+    uint64_t sum;
+    at = find.resolve(b, by, target, sum);
+    if (look == 0 || (look == 1 && (b < cut || at < cut_at))) cut = b, cut_at = at, total = within(b, sum);
+    if (look == 2 && b == cut && at > cut_at) at = cut_at;
+  }
   if (tid == 0) {
-    const double log2_total = log2((double)total) - kPoint;
-    const double n_at = grid(logit_of(at), c, rest);
+    const double log2_total = log2((double)total) - kUnits;
+    const int bin = find.bin_of(logit_of(at), rest);
     a.tokens[row] = (int64_t)(uint32_t)at;
-    a.logprobs[row] = (float)((((n_at - ref) + rest) / 16 - log2_total) * 0.6931471805599453);
+    a.logprobs[row] = (float)(((rest - bin) / 16 - log2_total) * 0.6931471805599453);
     if (a.rows) a.rows[row] = RowState{c, ref, low, log2_total, cut_at, cut, 0};
   }
 }
@@ -549,6 +578,7 @@ __global__ __launch_bounds__(PT) void sample_probs(SampleArgs a, int blocks) {
   const int row = (int)(blockIdx.x / (uint32_t)blocks), block = (int)(blockIdx.x - (uint32_t)row * blocks);
   const RowReader<T> r(a, row);
   const RowState s = a.rows[row];
+  const Grid g(s.c, s.ref);
   float* out = a.probs + (int64_t)row * a.ld_probs;
 #pragma unroll
   for (int j = 0; j < PIECES; ++j) {
@@ -558,12 +588,12 @@ __global__ __launch_bounds__(PT) void sample_probs(SampleArgs a, int blocks) {
 #pragma unroll
     for (int e = 0; e < RowReader<T>::W; ++e) {
       const float x = finite_top(r.at(w, e));
-      double rest;
-      const double n = grid(x, s.c, rest), d = s.ref - n;
+      const double on = g.on(x);
+      const uint64_t bin = g.below(on);
       p[e] = 0.f;
-      if (s.cut >= 0 && d <= s.cut && (double)x * s.c >= s.low && (d < s.cut || place(x, i0 + e) <= s.cut_at)) {
+      if (s.cut >= 0 && bin <= (uint64_t)s.cut && (double)x * s.c >= s.low && (bin < (uint64_t)s.cut || place(x, i0 + e) <= s.cut_at)) {
         // 2^whole 2^part: the exponential sees a small number
-        const double y = (rest - d) / 16 - s.log2_total, whole = rint(y);
+        const double y = (g.rest(x, on) - (double)(int)bin) / 16 - s.log2_total, whole = rint(y);
         p[e] = ldexpf(__builtin_amdgcn_exp2f((float)(y - whole)), (int)whole);
       }
       if (s.cut == kOneHot) p[e] = i0 + e == s.token ? 1.f : 0.f;
@@ -580,17 +610,16 @@ __global__ __launch_bounds__(PT) void sample_probs(SampleArgs a, int blocks) {
 // Chunks of 16384 logits where they fill the CUs, else of 4096.
 struct Plan {
   int64_t chunk, chunks;
-  int64_t heads, weights, counts, rows;  // bytes
-  int64_t bytes() const { return heads + weights + counts + rows; }
+  int64_t heads, bins, rows;  // bytes
+  int64_t bytes() const { return heads + bins + rows; }
 };
 
-Plan plan_of(int64_t B, int64_t V, bool counted, bool probs) {
+Plan plan_of(int64_t B, int64_t V, bool probs) {
   Plan p;
-  p.chunk = B * ((V + 16383) / 16384) >= 1024 ? 16384 : 4096;
+  p.chunk = B * ((V + kMaxChunk - 1) / kMaxChunk) >= 1024 ? kMaxChunk : 4096;
   p.chunks = (V + 7 + p.chunk - 1) / p.chunk;  // 7: a row may begin inside its first piece
   p.heads = B * p.chunks * (int64_t)sizeof(ChunkHead);
-  p.weights = B * p.chunks * kBins * 8;
-  p.counts = counted ? B * p.chunks * kBins * 4 : 0;
+  p.bins = B * p.chunks * kBins * 8;
   p.rows = probs ? B * (int64_t)sizeof(RowState) : 0;
   return p;
 }
@@ -598,8 +627,8 @@ Plan plan_of(int64_t B, int64_t V, bool counted, bool probs) {
 template <typename T>
 int32_t launch(const SampleArgs& a, const Plan& p, hipStream_t st) {
   const dim3 grid((uint32_t)(a.B * p.chunks));
-  if (p.chunk == 16384)
-    sample_chunks<T, 32><<<grid, dim3(CT), 0, st>>>(a);
+  if (p.chunk == kMaxChunk)
+    sample_chunks<T, kMaxChunk / CT><<<grid, dim3(CT), 0, st>>>(a);
   else
     sample_chunks<T, 8><<<grid, dim3(CT), 0, st>>>(a);
   CATOPT_LAUNCH_CHECK();
@@ -627,10 +656,10 @@ bool overlaps(const void* p, int64_t n, const void* q, int64_t m) {
 
 using namespace catopt;
 
-extern "C" int64_t catopt_hip_sample_workspace_bytes(int64_t B, int64_t V, int32_t counted, int32_t probs) {
+extern "C" int64_t catopt_hip_sample_workspace_bytes(int64_t B, int64_t V, int32_t probs) {
   if (B < 0 || V < 1 || V > kMaxVocab || B > (1 << 20)) return -1;
   if (B * V >= (1LL << 36)) return -1;
-  return plan_of(B, V, counted != 0, probs != 0).bytes();
+  return plan_of(B, V, probs != 0).bytes();
 }
 
 extern "C" int32_t catopt_hip_sample(int32_t dtype, int64_t B, int64_t V, const void* logits, int64_t ld, const float* u,
@@ -640,8 +669,7 @@ extern "C" int32_t catopt_hip_sample(int32_t dtype, int64_t B, int64_t V, const 
                                      void* workspace, int64_t workspace_bytes, void* stream) {
   if (B < 0 || V < 1) return CATOPT_E_INVAL;
   if (dtype != CATOPT_F32 && dtype != CATOPT_BF16) return CATOPT_E_UNSUPPORTED;
-  const bool counted = top_k || top_k_all > 1;
-  const int64_t need = catopt_hip_sample_workspace_bytes(B, V, counted, probs != nullptr);
+  const int64_t need = catopt_hip_sample_workspace_bytes(B, V, probs != nullptr);
   if (need < 0) return CATOPT_E_UNSUPPORTED;
   if (B == 0) return CATOPT_OK;
   if (!logits || !u || !tokens || !logprobs || ld < 0 || (B > 1 && ld_probs < V && probs)) return CATOPT_E_INVAL;
@@ -659,7 +687,7 @@ extern "C" int32_t catopt_hip_sample(int32_t dtype, int64_t B, int64_t V, const 
       if (overlaps(out[i].p, out[i].n, x.p, x.n)) return CATOPT_E_INVAL;
   }
   if (!workspace || workspace_bytes < need || !aligned16(workspace)) return CATOPT_E_WORKSPACE;
-  const Plan p = plan_of(B, V, counted, probs != nullptr);
+  const Plan p = plan_of(B, V, probs != nullptr);
   if (!grid_fits(B * p.chunks, CT) || !grid_fits(B, RT) || !grid_fits(B * ((V + 4095) / 4096 + 1), PT)) return CATOPT_E_UNSUPPORTED;
   SampleArgs a{};
   a.x = logits, a.ld = B > 1 ? ld : 0, a.ld_probs = B > 1 ? ld_probs : 0, a.V = (int)V, a.B = (int)B, a.chunks = (int)p.chunks;
@@ -669,11 +697,9 @@ extern "C" int32_t catopt_hip_sample(int32_t dtype, int64_t B, int64_t V, const 
   char* ws = static_cast<char*>(workspace);
   a.rows = probs ? reinterpret_cast<RowState*>(ws) : nullptr;
   ws += p.rows;
-  a.weights = reinterpret_cast<uint64_t*>(ws);
-  ws += p.weights;
+  a.bins = reinterpret_cast<uint64_t*>(ws);
+  ws += p.bins;
   a.heads = reinterpret_cast<ChunkHead*>(ws);
-  ws += p.heads;
-  a.counts = reinterpret_cast<uint32_t*>(ws);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return dtype == CATOPT_F32 ? launch<float>(a, p, st) : launch<uint16_t>(a, p, st);
 }

@@ -8,12 +8,19 @@ namespace catopt {
 // Weights exp((x - max) / T) lie on a grid of 16 steps to a factor of 2: with y =
 // x 16 log2(e) / T and n = rint(y), a logit belongs to the bin n and weighs
 // 2^(n / 16) 2^((y - n) / 16).  The second factor, between 0.978 and 1.022, is
-// rounded to 42 bits behind the point: a bin's weight is then a sum of integers,
-// the same in every order, whichever chunk of the row a logit lies in.  A bin 768
-// steps below the largest logit's weighs 2^-48 of it or less and counts as nothing.
+// rounded to 34 bits behind the point: a bin's weight is then a sum of integers,
+// the same in every order, whichever chunk of the row a logit lies in.  What a
+// choice can be off by is what such sums are off by, 2^-35 of a weight at random
+// and 2^-38 with one sign: a step of u is 2^-24.  A bin 768 steps below the largest
+// logit's weighs 2^-48 of it or less and counts as nothing.
+//
+// A chunk's bin holds the sum below bit 49 and the number of logits above.
 constexpr int kBins = 768;
-constexpr int kPoint = 42;
-constexpr int64_t kMaxVocab = 1LL << 21;  // a bin's sum stays below 2^(21 + 42.04)
+constexpr int kPoint = 34, kCount = 49;
+constexpr int kMaxChunk = 1 << 14;        // its sum stays below 2^(14 + 34.04), its number fits 15 bits
+constexpr int64_t kMaxVocab = 1LL << 21;
+// Sums over bins are in units of 2^-42 of bin 0's weight: below 2^(21 + 42.04).
+constexpr int kUnits = 42;
 
 struct SampleArgs {
   const void* x;
@@ -28,8 +35,7 @@ struct SampleArgs {
   int64_t* tokens;
   float *logprobs, *probs;
   struct ChunkHead* heads;  // [B][chunks]
-  uint64_t* weights;        // [B][chunks][kBins]
-  uint32_t* counts;         // the same, of rows with a top-k
+  uint64_t* bins;           // [B][chunks][kBins]
   struct RowState* rows;    // [B], for the probabilities
 };
 
@@ -41,7 +47,7 @@ struct ChunkHead {
 
 // What the probabilities of a row are worked out from.
 struct RowState {
-  double c, ref, low, log2_total;  // y = c x; the largest logit's n; the least y; log2 of the kept weights
+  double c, ref, low, log2_total;  // y = c x; the largest logit's n on the grid; the least y; log2 of the kept weights
   uint64_t cut_at;                 // in the cut's bin the last place that is kept
   int32_t cut, token;              // the last bin that is kept (some of it); kOneHot, kNone: the token alone, NaN
 };
@@ -66,31 +72,46 @@ __device__ __forceinline__ Settings settings(const SampleArgs& a, int row) {
 }
 
 // y's factor: at most 2^40 for the largest logit, where all that is not equal to it
-// lies far behind the last bin, so that n is exact.
+// lies far behind the last bin, so that n is exact; above 0 for -inf to stay -inf.
 __device__ __forceinline__ double factor(double t, float max) {
-  return fmin(16 * 1.4426950408889634 / t, 0x1p40 / fmax(fabs((double)max), 0x1p-120));
+  return fmax(fmin(16 * 1.4426950408889634 / t, 0x1p40 / fmax(fabs((double)max), 0x1p-120)), 0x1p-160);
 }
 
-// A logit's n; and its place in the bin, y - n.
-__device__ __forceinline__ double grid(float x, double c, double& rest) {
-  const double magic = 0x1.8p52;
-  const double n = __builtin_fma((double)x, c, magic) - magic;
-  rest = __builtin_fma((double)x, c, -n);
-  return n;
-}
+// y rounded to a whole number n, on top of 1.5 2^52: that number's low bits are n,
+// and two such numbers' bits as far apart as their n are.
+constexpr double kGrid = 0x1.8p52;
+__device__ __forceinline__ uint64_t bits_of(double v) { return __builtin_bit_cast(uint64_t, v); }
 
-// 2^(rest / 16) in fixed point, |rest| <= 1/2: the series to the fifth power, off by
-// less than 1.5e-13, with the sum's last addend 2^52 making the mantissa an integer.
-__device__ __forceinline__ uint64_t fixed(double rest) {
-  constexpr double l = 0.6931471805599453 / 16, one = 1LL << kPoint;
-  double s = one * (l * l * l * l * l / 120);
-  s = __builtin_fma(s, rest, one * (l * l * l * l / 24));
-  s = __builtin_fma(s, rest, one * (l * l * l / 6));
-  s = __builtin_fma(s, rest, one * (l * l / 2));
-  s = __builtin_fma(s, rest, one * l);
-  s = __builtin_fma(s, rest, one + 0x1p52);
-  return __builtin_bit_cast(uint64_t, s) & 0xfffffffffffffull;
-}
+// A row's grid.  The constants of a logit's weight stay in scalar registers: left to
+// itself the compiler sets them anew for every logit of an unrolled loop, a third of
+// its instructions.
+struct Grid {
+  double c, ref;  // y's factor, the largest logit's n on the grid
+  double shift = kGrid, back = -kGrid, s4, s3, s2, s1, s0;
+
+  __device__ __forceinline__ Grid(double t, float max) : Grid(factor(t, max), 0.0) { ref = on(max); }
+  __device__ __forceinline__ Grid(double c_, double ref_) : c(c_), ref(ref_) {
+    constexpr double one = 1LL << kPoint;
+    s4 = one * 1.4676443279006634e-07, s3 = one * 1.3551205157586767e-05, s2 = one * 0.0009383847924891109;
+    s1 = one * 0.04332169876016021, s0 = one * 1.0000000000000044 + 0x1p52;
+    asm("" : "+s"(shift), "+s"(back), "+s"(s4), "+s"(s3), "+s"(s2), "+s"(s1), "+s"(s0));
+  }
+  __device__ __forceinline__ double on(float x) const { return __builtin_fma((double)x, c, shift); }
+  // Bins from the largest logit's down to the one `on`, as far as they go.
+  __device__ __forceinline__ uint64_t below(double on) const { return bits_of(ref) - bits_of(on); }
+  // y - n.
+  __device__ __forceinline__ double rest(float x, double on) const { return __builtin_fma((double)x, c, -(on + back)); }
+  // 2^(rest / 16) in fixed point, |rest| <= 1/2: the polynomial of the fourth power
+  // that Chebyshev's expansion gives, off by 2^-38.5 of it at most (one of the third
+  // by 2^-29.7), with 2^52 in the sum's last addend making the mantissa an integer.
+  __device__ __forceinline__ uint64_t weight(double rest) const {
+    double s = __builtin_fma(s4, rest, s3);
+    s = __builtin_fma(s, rest, s2);
+    s = __builtin_fma(s, rest, s1);
+    s = __builtin_fma(s, rest, s0);
+    return bits_of(s) & 0xfffffffffffffull;  // below 2^35
+  }
+};
 
 // The order of a row, as ascending numbers: the largest logit first, the lowest
 // index first among equals (-0 as 0).
@@ -135,6 +156,7 @@ struct RowReader {
     }
     return w;
   }
+  __device__ __forceinline__ float value(int i) const { return load_f32(row, i); }
   // Logit e of a piece.
   static __device__ __forceinline__ float at(const u32x4& w, int e) {
     const uint32_t word = sizeof(T) == 4 ? w[e] : w[e / 2];
@@ -142,7 +164,11 @@ struct RowReader {
   }
 };
 
-// +inf as the largest finite number.
-__device__ __forceinline__ float finite_top(float x) { return __builtin_fminf(x, 0x1.fffffep127f); }
+// +inf as the largest finite number (one instruction: fminf makes NaNs quiet first).
+__device__ __forceinline__ float finite_top(float x) {
+  float y;
+  asm("v_min_f32 %0, %1, %2" : "=v"(y) : "s"(0x1.fffffep127f), "v"(x));
+  return y;
+}
 
 }  // namespace catopt

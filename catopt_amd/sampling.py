@@ -23,8 +23,8 @@ SAMPLE_MAX_VOCAB = 1 << 21
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace(B: int, V: int, counted: bool, probs: bool) -> int:
-    n = L.load().catopt_hip_sample_workspace_bytes(B, V, counted, probs)
+def _workspace(B: int, V: int, probs: bool) -> int:
+    n = L.load().catopt_hip_sample_workspace_bytes(B, V, probs)
     if n < 0:
         raise NotImplementedError(f"sample takes vocabularies of up to {SAMPLE_MAX_VOCAB}, got {B} rows of {V}")
     return n
@@ -69,9 +69,9 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: float | to
     NaN, with nothing above ``-inf`` or with a temperature that is negative or
     NaN gives token -1 and NaN.
 
-    Weights are in 64 bits, each off by 2^-42 of itself at most, and added up as
-    integers, so the outcome does not depend on the run; those below 2^-42 of the
-    largest count as nothing."""
+    Weights are in fixed point, each off by 2^-34 of itself at most, and added up
+    as integers, so the outcome does not depend on the run; those below 2^-42 of
+    the largest count as nothing."""
     ts = (logits, uniforms) + tuple(v for v in (temperature, top_k, top_p, min_p) if isinstance(v, torch.Tensor))
     dev = _device(ts)
     dt = _DT.get(logits.dtype)
@@ -94,7 +94,7 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: float | to
     probs = uniforms.new_empty((B, V)) if return_probs else None
     if B:
         k_all = min(int(k_all), V)
-        wsb = _workspace(B, V, k is not None or k_all > 1, return_probs)
+        wsb = _workspace(B, V, return_probs)
         ws = uniforms.new_empty(wsb // 4 + 1)
         st = _launch(dev, L.load().catopt_hip_sample, dt, B, V, logits.data_ptr(), logits.stride(0), uniforms.data_ptr(),
                      t if t is None else t.data_ptr(), t_all, k if k is None else k.data_ptr(), k_all,

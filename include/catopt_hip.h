@@ -764,15 +764,15 @@ int32_t catopt_hip_paged_prefix_attn_fwd(
  * everyone's, 0 for the others.  T = 0 takes the first largest logit.  A row
  * with a NaN, with nothing above -inf or with T < 0 gives -1 and NaN.  A logit
  * of +inf counts as the largest finite number.
- * Weights have an error of 2^-42 of themselves and those below 2^-42 of the
- * largest count as nothing; sums are of integers, the same on every run.
+ * Weights are off by 2^-34 of themselves at most (at random; 2^-38 with one sign),
+ * those below 2^-42 of the largest count as nothing; sums are of integers, the
+ * same on every run.
  * temperature, top_k, top_p, min_p ([B], device, optional) hold each row's own
  * settings; NULL: the *_all value for all rows.  V <= 2^21.
- * Workspace: catopt_hip_sample_workspace_bytes(B, V, counted, with probs) bytes,
- * 16-byte aligned, any contents; counted where top_k is given or top_k_all > 1.
+ * Workspace: catopt_hip_sample_workspace_bytes(B, V, with probs) bytes, 16-byte
+ * aligned, any contents (-1: invalid arguments).
  */
-int64_t catopt_hip_sample_workspace_bytes(int64_t B, int64_t V,
-                                          int32_t counted, int32_t probs);
+int64_t catopt_hip_sample_workspace_bytes(int64_t B, int64_t V, int32_t probs);
 int32_t catopt_hip_sample(
     int32_t dtype, int64_t B, int64_t V, const void* logits, int64_t ld,
     const float* u, const float* temperature, double temperature_all,

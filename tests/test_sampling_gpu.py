@@ -20,9 +20,10 @@ def gen(seed):
 
 def row_ref(x, u, t, k, p, low):
     """(token, log probability, probabilities, how near u and the borders come to a sum, how far off sums may be), the
-    last two relative to the whole.  A weight is rounded to 2^-42 of itself (half of it off at most) and its series is
-    off by 2^-42.6, so a sum is off by less than 2^-41 of itself; each of 768 bins' sums is rounded to 2^-42 of the
-    largest weight, which is at most the whole; and weights below 2^-41 of the largest may count as nothing."""
+    last two relative to the whole.  A weight is rounded to 2^-34 of about itself (half of that off at most, at random:
+    a standard deviation of 2^-35 / sqrt(3), and seven of a sum of n alike weights' are 2^-33 / sqrt(n) of it) and its series
+    is off by 2^-38.5; each of 768 bins' sums is rounded to 2^-42 of the largest weight, which is at most the whole; and
+    weights below 2^-41 of the largest may count as nothing."""
     V = len(x)
     if np.isnan(x).any() or not (x > -np.inf).any() or not t >= 0:
         return -1, math.nan, np.full(V, np.nan), 1.0, 0.0
@@ -35,7 +36,8 @@ def row_ref(x, u, t, k, p, low):
         order, w = order[:1], np.ones(1)
     else:
         w = np.exp((x[order] - x[order[0]]) / t)
-    off = 2.0 ** -40 + 768 * 2.0 ** -43 + w[w < 2.0 ** -41].sum()  # in both sums that are compared
+    many = np.sqrt((w * w).sum()) / w.sum()  # 1 / sqrt(n) of alike ones
+    off = 2 * (2.0 ** -33 * many + 2.0 ** -38.5) + 768 * 2.0 ** -43 + w[w < 2.0 ** -41].sum()  # in both sums that are compared
     near = 1.0
     if p < 1:
         cum = np.cumsum(w)
