@@ -92,7 +92,7 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
 
 // ------------------------------------------------------------------ rows
 
-constexpr int RT = 1024, WAVES = RT / 64;
+constexpr int RT = 512, WAVES = RT / 64;
 constexpr int kList = 8192;   // logits of a row that are kept in LDS
 constexpr int kParts = 256;   // of a range
 constexpr int kMaxChunks = 520;
@@ -156,12 +156,15 @@ __device__ __forceinline__ V wave_scan(V v) {
   return v;
 }
 
-// The wave's places (~0 behind the last) in ascending order, lane by lane.
-__device__ __forceinline__ uint64_t sorted(uint64_t mine, int n) {
+// How many of lanes j, j + step ... below n hold less than this one.
+__device__ __forceinline__ int lanes_below(uint64_t mine, int j, int n, int step) {
+  int below = 0;
+  for (; j < n; j += step) below += lane_u64(mine, j) < mine;
+  return below;
+}
+// The wave's places (~0 behind the last of n) by their ranks, lane by lane.
+__device__ __forceinline__ uint64_t by_rank_of(uint64_t mine, int rank, int n) {
   const int lane = threadIdx.x & 63;
-  int rank = 0;
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) rank += lane_u64(mine, j) < mine;
   if (lane >= n) rank = lane;
   const uint32_t hi = __builtin_amdgcn_ds_permute(4 * rank, (int)(mine >> 32));
   const uint32_t lo = __builtin_amdgcn_ds_permute(4 * rank, (int)(uint32_t)mine);
@@ -195,10 +198,21 @@ struct Search {
   RowLds& s;
   const RowReader<T> r;
   const Grid g;
-  static constexpr int U = 4;  // pieces at a time
+  static constexpr int W = RowReader<T>::W, U = 32 / W;  // logits of a piece, pieces at a time
+  u32x4 ahead[U];                         // the next ones, on their way
   int step = 0;
   uint32_t n_list = 0;
   Bins listed = kNoBins, listed2 = kNoBins;  // the list holds all their logits
+
+  // A row's search begins with its first pieces on their way.
+  __device__ __forceinline__ Search(RowLds& s_, const RowReader<T>& r_, const Grid& g_, const u32x4* first) : s(s_), r(r_), g(g_) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) ahead[j] = first[j];
+  }
+  static __device__ __forceinline__ void start(const RowReader<T>& r, u32x4* first) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) first[j] = r.load(threadIdx.x + j * RT);
+  }
 
   __device__ __forceinline__ int bin_of(float x, double& rest) const {
     const double on = g.on(x);
@@ -224,73 +238,94 @@ struct Search {
     return s.steps[step++ % 3];
   }
 
-  // f(first piece, a bit for each logit of four pieces that may be in either of the
-  // bins), by whole waves.  Two comparisons a logit; a bin's neighbours' edges come
-  // along.
-  template <typename F>
-  __device__ __forceinline__ void scan_row(Bins a, Bins b, F f) const {
+  // f(first piece, a bit for each logit of U pieces that may be in either of the
+  // bins), by whole waves.  A bin's neighbours' edges come along.
+  template <bool TWO, typename F>
+  __device__ __forceinline__ void scan_row(Bins a, Bins b, F f) {
     const float lo = floor_of(a.last), hi = top_of(a.first);
-    const bool two = b.first <= b.last;
-    const float lo2 = two ? floor_of(b.last) : __builtin_inff(), hi2 = two ? top_of(b.first) : -__builtin_inff();
-    const int n = r.pieces();
+    const float lo2 = TWO ? floor_of(b.last) : lo, hi2 = TWO ? top_of(b.first) : hi;
+    const int n = r.pieces(), wave0 = threadIdx.x & ~63;
 #pragma unroll 1
-    for (int p0 = threadIdx.x; p0 - (int)(threadIdx.x & 63) < n; p0 += U * RT) {
-      u32x4 w[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) w[j] = r.load(p0 + j * RT);
+    for (int p0 = 0; p0 + wave0 < n; p0 += U * RT) {
       uint32_t some = 0;
 #pragma unroll
       for (int j = 0; j < U; ++j)
 #pragma unroll
-        for (int e = 0; e < RowReader<T>::W; ++e) {
-          const float x = r.at(w[j], e);
-          some |= ((x >= lo && x <= hi) || (x >= lo2 && x <= hi2)) ? 1u << (j * RowReader<T>::W + e) : 0u;
+        for (int e = 0; e < W; ++e) {
+          const float x = r.at(ahead[j], e);
+          bool in = __builtin_amdgcn_fmed3f(x, lo, hi) == x;
+          if (TWO) in = in || __builtin_amdgcn_fmed3f(x, lo2, hi2) == x;
+          some |= in ? 1u << (j * W + e) : 0u;
         }
-      if (__ballot(some != 0)) f(p0, some);
+      const int next = p0 + U * RT + wave0 < n ? p0 + U * RT : 0;  // or the first ones again
+#pragma unroll
+      for (int j = 0; j < U; ++j) ahead[j] = r.load(next + j * RT + (int)threadIdx.x);
+      if (__ballot(some != 0)) f(p0 + (int)threadIdx.x, some);
     }
-  }
-  // The index of bit i, and the place of the logit with an index.
-  __device__ __forceinline__ int index_of(int p0, int i) const {
-    return r.first(p0 + i / RowReader<T>::W * RT) + i % RowReader<T>::W;
   }
   __device__ __forceinline__ uint64_t place_of(int i) const { return place(finite_top(r.value(i)), i); }
 
-  // f(place, rest) for the row's logits in a bin.
+  // f(place, rest) for the row's logits in a bin, one by one.
   template <typename F>
   __device__ __forceinline__ void each_in_row(int b, F f) const {
-    scan_row(Bins{b, b}, kNoBins, [&](int p0, uint32_t some) {
-      for (; some; some &= some - 1) {
-        const uint64_t at = place_of(index_of(p0, __builtin_ctz(some)));
-        double rest;
-        if (bin_of(logit_of(at), rest) == b) f(at, rest);
-      }
-    });
+#pragma unroll 1
+    for (int i = threadIdx.x; i < r.V; i += RT) {
+      const uint64_t at = place_of(i);
+      double rest;
+      if (bin_of(logit_of(at), rest) == b) f(at, rest);
+    }
+  }
+  // The same of the list.
+  template <typename F>
+  __device__ __forceinline__ void each_in_list(int b, F f) const {
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x; i < n_list; i += RT) {
+      const uint64_t at = s.list[i];
+      double rest;
+      if (bin_of(logit_of(at), rest) == b) f(at, rest);
+    }
   }
 
-  // The logits that may be in those bins into the list, as far as it holds them;
-  // their number.  The indexes come first, by a sum over each wave, then the places.
-  __device__ __forceinline__ uint32_t gather(Bins a, Bins b) {
+  __device__ __forceinline__ bool has(int b) const { return listed.has(b) || listed2.has(b); }
+
+  // The logits that may be in those bins into the list, to be searched in
+  // afterwards if it holds them all: the indexes first, by a sum over each wave,
+  // then the places.
+  __device__ __forceinline__ void list_bins(Bins a, Bins b) {
     Step& t = begin();
-    scan_row(a, b, [&](int p0, uint32_t some) {
+    auto append = [&](int p0, uint32_t some) {
       const uint32_t mine = __builtin_popcount(some), upto = wave_scan(mine);
       uint32_t base = 0;
       if ((threadIdx.x & 63) == 63) base = atomicAdd(&t.count, upto);
       uint32_t i = (uint32_t)__builtin_amdgcn_readlane((int)base, 63) + upto - mine;
-      for (; some; some &= some - 1, ++i)
-        if (i < kList) s.list[i] = (uint32_t)index_of(p0, __builtin_ctz(some));
-    });
+#pragma unroll 1
+      for (; some; some &= some - 1, ++i) {
+        const int bit = __builtin_ctz(some);
+        if (i < kList) s.list[i] = (uint32_t)(r.first(p0 + bit / W * RT) + bit % W);
+      }
+    };
+    if (b.first <= b.last)
+      scan_row<true>(a, b, append);
+    else
+      scan_row<false>(a, b, append);
     __syncthreads();
-    const uint32_t n = t.count;
-    for (uint32_t i = threadIdx.x; i < n && i < kList; i += RT) s.list[i] = place_of((int)(uint32_t)s.list[i]);
-    __syncthreads();
-    return n;
-  }
-
-  // The same to be searched in afterwards, if it holds them.
-  __device__ __forceinline__ void list_bins(Bins a, Bins b) {
-    n_list = gather(a, b);
-    const bool all = n_list <= kList;
+    const bool all = t.count <= kList;
+    n_list = all ? t.count : 0;
+    constexpr int A = 8;  // loads ahead of their use
+#pragma unroll 1
+    for (uint32_t i0 = threadIdx.x; i0 < n_list; i0 += A * RT) {
+      int at[A];
+      float x[A];
+#pragma unroll
+      for (int i = 0; i < A; ++i) at[i] = i0 + i * RT < n_list ? (int)(uint32_t)s.list[i0 + i * RT] : 0;
+#pragma unroll
+      for (int i = 0; i < A; ++i) x[i] = r.value(at[i]);
+#pragma unroll
+      for (int i = 0; i < A; ++i)
+        if (i0 + i * RT < n_list) s.list[i0 + i * RT] = place(finite_top(x[i]), at[i]);
+    }
     listed = all ? a : kNoBins, listed2 = all ? b : kNoBins;
+    __syncthreads();
   }
 
   // The first bin whose running sum (or count) meets the target, kBins - 1 where none does.
@@ -308,14 +343,8 @@ struct Search {
     const int lane = threadIdx.x & 63;
     uint64_t lo = place(top_of(b), 0), hi = place(floor_of(b), -1), before = 0;
     uint32_t n_before = 0, n = s.cum_n[b] - (b ? s.cum_n[b - 1] : 0);
-    bool list = listed.has(b) || listed2.has(b), own = false;  // own: the list is this call's
-    bool narrowed = false;  // more logits than the list holds: the row is read for each step
+    const bool list = has(b);  // else more logits than it holds: the row is read for each step
     for (;;) {
-      if (!list && n <= kList && !narrowed) {
-        listed = listed2 = kNoBins;
-        n = n_list = gather(Bins{b, b}, kNoBins);
-        list = own = n <= kList;  // not so where the neighbours' edges were too many
-      }
       // one key alone: its indexes end with the row
       if (lo >> 32 == hi >> 32) hi = least_of(hi, (hi & ~0xffffffffull) | (uint32_t)(r.V - 1));
       const bool few = n <= 64;
@@ -331,21 +360,15 @@ struct Search {
           atomicAdd(t.n + i, 1u);
         }
       };
-      if (list) {
-#pragma unroll 1
-        for (uint32_t i = threadIdx.x; i < n_list; i += RT) {
-          const uint64_t at = s.list[i];
-          double rest;
-          if (bin_of(logit_of(at), rest) == b) take(at, rest);
-        }
-      } else {
+      if (list)
+        each_in_list(b, take);
+      else
         each_in_row(b, take);
-      }
       __syncthreads();
       auto& found = s.found[step & 1];
       if (threadIdx.x < 64 && few) {  // in order
         const int m = min((int)t.count, 64);
-        const uint64_t at = sorted(lane < m ? t.last[lane] : ~0ull, m);
+        const uint64_t last = lane < m ? t.last[lane] : ~0ull, at = by_rank_of(last, lanes_below(last, 0, m, 1), m);
         double rest;
         bin_of(logit_of(at), rest);
         const uint64_t upto = wave_scan(lane < m ? g.weight(rest) : 0) + before;
@@ -382,11 +405,9 @@ struct Search {
       }
       __syncthreads();
       if (few) {
-        if (own) listed = listed2 = kNoBins;
         sum = found.sum;
         return found.lo;
       }
-      narrowed = true;
       lo = found.lo, before = found.sum, n_before = found.n_before, n = found.n;
       hi = least_of(hi, lo + ((1ull << shift) - 1));
     }
@@ -400,6 +421,9 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Settings set = settings(a, row);
   const ChunkHead* heads = a.heads + (int64_t)row * a.chunks;
+  const RowReader<T> reader(a, row);
+  u32x4 first[Search<T>::U];
+  Search<T>::start(reader, first);
   float m = -__builtin_inff();
   int nan = 0;
   for (int i = lane; i < a.chunks; i += 64) {
@@ -412,20 +436,20 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const bool valid = set.valid && __ballot(nan != 0) == 0 && m != -__builtin_inff();
   if (!valid || set.greedy) {
-    int first = 0x7fffffff;
+    int top = 0x7fffffff;
     if (valid)
-      for (int i = lane; i < a.chunks; i += 64) first = heads[i].max == m ? min(first, heads[i].first) : first;
+      for (int i = lane; i < a.chunks; i += 64) top = heads[i].max == m ? min(top, heads[i].first) : top;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
+    for (int o = 32; o > 0; o >>= 1) top = min(top, __shfl_xor(top, o, 64));
     if (tid == 0) {
-      a.tokens[row] = valid ? first : -1;
+      a.tokens[row] = valid ? top : -1;
       a.logprobs[row] = valid ? 0.f : __builtin_nanf("");
-      if (a.rows) a.rows[row] = RowState{0, 0, 0, 0, 0, valid ? kOneHot : kNone, first};
+      if (a.rows) a.rows[row] = RowState{0, 0, 0, 0, 0, valid ? kOneHot : kNone, top};
     }
     return;
   }
   double rest;
-  Search<T> find{s, RowReader<T>(a, row), Grid(set.t, m)};
+  Search<T> find(s, reader, Grid(set.t, m), first);
   const double c = find.g.c, ref = find.g.ref;
   // ---- the row's bins from the chunks'
   for (int i = tid; i < a.chunks; i += RT) {
@@ -436,28 +460,35 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   if (tid < kParts) s.steps[0].weight[tid] = 0, s.steps[0].n[tid] = 0;
   if (tid == 0) s.steps[0].count = 0;
   __syncthreads();
-  uint64_t w = 0;
-  uint32_t n = 0;
-  if (tid < kBins) {
-    const uint64_t* bins = a.bins + (int64_t)row * a.chunks * kBins + tid;
+  uint64_t w[2] = {0, 0};  // two bins a thread
+  uint32_t n[2] = {0, 0};
+  if (tid < kBins / 2) {
+    const uint64_t* bins = a.bins + (int64_t)row * a.chunks * kBins + 2 * tid;
 #pragma unroll 4
     for (int i = 0; i < a.chunks; ++i) {
       const int o = s.off[i];
-      const uint64_t v = tid >= o ? bins[(int64_t)i * kBins - o] : 0;
-      w += v & ((1ull << kCount) - 1);
-      n += (uint32_t)(v >> kCount);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint64_t v = 2 * tid + e >= o ? bins[(int64_t)i * kBins + e - o] : 0;
+        w[e] += v & ((1ull << kCount) - 1);
+        n[e] += (uint32_t)(v >> kCount);
+      }
     }
-    w = (uint64_t)rint((double)w * scale_of(tid));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) w[e] = (uint64_t)rint((double)w[e] * scale_of(2 * tid + e));
   }
   {
-    const uint64_t sw = wave_scan(w);
-    const uint32_t sn = wave_scan(n);
+    const uint64_t sw = wave_scan(w[0] + w[1]);
+    const uint32_t sn = wave_scan(n[0] + n[1]);
     if (lane == 63) s.wave_sums[wave] = sw, s.wave_counts[wave] = sn;
     __syncthreads();
     uint64_t bw = 0;
     uint32_t bn = 0;
     for (int i = 0; i < wave; ++i) bw += s.wave_sums[i], bn += s.wave_counts[i];
-    if (tid < kBins) s.cum[tid] = bw + sw, s.cum_n[tid] = bn + sn;
+    if (tid < kBins / 2) {
+      s.cum[2 * tid] = bw + sw - w[1], s.cum_n[2 * tid] = bn + sn - n[1];
+      s.cum[2 * tid + 1] = bw + sw, s.cum_n[2 * tid + 1] = bn + sn;
+    }
   }
   __syncthreads();
   // ---- the kept prefix: up to `cut_at` in bin `cut`, `total` in all
@@ -472,9 +503,10 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   auto before_n = [&](int b) { return b > 0 ? s.cum_n[b - 1] : 0u; };
   auto within = [&](int b, uint64_t sum) { return before(b) + (uint64_t)rint((double)sum * scale_of(b)); };
   Bins list = kNoBins, list2 = kNoBins;
+  int end = kBins - 1;
   if (by_rank || by_sum || by_low) {
     if (by_rank) cut = find.find_bin(kRank, (double)(set.k - 1));
-    int end = by_rank || !by_sum ? cut : find.find_bin(kReaches, set.p * (double)total);
+    end = by_rank || !by_sum ? cut : find.find_bin(kReaches, set.p * (double)total);
     // a border behind min-p's does nothing, but for a rank's that says what top-p is a share of
     by_low = low_bin <= end;
     if (low_bin < end && !(by_rank && by_sum)) by_rank = by_sum = false, end = (int)low_bin;
@@ -488,13 +520,44 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
       const uint32_t there = pick.first <= pick.last ? s.cum_n[pick.last] - before_n(pick.first) : 0;
       if (here + there <= kList) list = Bins{end, end}, list2 = pick;
     }
-    if (list.has(end)) find.list_bins(list, list2);
-    if (find.listed.first == 0 && find.n_list <= 64) {
-      // all that may be kept is in one wave: the definition, lane by lane
+  }
+  uint64_t at = 0, sum;
+#pragma unroll 1
+  for (int look = list.has(end) ? 0 : 1; look < 5; ++look) {  // for top-k's border, top-p's, min-p's, and for the token
+    Find by = kRank;
+    double target = 0;
+    int b = cut;
+    if (look == 1) {
+      if (!by_rank) continue;
+      if (s.cum_n[cut] == set.k) {
+        total = s.cum[cut];
+        continue;
+      }
+      target = (double)(set.k - 1 - before_n(cut));
+    } else if (look == 3) {
+      if (!by_low || low_bin > cut) continue;
+      b = (int)low_bin;
+    } else if (look > 0) {
+      if (look == 2 && !by_sum) continue;
+      by = look == 2 ? kReaches : kPasses;
+      target = (look == 2 ? set.p : u) * (double)total;
+      b = min(find.find_bin(by, target), cut);
+      target = (target - (double)before(b)) / scale_of(b);
+    }
+    if (look > 0) list = Bins{b, b}, list2 = kNoBins;
+    if (look == 0 || !find.has(b)) find.list_bins(list, list2);
+    if (look == 0) {
+      const int n_list = (int)find.n_list;
+      if (find.listed.first != 0 || n_list > 64) continue;
+      // all that may be kept is in one wave: the definition, lane by lane, after the waves have ranked them together
+      at = lane < n_list ? s.list[lane] : ~0ull;
+      Step& t = find.begin();
+      atomicAdd(&t.n[lane], (uint32_t)lanes_below(at, wave, n_list, WAVES));
+      __syncthreads();
       if (wave > 0) return;
-      const uint64_t at = sorted(lane < (int)find.n_list ? s.list[lane] : ~0ull, (int)find.n_list);
+      at = by_rank_of(at, (int)t.n[lane], n_list);
       const int bin = find.bin_of(logit_of(at), rest);
-      const int n_all = __builtin_popcountll(__ballot(lane < (int)find.n_list && bin <= end));
+      const int n_all = __builtin_popcountll(__ballot(lane < n_list && bin <= end));
       const double sums = wave_scan(lane < n_all ? (double)find.g.weight(rest) * scale_of(bin) : 0);
       const double whole = by_rank ? lane_f64(sums, (int)set.k - 1) : (double)total;
       bool kept = lane < (by_rank ? (int)set.k : n_all);
@@ -515,50 +578,26 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
       if (lane == last && a.rows) a.rows[row] = RowState{c, ref, low, log2_total, at, bin, 0};
       return;
     }
-  }
-  uint64_t at = 0;
-#pragma unroll 1
-  for (int look = 0; look < 3; ++look) {  // for top-k's border, for top-p's, for the token
-    Find by = kRank;
-    double target = 0;
-    int b = cut;
-    if (look == 0) {
-      if (!by_rank) continue;
-      if (s.cum_n[cut] == set.k) {
-        total = s.cum[cut];
-        continue;
-      }
-      target = (double)(set.k - 1 - before_n(cut));
-    } else {
-      if (look == 1 && !by_sum) continue;
-      if (look == 2 && by_low && low_bin <= cut) {
-        // of the border's bin those whose y is not below it
-        b = (int)low_bin;
-        Step& t = find.begin();
-        uint64_t mine = 0;
-        auto take = [&](uint64_t place, double rs) {
-          if ((double)logit_of(place) * c >= low && (b < cut || place <= cut_at)) mine += find.g.weight(rs);
-        };
-        if (find.listed.has(b)) {
-          for (uint32_t i = tid; i < find.n_list; i += RT)
-            if (find.bin_of(logit_of(s.list[i]), rest) == b) take(s.list[i], rest);
-        } else {
-          find.each_in_row(b, take);
-        }
-        if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(t.weight), (unsigned long long)mine);
-        __syncthreads();
-        total = least_of(total, within(b, t.weight[0]));
-        if (b < cut) cut = b, cut_at = ~0ull;
-      }
-      by = look == 1 ? kReaches : kPasses;
-      target = (look == 1 ? set.p : u) * (double)total;
-      b = min(find.find_bin(by, target), cut);
-      target = (target - (double)before(b)) / scale_of(b);
+    if (look == 3) {
+      // of the border's bin those whose y is not below it
+      Step& t = find.begin();
+      uint64_t mine = 0;
+      auto take = [&](uint64_t place, double rs) {
+        if ((double)logit_of(place) * c >= low && (b < cut || place <= cut_at)) mine += find.g.weight(rs);
+      };
+      if (find.has(b))
+        find.each_in_list(b, take);
+      else
+        find.each_in_row(b, take);
+      if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(t.weight), (unsigned long long)mine);
+      __syncthreads();
+      total = least_of(total, within(b, t.weight[0]));
+      if (b < cut) cut = b, cut_at = ~0ull;
+      continue;
     }
-    uint64_t sum;
     at = find.resolve(b, by, target, sum);
-    if (look == 0 || (look == 1 && (b < cut || at < cut_at))) cut = b, cut_at = at, total = within(b, sum);
-    if (look == 2 && b == cut && at > cut_at) at = cut_at;
+    if (look == 1 || (look == 2 && (b < cut || at < cut_at))) cut = b, cut_at = at, total = within(b, sum);
+    if (look == 4 && b == cut && at > cut_at) at = cut_at;
   }
   if (tid == 0) {
     const double log2_total = log2((double)total) - kUnits;
