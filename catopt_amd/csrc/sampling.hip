@@ -93,14 +93,14 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
 // ------------------------------------------------------------------ rows
 
 constexpr int RT = 512, WAVES = RT / 64;
-constexpr int kList = 8192;   // logits of a row that are kept in LDS
-constexpr int kParts = 256;   // of a range
+constexpr int kList = 6144;   // logits of a row that are kept in LDS: two workgroups fit a CU
+constexpr int kParts = 128;   // of a range
 constexpr int kMaxChunks = 520;
 
 // What one step of a search adds up.  Three of them take turns: a step clears the
 // next one's, which was last read before the barriers of the step before.
 struct Step {
-  uint64_t weight[kParts];
+  uint64_t weight[kParts], least[kParts], most[kParts];  // the places' bounds
   uint64_t last[64];
   uint32_t n[kParts];
   uint32_t count;
@@ -111,7 +111,7 @@ struct RowLds {
   uint64_t list[kList];
   Step steps[3];
   struct {
-    uint64_t lo, sum;
+    uint64_t lo, hi, sum;
     uint32_t n_before, n;
   } found[2];  // what the first wave has decided, in turn
   uint64_t wave_sums[WAVES];
@@ -231,10 +231,14 @@ struct Search {
     return f + fabsf(f) * 0x1p-22f + 0x1p-140f;
   }
 
+  static __device__ __forceinline__ void clear(Step& t) {
+    const int i = threadIdx.x;
+    if (i < kParts) t.weight[i] = 0, t.least[i] = ~0ull, t.most[i] = 0, t.n[i] = 0;
+    if (i == 0) t.count = 0;
+  }
   __device__ __forceinline__ Step& begin() {
     Step& next = s.steps[(step + 1) % 3];
-    if (threadIdx.x < kParts) next.weight[threadIdx.x] = 0, next.n[threadIdx.x] = 0;
-    if (threadIdx.x == 0) next.count = 0;
+    clear(next);
     return s.steps[step++ % 3];
   }
 
@@ -345,10 +349,8 @@ struct Search {
     uint32_t n_before = 0, n = s.cum_n[b] - (b ? s.cum_n[b - 1] : 0);
     const bool list = has(b);  // else more logits than it holds: the row is read for each step
     for (;;) {
-      // one key alone: its indexes end with the row
-      if (lo >> 32 == hi >> 32) hi = least_of(hi, (hi & ~0xffffffffull) | (uint32_t)(r.V - 1));
       const bool few = n <= 64;
-      const int bits = 64 - __builtin_clzll((hi - lo) | 1), shift = max(bits - 8, 0);
+      const int bits = 64 - __builtin_clzll((hi - lo) | 1), shift = max(bits - 7, 0);
       Step& t = begin();
       auto take = [&](uint64_t at, double rest) {
         if (at < lo || at > hi) return;
@@ -357,6 +359,8 @@ struct Search {
         } else {
           const int i = (int)((at - lo) >> shift);
           atomicAdd(reinterpret_cast<unsigned long long*>(t.weight + i), (unsigned long long)g.weight(rest));
+          atomicMin(reinterpret_cast<unsigned long long*>(t.least + i), (unsigned long long)at);
+          atomicMax(reinterpret_cast<unsigned long long*>(t.most + i), (unsigned long long)at);
           atomicAdd(t.n + i, 1u);
         }
       };
@@ -377,12 +381,12 @@ struct Search {
         if (lane == from) found.lo = at, found.sum = upto;
       }
       if (threadIdx.x < 64 && !few) {
-        // four parts a lane: the part that the logit is in, the last that holds one where none meets the target
-        uint64_t w[4], all = 0;
-        uint32_t k[4], all_n = 0;
+        // two parts a lane: the part that the logit is in, the last that holds one where none meets the target
+        uint64_t w[2], all = 0;
+        uint32_t k[2], all_n = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = t.weight[4 * lane + i], k[i] = t.n[4 * lane + i];
+        for (int i = 0; i < 2; ++i) {
+          w[i] = t.weight[2 * lane + i], k[i] = t.n[2 * lane + i];
           all += w[i], all_n += k[i];
         }
         uint64_t upto = wave_scan(all) - all + before, at_sum = 0;
@@ -390,16 +394,16 @@ struct Search {
         int at = -1;
         bool met = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           if (k[i] && !met) {
-            at = 4 * lane + i, at_sum = upto, at_n = upto_n, here = k[i];
+            at = 2 * lane + i, at_sum = upto, at_n = upto_n, here = k[i];
             met = meets(find, target, upto + w[i], upto_n + k[i]);
           }
           upto += w[i], upto_n += k[i];
         }
         const uint64_t some = __ballot(met), held = __ballot(at >= 0);
         if (lane == (some ? __builtin_ctzll(some) : 63 - __builtin_clzll(held | 1))) {
-          found.lo = lo + ((uint64_t)max(at, 0) << shift);
+          found.lo = t.least[max(at, 0)], found.hi = t.most[max(at, 0)];
           found.sum = at_sum, found.n_before = at_n, found.n = here;
         }
       }
@@ -408,8 +412,7 @@ struct Search {
         sum = found.sum;
         return found.lo;
       }
-      lo = found.lo, before = found.sum, n_before = found.n_before, n = found.n;
-      hi = least_of(hi, lo + ((1ull << shift) - 1));
+      lo = found.lo, hi = found.hi, before = found.sum, n_before = found.n_before, n = found.n;
     }
   }
 };
@@ -457,8 +460,7 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     // by the row's factor: it is the chunk's too wherever the chunk has a bin of the row's
     s.off[i] = find.bin_of(cm, rest);
   }
-  if (tid < kParts) s.steps[0].weight[tid] = 0, s.steps[0].n[tid] = 0;
-  if (tid == 0) s.steps[0].count = 0;
+  find.clear(s.steps[0]);
   __syncthreads();
   uint64_t w[2] = {0, 0};  // two bins a thread
   uint32_t n[2] = {0, 0};
