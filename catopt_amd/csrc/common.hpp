@@ -97,7 +97,7 @@ __device__ __forceinline__ constexpr int acc_row(int r, int g) {
 // fewer than 2^32 work-items in it.
 inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks * threads < (1LL << 32); }
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+__host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // γ^k for an integer k >= 0 from lg = log2|γ| and neg = (γ < 0), as pow
 // gives it for an integer exponent: 1 at k = 0 (0^0 included, where

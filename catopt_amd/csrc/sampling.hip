@@ -29,12 +29,15 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
   u32x4 w[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) w[j] = r.load(piece0 + j * CT);
+  // the first chunk takes the logits outside the pieces, too
+  const int edge = chunk == 0 && tid < r.edges() ? r.edge(tid) : -1;
+  const float at_edge = edge >= 0 ? r.value(edge) : -__builtin_inff();
   const Settings s = settings(a, row);
   const bool binned = s.valid && !s.greedy;
   if (binned)
     for (int i = tid; i < kBins; i += CT) bins[i] = 0;
-  float m = -__builtin_inff();
-  bool nan = false;
+  float m = at_edge;
+  bool nan = m != m;
 #pragma unroll
   for (int j = 0; j < P; ++j)
 #pragma unroll
@@ -53,7 +56,7 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
   for (int i = 0; i < CT / 64; ++i) m = fmaxf(m, maxima[i]);
   ChunkHead* head = a.heads + (int64_t)row * a.chunks + chunk;
   if (s.greedy) {
-    int first = 0x7fffffff;
+    int first = finite_top(at_edge) == m && edge >= 0 ? edge : 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < P; ++j)
 #pragma unroll
@@ -74,17 +77,18 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
   }
   if (!binned || m == -__builtin_inff()) return;
   const Grid g(s.t, m);
+  auto add = [&](float x) {
+    const double on = g.on(x);
+    const uint64_t bin = g.below(on);
+    if (bin < kBins)
+      atomicAdd(reinterpret_cast<unsigned long long*>(bins + bin),
+                (unsigned long long)(g.weight(g.rest(x, on)) | 1ull << kCount));
+  };
 #pragma unroll
   for (int j = 0; j < P; ++j)
 #pragma unroll
-    for (int e = 0; e < W; ++e) {
-      const float x = finite_top(r.at(w[j], e));
-      const double on = g.on(x);
-      const uint64_t bin = g.below(on);
-      if (bin < kBins)
-        atomicAdd(reinterpret_cast<unsigned long long*>(bins + bin),
-                  (unsigned long long)(g.weight(g.rest(x, on)) | 1ull << kCount));
-    }
+    for (int e = 0; e < W; ++e) add(finite_top(r.at(w[j], e)));
+  if (chunk == 0) add(finite_top(at_edge));
   __syncthreads();
   const int64_t at = ((int64_t)row * a.chunks + chunk) * kBins;
   for (int i = tid; i < kBins; i += CT) a.bins[at + i] = bins[i];
@@ -93,7 +97,7 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
 // ------------------------------------------------------------------ rows
 
 constexpr int RT = 512, WAVES = RT / 64;
-constexpr int kList = 6144;   // logits of a row that are kept in LDS: two workgroups fit a CU
+constexpr int kList = 8192;   // logits of a row that are kept in LDS
 constexpr int kParts = 128;   // of a range
 constexpr int kMaxChunks = 520;
 
@@ -198,6 +202,7 @@ struct Search {
   RowLds& s;
   const RowReader<T> r;
   const Grid g;
+  static constexpr int kEdges = -1;
   static constexpr int W = RowReader<T>::W, U = 32 / W;  // logits of a piece, pieces at a time
   u32x4 ahead[U];                         // the next ones, on their way
   int step = 0;
@@ -243,28 +248,31 @@ struct Search {
   }
 
   // f(first piece, a bit for each logit of U pieces that may be in either of the
-  // bins), by whole waves.  A bin's neighbours' edges come along.
+  // bins), by whole waves; kEdges for the logits outside the pieces.  A bin's neighbours' edges come along.
   template <bool TWO, typename F>
   __device__ __forceinline__ void scan_row(Bins a, Bins b, F f) {
     const float lo = floor_of(a.last), hi = top_of(a.first);
     const float lo2 = TWO ? floor_of(b.last) : lo, hi2 = TWO ? top_of(b.first) : hi;
-    const int n = r.pieces(), wave0 = threadIdx.x & ~63;
+    auto in = [&](float x) {
+      return __builtin_amdgcn_fmed3f(x, lo, hi) == x || (TWO && __builtin_amdgcn_fmed3f(x, lo2, hi2) == x);
+    };
+    const int n = r.pieces, wave0 = threadIdx.x & ~63;
 #pragma unroll 1
     for (int p0 = 0; p0 + wave0 < n; p0 += U * RT) {
       uint32_t some = 0;
 #pragma unroll
       for (int j = 0; j < U; ++j)
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const float x = r.at(ahead[j], e);
-          bool in = __builtin_amdgcn_fmed3f(x, lo, hi) == x;
-          if (TWO) in = in || __builtin_amdgcn_fmed3f(x, lo2, hi2) == x;
-          some |= in ? 1u << (j * W + e) : 0u;
-        }
+        for (int e = 0; e < W; ++e)
+          some |= in(r.at(ahead[j], e)) ? 1u << (j * W + e) : 0u;
       const int next = p0 + U * RT + wave0 < n ? p0 + U * RT : 0;  // or the first ones again
 #pragma unroll
       for (int j = 0; j < U; ++j) ahead[j] = r.load(next + j * RT + (int)threadIdx.x);
       if (__ballot(some != 0)) f(p0 + (int)threadIdx.x, some);
+    }
+    if (wave0 == 0) {  // a lane each
+      const bool edge = (int)threadIdx.x < r.edges();
+      f(kEdges, edge && in(r.value(edge ? r.edge(threadIdx.x) : 0)) ? 1u : 0u);
     }
   }
   __device__ __forceinline__ uint64_t place_of(int i) const { return place(finite_top(r.value(i)), i); }
@@ -305,7 +313,7 @@ struct Search {
 #pragma unroll 1
       for (; some; some &= some - 1, ++i) {
         const int bit = __builtin_ctz(some);
-        if (i < kList) s.list[i] = (uint32_t)(r.first(p0 + bit / W * RT) + bit % W);
+        if (i < kList) s.list[i] = (uint32_t)(p0 == kEdges ? r.edge(threadIdx.x) : r.first(p0 + bit / W * RT) + bit % W);
       }
     };
     if (b.first <= b.last)
@@ -447,7 +455,7 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     if (tid == 0) {
       a.tokens[row] = valid ? top : -1;
       a.logprobs[row] = valid ? 0.f : __builtin_nanf("");
-      if (a.rows) a.rows[row] = RowState{0, 0, 0, 0, 0, valid ? kOneHot : kNone, top};
+      if (a.rows) a.rows[row] = RowState{0, 0, 0, 0, 0, valid ? kOneHot : kNone, top, 0.f};
     }
     return;
   }
@@ -577,7 +585,7 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
         a.tokens[row] = (int64_t)(uint32_t)at;
         a.logprobs[row] = (float)(((rest - bin) / 16 - log2_total) * 0.6931471805599453);
       }
-      if (lane == last && a.rows) a.rows[row] = RowState{c, ref, low, log2_total, at, bin, 0};
+      if (lane == last && a.rows) a.rows[row] = RowState{c, ref, low, log2_total, at, bin, 0, find.floor_of(bin)};
       return;
     }
     if (look == 3) {
@@ -606,13 +614,13 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     const int bin = find.bin_of(logit_of(at), rest);
     a.tokens[row] = (int64_t)(uint32_t)at;
     a.logprobs[row] = (float)(((rest - bin) / 16 - log2_total) * 0.6931471805599453);
-    if (a.rows) a.rows[row] = RowState{c, ref, low, log2_total, cut_at, cut, 0};
+    if (a.rows) a.rows[row] = RowState{c, ref, low, log2_total, cut_at, cut, 0, find.floor_of(cut)};
   }
 }
 
 // --------------------------------------------------------- probabilities
 
-constexpr int PT = 256, PIECES = 4;
+constexpr int PT = 256, PIECES = 2;
 
 template <typename T>
 __global__ __launch_bounds__(PT) void sample_probs(SampleArgs a, int blocks) {
@@ -621,28 +629,41 @@ __global__ __launch_bounds__(PT) void sample_probs(SampleArgs a, int blocks) {
   const RowState s = a.rows[row];
   const Grid g(s.c, s.ref);
   float* out = a.probs + (int64_t)row * a.ld_probs;
+  // the rows without weights have one number but for the token's place
+  const bool plain = s.cut < 0;
+  const float rest_of_row = s.cut == kNone ? __builtin_nanf("") : 0.f;
+  auto prob = [&](float x, int i) {
+    if (plain) return s.cut == kOneHot && i == s.token ? 1.f : rest_of_row;
+    if (!(x >= s.floor)) return 0.f;
+    const double on = g.on(x);
+    const uint64_t bin = g.below(on);
+    if (bin > (uint64_t)s.cut || !((double)x * s.c >= s.low) || (bin == (uint64_t)s.cut && place(x, i) > s.cut_at)) return 0.f;
+    // 2^whole 2^part: the exponential sees a small number
+    const double y = (g.rest(x, on) - (double)(int)bin) / 16 - s.log2_total, whole = rint(y);
+    return ldexpf(__builtin_amdgcn_exp2f((float)(y - whole)), (int)whole);
+  };
+  const bool wide = aligned16(out + r.head);
 #pragma unroll
   for (int j = 0; j < PIECES; ++j) {
     const int piece = (block * PIECES + j) * PT + threadIdx.x, i0 = r.first(piece);
+    if (piece >= r.pieces) continue;
     const u32x4 w = r.load(piece);
-    float p[RowReader<T>::W];
 #pragma unroll
-    for (int e = 0; e < RowReader<T>::W; ++e) {
-      const float x = finite_top(r.at(w, e));
-      const double on = g.on(x);
-      const uint64_t bin = g.below(on);
-      p[e] = 0.f;
-      if (s.cut >= 0 && bin <= (uint64_t)s.cut && (double)x * s.c >= s.low && (bin < (uint64_t)s.cut || place(x, i0 + e) <= s.cut_at)) {
-        // 2^whole 2^part: the exponential sees a small number
-        const double y = (g.rest(x, on) - (double)(int)bin) / 16 - s.log2_total, whole = rint(y);
-        p[e] = ldexpf(__builtin_amdgcn_exp2f((float)(y - whole)), (int)whole);
+    for (int e = 0; e < RowReader<T>::W; e += 4) {
+      f32x4 p;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) p[k] = prob(finite_top(r.at(w, e + k)), i0 + e + k);
+      if (wide) {
+        *reinterpret_cast<f32x4*>(out + i0 + e) = p;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out[i0 + e + k] = p[k];
       }
-      if (s.cut == kOneHot) p[e] = i0 + e == s.token ? 1.f : 0.f;
-      if (s.cut == kNone) p[e] = __builtin_nanf("");
     }
-#pragma unroll
-    for (int e = 0; e < RowReader<T>::W; ++e)
-      if (i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = p[e];
+  }
+  if (block == 0 && (int)threadIdx.x < r.edges()) {
+    const int i = r.edge(threadIdx.x);
+    out[i] = prob(finite_top(r.value(i)), i);
   }
 }
 
@@ -658,7 +679,7 @@ struct Plan {
 Plan plan_of(int64_t B, int64_t V, bool probs) {
   Plan p;
   p.chunk = B * ((V + kMaxChunk - 1) / kMaxChunk) >= 1024 ? kMaxChunk : 4096;
-  p.chunks = (V + 7 + p.chunk - 1) / p.chunk;  // 7: a row may begin inside its first piece
+  p.chunks = (V + p.chunk - 1) / p.chunk;
   p.heads = B * p.chunks * (int64_t)sizeof(ChunkHead);
   p.bins = B * p.chunks * kBins * 8;
   p.rows = probs ? B * (int64_t)sizeof(RowState) : 0;
@@ -680,7 +701,7 @@ int32_t launch(const SampleArgs& a, const Plan& p, hipStream_t st) {
   CATOPT_LAUNCH_CHECK();
   if (a.probs) {
     constexpr int64_t per = PT * PIECES * RowReader<T>::W;
-    const int64_t blocks = (a.V + RowReader<T>::W - 1 + per - 1) / per;
+    const int64_t blocks = (a.V + per - 1) / per;
     sample_probs<T><<<dim3((uint32_t)(a.B * blocks)), dim3(PT), 0, st>>>(a, (int)blocks);
     CATOPT_LAUNCH_CHECK();
   }

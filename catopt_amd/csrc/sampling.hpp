@@ -50,6 +50,7 @@ struct RowState {
   double c, ref, low, log2_total;  // y = c x; the largest logit's n on the grid; the least y; log2 of the kept weights
   uint64_t cut_at;                 // in the cut's bin the last place that is kept
   int32_t cut, token;              // the last bin that is kept (some of it); kOneHot, kNone: the token alone, NaN
+  float floor;                     // nothing below it is kept
 };
 constexpr int kOneHot = -1, kNone = -2;
 
@@ -125,43 +126,37 @@ __device__ __forceinline__ float logit_of(uint64_t place) {
   return __builtin_bit_cast(float, key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-// A row in pieces of 16 bytes from the aligned address at or before its first
-// logit: piece i holds logits W i - shift on.  Pieces at the row's ends are read
-// logit by logit; what is not in the row reads as -inf.
+// A row in aligned pieces of 16 bytes, W logits each, and the few logits before the
+// first and behind the last of them.
 template <typename T>
 struct RowReader {
   static constexpr int W = 16 / sizeof(T);
   const T* row;
-  int V, shift;
+  int V, head, pieces;
 
   __device__ __forceinline__ RowReader(const SampleArgs& a, int r)
       : row(static_cast<const T*>(a.x) + (int64_t)r * a.ld), V(a.V) {
-    shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    head = min(shift ? W - shift : 0, V);
+    pieces = (V - head) / W;
   }
-  __device__ __forceinline__ int pieces() const { return (V + shift + W - 1) / W; }
-  __device__ __forceinline__ int first(int piece) const { return piece * W - shift; }
+  __device__ __forceinline__ int first(int piece) const { return head + piece * W; }
+  // -inf behind the last piece.
   __device__ __forceinline__ u32x4 load(int piece) const {
-    const int i = first(piece);
-    if (i >= 0 && i + W <= V) return *reinterpret_cast<const u32x4*>(row + i);
     const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
     u32x4 w = {none, none, none, none};
-    if (i + W <= 0 || i >= V) return w;
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-      if (i + e < 0 || i + e >= V) continue;
-      if constexpr (sizeof(T) == 4)
-        w[e] = __builtin_bit_cast(uint32_t, row[i + e]);
-      else
-        w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | (uint32_t)row[i + e] << 16 : (w[e / 2] & 0xffff0000u) | row[i + e];
-    }
+    if (piece < pieces) w = *reinterpret_cast<const u32x4*>(row + first(piece));
     return w;
   }
-  __device__ __forceinline__ float value(int i) const { return load_f32(row, i); }
   // Logit e of a piece.
   static __device__ __forceinline__ float at(const u32x4& w, int e) {
     const uint32_t word = sizeof(T) == 4 ? w[e] : w[e / 2];
     return __builtin_bit_cast(float, sizeof(T) == 4 ? word : e & 1 ? word & 0xffff0000u : word << 16);
   }
+  // Those outside the pieces, less than 2 W.
+  __device__ __forceinline__ int edges() const { return V - pieces * W; }
+  __device__ __forceinline__ int edge(int i) const { return i < head ? i : pieces * W + i; }
+  __device__ __forceinline__ float value(int i) const { return load_f32(row, i); }
 };
 
 // +inf as the largest finite number (one instruction: fminf makes NaNs quiet first).
