@@ -98,6 +98,7 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
 
 constexpr int RT = 512, WAVES = RT / 64;
 constexpr int kList = 8192;   // logits of a row that are kept in LDS
+constexpr int kShort = 1024;  // as many are looked through as quickly as a bin of them
 constexpr int kParts = 128;   // of a range
 constexpr int kMaxChunks = 520;
 
@@ -287,12 +288,13 @@ struct Search {
       if (bin_of(logit_of(at), rest) == b) f(at, rest);
     }
   }
-  // The same of the list.
+  // The same of the list, for places from lo to hi.
   template <typename F>
-  __device__ __forceinline__ void each_in_list(int b, F f) const {
-#pragma unroll 1
+  __device__ __forceinline__ void each_in_list(int b, uint64_t lo, uint64_t hi, F f) const {
+#pragma unroll 4
     for (uint32_t i = threadIdx.x; i < n_list; i += RT) {
       const uint64_t at = s.list[i];
+      if (at < lo || at > hi) continue;
       double rest;
       if (bin_of(logit_of(at), rest) == b) f(at, rest);
     }
@@ -373,7 +375,7 @@ struct Search {
         }
       };
       if (list)
-        each_in_list(b, take);
+        each_in_list(b, lo, hi, take);
       else
         each_in_row(b, take);
       __syncthreads();
@@ -520,7 +522,7 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     // a border behind min-p's does nothing, but for a rank's that says what top-p is a share of
     by_low = low_bin <= end;
     if (low_bin < end && !(by_rank && by_sum)) by_rank = by_sum = false, end = (int)low_bin;
-    if (s.cum_n[end] <= kList) {
+    if (s.cum_n[end] <= (by_rank ? kList : kShort)) {
       list = Bins{0, end};
     } else if (!by_rank) {
       // the border lies in bin `end`, the token where u says for a whole between the sums before and behind it: both
@@ -596,7 +598,7 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
         if ((double)logit_of(place) * c >= low && (b < cut || place <= cut_at)) mine += find.g.weight(rs);
       };
       if (find.has(b))
-        find.each_in_list(b, take);
+        find.each_in_list(b, 0, ~0ull, take);
       else
         find.each_in_row(b, take);
       if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(t.weight), (unsigned long long)mine);
