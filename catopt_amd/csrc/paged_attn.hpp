@@ -26,7 +26,7 @@ struct PagedArgs {
   int B, Hq, Hkv, G, d, cap, normalize, causal;
   int splits, min_keys;  // key ranges per tile at most, keys of one at least
   float scale;
-  // Of the calls that combine carriers of two sets of keys (CARRIERS), a set's part:
+  // Of the calls over two sets of keys, a set's part:
   const int32_t* groups;  // the set's sequences are groups of the call's (NULL: they are those), their first ones
   int n_seq;              // the call's sequences
   int part_ld, part_first;  // of a row's carriers: all, and the set's first
@@ -47,18 +47,35 @@ struct PagedTile {
   bool split;                      // it has several
 };
 
+// What a tile's workgroup does: the rows of a call over one set of keys; a set's
+// carriers of a call over two; such a call's rows over the first set and then, with
+// the same accumulators, over the second (the groups then have one more at either
+// end, of the sequences outside them, without keys).
+enum Form { kRows, kCarriers, kBothSets };
+
 // The rows of sequence b, or of group b of them.
-template <bool CARRIERS>
+template <Form F>
 __device__ __forceinline__ void set_rows(const PagedArgs& a, int b, int& row0, int& nq) {
-  if (!CARRIERS || !a.groups) return seq_rows(a.starts, b, a.N, row0, nq);
+  if (F == kRows || !a.groups) return seq_rows(a.starts, b, a.N, row0, nq);
   const int n = (int)a.N;
-  row0 = min(max(a.starts[min(max(a.groups[b], 0), a.n_seq)], 0), n);
-  nq = max(min(max(a.starts[min(max(a.groups[b + 1], 0), a.n_seq)], 0), n) - row0, 0);
+  int first, next;
+  if (F == kBothSets)
+    first = b == 0 ? 0 : a.groups[b - 1], next = b == a.B - 1 ? a.n_seq : a.groups[b];
+  else
+    first = a.groups[b], next = a.groups[b + 1];
+  row0 = min(max(a.starts[min(max(first, 0), a.n_seq)], 0), n);
+  nq = max(min(max(a.starts[min(max(next, 0), a.n_seq)], 0), n) - row0, 0);
+}
+// Its keys.
+template <Form F>
+__device__ __forceinline__ int set_len(const PagedArgs& a, int b) {
+  if (F == kBothSets && (b == 0 || b == a.B - 1)) return 0;
+  return min(max(a.lens[F == kBothSets ? b - 1 : b], 0), a.cap);
 }
 
 // Lane i looks at sequence i (of 64 at a time), so that the search and the
 // sequence's own numbers are one memory latency.
-template <int R, bool CARRIERS>
+template <int R, Form F>
 __device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, int t) {
   const int lane = threadIdx.x & 63;
   PagedTile x{};
@@ -69,8 +86,8 @@ __device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, int t) {
     int row0 = 0, nq = 0, len = 0;
     bool le = false;
     if (i < a.B) {
-      set_rows<CARRIERS>(a, i, row0, nq);
-      len = min(max(a.lens[i], 0), a.cap);
+      set_rows<F>(a, i, row0, nq);
+      len = set_len<F>(a, i);
       le = (int64_t)row0 * a.G / R + i <= t;
     }
     const int n = __popcll(__ballot(le));
@@ -116,13 +133,13 @@ __device__ __forceinline__ void decode_block(const PagedArgs& a, uint32_t block,
 
 // Where range `split` of row i has its carrier, counted in carriers; and where
 // their numerators begin.
-template <bool CARRIERS>
+template <Form F>
 __device__ __forceinline__ int64_t part_at(const PagedArgs& a, int64_t i, int split) {
-  return CARRIERS ? i * a.part_ld + a.part_first + split : i * a.splits + split;
+  return F == kCarriers ? i * a.part_ld + a.part_first + split : i * a.splits + split;
 }
-template <bool CARRIERS>
+template <Form F>
 __device__ __forceinline__ float* part_numerators(const PagedArgs& a) {
-  return a.part + ((2 * a.N * a.Hq * (CARRIERS ? a.part_ld : a.splits) + 3) & ~(int64_t)3);
+  return a.part + ((2 * a.N * a.Hq * (F == kCarriers ? a.part_ld : a.splits) + 3) & ~(int64_t)3);
 }
 
 // exp2((from - to) c), 0 for an empty `from`.

@@ -6,7 +6,7 @@ namespace {
 
 template <int D, bool WIDE>
 __global__ __launch_bounds__((Few<D, WIDE>::NT), 2) void paged_few_kernel(PagedArgs a) {
-  paged_few<D, Few<D, WIDE>, false>(a, blockIdx.x);
+  paged_few<D, Few<D, WIDE>, kRows>(a, blockIdx.x);
 }
 
 template <int D, bool WIDE>

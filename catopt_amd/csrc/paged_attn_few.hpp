@@ -56,14 +56,14 @@ __device__ __forceinline__ void wait_stage(bool newer) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <int D, typename L, bool CARRIERS>
+template <int D, typename L, Form F>
 __device__ __forceinline__ void paged_few(const PagedArgs& a, uint32_t block) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int h, t, split;
   decode_block(a, block, h, t, split);
-  PagedTile x = paged_tile<kFewRows, CARRIERS>(a, t);
+  PagedTile x = paged_tile<kFewRows, F>(a, t);
   if (x.rows == 0) return;
   paged_ranges(a, x);
   if (!has_range(x, split)) return;
@@ -115,6 +115,23 @@ __device__ __forceinline__ void paged_few(const PagedArgs& a, uint32_t block) {
     }
   };
 
+  // With one stage of LDS, K and V on their own: the next K rows are loaded once the
+  // scores have been formed, the next V rows once these have been read, so that one
+  // of both is on its way all the time.
+  constexpr bool APART = F == kCarriers && L::STAGES == 1;
+  auto issue_k = [&](int lane0, const KeyGroup& at) {
+#pragma unroll
+    for (int k = 0; k < L::LOADS; k += 2)
+      dma_rows_once(k_rsrc(at, lane0 + k * L::ROWS / 8), koff[k & 3], k_rsrc(at, lane0 + (k + 1) * L::ROWS / 8),
+                    koff[(k + 1) & 3], lds0 + k * 1024, 1024);
+  };
+  auto issue_v = [&](int lane0, const KeyGroup& at) {
+#pragma unroll
+    for (int k = 0; k < L::LOADS; k += 2)
+      dma_rows_once(v_rsrc(at, lane0 + k * L::ROWS / 8), voff[k & 1], v_rsrc(at, lane0 + (k + 1) * L::ROWS / 8),
+                    voff[(k + 1) & 1], lds0 + L::HALF + k * 1024, 1024);
+  };
+
   f32x16 acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
@@ -138,10 +155,16 @@ __device__ __forceinline__ void paged_few(const PagedArgs& a, uint32_t block) {
   for (int st = 0; st < stages; ++st) {
     const int in = st & 15;  // of the 16 stages whose groups the lanes hold
     if (in == 0 && st > 0) places(st, group_page(a, table, lane_key(st), lane_key(st) < k_end ? x.len : 0));
-    if (in == 0 || L::STAGES == 1) issue(st, 4 * in, at);
-    const bool newer = L::STAGES == 2 && in < 15 && st + 1 < stages;
-    if (newer) issue(st + 1, 4 * in + 4, at);
-    wait_stage<2 * L::LOADS>(newer);
+    // the next stage's loads are in flight while this one is used
+    const bool newer = (L::STAGES == 2 || APART) && in < 15 && st + 1 < stages;
+    if constexpr (APART) {
+      if (in == 0) issue_k(0, at), issue_v(0, at);
+      wait_stage<L::LOADS>(true);  // all but V's
+    } else {
+      if (in == 0 || L::STAGES == 1) issue(st, 4 * in, at);
+      if (newer) issue(st + 1, 4 * in + 4, at);
+      wait_stage<2 * L::LOADS>(newer);
+    }
     const int key0 = key_of(st);
     const uint32_t bad_now = (uint32_t)(bad >> (4 * in)) & 15u;
     const char* Ks = lds + wave * L::WAVE_BYTES + (st & (L::STAGES - 1)) * L::STAGE;
@@ -153,6 +176,10 @@ __device__ __forceinline__ void paged_few(const PagedArgs& a, uint32_t block) {
 #pragma unroll
     for (int j = 0; j < D / 16; ++j)
       s = mfma32x32x16(*reinterpret_cast<const bf16x8*>(Ks + tile_off<D>(l32, 2 * j + g)), qf[j], s);
+    if constexpr (APART) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K's reads are done
+      if (newer) issue_k(4 * in + 4, at);
+    }
     // some row does not see some key: the first row sees the fewest
     const bool masked = key0 + 32 > x.len || key0 + 31 > lim0 || bad_now;
     if (masked) mask_scores(s, lim - key0, bad_now);
@@ -188,13 +215,19 @@ __device__ __forceinline__ void paged_few(const PagedArgs& a, uint32_t block) {
         for (int r = 0; r < 16; ++r) acc[i][r] *= alpha;
     }
     bf16x8 vf[D / 16];
+    if constexpr (APART) wait_stage<L::LOADS>(newer);  // V's rows; the next K's are younger
     read_v<D>(Vs, 0, vf);
+    if constexpr (APART) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V's reads are done
+      if (newer) issue_v(4 * in + 4, at);
+    }
     if (masked && odd_values<D>(vf)) take_odd_values<D>(vf, lim - key0, bad_now, acc);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
       for (int u = 0; u < 2; ++u) acc[db] = mfma32x32x16(vf[2 * db + u], p[u], acc[db]);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage's LDS reads are done: it may be loaded again
+    if constexpr (!APART)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage's LDS reads are done: it may be loaded again
   }
 
   // ---- the waves' carriers meet in LDS: [wave][row][d] numerators, then
@@ -233,13 +266,13 @@ __device__ __forceinline__ void paged_few(const PagedArgs& a, uint32_t block) {
     }
     const int tk = (int)a.group.div(x.r0 + r), hr = h * a.G + x.r0 + r - tk * a.G;
     const int64_t i = (int64_t)(x.row0 + tk) * a.Hq + hr;
-    if (CARRIERS || x.split) {
-      const int64_t at = part_at<CARRIERS>(a, i, split);
+    if (F == kCarriers || x.split) {
+      const int64_t at = part_at<F>(a, i, split);
       if (d == 0) {
         a.part[2 * at] = mx;
         a.part[2 * at + 1] = lt;
       }
-      *reinterpret_cast<f32x4*>(part_numerators<CARRIERS>(a) + at * D + d) = y;
+      *reinterpret_cast<f32x4*>(part_numerators<F>(a) + at * D + d) = y;
     } else {
       uint16_t* orow = a.o + (int64_t)(x.row0 + tk) * a.o_t + (int64_t)hr * a.o_h;
 #pragma unroll

@@ -6,7 +6,7 @@ namespace {
 
 template <int D>
 __global__ __launch_bounds__((kTileThreads), (D == 64 ? 3 : 2)) void paged_tile_kernel(PagedArgs a, int tiles) {
-  paged_tile_rows<D, false>(a, blockIdx.x, tiles);
+  paged_tile_rows<D, kRows>(a, a, blockIdx.x, tiles);
 }
 
 template <int D>

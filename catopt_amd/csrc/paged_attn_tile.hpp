@@ -55,15 +55,29 @@ struct TileLds {
 __device__ __forceinline__ void pin(const bf16x8& x) { asm volatile("" ::"v"(__builtin_bit_cast(u32x4, x))); }
 __device__ __forceinline__ void pin(float x) { asm volatile("" ::"v"(x)); }
 
-template <int D, bool CARRIERS>
-__device__ __forceinline__ void paged_tile_rows(const PagedArgs& a, uint32_t block, int tiles) {
+// The last of n ascending starts that is not above x; -1 where none is.
+__device__ __forceinline__ int last_start(const int32_t* starts, int n, int most, int x) {
+  const int lane = threadIdx.x & 63;
+  int at = -1;
+  for (int c = 0; c < n; c += 64) {
+    const int i = c + lane;
+    const int k = __popcll(__ballot(i < n && min(max(starts[min(i, n - 1)], 0), most) <= x));
+    at += k;
+    if (k < 64) break;
+  }
+  return at;
+}
+
+// `own`: the second set of a call over both.
+template <int D, Form F>
+__device__ __forceinline__ void paged_tile_rows(const PagedArgs& a, const PagedArgs& own, uint32_t block, int tiles) {
   using L = TileLds<D>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int h, tr, split;
   decode_block(a, block, h, tr, split);
-  PagedTile x = paged_tile<kTileRows, CARRIERS>(a, tiles - 1 - tr);
+  PagedTile x = paged_tile<kTileRows, F>(a, tiles - 1 - tr);
   if (x.rows == 0) return;
   paged_ranges(a, x);
   if (!has_range(x, split)) return;
@@ -71,10 +85,10 @@ __device__ __forceinline__ void paged_tile_rows(const PagedArgs& a, uint32_t blo
 
   const int row = x.r0 + 32 * wave + l32, tok = (int)a.group.div(row), hq = h * a.G + row - tok * a.G;
   const bool live = 32 * wave + l32 < x.rows;
-  const int lim = min(x.off + tok, x.len - 1);  // last key this row sees
+  int lim = min(x.off + tok, x.len - 1);  // last key this row sees
   // of the wave's rows the first sees the fewest keys, the last the most
   const int w0 = x.r0 + 32 * wave, w1 = min(w0 + 31, x.r0 + x.rows - 1);
-  const int lim0 = __builtin_amdgcn_readfirstlane(x.off + (int)a.group.div(w0));
+  int lim0 = __builtin_amdgcn_readfirstlane(x.off + (int)a.group.div(w0));
   const int lim1 = __builtin_amdgcn_readfirstlane(x.off + (int)a.group.div(max(w1, 0)));
   const bool wave_live = 32 * wave < x.rows;
 
@@ -86,9 +100,9 @@ __device__ __forceinline__ void paged_tile_rows(const PagedArgs& a, uint32_t blo
   float m_run = kNegInf, m_true = kNegInf, l_run = 0.f;  // maxima in units of q . k
 
   const int k_end = min(x.kend, (split + 1) * x.keys);
-  const int t0 = split * x.keys / KVB, t1 = (k_end + KVB - 1) / KVB;
-  const int wave_end = wave_live ? min(k_end, lim1 + 1) : 0;
-  const int32_t* table = a.table + (int64_t)x.b * a.table_ld;
+  int t0 = split * x.keys / KVB, t1 = (k_end + KVB - 1) / KVB;
+  int wave_end = wave_live ? min(k_end, lim1 + 1) : 0;
+  const int32_t* table = a.table + (int64_t)(F == kBothSets ? x.b - 1 : x.b) * a.table_ld;
   const uint16_t *kb = a.k + (int64_t)h * a.k_h, *vb = a.v + (int64_t)h * a.v_h;
   // a lane's 16 bytes of load i: tile row (4 i + wave) ROWS + sub, whose place
   // in its 8 keys and whose swizzles do not depend on i
@@ -119,7 +133,7 @@ __device__ __forceinline__ void paged_tile_rows(const PagedArgs& a, uint32_t blo
 
   uint32_t bad = 0, bad_next = 0;  // a bit for each 8 keys of the tile whose page is invalid
   bf16x8 qf[D / 16];
-  if (t0 < t1) {
+  if (t0 < t1 || F == kBothSets) {
     // the first pages' ids, the queries and the first tile are on their way
     // together; the queries as whole rows through the second stage, four times
     // fewer lines a load than as fragments
@@ -268,23 +282,59 @@ __device__ __forceinline__ void paged_tile_rows(const PagedArgs& a, uint32_t blo
       __syncthreads();
     }
   };
-  for (int t = t0; t < t1; t += 2) {
-    tile(t, std::integral_constant<int, 0>{});
-    if (t + 1 < t1) tile(t + 1, std::integral_constant<int, 1>{});
-  }
+  // The next sequence of the tile that has keys of its own: its rows see them, the others none.
+  int b = -1;
+  const int n0 = x.row0 + (int)a.group.div(x.r0), n1 = x.row0 + (int)a.group.div(x.r0 + x.rows - 1);  // the tile's tokens
+  auto next_sequence = [&]() -> bool {
+    if (b < 0) b = last_start(own.starts, own.B, (int)own.N, n0) - 1;
+    for (;;) {
+      if (++b >= own.B) return false;
+      int row0, nq;
+      seq_rows(own.starts, b, own.N, row0, nq);
+      row0 = __builtin_amdgcn_readfirstlane(row0), nq = __builtin_amdgcn_readfirstlane(nq);
+      if (row0 > n1) return false;
+      x.len = __builtin_amdgcn_readfirstlane(min(max(own.lens[b], 0), own.cap));
+      if (row0 + nq <= n0 || x.len == 0) continue;
+      const int off = (own.causal ? x.len - nq : 0x3fffffff) - row0, last = row0 + nq - 1;  // token n sees keys <= off + n
+      const int kend = max(min(x.len, off + min(n1, last) + 1), 0);
+      if (kend == 0) continue;
+      const int n = x.row0 + tok;
+      lim = live && n >= row0 && n <= last ? min(off + n, x.len - 1) : -1;
+      const int wn0 = __builtin_amdgcn_readfirstlane(x.row0 + (int)a.group.div(w0));
+      const int wn1 = __builtin_amdgcn_readfirstlane(x.row0 + (int)a.group.div(max(w1, 0)));
+      lim0 = wn0 >= row0 && wn1 <= last ? off + wn0 : -1;
+      wave_end = wave_live && wn0 <= last && wn1 >= row0 ? max(min(kend, off + min(wn1, last) + 1), 0) : 0;
+      t0 = 0, t1 = (kend + KVB - 1) / KVB;
+      table = own.table + (int64_t)b * own.table_ld;
+      __syncthreads();  // the stages have been read
+      next_page = group_page(a, table, key_of(0), x.len);
+      places(0);
+      bad = (uint32_t)bads & 0xffu;
+      issue(0, 0);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      return true;
+    }
+  };
+  do {
+    for (int t = t0; t < t1; t += 2) {
+      tile(t, std::integral_constant<int, 0>{});
+      if (t + 1 < t1) tile(t + 1, std::integral_constant<int, 1>{});
+    }
+  } while (F == kBothSets && next_sequence());
 
   // ---- epilogue: back to the true max, then the row or its range's carrier
   const float fix = m_true != kNegInf && m_run != kNegInf ? __builtin_amdgcn_exp2f((m_run - m_true) * c) : 1.f;
   const float l_sum = l_run + __shfl_xor(l_run, 32, 64);
   const int64_t i = (int64_t)(x.row0 + tok) * a.Hq + hq;
-  if (CARRIERS || x.split) {
+  if (F == kCarriers || x.split) {
     if (!live) return;
-    const int64_t at = part_at<CARRIERS>(a, i, split);
+    const int64_t at = part_at<F>(a, i, split);
     if (g == 0) {
       a.part[2 * at] = m_true;
       a.part[2 * at + 1] = l_sum * fix;
     }
-    float* num = part_numerators<CARRIERS>(a) + at * D;
+    float* num = part_numerators<F>(a) + at * D;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll

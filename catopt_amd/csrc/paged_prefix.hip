@@ -28,107 +28,144 @@ constexpr int lds_of() {
 template <int D, bool FEW>
 __device__ __forceinline__ void attend(const PagedArgs& a, uint32_t block, int tiles) {
   if constexpr (FEW)
-    paged_few<D, FewFour<D>, true>(a, block);
+    paged_few<D, FewFour<D>, kCarriers>(a, block);
   else
-    paged_tile_rows<D, true>(a, block, tiles);
+    paged_tile_rows<D, kCarriers>(a, a, block, tiles);
 }
 
 // p: the prefixes, o: the sequences' own keys.
 template <int D, bool PFEW, bool OFEW>
 __global__ __launch_bounds__(NT, 2) void paged_prefix_kernel(PagedArgs p, PagedArgs o, uint32_t p_blocks, int p_tiles,
                                                               int o_tiles) {
-  if (blockIdx.x < p_blocks)
-    attend<D, PFEW>(p, blockIdx.x, p_tiles);
+  const bool prefix = blockIdx.x < p_blocks;
+  const uint32_t block = prefix ? blockIdx.x : blockIdx.x - p_blocks;
+  if constexpr (PFEW == OFEW)  // the same code for both
+    attend<D, PFEW>(prefix ? p : o, block, prefix ? p_tiles : o_tiles);
+  else if (prefix)
+    attend<D, PFEW>(p, block, p_tiles);
   else
-    attend<D, OFEW>(o, blockIdx.x - p_blocks, o_tiles);
+    attend<D, OFEW>(o, block, o_tiles);
 }
 
-// The last of n ascending starts that is not above x; -1 where none is.
-__device__ __forceinline__ int last_start(const int32_t* starts, int n, int most, int x) {
-  const int lane = threadIdx.x & 63;
-  int at = -1;
-  for (int c = 0; c < n; c += 64) {
-    const int i = c + lane;
-    const int k = __popcll(__ballot(i < n && min(max(starts[min(i, n - 1)], 0), most) <= x));
-    at += k;
-    if (k < 64) break;
-  }
-  return at;
+// Rows enough to fill the CUs: a tile's rows see their group's prefix and then, with
+// the same accumulators, their sequences' own keys, one sequence after the other.
+template <int D>
+__global__ __launch_bounds__(NT, D == 64 ? 3 : 2) void paged_prefix_whole(PagedArgs p, PagedArgs o, int tiles) {
+  paged_tile_rows<D, kBothSets>(p, o, blockIdx.x, tiles);
 }
 
-// WAVES waves a row, D / 4 lanes to a carrier's numerators.
-template <int D, int WAVES>
-__global__ __launch_bounds__(NT) void paged_prefix_combine(PagedArgs p, PagedArgs o, int p_rows, int o_rows) {
-  constexpr int TPR = D / 4, GROUPS = 64 * WAVES / TPR;
-  const int lane = threadIdx.x & 63, tid = WAVES == 4 ? threadIdx.x : lane;
-  const int row = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + (int)(threadIdx.x >> 6);  // N Hq < 2^30
-  if (row >= o.N * o.Hq) return;
-  const int n = (int)o.q_heads.div(row), hq = row - n * o.Hq;
+// A token's own sequence and its group (-1: none); -1 where the token is no sequence's.
+__device__ __forceinline__ int find_sets(const PagedArgs& p, const PagedArgs& o, int n, int& group) {
   const int b = last_start(o.starts, o.B, (int)o.N, n);
-  if (b < 0) return;
-  // the ranges of the row's tiles: the own keys' behind the prefix'
-  uint64_t ranges = 0;
-  auto add = [&](const PagedArgs& a, int i, int tile_rows) {
-    PagedTile x{};
-    x.b = i;
-    set_rows<true>(a, i, x.row0, x.nq);
-    if (n < x.row0 || n >= x.row0 + x.nq) return false;
-    x.len = min(max(a.lens[i], 0), a.cap);
-    x.r0 = ((n - x.row0) * a.G + hq - (int)a.group.div(hq) * a.G) / tile_rows * tile_rows;
-    x.rows = min(tile_rows, x.nq * a.G - x.r0);
-    paged_ranges(a, x);
-    ranges |= __ballot(lane < a.splits && has_range(x, lane)) << a.part_first;
-    return true;
-  };
-  if (!add(o, b, o_rows)) return;
-  const int group = p.B > 0 ? last_start(p.groups, p.B, p.n_seq, b) : -1;
-  if (group >= 0) add(p, group, p_rows);
-  const int slots = o.part_ld;
+  group = b >= 0 && p.B > 0 ? last_start(p.groups, p.B, p.n_seq, b) : -1;
+  return b;
+}
+
+// Set a's ranges of row (n, hq), a bit for each of the row's carriers; none where
+// its sequence i does not have the token.
+__device__ __forceinline__ uint64_t set_ranges(const PagedArgs& a, int i, int n, int hq, int tile_rows) {
+  PagedTile x{};
+  x.b = i;
+  set_rows<kCarriers>(a, i, x.row0, x.nq);
+  if (n < x.row0 || n >= x.row0 + x.nq) return 0;
+  x.len = min(max(a.lens[i], 0), a.cap);
+  x.r0 = ((n - x.row0) * a.G + hq - (int)a.group.div(hq) * a.G) / tile_rows * tile_rows;
+  x.rows = min(tile_rows, x.nq * a.G - x.r0);
+  paged_ranges(a, x);
+  const int lane = threadIdx.x & 63;
+  return __ballot(lane < a.splits && has_range(x, lane)) << a.part_first;
+}
+
+// Rows of carriers to results: WAVES waves to ROWS rows, D / 4 lanes to a
+// carrier's numerators.  Four waves to a row where the rows alone do not fill the
+// CUs; else a wave to four rows, whose loads are on their way together.
+template <int D, int WAVES, int ROWS>
+__global__ __launch_bounds__(NT) void paged_prefix_combine(PagedArgs p, PagedArgs o, int p_rows, int o_rows) {
+  constexpr int TPR = D / 4, GROUPS = 64 * WAVES / TPR, U = 8 / ROWS;  // carriers at a time: U GROUPS of each row
+  const int lane = threadIdx.x & 63, tid = WAVES == 4 ? threadIdx.x : lane;
+  const int row0 = (WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + (int)(threadIdx.x >> 6)) * ROWS;  // N Hq < 2^30
+  const int rows = (int)o.N * o.Hq, slots = o.part_ld, k0 = tid / TPR;
   const float c = o.scale * kLog2e;
-  const float* ml = o.part + (int64_t)2 * row * slots;
-  const float* num = part_numerators<true>(o) + (int64_t)row * slots * D + 4 * (tid % TPR);
-  const bool mine = (ranges >> lane) & 1;
-  const float ms = mine ? ml[2 * lane] : kNegInf, ls = mine ? ml[2 * lane + 1] : 0.f;
-  float mx = ms;
+  const float* nums = part_numerators<kCarriers>(o) + 4 * (tid % TPR);
+  uint64_t ranges[ROWS];
+  float ms[ROWS], ls[ROWS];
+  f32x4 y[ROWS];
+  int last = -1, b = -1, group = -1;
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s, 64));
-  const float f = mine ? move_factor(ms, mx, c) : 0.f;
-  float lt = mine ? ls * f : 0.f;
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) lt += __shfl_xor(lt, s, 64);
-  f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
-  constexpr int U = 8;  // loads ahead of their additions
-  for (int s0 = 0; s0 < slots; s0 += U * GROUPS) {  // every lane stays: the factors come from lanes
-    f32x4 ys[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int s = s0 + i * GROUPS + tid / TPR;
-      ys[i] = s < slots && (ranges >> s) & 1 ? *reinterpret_cast<const f32x4*>(num + (int64_t)s * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < ROWS; ++i) {
+    const int row = row0 + i;
+    ranges[i] = 0, ms[i] = kNegInf, ls[i] = 0.f, y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (row >= rows) continue;
+    const int n = (int)o.q_heads.div(row), hq = row - n * o.Hq;
+    if (n != last) b = find_sets(p, o, n, group), last = n;
+    if (b < 0) continue;
+    ranges[i] = set_ranges(o, b, n, hq, o_rows);
+    if (ranges[i] && group >= 0) ranges[i] |= set_ranges(p, group, n, hq, p_rows);
+    if (ranges[i] >> lane & 1) {
+      const float* ml = o.part + (int64_t)2 * row * slots + 2 * lane;
+      ms[i] = ml[0], ls[i] = ml[1];
     }
+  }
+  f32x4 ys[ROWS][U];
+  auto load = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) y += ys[i] * __shfl(f, min(s0 + i * GROUPS + tid / TPR, 63), 64);
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = s0 + u * GROUPS + k0;
+        ys[i][u] = k < slots && (ranges[i] >> k & 1)
+                       ? *reinterpret_cast<const f32x4*>(nums + ((int64_t)(row0 + i) * slots + k) * D)
+                       : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+  };
+  load(0);
+  float f[ROWS], mx[ROWS], lt[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    mx[i] = ms[i];
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) mx[i] = fmaxf(mx[i], __shfl_xor(mx[i], s, 64));
+    f[i] = ranges[i] >> lane & 1 ? move_factor(ms[i], mx[i], c) : 0.f;
+    lt[i] = ls[i] * f[i];
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) lt[i] += __shfl_xor(lt[i], s, 64);
+  }
+  for (int s0 = 0; s0 < slots; s0 += U * GROUPS) {  // every lane stays: the factors come from lanes
+    if (s0 > 0) load(s0);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+      for (int u = 0; u < U; ++u) y[i] += ys[i][u] * __shfl(f[i], min(s0 + u * GROUPS + k0, 63), 64);
   }
   if constexpr (WAVES == 4) {
     __shared__ f32x4 sums[GROUPS][TPR];
-    sums[tid / TPR][tid % TPR] = y;
+    sums[k0][tid % TPR] = y[0];
     __syncthreads();
     if (tid < TPR) {
 #pragma unroll
-      for (int i = 1; i < GROUPS; ++i) y += sums[i][tid];
+      for (int i = 1; i < GROUPS; ++i) y[0] += sums[i][tid];
     }
   } else {
 #pragma unroll
-    for (int s = TPR; s < 64; s <<= 1)
+    for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], s, 64);
-  }
-  if (tid < TPR && 4 * tid < o.d) {
+      for (int s = TPR; s < 64; s <<= 1)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = finish(y[e], lt, o.normalize);
-    *reinterpret_cast<u32x2*>(o.o + (int64_t)n * o.o_t + (int64_t)hq * o.o_h + 4 * tid) =
-        u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+        for (int e = 0; e < 4; ++e) y[i][e] += __shfl_xor(y[i][e], s, 64);
   }
-  if (tid == 0) row_stats(o, row, mx, lt);
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    if (!ranges[i]) continue;  // no sequence's row: it stays as it is
+    const int row = row0 + i, n = (int)o.q_heads.div(row), hq = row - n * o.Hq;
+    if (tid < TPR && 4 * tid < o.d) {
+      f32x4 z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = finish(y[i][e], lt[i], o.normalize);
+      *reinterpret_cast<u32x2*>(o.o + (int64_t)n * o.o_t + (int64_t)hq * o.o_h + 4 * tid) =
+          u32x2{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
+    }
+    if (tid == 0) row_stats(o, row, mx[i], lt[i]);
+  }
 }
 
 // ------------------------------------------------------------------ host
@@ -142,33 +179,69 @@ struct Set {
 
 Set set_of(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t cap, bool few) {
   Set s{};
-  s.few = few;
-  s.splits = 0, s.min_keys = 128;
+  s.few = few, s.min_keys = 128;
   if (B == 0 || cap == 0) return s;
   s.tiles = paged_tiles(N, G, B, few ? kFewRows : kTileRows);
-  const int64_t groups = s.tiles * Hkv;
-  int64_t n = (512 + groups - 1) / groups;
-  const int64_t most = (cap + 255) / 256;
+  s.splits = 1;
+  return s;
+}
+void split(Set& s, int64_t Hkv, int n) { s.splits = n, s.blocks = s.tiles * Hkv * n; }
+
+// Ranges of few-row tiles: so many that 2048 workgroups share them out, of 128 keys
+// at least.
+int few_splits(int64_t groups, int64_t cap) {
+  int64_t n = (2048 + groups - 1) / groups;
+  const int64_t most = (cap + 127) / 128;
   if (n > most) n = most;
   if (n > kMaxSplits / 2) n = kMaxSplits / 2;
-  s.splits = n < 1 ? 1 : (int)n;
-  s.blocks = groups * s.splits;
-  return s;
+  return n < 1 ? 1 : (int)n;
+}
+
+// Ranges of 128-row tiles: the fewest (their carriers go through memory, at 6 TB/s)
+// in which they are not what the launch takes longest for, by the times that
+// paged attention goes by; `beside`: what the other set takes meanwhile, in us.
+int tile_splits(int64_t groups, int64_t rows, int64_t D, int64_t cap, double beside) {
+  const double alone = D == 128 ? 1.7 : 1.0, shared = D == 128 ? 2.4 : 1.5;
+  double best = 0;
+  int splits = 1;
+  for (int s = 1; s <= kMaxSplits / 2; ++s) {
+    const int64_t keys = ((cap + s - 1) / s + 127) / 128 * 128, wgs = groups * s;
+    const double rounds = wgs <= 512 ? 1 : wgs / 512.0, tile = wgs <= 256 && beside == 0 ? alone : shared;
+    const double own = rounds * (keys / 64) * tile;
+    const double us = (own > beside ? own : beside) + (double)rows * s * D * 8 / 6e6;
+    if (s == 1 || us < best) best = us, splits = s;
+    if (keys <= 128) break;
+  }
+  return splits;
 }
 
 struct Plan {
   Set p, o;
+  bool whole;
   int64_t carriers;
   int64_t bytes(int64_t rows, int64_t D) const { return 4 * (((2 * rows * carriers + 3) & ~(int64_t)3) + rows * carriers * D); }
 };
 
-Plan plan_of(int64_t P, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t p_cap, int64_t cap) {
+// Few rows: 32-row tiles whenever the sequences (or groups) have 32 rows per key
+// head or fewer on average.  The groups have more than their members, so three of
+// the four forms are there.
+Plan plan_of(int64_t P, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t d, int64_t p_cap, int64_t cap) {
   Plan x;
-  const int64_t G = Hq / Hkv;
+  const int64_t G = Hq / Hkv, D = d <= 64 ? 64 : 128, rows = N * Hq;
+  if (cap < 1) cap = 1;  // without own keys their empty carriers
   const bool o_few = N * G <= kFewRows * B, p_few = o_few && N * G <= kFewRows * P;
   x.p = set_of(P, N, G, Hkv, p_cap, p_few);
-  x.o = set_of(B, N, G, Hkv, cap < 1 ? 1 : cap, o_few);  // without own keys its empty carriers
-  x.carriers = x.p.splits + x.o.splits;
+  x.o = set_of(B, N, G, Hkv, cap, o_few);
+  split(x.o, Hkv, o_few ? few_splits(x.o.tiles * Hkv, cap) : tile_splits(x.o.tiles * Hkv, rows, D, cap, 0));
+  if (x.p.splits) {
+    // half of what the own keys' bytes take, were every sequence as long as its table: so much is there for sure
+    // beside them
+    const double beside = o_few ? (double)B * cap * Hkv * d * 4 / 5e6 / 2 : 0;
+    split(x.p, Hkv, p_few ? few_splits(x.p.tiles * Hkv, p_cap) : tile_splits(x.p.tiles * Hkv, rows, D, p_cap, beside));
+  }
+  x.whole = x.p.splits == 1 && x.o.splits == 1 && !o_few;
+  if (x.whole) x.p.tiles = paged_tiles(N, G, P + 2, kTileRows), x.p.blocks = x.p.tiles * Hkv, x.o.blocks = 0;
+  x.carriers = x.whole ? 0 : x.p.splits + x.o.splits;
   return x;
 }
 
@@ -181,21 +254,33 @@ int32_t launch(const PagedArgs& p, const PagedArgs& o, const Plan& x, hipStream_
   if (r != CATOPT_OK) return r;
   const int64_t blocks = x.p.blocks + x.o.blocks, rows = o.N * o.Hq;
   const bool wide = rows < 2048;  // four waves a row where the rows alone do not fill the CUs
-  const int64_t nc = wide ? rows : (rows + 3) / 4;
+  const int64_t nc = wide ? rows : (rows + 15) / 16;
   if (!grid_fits(blocks, NT) || !grid_fits(nc, NT)) return CATOPT_E_UNSUPPORTED;
   kernel<<<dim3((uint32_t)blocks), dim3(NT), bytes, s>>>(p, o, (uint32_t)x.p.blocks, (int)x.p.tiles, (int)x.o.tiles);
   CATOPT_LAUNCH_CHECK();
   const int p_rows = PFEW ? kFewRows : kTileRows, o_rows = OFEW ? kFewRows : kTileRows;
   if (wide)
-    paged_prefix_combine<D, 4><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
+    paged_prefix_combine<D, 4, 1><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
   else
-    paged_prefix_combine<D, 1><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
+    paged_prefix_combine<D, 1, 4><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
+  CATOPT_LAUNCH_CHECK();
+  return CATOPT_OK;
+}
+
+template <int D>
+int32_t launch_whole(const PagedArgs& p, const PagedArgs& o, const Plan& x, hipStream_t s) {
+  static bool done[kDevices] = {};
+  const int32_t r = allow_lds(reinterpret_cast<const void*>(&paged_prefix_whole<D>), TileLds<D>::BYTES, done);
+  if (r != CATOPT_OK) return r;
+  if (!grid_fits(x.p.blocks, NT)) return CATOPT_E_UNSUPPORTED;
+  paged_prefix_whole<D><<<dim3((uint32_t)x.p.blocks), dim3(NT), TileLds<D>::BYTES, s>>>(p, o, (int)x.p.tiles);
   CATOPT_LAUNCH_CHECK();
   return CATOPT_OK;
 }
 
 template <int D>
 int32_t launch_form(const PagedArgs& p, const PagedArgs& o, const Plan& x, hipStream_t s) {
+  if (x.whole) return launch_whole<D>(p, o, x, s);
   if (x.p.few) return launch<D, true, true>(p, o, x, s);
   return x.o.few ? launch<D, false, true>(p, o, x, s) : launch<D, false, false>(p, o, x, s);
 }
@@ -215,7 +300,7 @@ extern "C" int64_t catopt_hip_paged_prefix_attn_workspace_bytes(int64_t P, int64
   if (n_table > lim || n_prefix_table > lim || page_size > lim || n_table * page_size >= lim || n_prefix_table * page_size >= lim)
     return -1;
   if (B == 0 || N == 0) return 0;
-  return plan_of(P, B, N, Hq, Hkv, n_prefix_table * page_size, n_table * page_size).bytes(N * Hq, d <= 64 ? 64 : 128);
+  return plan_of(P, B, N, Hq, Hkv, d, n_prefix_table * page_size, n_table * page_size).bytes(N * Hq, d <= 64 ? 64 : 128);
 }
 
 extern "C" int32_t catopt_hip_paged_prefix_attn_fwd(
@@ -248,8 +333,8 @@ extern "C" int32_t catopt_hip_paged_prefix_attn_fwd(
     return CATOPT_E_INVAL;
   // the rows of one load lie within 31 bits of its resource's base
   if (s[4] > (1 << 26) || s[7] > (1 << 26)) return CATOPT_E_UNSUPPORTED;
-  if (!workspace || !aligned16(workspace) || workspace_bytes < need) return CATOPT_E_WORKSPACE;
-  const Plan x = plan_of(P, B, N, Hq, Hkv, n_prefix_table * page_size, n_table * page_size);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return CATOPT_E_WORKSPACE;
+  const Plan x = plan_of(P, B, N, Hq, Hkv, d, n_prefix_table * page_size, n_table * page_size);
   PagedArgs a{};
   a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k_pages);
   a.v = static_cast<const uint16_t*>(v_pages), a.o = static_cast<uint16_t*>(o);
@@ -268,6 +353,7 @@ extern "C" int32_t catopt_hip_paged_prefix_attn_fwd(
   set(p, x.p, P, prefix_table, prefix_ld, n_prefix_table * page_size, prefix_lens);
   set(own, x.o, B, block_table, table_ld, n_table * page_size, kv_lens);
   p.groups = prefix_starts, own.causal = causal != 0, own.part_first = x.p.splits;
+  if (x.whole) p.B = (int)P + 2;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return d <= 64 ? launch_form<64>(p, own, x, st) : launch_form<128>(p, own, x, st);
 }

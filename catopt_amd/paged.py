@@ -404,12 +404,14 @@ def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         mp, lp = m.data_ptr(), l.data_ptr()
     if B and N:
         wsb = _prefix_workspace(P, B, N, Hq, Hkv, d, n_prefix, n_table, page)
-        ws = q.new_empty(wsb // 2)
+        if wsb:
+            ws = q.new_empty(wsb // 2)
+            ws_at = ws.data_ptr()
         st = _launch(dev, L.load().catopt_hip_paged_prefix_attn_fwd, L.BF16, P, B, N, Hq, Hkv, d, q_at, k_pages.data_ptr(),
                      v_pages.data_ptr(), n_pages, page, p_table.data_ptr(), p_ld, n_prefix, prefix_lens.data_ptr(),
                      prefix_starts.data_ptr(), table.data_ptr(), table_ld, n_table, kv_lens.data_ptr(), q_starts.data_ptr(),
                      scale, 1 if causal else 0, 2 if empty_rows == "zero" else 1, out.data_ptr(), mp, lp,
-                     _S10(q0, q1, *ks, *vs, o0, o1), ws.data_ptr(), wsb)
+                     _S10(q0, q1, *ks, *vs, o0, o1), ws_at, wsb)
         if st:
             _check("paged_prefix_attention", st)
     return (out, m, l) if return_ml else out
