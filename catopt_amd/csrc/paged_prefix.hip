@@ -37,14 +37,11 @@ __device__ __forceinline__ void attend(const PagedArgs& a, uint32_t block, int t
 template <int D, bool PFEW, bool OFEW>
 __global__ __launch_bounds__(NT, 2) void paged_prefix_kernel(PagedArgs p, PagedArgs o, uint32_t p_blocks, int p_tiles,
                                                               int o_tiles) {
-  const bool prefix = blockIdx.x < p_blocks;
-  const uint32_t block = prefix ? blockIdx.x : blockIdx.x - p_blocks;
-  if constexpr (PFEW == OFEW)  // the same code for both
-    attend<D, PFEW>(prefix ? p : o, block, prefix ? p_tiles : o_tiles);
-  else if (prefix)
-    attend<D, PFEW>(p, block, p_tiles);
+  // (one copy of the code for two sets of one kind, by pointers, is a us slower at 4 steps and at 22 short questions)
+  if (blockIdx.x < p_blocks)
+    attend<D, PFEW>(p, blockIdx.x, p_tiles);
   else
-    attend<D, OFEW>(o, block, o_tiles);
+    attend<D, OFEW>(o, blockIdx.x - p_blocks, o_tiles);
 }
 
 // Rows enough to fill the CUs: a tile's rows see their group's prefix and then, with
@@ -76,96 +73,68 @@ __device__ __forceinline__ uint64_t set_ranges(const PagedArgs& a, int i, int n,
   return __ballot(lane < a.splits && has_range(x, lane)) << a.part_first;
 }
 
-// Rows of carriers to results: WAVES waves to ROWS rows, D / 4 lanes to a
-// carrier's numerators.  Four waves to a row where the rows alone do not fill the
-// CUs; else a wave to four rows, whose loads are on their way together.
-template <int D, int WAVES, int ROWS>
+// A row's carriers to its result: WAVES waves, D / 4 lanes to a carrier's numerators.
+template <int D, int WAVES>
 __global__ __launch_bounds__(NT) void paged_prefix_combine(PagedArgs p, PagedArgs o, int p_rows, int o_rows) {
-  constexpr int TPR = D / 4, GROUPS = 64 * WAVES / TPR, U = 8 / ROWS;  // carriers at a time: U GROUPS of each row
+  constexpr int TPR = D / 4, GROUPS = 64 * WAVES / TPR, U = 8;  // loads ahead of their additions
   const int lane = threadIdx.x & 63, tid = WAVES == 4 ? threadIdx.x : lane;
-  const int row0 = (WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + (int)(threadIdx.x >> 6)) * ROWS;  // N Hq < 2^30
-  const int rows = (int)o.N * o.Hq, slots = o.part_ld, k0 = tid / TPR;
+  const int row = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + (int)(threadIdx.x >> 6);  // N Hq < 2^30
+  if (row >= o.N * o.Hq) return;
+  const int n = (int)o.q_heads.div(row), hq = row - n * o.Hq;
+  int group;
+  const int b = find_sets(p, o, n, group);
+  uint64_t ranges = b >= 0 ? set_ranges(o, b, n, hq, o_rows) : 0;
+  if (!ranges) return;  // no sequence's row
+  if (group >= 0) ranges |= set_ranges(p, group, n, hq, p_rows);
+  const int slots = o.part_ld, k0 = tid / TPR;
   const float c = o.scale * kLog2e;
-  const float* nums = part_numerators<kCarriers>(o) + 4 * (tid % TPR);
-  uint64_t ranges[ROWS];
-  float ms[ROWS], ls[ROWS];
-  f32x4 y[ROWS];
-  int last = -1, b = -1, group = -1;
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int row = row0 + i;
-    ranges[i] = 0, ms[i] = kNegInf, ls[i] = 0.f, y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (row >= rows) continue;
-    const int n = (int)o.q_heads.div(row), hq = row - n * o.Hq;
-    if (n != last) b = find_sets(p, o, n, group), last = n;
-    if (b < 0) continue;
-    ranges[i] = set_ranges(o, b, n, hq, o_rows);
-    if (ranges[i] && group >= 0) ranges[i] |= set_ranges(p, group, n, hq, p_rows);
-    if (ranges[i] >> lane & 1) {
-      const float* ml = o.part + (int64_t)2 * row * slots + 2 * lane;
-      ms[i] = ml[0], ls[i] = ml[1];
-    }
-  }
-  f32x4 ys[ROWS][U];
+  const float* ml = o.part + (int64_t)2 * row * slots;
+  const float* num = part_numerators<kCarriers>(o) + (int64_t)row * slots * D + 4 * (tid % TPR);
+  const bool mine = ranges >> lane & 1;
+  const float ms = mine ? ml[2 * lane] : kNegInf, ls = mine ? ml[2 * lane + 1] : 0.f;
+  f32x4 ys[U];
   auto load = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = s0 + u * GROUPS + k0;
-        ys[i][u] = k < slots && (ranges[i] >> k & 1)
-                       ? *reinterpret_cast<const f32x4*>(nums + ((int64_t)(row0 + i) * slots + k) * D)
-                       : f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+    for (int i = 0; i < U; ++i) {
+      const int k = s0 + i * GROUPS + k0;
+      ys[i] = k < slots && (ranges >> k & 1) ? *reinterpret_cast<const f32x4*>(num + (int64_t)k * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
   };
   load(0);
-  float f[ROWS], mx[ROWS], lt[ROWS];
+  float mx = ms;
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    mx[i] = ms[i];
+  for (int s = 32; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor(mx, s, 64));
+  const float f = mine ? move_factor(ms, mx, c) : 0.f;
+  float lt = ls * f;
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) mx[i] = fmaxf(mx[i], __shfl_xor(mx[i], s, 64));
-    f[i] = ranges[i] >> lane & 1 ? move_factor(ms[i], mx[i], c) : 0.f;
-    lt[i] = ls[i] * f[i];
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) lt[i] += __shfl_xor(lt[i], s, 64);
-  }
+  for (int s = 32; s > 0; s >>= 1) lt += __shfl_xor(lt, s, 64);
+  f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < slots; s0 += U * GROUPS) {  // every lane stays: the factors come from lanes
     if (s0 > 0) load(s0);
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-      for (int u = 0; u < U; ++u) y[i] += ys[i][u] * __shfl(f[i], min(s0 + u * GROUPS + k0, 63), 64);
+    for (int i = 0; i < U; ++i) y += ys[i] * __shfl(f, min(s0 + i * GROUPS + k0, 63), 64);
   }
   if constexpr (WAVES == 4) {
     __shared__ f32x4 sums[GROUPS][TPR];
-    sums[k0][tid % TPR] = y[0];
+    sums[k0][tid % TPR] = y;
     __syncthreads();
     if (tid < TPR) {
 #pragma unroll
-      for (int i = 1; i < GROUPS; ++i) y[0] += sums[i][tid];
+      for (int i = 1; i < GROUPS; ++i) y += sums[i][tid];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i)
+    for (int s = TPR; s < 64; s <<= 1)
 #pragma unroll
-      for (int s = TPR; s < 64; s <<= 1)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[i][e] += __shfl_xor(y[i][e], s, 64);
+      for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], s, 64);
   }
+  if (tid < TPR && 4 * tid < o.d) {
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    if (!ranges[i]) continue;  // no sequence's row: it stays as it is
-    const int row = row0 + i, n = (int)o.q_heads.div(row), hq = row - n * o.Hq;
-    if (tid < TPR && 4 * tid < o.d) {
-      f32x4 z;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) z[e] = finish(y[i][e], lt[i], o.normalize);
-      *reinterpret_cast<u32x2*>(o.o + (int64_t)n * o.o_t + (int64_t)hq * o.o_h + 4 * tid) =
-          u32x2{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3])};
-    }
-    if (tid == 0) row_stats(o, row, mx[i], lt[i]);
+    for (int e = 0; e < 4; ++e) y[e] = finish(y[e], lt, o.normalize);
+    *reinterpret_cast<u32x2*>(o.o + (int64_t)n * o.o_t + (int64_t)hq * o.o_h + 4 * tid) =
+        u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
   }
+  if (tid == 0) row_stats(o, row, mx, lt);
 }
 
 // ------------------------------------------------------------------ host
@@ -187,10 +156,14 @@ Set set_of(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t cap, bool few) 
 }
 void split(Set& s, int64_t Hkv, int n) { s.splits = n, s.blocks = s.tiles * Hkv * n; }
 
-// Ranges of few-row tiles: so many that 2048 workgroups share them out, of 128 keys
-// at least.
+// Ranges of few-row tiles: of 1024 keys, which evens out sequences of unlike
+// lengths, or as many as 1024 workgroups need, of 128 keys at least.  More cost their
+// workgroups' starts: 64 steps of 100 to 1500 own keys take 48.8 us in two, 52.0 in
+// three and 55.6 in four; 4 steps over 500 and 200 keys 10.6 in four and two and
+// 13.9 in one.
 int few_splits(int64_t groups, int64_t cap) {
-  int64_t n = (2048 + groups - 1) / groups;
+  int64_t n = (1024 + groups - 1) / groups;
+  if (n < cap / 1024) n = cap / 1024;
   const int64_t most = (cap + 127) / 128;
   if (n > most) n = most;
   if (n > kMaxSplits / 2) n = kMaxSplits / 2;
@@ -254,15 +227,15 @@ int32_t launch(const PagedArgs& p, const PagedArgs& o, const Plan& x, hipStream_
   if (r != CATOPT_OK) return r;
   const int64_t blocks = x.p.blocks + x.o.blocks, rows = o.N * o.Hq;
   const bool wide = rows < 2048;  // four waves a row where the rows alone do not fill the CUs
-  const int64_t nc = wide ? rows : (rows + 15) / 16;
+  const int64_t nc = wide ? rows : (rows + 3) / 4;
   if (!grid_fits(blocks, NT) || !grid_fits(nc, NT)) return CATOPT_E_UNSUPPORTED;
   kernel<<<dim3((uint32_t)blocks), dim3(NT), bytes, s>>>(p, o, (uint32_t)x.p.blocks, (int)x.p.tiles, (int)x.o.tiles);
   CATOPT_LAUNCH_CHECK();
   const int p_rows = PFEW ? kFewRows : kTileRows, o_rows = OFEW ? kFewRows : kTileRows;
   if (wide)
-    paged_prefix_combine<D, 4, 1><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
+    paged_prefix_combine<D, 4><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
   else
-    paged_prefix_combine<D, 1, 4><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
+    paged_prefix_combine<D, 1><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
   CATOPT_LAUNCH_CHECK();
   return CATOPT_OK;
 }

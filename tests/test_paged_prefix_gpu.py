@@ -73,6 +73,48 @@ def test_both_sets(pre, groups, nq, own, Hq, Hkv, d, page):
     _run(pre, groups, nq, own, Hq, Hkv, d, page, seed=sum(own) + d)
 
 
+# enough rows for one tile loop over both sets (no carriers): 128-row tiles of several sequences, of one and a part of one
+WHOLE = [
+    ([300], [0, 40], [52] * 40, [52 + 3 * i for i in range(40)], 32, 8, 64, 16, True),
+    ([90, 257], [1, 3, 7], [300, 1, 700, 33, 0, 900, 40, 350], [300, 60, 700, 400, 9, 950, 40, 350], 32, 8, 64, 32, True),
+    ([200], [0, 3], [1000, 500, 600], [1000, 800, 600], 32, 32, 128, 64, True),
+    ([64, 0], [0, 25, 50], [44] * 50, [44] * 50, 30, 10, 40, 8, False),
+]
+
+
+@pytest.mark.parametrize("pre,groups,nq,own,Hq,Hkv,d,page,causal", WHOLE)
+def test_many_rows(pre, groups, nq, own, Hq, Hkv, d, page, causal):
+    c, q, o = _run(pre, groups, nq, own, Hq, Hkv, d, page, seed=len(nq), causal=causal, slot_major=not causal)
+    n, width = sum(nq), c.cache.table.shape[1]
+    assert P._prefix_workspace(len(pre), len(nq), n, Hq, Hkv, d, width, width, page) == 0
+    if not causal:
+        return
+    # values that are not finite, invalid pages, rows that see nothing, padded rows
+    cache = c.cache
+    for b, j, x in ((0, 3, float("inf")), (len(pre), 20, float("nan")), (len(pre) + 2, 40, float("-inf"))):
+        page_at, s = (t[j] for t in cache.where(b, cache.lens[b]))
+        cache.v[page_at, 0, s, 5] = x
+    o, m, l = c.call(q, nq, d ** -0.5, return_ml=True)
+    check_attention(c, q, nq, c.lens(), o, scale=d ** -0.5, m=m, l=l)
+    out = torch.full((n + 5, Hq, d), 9.0, device=DEV, dtype=BF16)
+    padded = torch.cat([q, torch.full_like(q[:5], float("nan"))])
+    c.call(padded, nq, d ** -0.5, out=out)
+    assert (out[n:] == 9).all() and torch.equal(torch.nan_to_num(out[:n]), torch.nan_to_num(o))
+    good = cache.table.clone()
+    cache.table[0, 1], cache.table[len(pre), 0] = -1, cache.n_pages
+    bad = c.call(q, nq, d ** -0.5)
+    cache.table.copy_(good)
+    keep = [torch.ones(k, dtype=torch.bool, device=DEV) for k in c.lens()]
+    for b in range(len(nq)):
+        if c.group(b) == 0:
+            keep[b][page:min(2 * page, pre[0])] = False
+    at = pre[c.group(0)] if c.group(0) is not None else 0
+    keep[0][at:at + page] = False
+    check_attention(c, q, nq, c.lens(), bad, scale=d ** -0.5, keep=keep)
+    none = c.call(q, nq, d ** -0.5, pre_lens=ints([0] * len(pre)), lens=ints([0] * len(nq)), empty_rows="zero")
+    assert (none == 0).all()
+
+
 @pytest.mark.parametrize("pre,groups,nq,own,Hq,Hkv,d,page", CASES[2::4])
 def test_all_own_keys_seen(pre, groups, nq, own, Hq, Hkv, d, page):
     _run(pre, groups, nq, own, Hq, Hkv, d, page, seed=d, causal=False, slot_major=True)
