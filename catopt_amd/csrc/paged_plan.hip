@@ -5,9 +5,10 @@
 // prefix sum over the sequences, the new pages' places in the pool another one.
 // Every workgroup forms the sums it needs by itself, 512 sequences at a time, so
 // one launch does without a barrier over workgroups; block 0 writes what belongs
-// to the sequences, the others a slice of the tokens each.  A slice looks its
-// sequence up in LDS and takes a new token's page from the pool, where block 0
-// takes it for the table from, so that no block reads what another one writes.
+// to the sequences, the others a slice of the tokens each, with the table's new
+// entries: a new page's first key is a new token's.  A slice looks its sequences up
+// in LDS and takes new pages from the pool by their number, so that no block reads
+// what another one writes.
 #include "paged.hpp"
 
 namespace catopt {
@@ -103,10 +104,6 @@ __global__ __launch_bounds__(NT) void paged_extend_kernel(ExtendArgs a, int stat
         if (b == a.B - 1) a.starts[a.B] = end;
         a.lens_out[b] = after;
       }
-      for (int j = pages + tid; j < pages + all_pages; j += NT) {
-        const int i = find_last(c.first, here, j);  // the last one that starts there: it has a page
-        a.table[(int64_t)(b0 + i) * a.table_ld + c.held[i] + j - c.first[i]] = pool_page(a, count, j);
-      }
     }
     const int next = min(sum + all, a.N);
     for (int t = max(t0, sum) + tid; t < min(t1, next); t += NT) {
@@ -114,8 +111,16 @@ __global__ __launch_bounds__(NT) void paged_extend_kernel(ExtendArgs a, int stat
       int64_t slot = -1;
       if (key < a.reach) {
         const int p = (int)a.page.div(key);
-        const int id = p < c.held[i] ? a.table[(int64_t)(b0 + i) * a.table_ld + p] : pool_page(a, count, c.first[i] + p - c.held[i]);
-        if (id >= 0) slot = (int64_t)id * a.page.d + (key - p * (int)a.page.d);
+        const int in = key - p * (int)a.page.d;
+        int32_t* entry = a.table + (int64_t)(b0 + i) * a.table_ld + p;
+        int id;
+        if (p < c.held[i]) {
+          id = *entry;
+        } else {  // a new page: its first key is a new one, whose token writes the table
+          id = pool_page(a, count, c.first[i] + p - c.held[i]);
+          if (in == 0) *entry = id;
+        }
+        if (id >= 0) slot = (int64_t)id * a.page.d + in;
       }
       a.slots[t] = slot;
       a.positions[t] = (int64_t)key + (a.offsets ? a.offsets[b0 + i] : 0);
