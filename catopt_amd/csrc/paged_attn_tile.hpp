@@ -286,7 +286,7 @@ __device__ __forceinline__ void paged_tile_rows(const PagedArgs& a, const PagedA
   int b = -1;
   const int n0 = x.row0 + (int)a.group.div(x.r0), n1 = x.row0 + (int)a.group.div(x.r0 + x.rows - 1);  // the tile's tokens
   auto next_sequence = [&]() -> bool {
-    if (b < 0) b = last_start(own.starts, own.B, (int)own.N, n0) - 1;
+    if (b < 0) b = max(last_start(own.starts, own.B, (int)own.N, n0), 0) - 1;
     for (;;) {
       if (++b >= own.B) return false;
       int row0, nq;

@@ -752,7 +752,7 @@ extern "C" int32_t catopt_hip_sample(int32_t dtype, int64_t B, int64_t V, const 
   }
   if (!workspace || workspace_bytes < need || !aligned16(workspace)) return CATOPT_E_WORKSPACE;
   const Plan p = plan_of(B, V, probs != nullptr);
-  if (!grid_fits(B * p.chunks, CT) || !grid_fits(B, RT) || !grid_fits(B * ((V + 4095) / 4096 + 1), PT)) return CATOPT_E_UNSUPPORTED;
+  if (!grid_fits(B * p.chunks, CT) || !grid_fits(B, RT) || !grid_fits(B * ((V + PT * PIECES * 4 - 1) / (PT * PIECES * 4)), PT)) return CATOPT_E_UNSUPPORTED;
   SampleArgs a{};
   a.x = logits, a.ld = B > 1 ? ld : 0, a.ld_probs = B > 1 ? ld_probs : 0, a.V = (int)V, a.B = (int)B, a.chunks = (int)p.chunks;
   a.t_row = temperature, a.p_row = top_p, a.low_row = min_p, a.k_row = top_k;
