@@ -76,13 +76,13 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
     *head = h;
   }
   if (!binned || m == -__builtin_inff()) return;
-  const Grid g(s.t, m);
+  const Grid g(factor(s.t, m), m);
   auto add = [&](float x) {
     const double on = g.on(x);
-    const uint64_t bin = g.below(on);
+    const uint32_t bin = g.bin(on);
     if (bin < kBins)
       atomicAdd(reinterpret_cast<unsigned long long*>(bins + bin),
-                (unsigned long long)(g.weight(g.rest(x, on)) | 1ull << kCount));
+                (unsigned long long)(g.weight(g.part(on)) | 1ull << kCount));
   };
 #pragma unroll
   for (int j = 0; j < P; ++j)
@@ -220,20 +220,20 @@ struct Search {
     for (int j = 0; j < U; ++j) first[j] = r.load(threadIdx.x + j * RT);
   }
 
-  __device__ __forceinline__ int bin_of(float x, double& rest) const {
+  __device__ __forceinline__ int bin_of(float x, uint32_t& part) const {
     const double on = g.on(x);
-    rest = g.rest(x, on);
-    const uint64_t bin = g.below(on);
+    part = g.part(on);
+    const uint32_t bin = g.bin(on);
     return bin < kBins ? (int)bin : kBins;
   }
 
   // Finite numbers that no logit of bins up to b is below, or from b on above.
   __device__ __forceinline__ float floor_of(int b) const {
-    const float f = (float)((g.ref - kGrid - b - 0.5) / g.c);
+    const float f = (float)((g.top - b - 0x1p-30) / g.c);
     return fmaxf(f - fabsf(f) * 0x1p-22f - 0x1p-140f, -0x1.fffffep127f);
   }
   __device__ __forceinline__ float top_of(int b) const {
-    const float f = (float)((g.ref - kGrid - b + 0.5) / g.c);
+    const float f = (float)((g.top - b + 1) / g.c);
     return f + fabsf(f) * 0x1p-22f + 0x1p-140f;
   }
 
@@ -278,14 +278,14 @@ struct Search {
   }
   __device__ __forceinline__ uint64_t place_of(int i) const { return place(finite_top(r.value(i)), i); }
 
-  // f(place, rest) for the row's logits in a bin, one by one.
+  // f(place, part) for the row's logits in a bin, one by one.
   template <typename F>
   __device__ __forceinline__ void each_in_row(int b, F f) const {
 #pragma unroll 1
     for (int i = threadIdx.x; i < r.V; i += RT) {
       const uint64_t at = place_of(i);
-      double rest;
-      if (bin_of(logit_of(at), rest) == b) f(at, rest);
+      uint32_t part;
+      if (bin_of(logit_of(at), part) == b) f(at, part);
     }
   }
   // The same of the list, for places from lo to hi.
@@ -295,8 +295,8 @@ struct Search {
     for (uint32_t i = threadIdx.x; i < n_list; i += RT) {
       const uint64_t at = s.list[i];
       if (at < lo || at > hi) continue;
-      double rest;
-      if (bin_of(logit_of(at), rest) == b) f(at, rest);
+      uint32_t part;
+      if (bin_of(logit_of(at), part) == b) f(at, part);
     }
   }
 
@@ -362,13 +362,13 @@ struct Search {
       const bool few = n <= 64;
       const int bits = 64 - __builtin_clzll((hi - lo) | 1), shift = max(bits - 7, 0);
       Step& t = begin();
-      auto take = [&](uint64_t at, double rest) {
+      auto take = [&](uint64_t at, uint32_t part) {
         if (at < lo || at > hi) return;
         if (few) {
           t.last[atomicAdd(&t.count, 1u) & 63] = at;
         } else {
           const int i = (int)((at - lo) >> shift);
-          atomicAdd(reinterpret_cast<unsigned long long*>(t.weight + i), (unsigned long long)g.weight(rest));
+          atomicAdd(reinterpret_cast<unsigned long long*>(t.weight + i), (unsigned long long)g.weight(part));
           atomicMin(reinterpret_cast<unsigned long long*>(t.least + i), (unsigned long long)at);
           atomicMax(reinterpret_cast<unsigned long long*>(t.most + i), (unsigned long long)at);
           atomicAdd(t.n + i, 1u);
@@ -383,9 +383,9 @@ struct Search {
       if (threadIdx.x < 64 && few) {  // in order
         const int m = min((int)t.count, 64);
         const uint64_t last = lane < m ? t.last[lane] : ~0ull, at = by_rank_of(last, lanes_below(last, 0, m, 1), m);
-        double rest;
-        bin_of(logit_of(at), rest);
-        const uint64_t upto = wave_scan(lane < m ? g.weight(rest) : 0) + before;
+        uint32_t part;
+        bin_of(logit_of(at), part);
+        const uint64_t upto = wave_scan(lane < m ? g.weight(part) : 0) + before;
         const uint64_t some = __ballot(lane < m && meets(find, target, upto, n_before + lane + 1));
         const int from = some ? __builtin_ctzll(some) : max(m - 1, 0);
         if (lane == from) found.lo = at, found.sum = upto;
@@ -457,18 +457,18 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     if (tid == 0) {
       a.tokens[row] = valid ? top : -1;
       a.logprobs[row] = valid ? 0.f : __builtin_nanf("");
-      if (a.rows) a.rows[row] = RowState{0, 0, 0, 0, 0, valid ? kOneHot : kNone, top, 0.f};
+      if (a.rows) a.rows[row] = RowState{0, 0, 0, 0, valid ? kOneHot : kNone, top, 0.f, 0.f};
     }
     return;
   }
-  double rest;
-  Search<T> find(s, reader, Grid(set.t, m), first);
-  const double c = find.g.c, ref = find.g.ref;
+  uint32_t part;
+  Search<T> find(s, reader, Grid(factor(set.t, m), m), first);
+  const double c = find.g.c;
   // ---- the row's bins from the chunks'
   for (int i = tid; i < a.chunks; i += RT) {
     const float cm = heads[i].max;
     // by the row's factor: it is the chunk's too wherever the chunk has a bin of the row's
-    s.off[i] = find.bin_of(cm, rest);
+    s.off[i] = find.bin_of(cm, part);
   }
   find.clear(s.steps[0]);
   __syncthreads();
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   uint64_t cut_at = ~0ull, total = s.cum[kBins - 1];
   bool by_rank = set.k && s.cum_n[kBins - 1] > set.k, by_sum = set.p < 1, by_low = set.low > 0;
   const double low = by_low ? (double)m * c + 16 * log2(fmin(set.low, 1.0)) : -__builtin_inf();
-  const double low_bin = by_low ? ref - kGrid - rint(low) : kBins;
+  const double low_bin = by_low ? find.g.top - floor(low) : kBins;
   auto before = [&](int b) { return b > 0 ? s.cum[b - 1] : 0ull; };
   auto before_n = [&](int b) { return b > 0 ? s.cum_n[b - 1] : 0u; };
   auto within = [&](int b, uint64_t sum) { return before(b) + (uint64_t)rint((double)sum * scale_of(b)); };
@@ -568,9 +568,9 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
       __syncthreads();
       if (wave > 0) return;
       at = by_rank_of(at, (int)t.n[lane], n_list);
-      const int bin = find.bin_of(logit_of(at), rest);
+      const int bin = find.bin_of(logit_of(at), part);
       const int n_all = __builtin_popcountll(__ballot(lane < n_list && bin <= end));
-      const double sums = wave_scan(lane < n_all ? (double)find.g.weight(rest) * scale_of(bin) : 0);
+      const double sums = wave_scan(lane < n_all ? (double)find.g.weight(part) * scale_of(bin) : 0);
       const double whole = by_rank ? lane_f64(sums, (int)set.k - 1) : (double)total;
       bool kept = lane < (by_rank ? (int)set.k : n_all);
       if (by_sum) {
@@ -585,17 +585,17 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
       const double log2_total = log2(kept_sum) - kUnits;
       if (lane == from) {
         a.tokens[row] = (int64_t)(uint32_t)at;
-        a.logprobs[row] = (float)(((rest - bin) / 16 - log2_total) * 0.6931471805599453);
+        a.logprobs[row] = (float)((Grid::log_weight(bin, part) / 16 - log2_total) * 0.6931471805599453);
       }
-      if (lane == last && a.rows) a.rows[row] = RowState{c, ref, low, log2_total, at, bin, 0, find.floor_of(bin)};
+      if (lane == last && a.rows) a.rows[row] = RowState{c, low, log2_total, at, bin, 0, m, find.floor_of(bin)};
       return;
     }
     if (look == 3) {
       // of the border's bin those whose y is not below it
       Step& t = find.begin();
       uint64_t mine = 0;
-      auto take = [&](uint64_t place, double rs) {
-        if ((double)logit_of(place) * c >= low && (b < cut || place <= cut_at)) mine += find.g.weight(rs);
+      auto take = [&](uint64_t place, uint32_t part) {
+        if ((double)logit_of(place) * c >= low && (b < cut || place <= cut_at)) mine += find.g.weight(part);
       };
       if (find.has(b))
         find.each_in_list(b, 0, ~0ull, take);
@@ -613,10 +613,10 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   }
   if (tid == 0) {
     const double log2_total = log2((double)total) - kUnits;
-    const int bin = find.bin_of(logit_of(at), rest);
+    const int bin = find.bin_of(logit_of(at), part);
     a.tokens[row] = (int64_t)(uint32_t)at;
-    a.logprobs[row] = (float)(((rest - bin) / 16 - log2_total) * 0.6931471805599453);
-    if (a.rows) a.rows[row] = RowState{c, ref, low, log2_total, cut_at, cut, 0, find.floor_of(cut)};
+    a.logprobs[row] = (float)((Grid::log_weight(bin, part) / 16 - log2_total) * 0.6931471805599453);
+    if (a.rows) a.rows[row] = RowState{c, low, log2_total, cut_at, cut, 0, m, find.floor_of(cut)};
   }
 }
 
@@ -629,7 +629,7 @@ __global__ __launch_bounds__(PT) void sample_probs(SampleArgs a, int blocks) {
   const int row = (int)(blockIdx.x / (uint32_t)blocks), block = (int)(blockIdx.x - (uint32_t)row * blocks);
   const RowReader<T> r(a, row);
   const RowState s = a.rows[row];
-  const Grid g(s.c, s.ref);
+  const Grid g(s.c, s.max);
   float* out = a.probs + (int64_t)row * a.ld_probs;
   // the rows without weights have one number but for the token's place
   const bool plain = s.cut < 0;
@@ -638,10 +638,10 @@ __global__ __launch_bounds__(PT) void sample_probs(SampleArgs a, int blocks) {
     if (plain) return s.cut == kOneHot && i == s.token ? 1.f : rest_of_row;
     if (!(x >= s.floor)) return 0.f;
     const double on = g.on(x);
-    const uint64_t bin = g.below(on);
-    if (bin > (uint64_t)s.cut || !((double)x * s.c >= s.low) || (bin == (uint64_t)s.cut && place(x, i) > s.cut_at)) return 0.f;
+    const uint32_t bin = g.bin(on);
+    if (bin > (uint32_t)s.cut || !((double)x * s.c >= s.low) || (bin == (uint32_t)s.cut && place(x, i) > s.cut_at)) return 0.f;
     // 2^whole 2^part: the exponential sees a small number
-    const double y = (g.rest(x, on) - (double)(int)bin) / 16 - s.log2_total, whole = rint(y);
+    const double y = Grid::log_weight((int)bin, g.part(on)) / 16 - s.log2_total, whole = rint(y);
     return ldexpf(__builtin_amdgcn_exp2f((float)(y - whole)), (int)whole);
   };
   const bool wide = aligned16(out + r.head);

@@ -6,20 +6,20 @@
 namespace catopt {
 
 // Weights exp((x - max) / T) lie on a grid of 16 steps to a factor of 2: with y =
-// x 16 log2(e) / T and n = rint(y), a logit belongs to the bin n and weighs
-// 2^(n / 16) 2^((y - n) / 16).  The second factor, between 0.978 and 1.022, is
-// rounded to 34 bits behind the point: a bin's weight is then a sum of integers,
-// the same in every order, whichever chunk of the row a logit lies in.  What a
-// choice can be off by is what such sums are off by, 2^-35 of a weight at random
-// and 2^-38 with one sign: a step of u is 2^-24.  A bin 768 steps below the largest
-// logit's weighs 2^-48 of it or less and counts as nothing.
+// x 16 log2(e) / T and n its whole part, a logit belongs to the bin n and weighs
+// 2^(n / 16) 2^((y - n) / 16).  The second factor, from 1 to 1.045, is rounded to 34
+// bits behind the point: a bin's weight is then a sum of integers, the same in
+// every order, whichever chunk of the row a logit lies in.  What a choice can be off
+// by is what such sums are off by, 2^-35 of a weight at random and 2^-38 with one
+// sign: a step of u is 2^-24.  A bin 768 steps below the largest logit's weighs
+// 2^-48 of it or less and counts as nothing.
 //
 // A chunk's bin holds the sum below bit 49 and the number of logits above.
 constexpr int kBins = 768;
 constexpr int kPoint = 34, kCount = 49;
-constexpr int kMaxChunk = 1 << 14;        // its sum stays below 2^(14 + 34.04), its number fits 15 bits
+constexpr int kMaxChunk = 1 << 14;        // its sum stays below 2^(14 + 34.07), its number fits 15 bits
 constexpr int64_t kMaxVocab = 1LL << 21;
-// Sums over bins are in units of 2^-42 of bin 0's weight: below 2^(21 + 42.04).
+// Sums over bins are in units of 2^-42 of bin 0's weight: below 2^(21 + 42.07).
 constexpr int kUnits = 42;
 
 struct SampleArgs {
@@ -47,10 +47,10 @@ struct ChunkHead {
 
 // What the probabilities of a row are worked out from.
 struct RowState {
-  double c, ref, low, log2_total;  // y = c x; the largest logit's n on the grid; the least y; log2 of the kept weights
-  uint64_t cut_at;                 // in the cut's bin the last place that is kept
-  int32_t cut, token;              // the last bin that is kept (some of it); kOneHot, kNone: the token alone, NaN
-  float floor;                     // nothing below it is kept
+  double c, low, log2_total;  // y = c x; the least y; log2 of the kept weights
+  uint64_t cut_at;            // in the cut's bin the last place that is kept
+  int32_t cut, token;         // the last bin that is kept (some of it); kOneHot, kNone: the token alone, NaN
+  float max, floor;           // the largest logit; nothing below the floor is kept
 };
 constexpr int kOneHot = -1, kNone = -2;
 
@@ -78,40 +78,47 @@ __device__ __forceinline__ double factor(double t, float max) {
   return fmax(fmin(16 * 1.4426950408889634 / t, 0x1p40 / fmax(fabs((double)max), 0x1p-120)), 0x1p-160);
 }
 
-// y rounded to a whole number n, on top of 1.5 2^52: that number's low bits are n,
-// and two such numbers' bits as far apart as their n are.
-constexpr double kGrid = 0x1.8p52;
 __device__ __forceinline__ uint64_t bits_of(double v) { return __builtin_bit_cast(uint64_t, v); }
 
-// A row's grid.  The constants of a logit's weight stay in scalar registers: left to
-// itself the compiler sets them anew for every logit of an unrolled loop, a third of
-// its instructions.
+// A row's grid: y, less a whole number near the largest logit's, on top of 1.5 2^20.
+// That sum's upper word then has y's whole part and its lower word the 32 bits behind
+// the point: a bin and a logit's part of it cost one fused multiply-add and one
+// subtraction.  The constants of a weight stay in registers: left to itself the
+// compiler sets them anew for every logit of an unrolled loop, a third of its
+// instructions.
 struct Grid {
-  double c, ref;  // y's factor, the largest logit's n on the grid
-  double shift = kGrid, back = -kGrid, s4, s3, s2, s1, s0;
+  double c, shift, top;  // y's factor; what is added; the largest logit's whole part
+  uint32_t ref;          // and its upper word
+  double s4, s3, s2, s1, s0;
 
-  __device__ __forceinline__ Grid(double t, float max) : Grid(factor(t, max), 0.0) { ref = on(max); }
-  __device__ __forceinline__ Grid(double c_, double ref_) : c(c_), ref(ref_) {
-    constexpr double one = 1LL << kPoint;
-    s4 = one * 1.4676443279006634e-07, s3 = one * 1.3551205157586767e-05, s2 = one * 0.0009383847924891109;
-    s1 = one * 0.04332169876016021, s0 = one * 1.0000000000000044 + 0x1p52;
-    asm("" : "+s"(shift), "+s"(back), "+s"(s4), "+s"(s3), "+s"(s2), "+s"(s1), "+s"(s0));
+  __device__ __forceinline__ Grid(double c_, float max) : c(c_) {
+    const double n = __builtin_fma((double)max, c, 0x1.8p52) - 0x1.8p52;
+    shift = 0x1.8p20 - n;
+    ref = (uint32_t)(bits_of(on(max)) >> 32);
+    top = n + (double)(int)(ref - 0x41380000u);
+    // Of 2^(part / 16), part from 0 to 1 in steps of 2^-32: the polynomial of the
+    // fourth power that Chebyshev's expansion gives, off by 2^-38.5 of it at most (one
+    // of the third by 2^-29.7), with 2^52 to make the sum's mantissa an integer.
+    constexpr double one = 1LL << kPoint, p = 0x1p-32;
+    s4 = one * p * p * p * p * 1.499781553911453e-07, s3 = one * p * p * p * 1.3547981600582377e-05;
+    s2 = one * p * p * 0.0009383858041510473, s1 = one * p * 0.04332169865843112, s0 = one * 1.000000000002533 + 0x1p52;
+    asm("" : "+s"(s4), "+v"(s3), "+s"(s2), "+s"(s1), "+s"(s0));
   }
   __device__ __forceinline__ double on(float x) const { return __builtin_fma((double)x, c, shift); }
-  // Bins from the largest logit's down to the one `on`, as far as they go.
-  __device__ __forceinline__ uint64_t below(double on) const { return bits_of(ref) - bits_of(on); }
-  // y - n.
-  __device__ __forceinline__ double rest(float x, double on) const { return __builtin_fma((double)x, c, -(on + back)); }
-  // 2^(rest / 16) in fixed point, |rest| <= 1/2: the polynomial of the fourth power
-  // that Chebyshev's expansion gives, off by 2^-38.5 of it at most (one of the third
-  // by 2^-29.7), with 2^52 in the sum's last addend making the mantissa an integer.
-  __device__ __forceinline__ uint64_t weight(double rest) const {
-    double s = __builtin_fma(s4, rest, s3);
-    s = __builtin_fma(s, rest, s2);
-    s = __builtin_fma(s, rest, s1);
-    s = __builtin_fma(s, rest, s0);
+  // Bins from the largest logit's down to this one's; a large number for one far below, -inf or a NaN.
+  __device__ __forceinline__ uint32_t bin(double on) const { return ref - (uint32_t)(bits_of(on) >> 32); }
+  static __device__ __forceinline__ uint32_t part(double on) { return (uint32_t)bits_of(on); }
+  // 2^(part / 16) in fixed point.
+  __device__ __forceinline__ uint64_t weight(uint32_t part) const {
+    const double u = (double)part;
+    double s = __builtin_fma(s4, u, s3);
+    s = __builtin_fma(s, u, s2);
+    s = __builtin_fma(s, u, s1);
+    s = __builtin_fma(s, u, s0);
     return bits_of(s) & 0xfffffffffffffull;  // below 2^35
   }
+  // log2 of a weight to the largest logit's bin's, times 16.
+  static __device__ __forceinline__ double log_weight(int bin, uint32_t part) { return (double)part * 0x1p-32 - bin; }
 };
 
 // The order of a row, as ascending numbers: the largest logit first, the lowest
