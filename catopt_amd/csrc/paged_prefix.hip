@@ -51,26 +51,42 @@ __global__ __launch_bounds__(NT, D == 64 ? 3 : 2) void paged_prefix_whole(PagedA
   paged_tile_rows<D, kBothSets>(p, o, blockIdx.x, tiles);
 }
 
-// A token's own sequence and its group (-1: none); -1 where the token is no sequence's.
-__device__ __forceinline__ int find_sets(const PagedArgs& p, const PagedArgs& o, int n, int& group) {
-  const int b = last_start(o.starts, o.B, (int)o.N, n);
-  group = b >= 0 && p.B > 0 ? last_start(p.groups, p.B, p.n_seq, b) : -1;
-  return b;
+// A set's sequences (or groups) c to c + 63, a lane each.
+struct SetLane {
+  int row0, nq, len;
+};
+__device__ __forceinline__ SetLane set_lane(const PagedArgs& a, int c) {
+  const int i = c + (int)(threadIdx.x & 63);
+  SetLane x{0x7fffffff, 0, 0};
+  if (i < a.B) {
+    set_rows<kCarriers>(a, i, x.row0, x.nq);
+    x.len = a.lens[i];
+  }
+  return x;
 }
 
 // Set a's ranges of row (n, hq), a bit for each of the row's carriers; none where
-// its sequence i does not have the token.
-__device__ __forceinline__ uint64_t set_ranges(const PagedArgs& a, int i, int n, int hq, int tile_rows) {
-  PagedTile x{};
-  x.b = i;
-  set_rows<kCarriers>(a, i, x.row0, x.nq);
-  if (n < x.row0 || n >= x.row0 + x.nq) return 0;
-  x.len = min(max(a.lens[i], 0), a.cap);
-  x.r0 = ((n - x.row0) * a.G + hq - (int)a.group.div(hq) * a.G) / tile_rows * tile_rows;
-  x.rows = min(tile_rows, x.nq * a.G - x.r0);
-  paged_ranges(a, x);
+// the last sequence that does not begin behind the token does not have it.  `x`:
+// the first 64 sequences.
+__device__ __forceinline__ uint64_t set_ranges(const PagedArgs& a, SetLane x, int n, int hq, int tile_rows) {
+  PagedTile t{};
+  for (int c = 0; c < a.B; c += 64) {
+    if (c > 0) x = set_lane(a, c);
+    const int k = __popcll(__ballot(x.row0 <= n));
+    if (k > 0) {
+      t.row0 = __builtin_amdgcn_readlane(x.row0, k - 1);
+      t.nq = __builtin_amdgcn_readlane(x.nq, k - 1);
+      t.len = __builtin_amdgcn_readlane(x.len, k - 1);
+    }
+    if (k < 64) break;
+  }
+  if (n < t.row0 || n >= t.row0 + t.nq) return 0;
+  t.len = min(max(t.len, 0), a.cap);
+  t.r0 = ((n - t.row0) * a.G + hq - (int)a.group.div(hq) * a.G) / tile_rows * tile_rows;
+  t.rows = min(tile_rows, t.nq * a.G - t.r0);
+  paged_ranges(a, t);
   const int lane = threadIdx.x & 63;
-  return __ballot(lane < a.splits && has_range(x, lane)) << a.part_first;
+  return __ballot(lane < a.splits && has_range(t, lane)) << a.part_first;
 }
 
 // A row's carriers to its result: WAVES waves, D / 4 lanes to a carrier's numerators.
@@ -81,11 +97,11 @@ __global__ __launch_bounds__(NT) void paged_prefix_combine(PagedArgs p, PagedArg
   const int row = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + (int)(threadIdx.x >> 6);  // N Hq < 2^30
   if (row >= o.N * o.Hq) return;
   const int n = (int)o.q_heads.div(row), hq = row - n * o.Hq;
-  int group;
-  const int b = find_sets(p, o, n, group);
-  uint64_t ranges = b >= 0 ? set_ranges(o, b, n, hq, o_rows) : 0;
+  // both sets' sequences at once: two memory latencies, the groups' being two
+  const SetLane own = set_lane(o, 0), shared = set_lane(p, 0);
+  uint64_t ranges = set_ranges(o, own, n, hq, o_rows);
   if (!ranges) return;  // no sequence's row
-  if (group >= 0) ranges |= set_ranges(p, group, n, hq, p_rows);
+  ranges |= set_ranges(p, shared, n, hq, p_rows);
   const int slots = o.part_ld, k0 = tid / TPR;
   const float c = o.scale * kLog2e;
   const float* ml = o.part + (int64_t)2 * row * slots;
