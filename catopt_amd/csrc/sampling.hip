@@ -100,7 +100,7 @@ constexpr int RT = 512, WAVES = RT / 64;
 constexpr int kList = 8192;   // logits of a row that are kept in LDS
 constexpr int kShort = 1024;  // as many are looked through as quickly as a bin of them
 constexpr int kParts = 128;   // of a range
-constexpr int kMaxChunks = 520;
+constexpr int kMaxChunks = (int)(kMaxVocab / kMaxChunk);
 
 // What one step of a search adds up.  Three of them take turns: a step clears the
 // next one's, which was last read before the barriers of the step before.
@@ -671,7 +671,12 @@ __global__ __launch_bounds__(PT) void sample_probs(SampleArgs a, int blocks) {
 
 // ------------------------------------------------------------------ host
 
-// Chunks of 16384 logits where they fill the CUs, else of 4096.
+// Chunks of 16384 logits: the fewer there are, the fewer bins are added up for a row
+// (top-k of 50 in 1 and 64 rows of 131072 fp32: 21.3 and 27.7 us, in chunks of 8192
+// 21.7 and 29.0, of 4096 23.8 and 33.1; 256 rows 55.0, 57.5, 65.6).  In rows of two of
+// them at most the chunks' own latency counts for more: 1 and 64 rows of 8000 take
+// 12.3 and 13.3 us, in chunks of 8192 11.6 and 12.6, of 4096 11.8 and 12.8.
+constexpr int kFewChunk = 8192, kFewLogits = 2 * kMaxChunk;
 struct Plan {
   int64_t chunk, chunks;
   int64_t heads, bins, rows;  // bytes
@@ -680,7 +685,7 @@ struct Plan {
 
 Plan plan_of(int64_t B, int64_t V, bool probs) {
   Plan p;
-  p.chunk = B * ((V + kMaxChunk - 1) / kMaxChunk) >= 1024 ? kMaxChunk : 4096;
+  p.chunk = V > kFewLogits ? kMaxChunk : kFewChunk;
   p.chunks = (V + p.chunk - 1) / p.chunk;
   p.heads = B * p.chunks * (int64_t)sizeof(ChunkHead);
   p.bins = B * p.chunks * kBins * 8;
@@ -694,7 +699,7 @@ int32_t launch(const SampleArgs& a, const Plan& p, hipStream_t st) {
   if (p.chunk == kMaxChunk)
     sample_chunks<T, kMaxChunk / CT><<<grid, dim3(CT), 0, st>>>(a);
   else
-    sample_chunks<T, 8><<<grid, dim3(CT), 0, st>>>(a);
+    sample_chunks<T, kFewChunk / CT><<<grid, dim3(CT), 0, st>>>(a);
   CATOPT_LAUNCH_CHECK();
   static bool done[kDevices] = {};
   const int32_t r = allow_lds(reinterpret_cast<const void*>(&sample_rows<T>), sizeof(RowLds), done);

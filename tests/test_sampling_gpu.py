@@ -125,6 +125,19 @@ def test_every_row_its_own_settings(V):
     assert all(torch.equal(m, n) for m, n in zip(a, b))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [8191, 8193, 16399, 24577, 32767, 32768, 32769, 32791, 49153])
+def test_rows_about_the_chunks_sizes(V, dtype):
+    """The last logit, the largest, is alone in its chunk, in aligned rows and in rows with logits outside the pieces."""
+    g = gen(V)
+    wide = logits(g, 4, V + 5, dtype)
+    for x in (wide[:, :V], wide[:, 3:V + 3]):
+        x = x.clone() if x.data_ptr() == wide.data_ptr() else x
+        x[1:3, -1] = 40.0
+        for setting in ((1.0, 0, 1.0, 0.0), (0.8, 60, 0.95, 0.001), (0.0, 0, 1.0, 0.0)):
+            check(x, torch.rand((4,), generator=g, device=DEV), *setting, ties=dtype is torch.bfloat16)
+
+
 @pytest.mark.parametrize("V", [9, 5000, 131072])
 @pytest.mark.parametrize("setting", [(1.0, 0, 1.0, 0.0), (1.0, 0, 0.5, 0.0), (1.0, 3, 1.0, 0.0), (2.0, 0, 0.3, 0.5), (1.0, 0, 1.0, 1.0)])
 def test_equal_logits_go_by_index(V, setting):
