@@ -89,12 +89,13 @@ __device__ __forceinline__ uint64_t set_ranges(const PagedArgs& a, SetLane x, in
   return __ballot(lane < a.splits && has_range(t, lane)) << a.part_first;
 }
 
-// A row's carriers to its result: WAVES waves, D / 4 lanes to a carrier's numerators.
-template <int D, int WAVES>
+// A row's carriers to its result by a wave, D / 4 lanes to a carrier's numerators.
+// (Four waves a row are level where the rows do not fill the CUs, 10.5 us a call to
+// 10.2 at 128 rows and 18.4 to 18.8 at 512, and slower at 2048, 51.2 to 47.7.)
+template <int D>
 __global__ __launch_bounds__(NT) void paged_prefix_combine(PagedArgs p, PagedArgs o, int p_rows, int o_rows) {
-  constexpr int TPR = D / 4, GROUPS = 64 * WAVES / TPR, U = 8;  // loads ahead of their additions
-  const int lane = threadIdx.x & 63, tid = WAVES == 4 ? threadIdx.x : lane;
-  const int row = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + (int)(threadIdx.x >> 6);  // N Hq < 2^30
+  constexpr int TPR = D / 4, GROUPS = 64 / TPR, U = 8;  // loads ahead of their additions
+  const int lane = threadIdx.x & 63, row = blockIdx.x * (NT / 64) + (int)(threadIdx.x >> 6);  // N Hq < 2^30
   if (row >= o.N * o.Hq) return;
   const int n = (int)o.q_heads.div(row), hq = row - n * o.Hq;
   // both sets' sequences at once: two memory latencies, the groups' being two
@@ -102,10 +103,10 @@ __global__ __launch_bounds__(NT) void paged_prefix_combine(PagedArgs p, PagedArg
   uint64_t ranges = set_ranges(o, own, n, hq, o_rows);
   if (!ranges) return;  // no sequence's row
   ranges |= set_ranges(p, shared, n, hq, p_rows);
-  const int slots = o.part_ld, k0 = tid / TPR;
+  const int slots = o.part_ld, k0 = lane / TPR;
   const float c = o.scale * kLog2e;
   const float* ml = o.part + (int64_t)2 * row * slots;
-  const float* num = part_numerators<kCarriers>(o) + (int64_t)row * slots * D + 4 * (tid % TPR);
+  const float* num = part_numerators<kCarriers>(o) + (int64_t)row * slots * D + 4 * (lane % TPR);
   const bool mine = ranges >> lane & 1;
   const float ms = mine ? ml[2 * lane] : kNegInf, ls = mine ? ml[2 * lane + 1] : 0.f;
   f32x4 ys[U];
@@ -130,27 +131,17 @@ __global__ __launch_bounds__(NT) void paged_prefix_combine(PagedArgs p, PagedArg
 #pragma unroll
     for (int i = 0; i < U; ++i) y += ys[i] * __shfl(f, min(s0 + i * GROUPS + k0, 63), 64);
   }
-  if constexpr (WAVES == 4) {
-    __shared__ f32x4 sums[GROUPS][TPR];
-    sums[k0][tid % TPR] = y;
-    __syncthreads();
-    if (tid < TPR) {
 #pragma unroll
-      for (int i = 1; i < GROUPS; ++i) y += sums[i][tid];
-    }
-  } else {
+  for (int s = TPR; s < 64; s <<= 1)
 #pragma unroll
-    for (int s = TPR; s < 64; s <<= 1)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], s, 64);
-  }
-  if (tid < TPR && 4 * tid < o.d) {
+    for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], s, 64);
+  if (lane < TPR && 4 * lane < o.d) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = finish(y[e], lt, o.normalize);
-    *reinterpret_cast<u32x2*>(o.o + (int64_t)n * o.o_t + (int64_t)hq * o.o_h + 4 * tid) =
+    *reinterpret_cast<u32x2*>(o.o + (int64_t)n * o.o_t + (int64_t)hq * o.o_h + 4 * lane) =
         u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
   }
-  if (tid == 0) row_stats(o, row, mx, lt);
+  if (lane == 0) row_stats(o, row, mx, lt);
 }
 
 // ------------------------------------------------------------------ host
@@ -242,16 +233,12 @@ int32_t launch(const PagedArgs& p, const PagedArgs& o, const Plan& x, hipStream_
   const int32_t r = allow_lds(reinterpret_cast<const void*>(kernel), bytes, done);
   if (r != CATOPT_OK) return r;
   const int64_t blocks = x.p.blocks + x.o.blocks, rows = o.N * o.Hq;
-  const bool wide = rows < 2048;  // four waves a row where the rows alone do not fill the CUs
-  const int64_t nc = wide ? rows : (rows + 3) / 4;
+  const int64_t nc = (rows + NT / 64 - 1) / (NT / 64);
   if (!grid_fits(blocks, NT) || !grid_fits(nc, NT)) return CATOPT_E_UNSUPPORTED;
   kernel<<<dim3((uint32_t)blocks), dim3(NT), bytes, s>>>(p, o, (uint32_t)x.p.blocks, (int)x.p.tiles, (int)x.o.tiles);
   CATOPT_LAUNCH_CHECK();
   const int p_rows = PFEW ? kFewRows : kTileRows, o_rows = OFEW ? kFewRows : kTileRows;
-  if (wide)
-    paged_prefix_combine<D, 4><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
-  else
-    paged_prefix_combine<D, 1><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
+  paged_prefix_combine<D><<<dim3((uint32_t)nc), dim3(NT), 0, s>>>(p, o, p_rows, o_rows);
   CATOPT_LAUNCH_CHECK();
   return CATOPT_OK;
 }
