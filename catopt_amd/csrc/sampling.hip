@@ -7,6 +7,13 @@
 // bins (one read of the row), and a row's workgroup finds the bins in which the
 // borders and the token lie, reads the row again for the logits of those alone, and
 // narrows them down to at most 64, which one wave ranks.
+//
+// Measured, 256 rows of 131072 fp32 logits, a share of 0.95: chunks 27 us (5.4 TB/s;
+// the arithmetic in 64 bits bounds them: VALU busy 0.55 at least, and bf16 logits,
+// half the bytes, take as long), rows 44, of which the row's read is 20 (7 TB/s), the
+// setup from the chunks' bins 7 and the borders of flat rows, with some thousand
+// logits in a bin, the rest.  64 rows of 50021 with settings of their own 6.7 and 12.2
+// us, one row of 32000 bf16 4.3 and 8.7: latency.
 #include "sampling.hpp"
 
 namespace catopt {
