@@ -212,3 +212,21 @@ def test_a_captured_step_goes_on_in_place(B, q):
         graphs[1].replay()
         pool, lens, count = release_ref(table, lens, ended, pool, count, page)
         assert p.tolist() == pool and kv.tolist() == lens and c.tolist() == [count]
+
+
+def test_table_past_32_bit_offsets():
+    """Rows of a table that lie more than 2^31 entries apart."""
+    ld = (1 << 30) + 24
+    wide = torch.empty((2 * ld + 16,), dtype=torch.int32, device=DEV)
+    t = wide.as_strided((3, 16), (ld, 1))
+    rng = random.Random(1)
+    table, lens, pool = _state(rng, 3, 100, 16, 16, 40)
+    t.copy_(ints(table))
+    new = [20, 1, 37]
+    r = P.paged_extend(t, ints(lens), ints(new), ints(pool), ints([len(pool)]), 60, 16)
+    want = extend_ref(table, lens, new, pool, len(pool), 60, 16)
+    assert t.tolist() == want[0] and r.slots.tolist() == want[3] and r.kv_lens.tolist() == want[4]
+    back, p = r.kv_lens.tolist(), ints(pool)
+    kv, c = P.paged_release(t, r.kv_lens, torch.tensor([True, False, True], device=DEV), p, r.free_count, 16)
+    after = release_ref(want[0], back, [True, False, True], pool, r.free_count.item(), 16)
+    assert p.tolist() == after[0] and kv.tolist() == after[1] and c.tolist() == [after[2]]

@@ -36,7 +36,7 @@ class Both:
         return own if p is None else torch.cat([self.cache.rows(pages, p), own], 1)
 
     def call(self, q, nq, scale, **kw):
-        args = dict(pre_lens=ints(self.pre), groups=ints(self.groups), lens=ints(self.own), starts=starts_of(nq))
+        args = dict(pre_lens=ints(self.pre), groups=ints(self.groups), lens=ints(self.own), starts=starts_of(nq or []))
         args.update({k: kw.pop(k) for k in list(kw) if k in args})
         return P.paged_prefix_attention(q, self.k, self.v, self.pre_table, args["pre_lens"], args["groups"], self.table,
                                         args["lens"], args["starts"], scale, **kw)
@@ -311,3 +311,85 @@ def test_nothing_to_do():
     out = torch.full_like(q, 5.0)
     P.paged_prefix_attention(q, c.k, c.v, c.pre_table, ints([40]), ints([0, 0]), c.table[:0], ints([]), ints([0]), 0.1, out=out)
     assert (out == 5).all()
+
+
+@pytest.mark.parametrize("nq,heads", [([1, 1], 16), ([1] * 70, 16), ([30, 64], 16), ([52] * 40, 32)])
+def test_pages_past_32_bit_offsets(nq, heads):
+    """The last pages of a cache of more than 2^31 elements (4 GiB of keys), in each form."""
+    page, Hkv, d = 64, 8, 128
+    small = Both([500], [0, len(nq)], [n + 90 for n in nq], Hkv, d, page, seed=2)
+    used, at = small.table.numel() + small.pre_table.numel(), (1 << 31) // (page * Hkv * d) + 9
+    k, v = (torch.empty((at + used, Hkv, page, d), dtype=BF16, device=DEV) for _ in range(2))
+    big = SimpleNamespace(table=torch.full_like(small.table, -1), pre_table=torch.full_like(small.pre_table, -1))
+    for to, table in ((big.table, small.table), (big.pre_table, small.pre_table)):
+        for b, i in (table >= 0).nonzero().tolist():
+            at += 1
+            to[b, i] = at
+            k[at], v[at] = small.k[table[b, i]], small.v[table[b, i]]
+    q = randn(gen(2), sum(nq), heads, d)
+    got = P.paged_prefix_attention(q, k, v, big.pre_table, ints([500]), ints([0, len(nq)]), big.table, ints(small.own),
+                                   starts_of(nq), 0.1)
+    assert torch.equal(got, small.call(q, nq, 0.1))
+    check_attention(small, q, nq, small.lens(), got, scale=0.1)
+
+
+@pytest.mark.parametrize("nq", [[1, 1, 1], [3, 5, 0]])
+@pytest.mark.parametrize("G", [33, 40, 130])
+def test_more_query_heads_than_a_tile_has_rows(G, nq):
+    _run([300], [0, 3], nq, [7, 90, 41], G, 1, 64, 16, seed=G)
+
+
+def test_a_captured_call_of_many_rows_replays_on_other_lengths():
+    """The tile loop over both sets, with rows that change their sequences between replays."""
+    nq, B = 52, 40
+    c = Both([300], [0, B], [nq + 60] * B, 8, 64, 16, seed=17)
+    q = randn(gen(17), B * nq, 32, 64)
+    pre, groups, lens, starts = ints([300]), ints([0, B]), ints(c.own), starts_of([nq] * B)
+
+    def run():
+        return P.paged_prefix_attention(q, c.k, c.v, c.pre_table, pre, groups, c.table, lens, starts, 0.1, return_ml=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for step in range(3):
+        new = [nq + (7 * b * step) % 40 * (-1) ** b for b in range(B)]
+        new[-1] += B * nq - sum(new)
+        c.pre, c.groups, c.own = [300 - 120 * step], [step, B - 2 * step], [min(n + 11 * step, nq + 60) for n in new]
+        c.cache.lens = c.pre + c.own
+        pre.copy_(ints(c.pre)), groups.copy_(ints(c.groups)), lens.copy_(ints(c.own)), starts.copy_(starts_of(new))
+        q.copy_(randn(gen(step), B * nq, 32, 64))
+        graph.replay()
+        assert all(torch.equal(torch.nan_to_num(x), torch.nan_to_num(y)) for x, y in zip(run(), out))
+        check_attention(c, q, new, c.lens(), out[0], scale=0.1, m=out[1], l=out[2])
+
+
+@pytest.mark.parametrize("nq", [1, 40, 700])
+def test_starts_that_do_not_ascend(nq):
+    """Nothing is promised for such rows; the padding stays and the next good call is as the one before."""
+    c = Both([90, 300], [0, 2, 3], [nq + 5] * 4, 8, 64, 16, seed=19)
+    n, end = 4 * nq, 2 ** 31 - 1
+    q = randn(gen(19), n + 2, 32, 64)
+    want = c.call(q[:n], [nq] * 4, 0.1)
+    for starts in ([0, 3 * nq, nq, 2 * nq, n], [end, 5, -1, -end, 0], [n, n, 0, 0, n], [0, end, 0, end, 0]):
+        out = torch.full_like(q, 7.0)
+        c.call(q[:n], [nq] * 4, 0.1, starts=ints(starts), out=out[:n])
+        assert (out[n:] == 7).all()
+    for groups in ([3, 1, 0], [end, -end, 4], [2, 0, end], [0, end, 0]):
+        c.call(q[:n], [nq] * 4, 0.1, groups=ints(groups))
+    assert torch.equal(c.call(q[:n], [nq] * 4, 0.1), want)
+
+
+@pytest.mark.parametrize("nq", [1, 40, 700])
+def test_rows_before_the_first_sequence_are_left_alone(nq):
+    c = Both([200], [0, 4], [nq + 30] * 4, 8, 64, 16, seed=23)
+    q = randn(gen(23), 4 * nq + 3, 32, 64)
+    out = torch.full_like(q, 5.0)
+    c.call(q, None, 0.1, starts=ints([3 + i * nq for i in range(5)]), out=out)
+    assert (out[:3] == 5).all()
+    check_attention(c, q[3:], [nq] * 4, c.lens(), out[3:], scale=0.1)

@@ -287,3 +287,39 @@ def test_two_captured_steps_and_an_eager_one():
             assert all(torch.equal(a, b) for a, b in zip(f(), o))
         assert all(torch.equal(a, b) for a, b in zip(eager, outs[1]))
         check(x, u, 0.8, k, 0.9)
+
+
+def test_rows_past_32_bit_offsets():
+    """Logits more than 2^31 elements apart, and probabilities of more than 2^31 elements from one row of logits."""
+    g, V, ld = gen(21), 4099, (1 << 30) + 8
+    x = torch.empty((2 * ld + V,), device=DEV).as_strided((3, V), (ld, 1))
+    small = logits(g, 3, V)
+    x.copy_(small)
+    u = torch.rand((3,), generator=g, device=DEV)
+    got = check(x, u, 0.9, 40, 0.9)
+    assert all(torch.equal(a, b) for a, b in zip(got, S.sample(small, u, 0.9, 40, 0.9, return_probs=True)))
+    V, B = 1 << 21, 1026
+    row = logits(g, 1, V)
+    u = torch.rand((B,), generator=g, device=DEV)
+    tokens, logs, probs = S.sample(row.expand(B, V), u, 0.9, 0, 0.5, return_probs=True)
+    for b in (0, 1023, 1024, B - 1):
+        one = S.sample(row, u[b:b + 1], 0.9, 0, 0.5, return_probs=True)
+        assert tokens[b] == one[0][0] and logs[b] == one[1][0] and torch.equal(probs[b], one[2][0])
+
+
+def test_calls_at_once_on_two_streams():
+    g = gen(22)
+    calls = [(logits(g, B, V, dt), torch.rand((B,), generator=g, device=DEV)) for B, V, dt in
+             ((40, 50021, torch.float32), (33, 70000, torch.bfloat16))]
+    want = [S.sample(x, u, 0.9, 0, 0.95, return_probs=True) for x, u in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for s, (x, u) in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(S.sample(x, u, 0.9, 0, 0.95, return_probs=True))
+    torch.cuda.synchronize()
+    for i, r in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(r, want[i % 2]))
