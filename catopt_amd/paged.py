@@ -559,11 +559,11 @@ def paged_extend(block_table: torch.Tensor, kv_lens: torch.Tensor, new_lens: tor
     if table is not block_table:
         raise ValueError(f"block_table is written in place and needs a contiguous last axis, got strides {block_table.stride()}")
     n_free = _pool(free_pages, free_count)
-    lens_out = kv_lens.new_empty((B,)) if kv_lens_out is None else _in_place("kv_lens_out", kv_lens_out, B)
-    count_out = kv_lens.new_empty((1,)) if free_count_out is None else _in_place("free_count_out", free_count_out, 1)
-    starts = kv_lens.new_empty((B + 1,))
-    positions = kv_lens.new_empty((n_tokens,), dtype=torch.int64)
-    slots = kv_lens.new_empty((n_tokens,), dtype=torch.int64)
+    lens_out = kv_lens.new_empty(B) if kv_lens_out is None else _in_place("kv_lens_out", kv_lens_out, B)
+    count_out = kv_lens.new_empty(1) if free_count_out is None else _in_place("free_count_out", free_count_out, 1)
+    starts = kv_lens.new_empty(B + 1)
+    positions = kv_lens.new_empty(n_tokens, dtype=torch.int64)
+    slots = torch.empty_like(positions)
     st = _launch(dev, L.load().catopt_hip_paged_extend, B, n_tokens, page_size, table.data_ptr(), table_ld, n_table,
                  kv_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), n_free, free_count.data_ptr(), offsets_at,
                  starts.data_ptr(), positions.data_ptr(), slots.data_ptr(), lens_out.data_ptr(), count_out.data_ptr())
@@ -591,13 +591,13 @@ def paged_release(block_table: torch.Tensor, kv_lens: torch.Tensor, released: to
     kv_lens, released = _vector("kv_lens", kv_lens, torch.int32, B), _vector("released", released, torch.bool, B)
     table, n_table, table_ld = _table("block_table", block_table, B)
     n_free = _pool(free_pages, free_count)
-    lens_out = kv_lens.new_empty((B,)) if kv_lens_out is None else _in_place("kv_lens_out", kv_lens_out, B)
-    count_out = kv_lens.new_empty((1,)) if free_count_out is None else _in_place("free_count_out", free_count_out, 1)
+    lens_out = kv_lens.new_empty(B) if kv_lens_out is None else _in_place("kv_lens_out", kv_lens_out, B)
+    count_out = kv_lens.new_empty(1) if free_count_out is None else _in_place("free_count_out", free_count_out, 1)
     lib = L.load()
     wsb = lib.catopt_hip_paged_release_workspace_bytes(B)
     ws_at = None
     if wsb > 0:
-        ws = kv_lens.new_empty((wsb // 4,))
+        ws = kv_lens.new_empty(wsb // 4)
         ws_at = ws.data_ptr()
     st = _launch(dev, lib.catopt_hip_paged_release, B, page_size, table.data_ptr(), table_ld, n_table, kv_lens.data_ptr(),
                  released.data_ptr(), free_pages.data_ptr(), n_free, free_count.data_ptr(), lens_out.data_ptr(),

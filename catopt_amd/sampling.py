@@ -26,7 +26,8 @@ SAMPLE_MAX_VOCAB = 1 << 21
 def _workspace(B: int, V: int, probs: bool) -> int:
     n = L.load().catopt_hip_sample_workspace_bytes(B, V, probs)
     if n < 0:
-        raise NotImplementedError(f"sample takes vocabularies of up to {SAMPLE_MAX_VOCAB}, got {B} rows of {V}")
+        raise NotImplementedError(f"sample takes up to {1 << 20} rows, vocabularies of up to {SAMPLE_MAX_VOCAB} and 2^36 "
+                                  f"logits in all, got {B} rows of {V}")
     return n
 
 
@@ -89,8 +90,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, temperature: float | to
     if (logits.stride(1) != 1 and V > 1) or (B > 1 and logits.stride(0) < 0):
         logits = logits.contiguous()
     uniforms = uniforms.contiguous()
-    tokens = uniforms.new_empty((B,), dtype=torch.int64)
-    logprobs = uniforms.new_empty((B,))
+    tokens = uniforms.new_empty(B, dtype=torch.int64)
+    logprobs = torch.empty_like(uniforms)
     probs = uniforms.new_empty((B, V)) if return_probs else None
     if B:
         k_all = min(int(k_all), V)
