@@ -5,8 +5,9 @@
 // token is the first kept one whose running sum of weights passes u times the kept
 // weights.  So nothing is sorted: a chunk's workgroup adds its logits' weights up in
 // bins (one read of the row), and a row's workgroup finds the bins in which the
-// borders and the token lie, reads the row again for the logits of those alone, and
-// narrows them down to at most 64, which one wave ranks.
+// borders and the token lie and reads the row again for the logits of those alone.
+// Where they are few they are ranked, and one wave follows the definition; else each
+// border is narrowed down to at most 64 of them.
 //
 // Measured, 256 rows of 131072 fp32 logits, a share of 0.95: chunks 27 us (5.4 TB/s;
 // the arithmetic in 64 bits bounds them: VALU busy 0.55 at least, and bf16 logits,
@@ -107,6 +108,10 @@ constexpr int RT = 512, WAVES = RT / 64;
 constexpr int kList = 8192;   // logits of a row that are kept in LDS
 constexpr int kShort = 1024;  // as many are looked through as quickly as a bin of them
 constexpr int kParts = 128;   // of a range
+// As many are ranked and the rest left to one wave, if they are all that may be kept:
+// 48 rows of 65536 bf16, a rank of 200 and a share of 0.98 of it, 14 us where three
+// searches by parts take 19.5.  (Twice as many would not fit a wave's registers.)
+constexpr int kRanked = 512;
 constexpr int kMaxChunks = (int)(kMaxVocab / kMaxChunk);
 
 // What one step of a search adds up.  Three of them take turns: a step clears the
@@ -135,12 +140,12 @@ struct RowLds {
 // (min and max of the headers take 64-bit integers as doubles.)
 __device__ __forceinline__ uint64_t least_of(uint64_t a, uint64_t b) { return a < b ? a : b; }
 
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {  // of a lane that is the same for the wave
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {  // of a lane that is the same for the wave
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
-__device__ __forceinline__ double lane_f64(double v, int lane) {
-  return __builtin_bit_cast(double, lane_u64(__builtin_bit_cast(uint64_t, v), lane));
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  return __builtin_bit_cast(double, lane_of(__builtin_bit_cast(uint64_t, v), lane));
 }
 // The value of the lane that a DPP control names, 0 where there is none (row_shr
 // by 1 to 8 within 16 lanes, then the ends of 16 and of 32 lanes to those behind).
@@ -171,7 +176,7 @@ __device__ __forceinline__ V wave_scan(V v) {
 // How many of lanes j, j + step ... below n hold less than this one.
 __device__ __forceinline__ int lanes_below(uint64_t mine, int j, int n, int step) {
   int below = 0;
-  for (; j < n; j += step) below += lane_u64(mine, j) < mine;
+  for (; j < n; j += step) below += lane_of(mine, j) < mine;
   return below;
 }
 // The wave's places (~0 behind the last of n) by their ranks, lane by lane.
@@ -434,6 +439,69 @@ struct Search {
   }
 };
 
+// What decides a row's token among the logits that may be kept: bins up to `end`.
+struct RowEnd {
+  const SampleArgs& a;
+  int row;
+  float m;
+  double low, c, u;
+  uint64_t total;  // without top-k
+  const Settings& set;
+  int end;
+  bool by_rank, by_sum, by_low;
+};
+
+// The row's result by one wave, E places in the order a lane, ~0 behind the n-th.
+// What is kept is a prefix by each of the three, so that counts say where it ends.
+template <typename T, int E>
+__device__ __forceinline__ void choose(const Search<T>& find, const RowEnd& r, const uint64_t (&at)[E], int n) {
+  const int lane = threadIdx.x & 63;
+  auto count = [&](auto f) {
+    int k = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) k += __builtin_popcountll(__ballot(f(E * lane + e, e)));
+    return k;
+  };
+  bool in[E];
+  double sums[E], run = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    uint32_t part;
+    const int bin = find.bin_of(logit_of(at[e]), part);
+    in[e] = E * lane + e < n && bin <= r.end;
+    if (in[e]) run += (double)find.g.weight(part) * scale_of(bin);
+    sums[e] = run;
+  }
+  const double upto = wave_scan(run), before = __shfl_up(upto, 1, 64);
+#pragma unroll
+  for (int e = 0; e < E; ++e) sums[e] = e == E - 1 ? upto : lane ? before + sums[e] : sums[e];
+  auto of = [&](const auto& v, int i) {  // of the i-th place, the same for the wave
+    auto x = v[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) x = i % E == e ? v[e] : x;
+    return lane_of(x, i / E);
+  };
+  int kept = r.by_rank ? (int)r.set.k : count([&](int i, int e) { return in[e]; });
+  const double whole = r.by_rank ? of(sums, kept - 1) : (double)r.total;
+  if (r.by_sum) kept = min(kept, 1 + count([&](int i, int e) { return i < kept && !(sums[e] >= r.set.p * whole); }));
+  if (r.by_low) kept = count([&](int i, int e) { return i < kept && (double)logit_of(at[e]) * r.c >= r.low; });
+  const int last = max(kept - 1, 0);
+  const double kept_sum = of(sums, last);
+  const int from = min(last, count([&](int i, int e) { return i <= last && !(sums[e] > r.u * kept_sum); }));
+  const double log2_total = log2(kept_sum) - kUnits;
+  uint32_t p;
+  const uint64_t token = of(at, from), cut = of(at, last);
+  const int token_bin = find.bin_of(logit_of(token), p);
+  if (lane == 0) {
+    r.a.tokens[r.row] = (int64_t)(uint32_t)token;
+    r.a.logprobs[r.row] = (float)((Grid::log_weight(token_bin, p) / 16 - log2_total) * 0.6931471805599453);
+    if (r.a.rows) {
+      const int bin = find.bin_of(logit_of(cut), p);
+      r.a.rows[r.row] = RowState{r.c, r.low, log2_total, cut, bin, 0, r.m, find.floor_of(bin)};
+    }
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -567,34 +635,45 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     if (look == 0 || !find.has(b)) find.list_bins(list, list2);
     if (look == 0) {
       const int n_list = (int)find.n_list;
-      if (find.listed.first != 0 || n_list > 64) continue;
-      // all that may be kept is in one wave: the definition, lane by lane, after the waves have ranked them together
-      at = lane < n_list ? s.list[lane] : ~0ull;
-      Step& t = find.begin();
-      atomicAdd(&t.n[lane], (uint32_t)lanes_below(at, wave, n_list, WAVES));
+      if (find.listed.first != 0) continue;
+      // All that may be kept is in the list.  Where a wave's lanes hold it, the definition:
+      const RowEnd row_end{a, row, m, low, c, u, total, set, end, by_rank, by_sum, by_low};
+      if (n_list <= 64) {  // the waves have ranked them together
+        at = lane < n_list ? s.list[lane] : ~0ull;
+        Step& t = find.begin();
+        atomicAdd(&t.n[lane], (uint32_t)lanes_below(at, wave, n_list, WAVES));
+        __syncthreads();
+        if (wave > 0) return;
+        const uint64_t one[1] = {by_rank_of(at, (int)t.n[lane], n_list)};
+        choose<T, 1>(find, row_end, one, n_list);
+        return;
+      }
+      const int n_all = (int)s.cum_n[end];
+      if (n_all > kRanked) continue;
+      __syncthreads();  // the counts have been read
+      // by bins, then within each: a bin's place is its count of logits up to it, counted down
+      uint64_t *grouped = s.list + kList - 2 * kRanked, *sorted = grouped + kRanked;
+      for (int i = tid; i < n_list; i += RT) {
+        const uint64_t x = s.list[i];
+        const int b = find.bin_of(logit_of(x), part);
+        if (b <= end) grouped[(atomicSub(&s.cum_n[b], 1u) - 1) & (kRanked - 1)] = x;
+      }
+      __syncthreads();
+      if (tid < n_all) {
+        const uint64_t x = grouped[tid];
+        const int b = find.bin_of(logit_of(x), part), first = (int)s.cum_n[b], last = b < end ? (int)s.cum_n[b + 1] : n_all;
+        int rank = first;
+#pragma unroll 4
+        for (int j = first; j < last; ++j) rank += grouped[j] < x;
+        sorted[rank & (kRanked - 1)] = x;
+      }
       __syncthreads();
       if (wave > 0) return;
-      at = by_rank_of(at, (int)t.n[lane], n_list);
-      const int bin = find.bin_of(logit_of(at), part);
-      const int n_all = __builtin_popcountll(__ballot(lane < n_list && bin <= end));
-      const double sums = wave_scan(lane < n_all ? (double)find.g.weight(part) * scale_of(bin) : 0);
-      const double whole = by_rank ? lane_f64(sums, (int)set.k - 1) : (double)total;
-      bool kept = lane < (by_rank ? (int)set.k : n_all);
-      if (by_sum) {
-        const uint64_t reach = __ballot(kept && sums >= set.p * whole);
-        if (reach) kept = lane <= __builtin_ctzll(reach);
-      }
-      if (by_low) kept = kept && (double)logit_of(at) * c >= low;
-      const int last = 63 - __builtin_clzll(__ballot(kept) | 1);
-      const double kept_sum = lane_f64(sums, last);
-      const uint64_t pass = __ballot(lane <= last && sums > u * kept_sum);
-      const int from = pass ? __builtin_ctzll(pass) : last;
-      const double log2_total = log2(kept_sum) - kUnits;
-      if (lane == from) {
-        a.tokens[row] = (int64_t)(uint32_t)at;
-        a.logprobs[row] = (float)((Grid::log_weight(bin, part) / 16 - log2_total) * 0.6931471805599453);
-      }
-      if (lane == last && a.rows) a.rows[row] = RowState{c, low, log2_total, at, bin, 0, m, find.floor_of(bin)};
+      constexpr int E = kRanked / 64;
+      uint64_t some[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) some[e] = E * lane + e < n_all ? sorted[E * lane + e] : ~0ull;
+      choose<T, E>(find, row_end, some, n_all);
       return;
     }
     if (look == 3) {

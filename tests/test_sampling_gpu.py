@@ -323,3 +323,19 @@ def test_calls_at_once_on_two_streams():
     torch.cuda.synchronize()
     for i, r in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(r, want[i % 2]))
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 130, 511, 512, 513, 1023, 1025])
+@pytest.mark.parametrize("equal", [False, True])
+def test_as_many_logits_as_may_be_kept(n, equal):
+    """n logits above the others, by far: whether they are ranked or searched in depends on their number."""
+    g, V = gen(n), 9000
+    x = torch.full((5, V), -200.0, device=DEV)
+    for b in range(5):
+        at = torch.randperm(V, generator=g, device=DEV)[:n]
+        x[b, at] = 1.5 if equal else torch.randn((n,), generator=g, device=DEV) * (0.01 + b)
+    u = torch.rand((5,), generator=g, device=DEV)
+    for setting in ((1.0, 0, 0.9, 0.0), (0.9, n, 1.0, 0.0), (0.9, n - 1, 0.77, 0.0), (1.0, n - 3, 0.995, 1e-3), (1.1, 0, 1.0, 1e-30),
+                    (1.0, 64, 0.5, 0.0)):
+        # a share of 1e-30 is nearer to every small weight than sums are off, but those here are below e^-180 = 1e-78
+        check(x, u, *setting, ties=equal or setting[3] == 1e-30)
