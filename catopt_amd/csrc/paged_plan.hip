@@ -10,9 +10,9 @@
 // in LDS and takes new pages from the pool by their number, so that no block reads
 // what another one writes.
 //
-// Measured: a step of 8 requests 3.6 us, of 73483 tokens of 500 requests 5.5 (1.4 MB);
-// the pages of 16 sequences given back in 2.6, of 512 with half of them ended, of up
-// to 16000 keys, in 4.5 + 6.0.  An empty launch takes some 2.
+// Measured: a step of 8 requests 3.5 us, of 73483 tokens of 500 requests 5.4 (1.4 MB);
+// the pages of 16 sequences given back in 2.7, of 512 with half of them ended, of up
+// to 16000 keys, in 4.5 + 5.9.  An empty launch takes some 2.
 #include "paged.hpp"
 
 namespace catopt {

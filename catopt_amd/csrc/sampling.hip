@@ -13,8 +13,8 @@
 // the arithmetic in 64 bits bounds them: VALU busy 0.55 at least, and bf16 logits,
 // half the bytes, take as long), rows 44, of which the row's read is 20 (7 TB/s), the
 // setup from the chunks' bins 7 and the borders of flat rows, with some thousand
-// logits in a bin, the rest.  64 rows of 50021 with settings of their own 6.7 and 12.2
-// us, one row of 32000 bf16 4.3 and 8.7: latency.
+// logits in a bin, the rest.  64 rows of 50021 with settings of their own 6.4 and 12.7
+// us, one row of 32000 bf16 4.3 and 8.9: latency.
 #include "sampling.hpp"
 
 namespace catopt {
