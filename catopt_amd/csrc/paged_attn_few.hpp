@@ -117,7 +117,8 @@ __device__ __forceinline__ void paged_few(const PagedArgs& a, uint32_t block) {
 
   // With one stage of LDS, K and V on their own: the next K rows are loaded once the
   // scores have been formed, the next V rows once these have been read, so that one
-  // of both is on its way all the time.
+  // of both is on its way all the time: 64 steps of 100 to 1500 own keys behind 8192
+  // shared ones 52.6 -> 48 us.
   constexpr bool APART = F == kCarriers && L::STAGES == 1;
   auto issue_k = [&](int lane0, const KeyGroup& at) {
 #pragma unroll

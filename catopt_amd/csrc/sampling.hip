@@ -106,11 +106,14 @@ __global__ __launch_bounds__(CT) void sample_chunks(SampleArgs a) {
 
 constexpr int RT = 512, WAVES = RT / 64;
 constexpr int kList = 8192;   // logits of a row that are kept in LDS
-constexpr int kShort = 1024;  // as many are looked through as quickly as a bin of them
+// As many are taken whole where a border would need a bin of them alone: 512 and 2048
+// measure level, 8192 slower (a share of 0.95 of 64 flat rows of 50021 29.7 -> 31.5 us).
+constexpr int kShort = 1024;
 constexpr int kParts = 128;   // of a range
 // As many are ranked and the rest left to one wave, if they are all that may be kept:
-// 48 rows of 65536 bf16, a rank of 200 and a share of 0.98 of it, 14 us where three
-// searches by parts take 19.5.  (Twice as many would not fit a wave's registers.)
+// 48 rows of 65536 bf16, a rank of 200 and a share of 0.98 of it, 25 us where searches
+// by parts take 30; 32 rows of 250 normal logits 15 for 18 to 20, of 500 equal ones 29
+// for 24 to 29.
 constexpr int kRanked = 512;
 constexpr int kMaxChunks = (int)(kMaxVocab / kMaxChunk);
 
@@ -126,6 +129,7 @@ struct Step {
 struct RowLds {
   uint64_t cum[kBins];  // weights up to a bin's end, in units of 2^-42 of bin 0's
   uint64_t list[kList];
+  uint64_t grouped[kRanked], sorted[kRanked];  // by bins, in order
   Step steps[3];
   struct {
     uint64_t lo, hi, sum;
@@ -652,27 +656,26 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
       if (n_all > kRanked) continue;
       __syncthreads();  // the counts have been read
       // by bins, then within each: a bin's place is its count of logits up to it, counted down
-      uint64_t *grouped = s.list + kList - 2 * kRanked, *sorted = grouped + kRanked;
       for (int i = tid; i < n_list; i += RT) {
         const uint64_t x = s.list[i];
         const int b = find.bin_of(logit_of(x), part);
-        if (b <= end) grouped[(atomicSub(&s.cum_n[b], 1u) - 1) & (kRanked - 1)] = x;
+        if (b <= end) s.grouped[(atomicSub(&s.cum_n[b], 1u) - 1) & (kRanked - 1)] = x;
       }
       __syncthreads();
       if (tid < n_all) {
-        const uint64_t x = grouped[tid];
+        const uint64_t x = s.grouped[tid];
         const int b = find.bin_of(logit_of(x), part), first = (int)s.cum_n[b], last = b < end ? (int)s.cum_n[b + 1] : n_all;
         int rank = first;
 #pragma unroll 4
-        for (int j = first; j < last; ++j) rank += grouped[j] < x;
-        sorted[rank & (kRanked - 1)] = x;
+        for (int j = first; j < last; ++j) rank += s.grouped[j] < x;
+        s.sorted[rank & (kRanked - 1)] = x;
       }
       __syncthreads();
       if (wave > 0) return;
       constexpr int E = kRanked / 64;
       uint64_t some[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) some[e] = E * lane + e < n_all ? sorted[E * lane + e] : ~0ull;
+      for (int e = 0; e < E; ++e) some[e] = E * lane + e < n_all ? s.sorted[E * lane + e] : ~0ull;
       choose<T, E>(find, row_end, some, n_all);
       return;
     }

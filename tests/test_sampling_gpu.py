@@ -339,3 +339,18 @@ def test_as_many_logits_as_may_be_kept(n, equal):
                     (1.0, 64, 0.5, 0.0)):
         # a share of 1e-30 is nearer to every small weight than sums are off, but those here are below e^-180 = 1e-78
         check(x, u, *setting, ties=equal or setting[3] == 1e-30)
+
+
+@pytest.mark.parametrize("p", [1.0, 0.9])
+@pytest.mark.parametrize("n", [8000, 9000])
+def test_many_logits_next_to_the_borders_bin(n, p):
+    """Weights in steps of 2^(1 / 16): a hundred logits in the first ten of them, thousands a rounding below those."""
+    g, V, step = gen(n), 20000, math.log(2) / 16
+    x = torch.full((4, V), -300.0, device=DEV)
+    below = np.nextafter(np.float32(-10 * step), np.float32(-1))
+    assert -10 * step * (1 + 2.0 ** -22) < below < -10 * step
+    for b in range(4):
+        at = torch.randperm(V, generator=g, device=DEV)
+        for i0, i1, value in ((0, 1, 0.0), (1, 61, -9.2 * step), (61, 100, -9.7 * step), (100, 100 + n, float(below))):
+            x[b, at[i0:i1]] = value
+    check(x, torch.rand((4,), generator=g, device=DEV), 1.0, 70, p, ties=True)
