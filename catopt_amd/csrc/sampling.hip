@@ -207,6 +207,11 @@ __device__ __forceinline__ double scale_of(int b) {
   return ldexp(x * y, kUnits - kPoint - (b >> 4));
 }
 
+// The log of a token's share, of the weight that the sum has: at most 0, and 0 for one alone.
+__device__ __forceinline__ float log_share(uint64_t weight, int bin, double total) {
+  return (float)log(fmin((double)weight * scale_of(bin) / total, 1.0));
+}
+
 struct Bins {
   int first, last;
   __device__ __forceinline__ bool has(int b) const { return b >= first && b <= last; }
@@ -498,7 +503,7 @@ __device__ __forceinline__ void choose(const Search<T>& find, const RowEnd& r, c
   const int token_bin = find.bin_of(logit_of(token), p);
   if (lane == 0) {
     r.a.tokens[r.row] = (int64_t)(uint32_t)token;
-    r.a.logprobs[r.row] = (float)((Grid::log_weight(token_bin, p) / 16 - log2_total) * 0.6931471805599453);
+    r.a.logprobs[r.row] = log_share(find.g.weight(p), token_bin, kept_sum);
     if (r.a.rows) {
       const int bin = find.bin_of(logit_of(cut), p);
       r.a.rows[r.row] = RowState{r.c, r.low, log2_total, cut, bin, 0, r.m, find.floor_of(bin)};
@@ -704,7 +709,7 @@ __global__ __launch_bounds__(RT) void sample_rows(SampleArgs a) {
     const double log2_total = log2((double)total) - kUnits;
     const int bin = find.bin_of(logit_of(at), part);
     a.tokens[row] = (int64_t)(uint32_t)at;
-    a.logprobs[row] = (float)((Grid::log_weight(bin, part) / 16 - log2_total) * 0.6931471805599453);
+    a.logprobs[row] = log_share(find.g.weight(part), bin, (double)total);
     if (a.rows) a.rows[row] = RowState{c, low, log2_total, cut_at, cut, 0, m, find.floor_of(cut)};
   }
 }

@@ -354,3 +354,21 @@ def test_many_logits_next_to_the_borders_bin(n, p):
         for i0, i1, value in ((0, 1, 0.0), (1, 61, -9.2 * step), (61, 100, -9.7 * step), (100, 100 + n, float(below))):
             x[b, at[i0:i1]] = value
     check(x, torch.rand((4,), generator=g, device=DEV), 1.0, 70, p, ties=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("setting", [(1.0, 0, 1.0, 0.0), (0.7, 0, 0.1, 0.0), (0.83, 0, 1.0, 1.0), (0.7, 60, 0.2, 0.9), (1e-3, 0, 0.9, 0.0)])
+def test_a_token_alone_has_all_the_weight(dtype, setting):
+    """Its log probability is 0, whatever its logit is a multiple of; no token's is above."""
+    g, V = gen(31), 32000
+    x = logits(g, 200, V, dtype)
+    u = torch.rand((200,), generator=g, device=DEV)
+    at = torch.randint(0, V, (200,), generator=g, device=DEV)
+    top = x.amax(1) + 4 + torch.arange(200, device=DEV, dtype=dtype) / 64
+    alone = x.clone() if setting[0] < 1 else torch.full_like(x, -math.inf)
+    alone.scatter_(1, at[:, None], top[:, None])
+    tokens, logs, probs = S.sample(alone, u, *setting, return_probs=True)
+    assert torch.equal(tokens, at) and (logs == 0).all()
+    # an exponential of one step, 2^-23, of a number that is off by 2^-33 at most
+    assert (probs.gather(1, at[:, None]) - 1).abs().max() <= 2.0 ** -22 and (probs > 0).sum() == 200
+    assert (S.sample(x, u, *setting)[1] <= 0).all()
